@@ -191,6 +191,64 @@ int see_cuda_xent_forward_static(const float* logits, const int32_t* labels, flo
 uint64_t see_cuda_static_max_rows(void);
 const char* see_cuda_static_last_error(void);
 
+/* ---- A block's own weights: norm, gated feed-forward, AdamW -----------------------
+ * No counterpart in the reference, whose plans train adapters beside frozen weights: what a step that also trains a
+ * block's norms and feed-forward weights needs, on device memory that the caller owns.  All pointers below are DEVICE
+ * pointers of the handle's device unless a line says otherwise; rows are row-major; work is enqueued on the handle's
+ * stream (see_cuda_set_stream), whatever device is current, and nothing is allocated, copied or waited for, so a call
+ * can be captured into a CUDA graph after a first call of its kind.  Calls share no memory but what they are given:
+ * calls that can overlap on the GPU need workspaces of their own.  A call that is refused (SEE_ERROR: a null, misaligned
+ * or overlapping operand, a size outside the stated range, a workspace too small) enqueues nothing.  Outputs may not
+ * overlap inputs or one another; two matrices may lie side by side in the rows of one buffer (equal strides). */
+enum { SEE_F32 = 0, SEE_BF16 = 1, SEE_F16 = 2 };        /* element types */
+enum { SEE_NORM_LAYER = 0, SEE_NORM_RMS = 1 };
+enum { SEE_ACT_RELU = 1, SEE_ACT_GELU = 2, SEE_ACT_SILU = 3 };   /* GELU: the tanh form, as in the plans */
+
+/* Rows of `cols` columns (1 .. 16384), up to 2^31 - 1 of them.  x_type: of x, dx and addend; y_type: of y and dy; equal,
+ * or x_type f32.  Strides: elements from a row to the next (0: cols), of x, dx and addend, and of y and dy; what lies
+ * between the rows stays as it is. */
+typedef struct see_norm_shape {
+  int32_t kind, x_type, y_type;
+  float eps;
+  uint64_t rows, cols, x_stride, y_stride;
+} see_norm_shape;
+/* Layer: y = (x - mean) rstd gamma + beta, mean and rstd = (var + eps)^-1/2 of each row kept for the backward pass.
+ * Rms: y = x rstd gamma, rstd = (mean of x^2 + eps)^-1/2; beta and mean are NULL.  gamma, beta [cols], mean, rstd [rows]
+ * are f32. */
+int see_cuda_norm_forward(see_cuda_backend* h, const see_norm_shape* shape, const void* x, const float* gamma,
+                          const float* beta, void* y, float* mean, float* rstd);
+/* dx (plus addend, unless NULL: the gradient that reaches x past the norm), dgamma [cols] and, layer, dbeta [cols]: f32
+ * sums over all rows, in an order that the sizes alone fix (zero rows: zeros).  Rms: mean and dbeta are NULL.
+ * workspace: at least see_cuda_norm_backward_workspace(rows, cols) bytes, 16-byte aligned. */
+uint64_t see_cuda_norm_backward_workspace(uint64_t rows, uint64_t cols);
+int see_cuda_norm_backward(see_cuda_backend* h, const see_norm_shape* shape, const void* dy, const void* x,
+                           const float* gamma, const float* mean, const float* rstd, const void* addend, void* dx,
+                           float* dgamma, float* dbeta, void* workspace, uint64_t workspace_bytes);
+
+/* One AdamW step over `count` tensors of n elements each, in the kAdamWStep instruction's expression.  p: f32 weights.
+ * g: their gradients.  copy: the new weights in 16 bits (copy_type SEE_BF16 or SEE_F16), or NULL with copy_type SEE_F32.
+ * state_bits 32: m, v f32 moments.  state_bits 8: m and v are e4m3 (one byte an element), v holding the ROOT of the second
+ * moment; m_scale, v_scale: an f32 for each block of SEE_ADAMW_BLOCK elements (the last may be short), whose product with
+ * an element is its value.  All zero bytes are the state before the first step.  A moment that is not finite makes its
+ * block's NaN.  The 8-bit rounding cuts at a point that depends on element and params->step alone.
+ * flags: SEE_ADAMW_NO_DECAY: weight decay 0.  grad_scale: an f32 that every gradient is multiplied by first, or NULL.
+ * `tensors` and `params` are HOST memory and are read before the call returns.  p, m, v, the scales and copy of all
+ * tensors are written and may not overlap. */
+enum { SEE_ADAMW_BLOCK = 256 };
+enum { SEE_ADAMW_NO_DECAY = 1 };
+typedef struct see_adamw_tensor {
+  float* p;
+  const void* g;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  void* copy;
+  uint64_t n;
+  int32_t g_type, copy_type;
+  uint32_t flags, pad;
+} see_adamw_tensor;
+int see_cuda_adamw_step(see_cuda_backend* h, const see_adamw_tensor* tensors, uint64_t count, int state_bits,
+                        const see_step_params* params, const float* grad_scale);
+
 /* ---- The dispatcher: UpdateEngine over the CUDA backend ----------------------
  * Mirrors the hot-path surface of seeml::update_rt::UpdateEngine (reference:
  * runtime/dispatcher/update_engine.h:211-367).  The engine owns the device slab

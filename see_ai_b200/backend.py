@@ -34,7 +34,16 @@ EXPORTED_SYMBOLS = [
     "see_cuda_xent_forward_static", "see_cuda_static_max_rows", "see_cuda_static_last_error",
     "see_cuda_quantize_columns", "see_cuda_set_lora_fold", "see_cuda_set_product_groups", "see_cuda_set_adapter_fma", "see_cuda_set_split_gemm", "see_cuda_set_cta_pairs", "see_cuda_set_adapter_tensor_backward", "see_cuda_set_attention_one_walk",
     "see_cuda_set_attention_slices", "see_cuda_attention_slices",
+    "see_cuda_norm_forward", "see_cuda_norm_backward", "see_cuda_norm_backward_workspace", "see_cuda_adamw_step",
 ]
+
+# Element types, norms and activations of the operators below.
+F32, BF16, F16 = 0, 1, 2
+TYPES = {"f32": F32, "bf16": BF16, "f16": F16}
+NORM_LAYER, NORM_RMS = 0, 1
+ACT_RELU, ACT_GELU, ACT_SILU = 1, 2, 3
+ACTS = {"relu": ACT_RELU, "gelu": ACT_GELU, "silu": ACT_SILU}
+ADAMW_BLOCK, ADAMW_NO_DECAY = 256, 1
 
 
 class StepParams(ctypes.Structure):
@@ -53,6 +62,18 @@ class ProfileRecord(ctypes.Structure):
     _fields_ = [("opcode", ctypes.c_uint16), ("absorbed", ctypes.c_uint16), ("index", ctypes.c_uint32),
                 ("ms", ctypes.c_float), ("kernel_ms", ctypes.c_float), ("m", ctypes.c_uint64),
                 ("n", ctypes.c_uint64), ("k", ctypes.c_uint64)]
+
+
+class NormShape(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int32), ("x_type", ctypes.c_int32), ("y_type", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("rows", ctypes.c_uint64), ("cols", ctypes.c_uint64), ("x_stride", ctypes.c_uint64),
+                ("y_stride", ctypes.c_uint64)]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale", "copy")] + [
+        ("n", ctypes.c_uint64), ("g_type", ctypes.c_int32), ("copy_type", ctypes.c_int32), ("flags", ctypes.c_uint32),
+        ("pad", ctypes.c_uint32)]
 
 
 class BackendError(RuntimeError):
@@ -115,6 +136,11 @@ def load_library() -> ctypes.CDLL:
     lib.see_cuda_set_attention_slices.argtypes = [vp, i32]
     lib.see_cuda_attention_slices.argtypes = [vp]
     lib.see_cuda_attention_slices.restype = u64
+    lib.see_cuda_norm_forward.argtypes = [vp, ctypes.POINTER(NormShape)] + [vp] * 6
+    lib.see_cuda_norm_backward.argtypes = [vp, ctypes.POINTER(NormShape)] + [vp] * 10 + [u64]
+    lib.see_cuda_norm_backward_workspace.argtypes = [u64, u64]
+    lib.see_cuda_norm_backward_workspace.restype = u64
+    lib.see_cuda_adamw_step.argtypes = [vp, ctypes.POINTER(AdamWTensor), u64, i32, ctypes.POINTER(StepParams), vp]
     lib.see_cuda_xent_forward_static.argtypes = [vp, vp, vp, vp, u64, u64, i32, vp]
     lib.see_cuda_static_max_rows.restype = u64
     lib.see_cuda_static_last_error.restype = ctypes.c_char_p
@@ -133,6 +159,23 @@ def xent_forward_static(logits_ptr: int, labels_ptr: int, loss_ptr: int, probs_p
                                           rows, classes, int(masked), ctypes.c_void_p(stream))
     if rc != SEE_OK:
         raise BackendError(lib.see_cuda_static_last_error().decode())
+
+
+def norm_backward_workspace(rows: int, cols: int) -> int:
+    """Bytes that `CudaBackend.norm_backward` needs beside its operands."""
+    return int(load_library().see_cuda_norm_backward_workspace(rows, cols))
+
+
+def adamw_tensors(tensors):
+    """The table `CudaBackend.adamw_step` takes, of dicts of DEVICE pointers p, g, m, v (and m_scale, v_scale with 8-bit
+    moments; copy), the number of elements n, g_type, copy_type and no_decay."""
+    table = (AdamWTensor * len(tensors))()
+    for entry, t in zip(table, tensors):
+        for key in ("p", "g", "m", "v", "m_scale", "v_scale", "copy"):
+            setattr(entry, key, t.get(key) or None)
+        entry.n, entry.g_type, entry.copy_type = t["n"], t.get("g_type", F32), t.get("copy_type", F32)
+        entry.flags = ADAMW_NO_DECAY if t.get("no_decay") else 0
+    return table
 
 
 def program_bytes(program) -> bytes:
@@ -294,6 +337,27 @@ class CudaBackend:
         """Per-column int8 quantisation of W [K, N] over DEVICE pointers."""
         self._check(self.lib.see_cuda_quantize_columns(self.h, ctypes.c_void_p(w_ptr), K, N,
                                                        ctypes.c_void_p(levels_ptr), ctypes.c_void_p(scales_ptr)))
+
+    def norm_forward(self, kind: int, rows: int, cols: int, x: int, gamma: int, beta: int, y: int, mean: int, rstd: int,
+                     x_type: int = F32, y_type: int = F32, eps: float = 1e-5, x_stride: int = 0, y_stride: int = 0):
+        """Layer norm (NORM_LAYER) or root-mean-square norm (NORM_RMS: beta and mean are 0) over DEVICE pointers."""
+        shape = NormShape(kind, x_type, y_type, eps, rows, cols, x_stride, y_stride)
+        self._check(self.lib.see_cuda_norm_forward(self.h, shape, x or None, gamma or None, beta or None, y or None, mean or None,
+                                                   rstd or None))
+
+    def norm_backward(self, kind: int, rows: int, cols: int, dy: int, x: int, gamma: int, mean: int, rstd: int, dx: int,
+                      dgamma: int, dbeta: int, workspace: int, workspace_bytes: int, addend: int = 0, x_type: int = F32,
+                      y_type: int = F32, x_stride: int = 0, y_stride: int = 0):
+        """Its backward pass with the gradients of gamma and beta (NORM_RMS: mean and dbeta are 0); `addend` joins dx.
+        The workspace has norm_backward_workspace(rows, cols) bytes."""
+        shape = NormShape(kind, x_type, y_type, 0.0, rows, cols, x_stride, y_stride)
+        self._check(self.lib.see_cuda_norm_backward(self.h, shape, dy or None, x or None, gamma or None, mean or None, rstd or None,
+                                                    addend or None, dx or None, dgamma or None, dbeta or None, workspace or None,
+                                                    workspace_bytes))
+
+    def adamw_step(self, tensors, params: StepParams, state_bits: int = 32, grad_scale: int = 0):
+        """One AdamW step over a table of adamw_tensors, moments in 8 bits or in 32."""
+        self._check(self.lib.see_cuda_adamw_step(self.h, tensors, len(tensors), state_bits, params, grad_scale or None))
 
     def set_profiling(self, on: bool):
         self._check(self.lib.see_cuda_set_profiling(self.h, int(on)))

@@ -1,0 +1,250 @@
+// The checks of the operators that train a block's own weights, and their dispatch: what see_cuda.h promises to refuse is
+// refused here, before anything is enqueued.
+#include "block_ops.h"
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "cuda_backend.h"
+
+namespace see {
+namespace {
+
+// The handle's device for the calls of a scope; the caller's current device is left as it was.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    ok_ = cudaGetDevice(&before_) == cudaSuccess && (before_ == device || cudaSetDevice(device) == cudaSuccess);
+    moved_ = ok_ && before_ != device;
+  }
+  ~OnDevice() {
+    if (moved_) cudaSetDevice(before_);
+  }
+  bool ok() const { return ok_; }
+
+ private:
+  int before_ = 0;
+  bool ok_ = false, moved_ = false;
+};
+
+uint64_t SizeOf(int type) { return type == SEE_F32 ? 4 : 2; }
+bool IsType(int type) { return type == SEE_F32 || type == SEE_BF16 || type == SEE_F16; }
+
+// A matrix operand: `rows` runs of `width` bytes, `pitch` bytes apart.
+struct Operand {
+  const char* name;
+  const void* p;
+  uint64_t rows, width, pitch, align;
+  bool written;
+  uint64_t begin() const { return reinterpret_cast<uint64_t>(p); }
+  uint64_t end() const { return rows ? begin() + (rows - 1) * pitch + width : begin(); }
+};
+Operand Vector(const char* name, const void* p, uint64_t bytes, uint64_t align, bool written) {
+  return {name, p, bytes ? 1u : 0u, bytes, 0, align, written};
+}
+
+bool Overlap(const Operand& a, const Operand& b) {
+  if (a.rows == 0 || b.rows == 0 || a.end() <= b.begin() || b.end() <= a.begin()) return false;
+  if (a.rows > 1 && b.rows > 1 && a.pitch == b.pitch) {   // side by side in the rows of one buffer
+    const uint64_t shift = b.begin() >= a.begin() ? (b.begin() - a.begin()) % a.pitch : (a.pitch - (a.begin() - b.begin()) % a.pitch) % a.pitch;
+    if (shift >= a.width && shift + b.width <= a.pitch) return false;
+  }
+  return true;
+}
+
+Status CheckOperands(const std::string& what, const std::vector<Operand>& ops) {
+  for (const Operand& o : ops) {
+    if (!o.p) return std::unexpected(what + ": " + o.name + " is null");
+    if (o.begin() % o.align) return std::unexpected(what + ": " + o.name + " is not aligned");
+    uint64_t span;
+    if (__builtin_mul_overflow(o.rows, o.pitch, &span) || span + o.width > (1ull << 56) || o.begin() > (1ull << 56))
+      return std::unexpected(what + ": " + o.name + " is too large");
+  }
+  for (size_t i = 0; i < ops.size(); ++i)
+    for (size_t j = i + 1; j < ops.size(); ++j)
+      if ((ops[i].written || ops[j].written) && Overlap(ops[i], ops[j]))
+        return std::unexpected(what + ": " + ops[i].name + " and " + ops[j].name + " overlap");
+  return {};
+}
+
+// Shape checks common to both directions; fills the strides.
+Status CheckNorm(const std::string& what, see_norm_shape* s) {
+  if (s->kind != SEE_NORM_LAYER && s->kind != SEE_NORM_RMS) return std::unexpected(what + ": unknown kind");
+  if (!IsType(s->x_type) || !IsType(s->y_type) || (s->x_type != s->y_type && s->x_type != SEE_F32))
+    return std::unexpected(what + ": x_type and y_type are equal, or x_type is f32");
+  if (!(s->eps >= 0.0f) || !std::isfinite(s->eps)) return std::unexpected(what + ": eps is not a finite number from 0 on");
+  if (s->cols == 0 || s->cols > k::kNormMaxCols) return std::unexpected(what + ": 1 to 16384 columns");
+  if (s->rows > 0x7FFFFFFFull) return std::unexpected(what + ": more than 2^31 - 1 rows");
+  if (s->x_stride == 0) s->x_stride = s->cols;
+  if (s->y_stride == 0) s->y_stride = s->cols;
+  if (s->x_stride < s->cols || s->y_stride < s->cols || s->x_stride > (1ull << 40) || s->y_stride > (1ull << 40))
+    return std::unexpected(what + ": a stride is smaller than a row, or over 2^40");
+  return {};
+}
+
+k::NormArgs ArgsOf(const see_norm_shape& s) {
+  k::NormArgs a;
+  a.rows = s.rows;
+  a.cols = static_cast<uint32_t>(s.cols);
+  a.x_stride = s.x_stride;
+  a.y_stride = s.y_stride;
+  a.x_type = s.x_type;
+  a.y_type = s.y_type;
+  a.rms = s.kind == SEE_NORM_RMS;
+  a.eps = s.eps;
+  return a;
+}
+
+}  // namespace
+
+uint64_t NormBackwardWorkspace(uint64_t rows, uint64_t cols) {
+  if (cols == 0 || cols > k::kNormMaxCols) return 0;
+  return std::max<uint64_t>(16, k::NormPartialRows(rows) * cols * 2 * sizeof(float));
+}
+
+Status CudaBackend::NormForward(const see_norm_shape& given, const void* x, const float* gamma, const float* beta, void* y, float* mean,
+                                float* rstd) {
+  const std::string what = "cuda: norm forward";
+  see_norm_shape s = given;
+  if (auto r = CheckNorm(what, &s); !r) return r;
+  const bool layer = s.kind == SEE_NORM_LAYER;
+  if (!layer && (beta || mean)) return std::unexpected(what + ": rms has neither beta nor mean");
+  const uint64_t xs = SizeOf(s.x_type), ys = SizeOf(s.y_type);
+  std::vector<Operand> ops = {{"x", x, s.rows, s.cols * xs, s.x_stride * xs, xs, false},
+                              {"y", y, s.rows, s.cols * ys, s.y_stride * ys, ys, true},
+                              Vector("gamma", gamma, s.cols * 4, 4, false),
+                              Vector("rstd", rstd, s.rows * 4, 4, true)};
+  if (layer) {
+    ops.push_back(Vector("beta", beta, s.cols * 4, 4, false));
+    ops.push_back(Vector("mean", mean, s.rows * 4, 4, true));
+  }
+  if (auto r = CheckOperands(what, ops); !r) return r;
+  if (s.rows == 0) return {};
+  k::NormArgs a = ArgsOf(s);
+  a.x = x;
+  a.gamma = gamma;
+  a.beta = beta;
+  a.y = y;
+  a.mean = mean;
+  a.rstd = rstd;
+  OnDevice on(device_);
+  if (!on.ok()) return Check(cudaGetLastError(), "norm forward: device");
+  if (auto r = Check(k::NormForward(a, sms_, stream_), "norm forward"); !r) return r;
+  ++counters_.kernel_launches;
+  return {};
+}
+
+Status CudaBackend::NormBackward(const see_norm_shape& given, const void* dy, const void* x, const float* gamma, const float* mean,
+                                 const float* rstd, const void* addend, void* dx, float* dgamma, float* dbeta, void* workspace,
+                                 uint64_t workspace_bytes) {
+  const std::string what = "cuda: norm backward";
+  see_norm_shape s = given;
+  if (auto r = CheckNorm(what, &s); !r) return r;
+  const bool layer = s.kind == SEE_NORM_LAYER;
+  if (!layer && (dbeta || mean)) return std::unexpected(what + ": rms has neither mean nor dbeta");
+  if (workspace_bytes < NormBackwardWorkspace(s.rows, s.cols)) return std::unexpected(what + ": the workspace is too small");
+  const uint64_t xs = SizeOf(s.x_type), ys = SizeOf(s.y_type);
+  std::vector<Operand> ops = {{"dy", dy, s.rows, s.cols * ys, s.y_stride * ys, ys, false},
+                              {"x", x, s.rows, s.cols * xs, s.x_stride * xs, xs, false},
+                              {"dx", dx, s.rows, s.cols * xs, s.x_stride * xs, xs, true},
+                              Vector("gamma", gamma, s.cols * 4, 4, false),
+                              Vector("rstd", rstd, s.rows * 4, 4, false),
+                              Vector("dgamma", dgamma, s.cols * 4, 4, true),
+                              Vector("workspace", workspace, workspace_bytes, 16, true)};
+  if (addend) ops.push_back({"addend", addend, s.rows, s.cols * xs, s.x_stride * xs, xs, false});
+  if (layer) {
+    ops.push_back(Vector("mean", mean, s.rows * 4, 4, false));
+    ops.push_back(Vector("dbeta", dbeta, s.cols * 4, 4, true));
+  }
+  if (auto r = CheckOperands(what, ops); !r) return r;
+  OnDevice on(device_);
+  if (!on.ok()) return Check(cudaGetLastError(), "norm backward: device");
+  if (s.rows == 0) {
+    if (auto r = Check(cudaMemsetAsync(dgamma, 0, s.cols * 4, stream_), "norm backward"); !r) return r;
+    return layer ? Check(cudaMemsetAsync(dbeta, 0, s.cols * 4, stream_), "norm backward") : Status{};
+  }
+  k::NormArgs a = ArgsOf(s);
+  a.x = x;
+  a.dy = dy;
+  a.addend = addend;
+  a.gamma = gamma;
+  a.mean = const_cast<float*>(mean);
+  a.rstd = const_cast<float*>(rstd);
+  a.dx = dx;
+  a.dgamma = dgamma;
+  a.dbeta = dbeta;
+  a.partials = static_cast<float*>(workspace);
+  int launches = 0;
+  const cudaError_t e = k::NormBackward(a, sms_, stream_, &launches);
+  counters_.kernel_launches += static_cast<uint64_t>(launches);
+  return Check(e, "norm backward");
+}
+
+Status CudaBackend::AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params,
+                                 const float* grad_scale) {
+  const std::string what = "cuda: adamw";
+  if (state_bits != 8 && state_bits != 32) return std::unexpected(what + ": moments have 8 or 32 bits");
+  if (params.step == 0) return std::unexpected(what + ": steps count from 1");
+  if (!(params.beta1 >= 0.0f && params.beta1 < 1.0f && params.beta2 >= 0.0f && params.beta2 < 1.0f))
+    return std::unexpected(what + ": beta1 and beta2 are from 0 on and below 1");
+  if (count && !tensors) return std::unexpected(what + ": tensors is null");
+  if (reinterpret_cast<uint64_t>(grad_scale) % 4) return std::unexpected(what + ": grad_scale is not aligned");
+  struct Span { uint64_t begin, end; bool written; };
+  std::vector<Span> spans;
+  spans.reserve(count * 7 + 1);
+  for (uint64_t i = 0; i < count; ++i) {
+    const see_adamw_tensor& t = tensors[i];
+    const std::string name = what + ": tensor " + std::to_string(i);
+    if (!IsType(t.g_type) || !IsType(t.copy_type)) return std::unexpected(name + ": unknown type");
+    if (t.flags & ~static_cast<uint32_t>(SEE_ADAMW_NO_DECAY)) return std::unexpected(name + ": unknown flag");
+    if ((t.copy_type == SEE_F32) != (t.copy == nullptr)) return std::unexpected(name + ": a copy has 16 bits, and none is null with type f32");
+    if (t.n == 0) continue;
+    if (t.n > (1ull << 42)) return std::unexpected(name + ": more than 2^42 elements");
+    const uint64_t blocks = (t.n + k::kAdamBlock - 1) / k::kAdamBlock, state = state_bits / 8;
+    const struct { const char* name; const void* p; uint64_t bytes, align; bool written; } ops[] = {
+        {"p", t.p, t.n * 4, 4, true},
+        {"g", t.g, t.n * SizeOf(t.g_type), SizeOf(t.g_type), false},
+        {"m", t.m, t.n * state, state, true},
+        {"v", t.v, t.n * state, state, true},
+        {"m_scale", t.m_scale, state == 1 ? blocks * 4 : 0, 4, true},
+        {"v_scale", t.v_scale, state == 1 ? blocks * 4 : 0, 4, true},
+        {"copy", t.copy, t.copy ? t.n * 2 : 0, 2, true}};
+    for (const auto& o : ops) {
+      if (o.bytes == 0) continue;
+      const uint64_t at = reinterpret_cast<uint64_t>(o.p);
+      if (!at) return std::unexpected(name + ": " + o.name + " is null");
+      if (at % o.align) return std::unexpected(name + ": " + o.name + " is not aligned");
+      spans.push_back({at, at + o.bytes, o.written});
+    }
+  }
+  if (grad_scale) spans.push_back({reinterpret_cast<uint64_t>(grad_scale), reinterpret_cast<uint64_t>(grad_scale) + 4, false});
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  uint64_t any = 0, written = 0;   // how far the spans so far reach
+  for (const Span& s : spans) {
+    if (s.begin < written || (s.written && s.begin < any)) return std::unexpected(what + ": operands overlap");
+    any = std::max(any, s.end);
+    if (s.written) written = std::max(written, s.end);
+  }
+  const k::AdamScalars sc = ScalarsOf(params);
+  k::AdamStepScalars a;
+  a.lr = sc.lr;
+  a.beta1 = sc.beta1;
+  a.beta2 = sc.beta2;
+  a.om_beta1 = 1.0f - sc.beta1;
+  a.om_beta2 = 1.0f - sc.beta2;
+  a.eps = sc.eps;
+  a.weight_decay = sc.weight_decay;
+  a.inv_bc1 = sc.inv_bc1;
+  a.inv_bc2 = sc.inv_bc2;
+  a.root_inv_bc2 = std::sqrt(sc.inv_bc2);
+  a.phase = static_cast<uint32_t>(params.step) * 0x6A09E667u;   // 2^32 (sqrt(2) - 1)
+  OnDevice on(device_);
+  if (!on.ok()) return Check(cudaGetLastError(), "adamw: device");
+  int launches = 0;
+  const cudaError_t e = k::AdamWTensors(tensors, count, state_bits, a, grad_scale, sms_, stream_, &launches);
+  counters_.kernel_launches += static_cast<uint64_t>(launches);
+  return Check(e, "adamw");
+}
+
+}  // namespace see

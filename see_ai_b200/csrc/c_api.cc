@@ -7,6 +7,7 @@
 #include <span>
 #include <string>
 
+#include "block_ops.h"
 #include "cuda_backend.h"
 #include "engine.h"
 #include "lora_umma.h"
@@ -51,6 +52,22 @@ int Fail(see_cuda_backend* h, const std::string& msg) {
 int Fail(see_engine* h, const std::string& msg) {
   h->error = msg;
   return CodeOf(msg);
+}
+// A call of an operator: nothing thrown leaves it (the host tables that it builds can run out of memory).
+template <typename F>
+int Guarded(see_cuda_backend* h, const char* what, const void* shape, F call) {
+  if (!h) return SEE_ERROR;
+  try {
+    if (!shape) return Fail(h, std::string("cuda: ") + what + ": null description");
+    const see::Status r = call();
+    return r ? SEE_OK : Fail(h, r.error());
+  } catch (const std::exception& e) {
+    try {
+      return Fail(h, std::string("cuda: ") + what + ": " + e.what());
+    } catch (...) {
+      return SEE_ERROR;
+    }
+  }
 }
 int Done(see_engine* h, const see::Status& r) { return r ? SEE_OK : Fail(h, r.error()); }
 
@@ -162,6 +179,28 @@ int see_cuda_quantize_columns(see_cuda_backend* h, const float* w, uint64_t K, u
                               int8_t* levels, float* scales) {
   auto r = h->backend->QuantizeColumns(w, K, N, levels, scales);
   return r ? SEE_OK : Fail(h, r.error());
+}
+
+uint64_t see_cuda_norm_backward_workspace(uint64_t rows, uint64_t cols) {
+  return see::NormBackwardWorkspace(rows, cols);
+}
+
+int see_cuda_norm_forward(see_cuda_backend* h, const see_norm_shape* shape, const void* x, const float* gamma,
+                          const float* beta, void* y, float* mean, float* rstd) {
+  return Guarded(h, "norm forward", shape, [&] { return h->backend->NormForward(*shape, x, gamma, beta, y, mean, rstd); });
+}
+
+int see_cuda_norm_backward(see_cuda_backend* h, const see_norm_shape* shape, const void* dy, const void* x,
+                           const float* gamma, const float* mean, const float* rstd, const void* addend, void* dx,
+                           float* dgamma, float* dbeta, void* workspace, uint64_t workspace_bytes) {
+  return Guarded(h, "norm backward", shape, [&] {
+    return h->backend->NormBackward(*shape, dy, x, gamma, mean, rstd, addend, dx, dgamma, dbeta, workspace, workspace_bytes);
+  });
+}
+
+int see_cuda_adamw_step(see_cuda_backend* h, const see_adamw_tensor* tensors, uint64_t count, int state_bits,
+                        const see_step_params* params, const float* grad_scale) {
+  return Guarded(h, "adamw", params, [&] { return h->backend->AdamWTensors(tensors, count, state_bits, ToParams(params), grad_scale); });
 }
 
 int see_cuda_flush(see_cuda_backend* h) {

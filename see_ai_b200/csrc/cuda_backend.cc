@@ -65,6 +65,7 @@ Status CudaBackend::Init() {
   cudaDeviceProp prop{};
   if (auto r = Check(cudaGetDeviceProperties(&prop, device_), "cudaGetDeviceProperties"); !r)
     return r;
+  sms_ = static_cast<uint32_t>(prop.multiProcessorCount);
   if (prop.major != 10)
     return std::unexpected(std::string("cuda: device '") + prop.name +
                            "' is not compute capability 10.x; the kernels are built for sm_100a only");
@@ -73,7 +74,7 @@ Status CudaBackend::Init() {
                   " SMs), relaxed GEMMs on tcgen05 bf16 tensor cores";
   if (auto r = Check(cudaStreamCreateWithFlags(&stream_, cudaStreamNonBlocking), "stream"); !r)
     return r;
-  own_stream_ = true;
+  own_stream_ = stream_;
   void* p = nullptr;
   const size_t scratch_bytes = 4096 + 256 * sizeof(double);
   if (auto r = Check(cudaMalloc(&p, scratch_bytes), "scratch"); !r) return r;
@@ -112,7 +113,7 @@ CudaBackend::~CudaBackend() {
   cudaFree(d_lora_partials_);
   if (h_published_) cudaFreeHost(h_published_);
   if (h_flush_) cudaFreeHost(h_flush_);
-  if (own_stream_ && stream_) cudaStreamDestroy(stream_);
+  if (own_stream_) cudaStreamDestroy(own_stream_);
 }
 
 // False: no pinned memory to be had (downloads then go range by range).

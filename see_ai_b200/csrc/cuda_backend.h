@@ -31,6 +31,7 @@
 #include <utility>
 #include <vector>
 
+#include "../../include/see_cuda.h"
 #include "extents.h"
 #include "kernels.h"
 #include "plan_abi.h"
@@ -185,6 +186,12 @@ class CudaBackend {
   // arithmetic bit for bit (reference: compiler/backend/allocation/arena_binder.cc:129-190).
   Status QuantizeColumns(const float* w, uint64_t K, uint64_t N, int8_t* levels, float* scales);
 
+  // The operators that train a block's own weights (see_cuda.h says what each takes and refuses; block_ops.cc).
+  Status NormForward(const see_norm_shape& shape, const void* x, const float* gamma, const float* beta, void* y, float* mean, float* rstd);
+  Status NormBackward(const see_norm_shape& shape, const void* dy, const void* x, const float* gamma, const float* mean, const float* rstd,
+                      const void* addend, void* dx, float* dgamma, float* dbeta, void* workspace, uint64_t workspace_bytes);
+  Status AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale);
+
   // Merge deltas launched as a run add their non-finite results to *tally (device memory) from now on; null: they do
   // not.  merge_counted(): how many deltas have been counted that way since the last call of this.
   void SetMergeTally(unsigned long long* tally) { merge_tally_ = tally; merge_counted_ = 0; }
@@ -218,9 +225,10 @@ class CudaBackend {
   T* Wr(uint64_t ref) const { return reinterpret_cast<T*>(d_arena_ + RefOffset(ref)); }
 
   int device_ = 0;
+  uint32_t sms_ = 0;
   std::string device_label_;
   cudaStream_t stream_ = nullptr;
-  bool own_stream_ = false;
+  cudaStream_t own_stream_ = nullptr;   // made by Init; stream_ may be the caller's
 
   uint8_t* host_arena_ = nullptr;
   uint64_t arena_bytes_ = 0;
