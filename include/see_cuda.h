@@ -225,6 +225,27 @@ int see_cuda_norm_backward(see_cuda_backend* h, const see_norm_shape* shape, con
                            const float* gamma, const float* mean, const float* rstd, const void* addend, void* dx,
                            float* dgamma, float* dbeta, void* workspace, uint64_t workspace_bytes);
 
+/* The gated feed-forward block up to its down projection: hidden = act(gate) * up with gate = x w_gate and up = x w_up.
+ * x [rows, d_in], w_gate, w_up [d_in, d_hidden], hidden, gate, up [rows, d_hidden]: all of one 16-bit type, products and
+ * activation in f32 and one rounding at the end.  gate and up are kept for the backward pass, or both NULL.  d_in and
+ * d_hidden: multiples of 8 up to 2^20; rows up to 2^31 - 256; addresses 16-byte aligned.  Strides: elements from a row to
+ * the next, multiples of 8 (0: d_in, d_hidden): x_stride of x and dx, hidden_stride of hidden, dhidden, gate and up. */
+typedef struct see_gated_shape {
+  int32_t type, act;
+  uint64_t rows, d_in, d_hidden, x_stride, hidden_stride;
+} see_gated_shape;
+int see_cuda_gated_forward(see_cuda_backend* h, const see_gated_shape* shape, const void* x, const void* w_gate,
+                           const void* w_up, void* hidden, void* gate, void* up);
+/* From dhidden and what the forward pass kept: dgate = dhidden up act'(gate) and dup = dhidden act(gate), rounded to the
+ * type as the products' operands (in f16 a gradient beyond 65504 overflows: scale the loss), then
+ * dx = dgate w_gate^T + dup w_up^T, dw_gate = x^T dgate, dw_up = x^T dup, sums in f32 and in an order that the sizes alone
+ * fix (zero rows: zeros).  dx, or dw_gate and dw_up together, may be NULL: not wanted.  workspace: at least
+ * see_cuda_gated_backward_workspace(rows, d_in, d_hidden) bytes, 128-byte aligned. */
+uint64_t see_cuda_gated_backward_workspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden);
+int see_cuda_gated_backward(see_cuda_backend* h, const see_gated_shape* shape, const void* dhidden, const void* x,
+                            const void* w_gate, const void* w_up, const void* gate, const void* up, void* dx,
+                            void* dw_gate, void* dw_up, void* workspace, uint64_t workspace_bytes);
+
 /* One AdamW step over `count` tensors of n elements each, in the kAdamWStep instruction's expression.  p: f32 weights.
  * g: their gradients.  copy: the new weights in 16 bits (copy_type SEE_BF16 or SEE_F16), or NULL with copy_type SEE_F32.
  * state_bits 32: m, v f32 moments.  state_bits 8: m and v are e4m3 (one byte an element), v holding the ROOT of the second

@@ -35,6 +35,7 @@ EXPORTED_SYMBOLS = [
     "see_cuda_quantize_columns", "see_cuda_set_lora_fold", "see_cuda_set_product_groups", "see_cuda_set_adapter_fma", "see_cuda_set_split_gemm", "see_cuda_set_cta_pairs", "see_cuda_set_adapter_tensor_backward", "see_cuda_set_attention_one_walk",
     "see_cuda_set_attention_slices", "see_cuda_attention_slices",
     "see_cuda_norm_forward", "see_cuda_norm_backward", "see_cuda_norm_backward_workspace", "see_cuda_adamw_step",
+    "see_cuda_gated_forward", "see_cuda_gated_backward", "see_cuda_gated_backward_workspace",
 ]
 
 # Element types, norms and activations of the operators below.
@@ -68,6 +69,11 @@ class NormShape(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int32), ("x_type", ctypes.c_int32), ("y_type", ctypes.c_int32), ("eps", ctypes.c_float),
                 ("rows", ctypes.c_uint64), ("cols", ctypes.c_uint64), ("x_stride", ctypes.c_uint64),
                 ("y_stride", ctypes.c_uint64)]
+
+
+class GatedShape(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("act", ctypes.c_int32)] + [
+        (n, ctypes.c_uint64) for n in ("rows", "d_in", "d_hidden", "x_stride", "hidden_stride")]
 
 
 class AdamWTensor(ctypes.Structure):
@@ -140,6 +146,10 @@ def load_library() -> ctypes.CDLL:
     lib.see_cuda_norm_backward.argtypes = [vp, ctypes.POINTER(NormShape)] + [vp] * 10 + [u64]
     lib.see_cuda_norm_backward_workspace.argtypes = [u64, u64]
     lib.see_cuda_norm_backward_workspace.restype = u64
+    lib.see_cuda_gated_forward.argtypes = [vp, ctypes.POINTER(GatedShape)] + [vp] * 6
+    lib.see_cuda_gated_backward.argtypes = [vp, ctypes.POINTER(GatedShape)] + [vp] * 10 + [u64]
+    lib.see_cuda_gated_backward_workspace.argtypes = [u64, u64, u64]
+    lib.see_cuda_gated_backward_workspace.restype = u64
     lib.see_cuda_adamw_step.argtypes = [vp, ctypes.POINTER(AdamWTensor), u64, i32, ctypes.POINTER(StepParams), vp]
     lib.see_cuda_xent_forward_static.argtypes = [vp, vp, vp, vp, u64, u64, i32, vp]
     lib.see_cuda_static_max_rows.restype = u64
@@ -164,6 +174,11 @@ def xent_forward_static(logits_ptr: int, labels_ptr: int, loss_ptr: int, probs_p
 def norm_backward_workspace(rows: int, cols: int) -> int:
     """Bytes that `CudaBackend.norm_backward` needs beside its operands."""
     return int(load_library().see_cuda_norm_backward_workspace(rows, cols))
+
+
+def gated_backward_workspace(rows: int, d_in: int, d_hidden: int) -> int:
+    """Bytes that `CudaBackend.gated_backward` needs beside its operands."""
+    return int(load_library().see_cuda_gated_backward_workspace(rows, d_in, d_hidden))
 
 
 def adamw_tensors(tensors):
@@ -354,6 +369,24 @@ class CudaBackend:
         self._check(self.lib.see_cuda_norm_backward(self.h, shape, dy or None, x or None, gamma or None, mean or None, rstd or None,
                                                     addend or None, dx or None, dgamma or None, dbeta or None, workspace or None,
                                                     workspace_bytes))
+
+    def gated_forward(self, rows: int, d_in: int, d_hidden: int, x: int, w_gate: int, w_up: int, hidden: int, gate: int = 0,
+                      up: int = 0, type: int = BF16, act: int = ACT_SILU, x_stride: int = 0, hidden_stride: int = 0):
+        """hidden = act(x w_gate) * (x w_up) over DEVICE pointers of a 16-bit type; gate and up are the two products, kept for
+        the backward pass (0: not kept)."""
+        shape = GatedShape(type, act, rows, d_in, d_hidden, x_stride, hidden_stride)
+        self._check(self.lib.see_cuda_gated_forward(self.h, shape, x or None, w_gate or None, w_up or None, hidden or None,
+                                                    gate or None, up or None))
+
+    def gated_backward(self, rows: int, d_in: int, d_hidden: int, dhidden: int, x: int, w_gate: int, w_up: int, gate: int, up: int,
+                       dx: int, dw_gate: int, dw_up: int, workspace: int, workspace_bytes: int, type: int = BF16,
+                       act: int = ACT_SILU, x_stride: int = 0, hidden_stride: int = 0):
+        """Its backward pass; dx, or dw_gate and dw_up, may be 0 (not wanted).  The workspace has
+        gated_backward_workspace(rows, d_in, d_hidden) bytes."""
+        shape = GatedShape(type, act, rows, d_in, d_hidden, x_stride, hidden_stride)
+        self._check(self.lib.see_cuda_gated_backward(self.h, shape, dhidden or None, x or None, w_gate or None, w_up or None,
+                                                     gate or None, up or None, dx or None, dw_gate or None, dw_up or None,
+                                                     workspace or None, workspace_bytes))
 
     def adamw_step(self, tensors, params: StepParams, state_bits: int = 32, grad_scale: int = 0):
         """One AdamW step over a table of adamw_tensors, moments in 8 bits or in 32."""

@@ -44,8 +44,9 @@ CU_SOURCES = {
     "k_lora_umma.cu": [],
     "k_block_norm.cu": [],
     "k_adamw.cu": ["-fmad=false"],
+    "k_gated_umma.cu": [],
 }
-CC_SOURCES = ["extents.cc", "cuda_backend.cc", "c_api.cc", "umma_gemm.cc", "engine.cc", "exchange.cc", "block_ops.cc"]
+CC_SOURCES = ["extents.cc", "cuda_backend.cc", "c_api.cc", "umma_gemm.cc", "engine.cc", "exchange.cc", "block_ops.cc", "gated.cc"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O3", "-lineinfo",
               "--expt-extended-lambda", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",

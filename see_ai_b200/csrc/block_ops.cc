@@ -6,67 +6,11 @@
 #include <cmath>
 #include <vector>
 
+#include "block_checks.h"
 #include "cuda_backend.h"
 
 namespace see {
 namespace {
-
-// The handle's device for the calls of a scope; the caller's current device is left as it was.
-class OnDevice {
- public:
-  explicit OnDevice(int device) {
-    ok_ = cudaGetDevice(&before_) == cudaSuccess && (before_ == device || cudaSetDevice(device) == cudaSuccess);
-    moved_ = ok_ && before_ != device;
-  }
-  ~OnDevice() {
-    if (moved_) cudaSetDevice(before_);
-  }
-  bool ok() const { return ok_; }
-
- private:
-  int before_ = 0;
-  bool ok_ = false, moved_ = false;
-};
-
-uint64_t SizeOf(int type) { return type == SEE_F32 ? 4 : 2; }
-bool IsType(int type) { return type == SEE_F32 || type == SEE_BF16 || type == SEE_F16; }
-
-// A matrix operand: `rows` runs of `width` bytes, `pitch` bytes apart.
-struct Operand {
-  const char* name;
-  const void* p;
-  uint64_t rows, width, pitch, align;
-  bool written;
-  uint64_t begin() const { return reinterpret_cast<uint64_t>(p); }
-  uint64_t end() const { return rows ? begin() + (rows - 1) * pitch + width : begin(); }
-};
-Operand Vector(const char* name, const void* p, uint64_t bytes, uint64_t align, bool written) {
-  return {name, p, bytes ? 1u : 0u, bytes, 0, align, written};
-}
-
-bool Overlap(const Operand& a, const Operand& b) {
-  if (a.rows == 0 || b.rows == 0 || a.end() <= b.begin() || b.end() <= a.begin()) return false;
-  if (a.rows > 1 && b.rows > 1 && a.pitch == b.pitch) {   // side by side in the rows of one buffer
-    const uint64_t shift = b.begin() >= a.begin() ? (b.begin() - a.begin()) % a.pitch : (a.pitch - (a.begin() - b.begin()) % a.pitch) % a.pitch;
-    if (shift >= a.width && shift + b.width <= a.pitch) return false;
-  }
-  return true;
-}
-
-Status CheckOperands(const std::string& what, const std::vector<Operand>& ops) {
-  for (const Operand& o : ops) {
-    if (!o.p) return std::unexpected(what + ": " + o.name + " is null");
-    if (o.begin() % o.align) return std::unexpected(what + ": " + o.name + " is not aligned");
-    uint64_t span;
-    if (__builtin_mul_overflow(o.rows, o.pitch, &span) || span + o.width > (1ull << 56) || o.begin() > (1ull << 56))
-      return std::unexpected(what + ": " + o.name + " is too large");
-  }
-  for (size_t i = 0; i < ops.size(); ++i)
-    for (size_t j = i + 1; j < ops.size(); ++j)
-      if ((ops[i].written || ops[j].written) && Overlap(ops[i], ops[j]))
-        return std::unexpected(what + ": " + ops[i].name + " and " + ops[j].name + " overlap");
-  return {};
-}
 
 // Shape checks common to both directions; fills the strides.
 Status CheckNorm(const std::string& what, see_norm_shape* s) {
@@ -103,14 +47,14 @@ uint64_t NormBackwardWorkspace(uint64_t rows, uint64_t cols) {
   return std::max<uint64_t>(16, k::NormPartialRows(rows) * cols * 2 * sizeof(float));
 }
 
-Status CudaBackend::NormForward(const see_norm_shape& given, const void* x, const float* gamma, const float* beta, void* y, float* mean,
-                                float* rstd) {
+Status CheckNormForward(see_norm_shape* shape, const void* x, const float* gamma, const float* beta, const void* y, const float* mean,
+                        const float* rstd) {
   const std::string what = "cuda: norm forward";
-  see_norm_shape s = given;
-  if (auto r = CheckNorm(what, &s); !r) return r;
+  if (auto r = CheckNorm(what, shape); !r) return r;
+  const see_norm_shape& s = *shape;
   const bool layer = s.kind == SEE_NORM_LAYER;
   if (!layer && (beta || mean)) return std::unexpected(what + ": rms has neither beta nor mean");
-  const uint64_t xs = SizeOf(s.x_type), ys = SizeOf(s.y_type);
+  const uint64_t xs = SizeOfType(s.x_type), ys = SizeOfType(s.y_type);
   std::vector<Operand> ops = {{"x", x, s.rows, s.cols * xs, s.x_stride * xs, xs, false},
                               {"y", y, s.rows, s.cols * ys, s.y_stride * ys, ys, true},
                               Vector("gamma", gamma, s.cols * 4, 4, false),
@@ -119,7 +63,13 @@ Status CudaBackend::NormForward(const see_norm_shape& given, const void* x, cons
     ops.push_back(Vector("beta", beta, s.cols * 4, 4, false));
     ops.push_back(Vector("mean", mean, s.rows * 4, 4, true));
   }
-  if (auto r = CheckOperands(what, ops); !r) return r;
+  return CheckOperands(what, ops);
+}
+
+Status CudaBackend::NormForward(const see_norm_shape& given, const void* x, const float* gamma, const float* beta, void* y, float* mean,
+                                float* rstd) {
+  see_norm_shape s = given;
+  if (auto r = CheckNormForward(&s, x, gamma, beta, y, mean, rstd); !r) return r;
   if (s.rows == 0) return {};
   k::NormArgs a = ArgsOf(s);
   a.x = x;
@@ -135,16 +85,16 @@ Status CudaBackend::NormForward(const see_norm_shape& given, const void* x, cons
   return {};
 }
 
-Status CudaBackend::NormBackward(const see_norm_shape& given, const void* dy, const void* x, const float* gamma, const float* mean,
-                                 const float* rstd, const void* addend, void* dx, float* dgamma, float* dbeta, void* workspace,
-                                 uint64_t workspace_bytes) {
+Status CheckNormBackward(see_norm_shape* shape, const void* dy, const void* x, const float* gamma, const float* mean, const float* rstd,
+                         const void* addend, const void* dx, const float* dgamma, const float* dbeta, const void* workspace,
+                         uint64_t workspace_bytes) {
   const std::string what = "cuda: norm backward";
-  see_norm_shape s = given;
-  if (auto r = CheckNorm(what, &s); !r) return r;
+  if (auto r = CheckNorm(what, shape); !r) return r;
+  const see_norm_shape& s = *shape;
   const bool layer = s.kind == SEE_NORM_LAYER;
   if (!layer && (dbeta || mean)) return std::unexpected(what + ": rms has neither mean nor dbeta");
   if (workspace_bytes < NormBackwardWorkspace(s.rows, s.cols)) return std::unexpected(what + ": the workspace is too small");
-  const uint64_t xs = SizeOf(s.x_type), ys = SizeOf(s.y_type);
+  const uint64_t xs = SizeOfType(s.x_type), ys = SizeOfType(s.y_type);
   std::vector<Operand> ops = {{"dy", dy, s.rows, s.cols * ys, s.y_stride * ys, ys, false},
                               {"x", x, s.rows, s.cols * xs, s.x_stride * xs, xs, false},
                               {"dx", dx, s.rows, s.cols * xs, s.x_stride * xs, xs, true},
@@ -157,7 +107,15 @@ Status CudaBackend::NormBackward(const see_norm_shape& given, const void* dy, co
     ops.push_back(Vector("mean", mean, s.rows * 4, 4, false));
     ops.push_back(Vector("dbeta", dbeta, s.cols * 4, 4, true));
   }
-  if (auto r = CheckOperands(what, ops); !r) return r;
+  return CheckOperands(what, ops);
+}
+
+Status CudaBackend::NormBackward(const see_norm_shape& given, const void* dy, const void* x, const float* gamma, const float* mean,
+                                 const float* rstd, const void* addend, void* dx, float* dgamma, float* dbeta, void* workspace,
+                                 uint64_t workspace_bytes) {
+  see_norm_shape s = given;
+  if (auto r = CheckNormBackward(&s, dy, x, gamma, mean, rstd, addend, dx, dgamma, dbeta, workspace, workspace_bytes); !r) return r;
+  const bool layer = s.kind == SEE_NORM_LAYER;
   OnDevice on(device_);
   if (!on.ok()) return Check(cudaGetLastError(), "norm backward: device");
   if (s.rows == 0) {
@@ -181,8 +139,7 @@ Status CudaBackend::NormBackward(const see_norm_shape& given, const void* dy, co
   return Check(e, "norm backward");
 }
 
-Status CudaBackend::AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params,
-                                 const float* grad_scale) {
+Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale) {
   const std::string what = "cuda: adamw";
   if (state_bits != 8 && state_bits != 32) return std::unexpected(what + ": moments have 8 or 32 bits");
   if (params.step == 0) return std::unexpected(what + ": steps count from 1");
@@ -204,7 +161,7 @@ Status CudaBackend::AdamWTensors(const see_adamw_tensor* tensors, uint64_t count
     const uint64_t blocks = (t.n + k::kAdamBlock - 1) / k::kAdamBlock, state = state_bits / 8;
     const struct { const char* name; const void* p; uint64_t bytes, align; bool written; } ops[] = {
         {"p", t.p, t.n * 4, 4, true},
-        {"g", t.g, t.n * SizeOf(t.g_type), SizeOf(t.g_type), false},
+        {"g", t.g, t.n * SizeOfType(t.g_type), SizeOfType(t.g_type), false},
         {"m", t.m, t.n * state, state, true},
         {"v", t.v, t.n * state, state, true},
         {"m_scale", t.m_scale, state == 1 ? blocks * 4 : 0, 4, true},
@@ -226,6 +183,12 @@ Status CudaBackend::AdamWTensors(const see_adamw_tensor* tensors, uint64_t count
     any = std::max(any, s.end);
     if (s.written) written = std::max(written, s.end);
   }
+  return {};
+}
+
+Status CudaBackend::AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params,
+                                 const float* grad_scale) {
+  if (auto r = CheckAdamW(tensors, count, state_bits, params, grad_scale); !r) return r;
   const k::AdamScalars sc = ScalarsOf(params);
   k::AdamStepScalars a;
   a.lr = sc.lr;

@@ -12,11 +12,6 @@
 #include "../../include/see_cuda.h"
 #include "kernels.h"
 
-namespace see {
-// Bytes for any shape of these sizes, whatever its types and alignment (0: sizes outside the range).
-uint64_t NormBackwardWorkspace(uint64_t rows, uint64_t cols);
-}  // namespace see
-
 namespace see::k {
 
 // ---- norm (k_block_norm.cu) ------------------------------------------------

@@ -7,7 +7,7 @@
 #include <span>
 #include <string>
 
-#include "block_ops.h"
+#include "block_checks.h"
 #include "cuda_backend.h"
 #include "engine.h"
 #include "lora_umma.h"
@@ -195,6 +195,23 @@ int see_cuda_norm_backward(see_cuda_backend* h, const see_norm_shape* shape, con
                            float* dgamma, float* dbeta, void* workspace, uint64_t workspace_bytes) {
   return Guarded(h, "norm backward", shape, [&] {
     return h->backend->NormBackward(*shape, dy, x, gamma, mean, rstd, addend, dx, dgamma, dbeta, workspace, workspace_bytes);
+  });
+}
+
+uint64_t see_cuda_gated_backward_workspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden) {
+  return see::GatedBackwardWorkspace(rows, d_in, d_hidden);
+}
+
+int see_cuda_gated_forward(see_cuda_backend* h, const see_gated_shape* shape, const void* x, const void* w_gate,
+                           const void* w_up, void* hidden, void* gate, void* up) {
+  return Guarded(h, "gated forward", shape, [&] { return h->backend->GatedForward(*shape, x, w_gate, w_up, hidden, gate, up); });
+}
+
+int see_cuda_gated_backward(see_cuda_backend* h, const see_gated_shape* shape, const void* dhidden, const void* x,
+                            const void* w_gate, const void* w_up, const void* gate, const void* up, void* dx,
+                            void* dw_gate, void* dw_up, void* workspace, uint64_t workspace_bytes) {
+  return Guarded(h, "gated backward", shape, [&] {
+    return h->backend->GatedBackward(*shape, dhidden, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, workspace, workspace_bytes);
   });
 }
 

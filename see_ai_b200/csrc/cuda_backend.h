@@ -190,6 +190,9 @@ class CudaBackend {
   Status NormForward(const see_norm_shape& shape, const void* x, const float* gamma, const float* beta, void* y, float* mean, float* rstd);
   Status NormBackward(const see_norm_shape& shape, const void* dy, const void* x, const float* gamma, const float* mean, const float* rstd,
                       const void* addend, void* dx, float* dgamma, float* dbeta, void* workspace, uint64_t workspace_bytes);
+  Status GatedForward(const see_gated_shape& shape, const void* x, const void* w_gate, const void* w_up, void* hidden, void* gate, void* up);
+  Status GatedBackward(const see_gated_shape& shape, const void* dhidden, const void* x, const void* w_gate, const void* w_up,
+                       const void* gate, const void* up, void* dx, void* dw_gate, void* dw_up, void* workspace, uint64_t workspace_bytes);
   Status AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale);
 
   // Merge deltas launched as a run add their non-finite results to *tally (device memory) from now on; null: they do

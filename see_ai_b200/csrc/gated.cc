@@ -1,0 +1,206 @@
+// Host side of the gated feed-forward block: what a call refuses, the tensor maps of its operands, and the choice of tiles.
+#include <algorithm>
+#include <atomic>
+
+#include "block_checks.h"
+#include "cuda_backend.h"
+#include "gated_umma.h"
+
+namespace see {
+namespace {
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                              CUtensorMapFloatOOBfill);
+
+EncodeFn Encoder() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found{};
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found);
+    return e == cudaSuccess && found == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeFn>(p) : nullptr;
+  }();
+  return fn;
+}
+
+// A row-major 16-bit matrix in boxes of box_rows x 64 elements under the 128-byte swizzle.
+bool MapOf(CUtensorMap* map, bool f16, const void* base, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t box_rows) {
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride * 2};
+  const cuuint32_t box[2] = {64, box_rows}, elem[2] = {1, 1};
+  return Encoder()(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides,
+                   box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+uint32_t Up(uint64_t n, uint64_t by) { return static_cast<uint32_t>((n + by - 1) / by); }
+
+Status CheckGated(const std::string& what, see_gated_shape* s) {
+  if (s->type != SEE_BF16 && s->type != SEE_F16) return std::unexpected(what + ": the type is bf16 or f16");
+  if (s->act != SEE_ACT_RELU && s->act != SEE_ACT_GELU && s->act != SEE_ACT_SILU) return std::unexpected(what + ": unknown activation");
+  if (s->d_in == 0 || s->d_hidden == 0 || s->d_in % 8 || s->d_hidden % 8 || s->d_in > (1u << 20) || s->d_hidden > (1u << 20))
+    return std::unexpected(what + ": d_in and d_hidden are multiples of 8 from 8 to 2^20");
+  if (s->rows > 0x7FFFFF00ull) return std::unexpected(what + ": more than 2^31 - 256 rows");
+  if (s->x_stride == 0) s->x_stride = s->d_in;
+  if (s->hidden_stride == 0) s->hidden_stride = s->d_hidden;
+  if (s->x_stride < s->d_in || s->hidden_stride < s->d_hidden || s->x_stride % 8 || s->hidden_stride % 8 || s->x_stride > (1ull << 36) ||
+      s->hidden_stride > (1ull << 36))
+    return std::unexpected(what + ": a stride is smaller than a row, not a multiple of 8, or over 2^36");
+  // (the tiles of any product are numbered in 32 bits)
+  if ((s->rows / 256 + 1) * (s->d_hidden / 64 + 1) > 0x7FFFFFFFull || (s->rows / 256 + 1) * (s->d_in / 128 + 1) > 0x7FFFFFFFull)
+    return std::unexpected(what + ": too many rows for these widths");
+  return {};
+}
+
+uint64_t SlopeBytes(uint64_t rows, uint64_t d_hidden) { return (rows * d_hidden * 2 + 127) / 128 * 128; }
+
+// Width of a pair's accumulator: 256 columns do a third more arithmetic per operand byte, 128 leave fewer pairs idle in the
+// last round.
+uint32_t TileWidth(const uint64_t (&tiles)[2], uint32_t sms) {
+  const uint64_t pairs = std::max<uint64_t>(1, sms / 2);
+  const double wide = static_cast<double>((tiles[0] + pairs - 1) / pairs), narrow = 0.6 * static_cast<double>((tiles[1] + pairs - 1) / pairs);
+  return wide <= narrow ? 256 : 128;
+}
+
+}  // namespace
+
+uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden) {
+  if (d_in == 0 || d_hidden == 0 || d_in % 8 || d_hidden % 8 || d_in > (1u << 20) || d_hidden > (1u << 20) || rows > 0x7FFFFF00ull) return 0;
+  return std::max<uint64_t>(128, 2 * SlopeBytes(rows, d_hidden));
+}
+
+Status CheckGatedForward(see_gated_shape* shape, const void* x, const void* w_gate, const void* w_up, const void* hidden, const void* gate,
+                         const void* up) {
+  const std::string what = "cuda: gated forward";
+  if (auto r = CheckGated(what, shape); !r) return r;
+  const see_gated_shape& s = *shape;
+  if (!gate != !up) return std::unexpected(what + ": gate and up are kept together or not at all");
+  const uint64_t weights = s.d_in * s.d_hidden * 2, width = s.d_hidden * 2, pitch = s.hidden_stride * 2;
+  std::vector<Operand> ops = {{"x", x, s.rows, s.d_in * 2, s.x_stride * 2, 16, false},
+                              Vector("w_gate", w_gate, weights, 16, false),
+                              Vector("w_up", w_up, weights, 16, false),
+                              {"hidden", hidden, s.rows, width, pitch, 16, true}};
+  if (gate) {
+    ops.push_back({"gate", gate, s.rows, width, pitch, 16, true});
+    ops.push_back({"up", up, s.rows, width, pitch, 16, true});
+  }
+  return CheckOperands(what, ops);
+}
+
+Status CheckGatedBackward(see_gated_shape* shape, const void* dhidden, const void* x, const void* w_gate, const void* w_up,
+                          const void* gate, const void* up, const void* dx, const void* dw_gate, const void* dw_up, const void* workspace,
+                          uint64_t workspace_bytes) {
+  const std::string what = "cuda: gated backward";
+  if (auto r = CheckGated(what, shape); !r) return r;
+  const see_gated_shape& s = *shape;
+  if (!dw_gate != !dw_up) return std::unexpected(what + ": dw_gate and dw_up are wanted together or not at all");
+  if (!dx && !dw_gate) return std::unexpected(what + ": no output is wanted");
+  if (workspace_bytes < GatedBackwardWorkspace(s.rows, s.d_in, s.d_hidden)) return std::unexpected(what + ": the workspace is too small");
+  const uint64_t weights = s.d_in * s.d_hidden * 2, width = s.d_hidden * 2, pitch = s.hidden_stride * 2;
+  std::vector<Operand> ops = {{"dhidden", dhidden, s.rows, width, pitch, 16, false},
+                              {"x", x, s.rows, s.d_in * 2, s.x_stride * 2, 16, false},
+                              Vector("w_gate", w_gate, weights, 16, false),
+                              Vector("w_up", w_up, weights, 16, false),
+                              {"gate", gate, s.rows, width, pitch, 16, false},
+                              {"up", up, s.rows, width, pitch, 16, false},
+                              Vector("workspace", workspace, workspace_bytes, 128, true)};
+  if (dx) ops.push_back({"dx", dx, s.rows, s.d_in * 2, s.x_stride * 2, 16, true});
+  if (dw_gate) {
+    ops.push_back(Vector("dw_gate", dw_gate, weights, 16, true));
+    ops.push_back(Vector("dw_up", dw_up, weights, 16, true));
+  }
+  return CheckOperands(what, ops);
+}
+
+Status CudaBackend::GatedForward(const see_gated_shape& given, const void* x, const void* w_gate, const void* w_up, void* hidden, void* gate,
+                                 void* up) {
+  see_gated_shape s = given;
+  if (auto r = CheckGatedForward(&s, x, w_gate, w_up, hidden, gate, up); !r) return r;
+  if (s.rows == 0) return {};
+  OnDevice on(device_);
+  if (!on.ok()) return Check(cudaGetLastError(), "gated forward: device");
+  if (!Encoder()) return std::unexpected("cuda: gated forward: the driver does not provide cuTensorMapEncodeTiled");
+  const bool f16 = s.type == SEE_F16;
+  k::GatedLaunch l = {};
+  k::GatedProblem& p = l.p[0];
+  const uint64_t tiles[2] = {static_cast<uint64_t>(Up(s.rows, 256)) * Up(s.d_hidden, 128), static_cast<uint64_t>(Up(s.rows, 256)) * Up(s.d_hidden, 64)};
+  const uint32_t tn = TileWidth(tiles, sms_);
+  bool ok = MapOf(&p.a[0], f16, x, s.rows, s.d_in, s.x_stride, 64) && MapOf(&p.b[0], f16, w_gate, s.d_in, s.d_hidden, s.d_hidden, 64) &&
+            MapOf(&p.b[1], f16, w_up, s.d_in, s.d_hidden, s.d_hidden, 64) && MapOf(&p.c, f16, hidden, s.rows, s.d_hidden, s.hidden_stride, 32);
+  if (gate)
+    ok = ok && MapOf(&l.gate, f16, gate, s.rows, s.d_hidden, s.hidden_stride, 32) && MapOf(&l.up, f16, up, s.rows, s.d_hidden, s.hidden_stride, 32);
+  if (!ok) return std::unexpected("cuda: gated forward: cuTensorMapEncodeTiled refused an operand layout");
+  p.M = static_cast<uint32_t>(s.rows);
+  p.N = static_cast<uint32_t>(s.d_hidden);
+  p.blocks[0] = Up(s.d_in, 64);
+  p.b_mn = 1;
+  p.tiles_m = Up(s.rows, 256);
+  p.tiles_n = Up(s.d_hidden, tn / 2);
+  l.count = 1;
+  l.f16 = f16;
+  l.act = s.act;
+  l.keep = gate != nullptr;
+  l.status = d_status_;
+  if (auto r = Check(k::GatedProducts(l, true, tn, sms_, stream_), "gated forward"); !r) return r;
+  ++counters_.kernel_launches;
+  return {};
+}
+
+Status CudaBackend::GatedBackward(const see_gated_shape& given, const void* dhidden, const void* x, const void* w_gate, const void* w_up,
+                                  const void* gate, const void* up, void* dx, void* dw_gate, void* dw_up, void* workspace,
+                                  uint64_t workspace_bytes) {
+  see_gated_shape s = given;
+  if (auto r = CheckGatedBackward(&s, dhidden, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, workspace, workspace_bytes); !r) return r;
+  OnDevice on(device_);
+  if (!on.ok()) return Check(cudaGetLastError(), "gated backward: device");
+  const uint64_t weights = s.d_in * s.d_hidden * 2;
+  if (s.rows == 0) {
+    for (void* w : {dw_gate, dw_up})
+      if (w)
+        if (auto r = Check(cudaMemsetAsync(w, 0, weights, stream_), "gated backward"); !r) return r;
+    return {};
+  }
+  if (!Encoder()) return std::unexpected("cuda: gated backward: the driver does not provide cuTensorMapEncodeTiled");
+  const bool f16 = s.type == SEE_F16;
+  void* dg = workspace;
+  void* du = static_cast<uint8_t*>(workspace) + SlopeBytes(s.rows, s.d_hidden);
+  k::GatedLaunch l = {};
+  l.f16 = f16;
+  l.status = d_status_;
+  const uint32_t rows = static_cast<uint32_t>(s.rows), d_in = static_cast<uint32_t>(s.d_in), d_hidden = static_cast<uint32_t>(s.d_hidden);
+  uint64_t tiles[2] = {0, 0};
+  auto problem = [&](uint32_t M, uint32_t N) -> k::GatedProblem& {
+    k::GatedProblem& p = l.p[l.count++];
+    p.M = M;
+    p.N = N;
+    p.tiles_m = Up(M, 256);
+    tiles[0] += static_cast<uint64_t>(p.tiles_m) * Up(N, 256);
+    tiles[1] += static_cast<uint64_t>(p.tiles_m) * Up(N, 128);
+    return p;
+  };
+  bool ok = true;
+  if (dx) {   // A: dg, then du, along their rows; B: the weights' rows are dx's columns
+    k::GatedProblem& p = problem(rows, d_in);
+    p.blocks[0] = p.blocks[1] = Up(d_hidden, 64);
+    ok = MapOf(&p.a[0], f16, dg, rows, d_hidden, d_hidden, 64) && MapOf(&p.a[1], f16, du, rows, d_hidden, d_hidden, 64) &&
+         MapOf(&p.b[0], f16, w_gate, d_in, d_hidden, d_hidden, 64) && MapOf(&p.b[1], f16, w_up, d_in, d_hidden, d_hidden, 64) &&
+         MapOf(&p.c, f16, dx, rows, d_in, s.x_stride, 32);
+  }
+  for (int which = 0; which < 2 && dw_gate && ok; ++which) {   // both operands down their columns
+    k::GatedProblem& p = problem(d_in, d_hidden);
+    p.a_mn = p.b_mn = 1;
+    p.blocks[0] = Up(rows, 64);
+    ok = MapOf(&p.a[0], f16, x, rows, d_in, s.x_stride, 64) && MapOf(&p.b[0], f16, which ? du : dg, rows, d_hidden, d_hidden, 64) &&
+         MapOf(&p.c, f16, which ? dw_up : dw_gate, d_in, d_hidden, d_hidden, 32);
+  }
+  if (!ok) return std::unexpected("cuda: gated backward: cuTensorMapEncodeTiled refused an operand layout");
+  const uint32_t tn = TileWidth(tiles, sms_);
+  for (uint32_t i = 0; i < l.count; ++i) l.p[i].tiles_n = Up(l.p[i].N, tn);
+  if (auto r = Check(k::GatedSlopes(dhidden, gate, up, dg, du, s.rows, d_hidden, s.hidden_stride, s.act, f16, sms_, stream_), "gated backward"); !r)
+    return r;
+  ++counters_.kernel_launches;
+  if (auto r = Check(k::GatedProducts(l, false, tn, sms_, stream_), "gated backward"); !r) return r;
+  ++counters_.kernel_launches;
+  return {};
+}
+
+}  // namespace see
