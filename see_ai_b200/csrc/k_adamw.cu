@@ -87,7 +87,7 @@ __device__ __forceinline__ BlockScale ScaleOf(uint32_t largest_bits) {
   const float largest = __uint_as_float(largest_bits);
   if (largest_bits >= 0x7F800000u) return {0.0f, __uint_as_float(0x7FC00000u)};
   if (largest < 7.888609052210118e-31f) return {0.0f, 0.0f};
-  return {448.0f / largest, largest * (1.0f / 448.0f)};
+  return {1.0f / largest * 448.0f, largest * (1.0f / 448.0f)};
 }
 
 template <int kBits, uint32_t kEntries>
