@@ -133,6 +133,7 @@ Status CudaBackend::NormBackward(const see_norm_shape& given, const void* dy, co
   a.dgamma = dgamma;
   a.dbeta = dbeta;
   a.partials = static_cast<float*>(workspace);
+  a.status = d_status_;
   int launches = 0;
   const cudaError_t e = k::NormBackward(a, sms_, stream_, &launches);
   counters_.kernel_launches += static_cast<uint64_t>(launches);

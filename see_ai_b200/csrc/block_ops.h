@@ -29,6 +29,7 @@ struct NormArgs {
   int x_type = SEE_F32, y_type = SEE_F32;
   bool rms = false;
   float eps = 0.0f;
+  DeviceStatus* status = nullptr;
 };
 inline uint64_t NormPartialRows(uint64_t rows) { return rows < kNormPartials ? rows : kNormPartials; }
 cudaError_t NormForward(const NormArgs& a, uint32_t sms, cudaStream_t s);

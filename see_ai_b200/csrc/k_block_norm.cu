@@ -11,8 +11,10 @@
 //
 // All sums are f32.  The forward pass takes the mean twice: the second pass over the registers sums the deviations from
 // the first result, which corrects it, beside their squares, so rows far from zero lose nothing to cancellation.
+#include "act_expr.cuh"
 #include "block_ops.h"
 #include "launch.cuh"
+#include "umma_device.cuh"
 #include "vec_types.cuh"
 
 namespace see::k {
@@ -20,20 +22,23 @@ namespace see::k {
 namespace {
 
 constexpr uint32_t kNormThreads = 512;
+constexpr size_t kRingBytes = 200 * 1024;   // of a block
 
-__device__ __forceinline__ float2 WarpSum2(float2 v) {
+template <bool kBoth>
+__device__ __forceinline__ float2 WarpSum(float2 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, o);
-    v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, o);
+    if (kBoth) v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, o);
   }
   return v;
 }
 
 // The sums of a group's T threads, in all of them.  `slots`: two sets of 16 per block, used in turn, so that one barrier
 // a sum is enough: who writes a set again has passed the barrier that the readers of its last use arrived at after it.
+template <bool kBoth>   // or v.x alone
 __device__ __forceinline__ float2 GroupSum(float2 v, uint32_t T, uint32_t group, float2 (*slots)[kNormThreads / 32], uint32_t& turn) {
-  v = WarpSum2(v);
+  v = WarpSum<kBoth>(v);
   if (T == 32) return v;
   float2* set = slots[turn] + group * (T / 32);
   turn ^= 1;
@@ -42,7 +47,7 @@ __device__ __forceinline__ float2 GroupSum(float2 v, uint32_t T, uint32_t group,
   float2 sum = set[0];
   for (uint32_t w = 1; w < T / 32; ++w) {
     sum.x += set[w].x;
-    sum.y += set[w].y;
+    if (kBoth) sum.y += set[w].y;
   }
   return sum;
 }
@@ -82,7 +87,7 @@ NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sum.x += kRms ? v[i][j] * v[i][j] : v[i][j];
   }
-  sum = GroupSum(sum, T, group, slots, turn);
+  sum = GroupSum<false>(sum, T, group, slots, turn);
   const float per_col = 1.0f / static_cast<float>(a.cols);
   float mean = 0.0f, var;
   if constexpr (kRms) {
@@ -100,7 +105,7 @@ NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
           sum.y += d * d;
         }
       }
-    sum = GroupSum(sum, T, group, slots, turn);
+    sum = GroupSum<true>(sum, T, group, slots, turn);
     const float shift = sum.x * per_col;
     if (isfinite(shift)) mean += shift;
     var = fmaxf(sum.y * per_col - shift * shift, 0.0f);
@@ -122,6 +127,164 @@ NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) g[j] = kRms ? v[i][j] * rstd * g[j] : (v[i][j] - mean) * rstd * g[j] + b[j];
       StoreCols<YT, VEC>(y + c, g);
+    }
+  }
+}
+
+// Eight columns as four pairs for the packed f32 instructions (the kernel below is short of issue slots, not of memory's).
+template <typename T> __device__ __forceinline__ void LoadPairs(const T* p, f32x2 (&v)[4]) {
+  float f[8];
+  Load8<T>(p, f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = PackF2(f[2 * j], f[2 * j + 1]);
+}
+template <typename T> __device__ __forceinline__ void StorePairs(T* p, const f32x2 (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) UnpackF2(v[j], &f[2 * j], &f[2 * j + 1]);
+  Store8<T>(p, f);
+}
+
+// ---- rows through a ring in shared memory -----------------------------------------------
+// Each group has `slots` of its own, filled by one thread's bulk copies (a whole row each, counted on the slot's mbarrier)
+// and emptied into registers; a slot is asked to be filled again as soon as the group has read it, so that between 60 and
+// 200 KB are on their way to an SM at any time.
+__device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(umma_dev::SmemAddr(dst)), "l"(src), "r"(bytes), "r"(umma_dev::SmemAddr(bar))
+               : "memory");
+}
+__device__ __forceinline__ void GroupBarrier(uint32_t T, uint32_t group) {
+  if (T == 32) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(T) : "memory");
+}
+// A bulk copy of this device's memory always lands; that nothing can wait for good even so, the wait is bounded, and a thread
+// that ran out raises the flag and goes on (the others of its group count on it at their barriers).
+__device__ __forceinline__ void AwaitRow(uint64_t* bar, uint32_t parity, DeviceStatus* status) {
+  if (umma_dev::MbarWait(bar, parity)) return;
+  status->wait_timeout = 1;
+  umma_dev::DrainDelay();
+}
+
+template <typename XT, typename YT, bool kRms, int NV, uint32_t kThreads>
+__global__ void __launch_bounds__(kThreads, 1)
+NormBwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots) {
+  constexpr bool kHoldGamma = kThreads < 512 || NV <= 2;   // in registers, as far as they go
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ float2 sums[2][kNormThreads / 32];
+  const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
+  const uint32_t x_bytes = a.cols * sizeof(XT), y_bytes = a.cols * sizeof(YT);
+  const uint32_t slot_bytes = x_bytes + y_bytes + (a.addend ? x_bytes : 0);
+  uint8_t* ring = dyn + static_cast<size_t>(group) * slots * slot_bytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + static_cast<size_t>(groups) * slots * slot_bytes) + group * slots;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups + group, step = static_cast<uint64_t>(gridDim.x) * groups;
+  if (t == 0) {
+    for (uint32_t i = 0; i < slots; ++i) umma_dev::MbarInit(&bars[i], 1);
+    umma_dev::MbarInitFence();
+  }
+  auto fill = [&](uint64_t row, uint32_t slot) {   // the group's thread 0
+    uint8_t* dst = ring + static_cast<size_t>(slot) * slot_bytes;
+    umma_dev::MbarExpectTx(&bars[slot], slot_bytes);
+    BulkLoad(dst, static_cast<const XT*>(a.x) + row * a.x_stride, x_bytes, &bars[slot]);
+    BulkLoad(dst + x_bytes, static_cast<const YT*>(a.dy) + row * a.y_stride, y_bytes, &bars[slot]);
+    if (a.addend) BulkLoad(dst + x_bytes + y_bytes, static_cast<const XT*>(a.addend) + row * a.x_stride, x_bytes, &bars[slot]);
+  };
+  AwaitPrevious();
+  if (t == 0)
+    for (uint32_t i = 0; i < slots && first + i * step < a.rows; ++i) fill(first + i * step, i);
+  const float per_col = 1.0f / static_cast<float>(a.cols);
+  uint32_t turn = 0;
+  f32x2 gamma[kHoldGamma ? NV : 1][4], sum_g[NV][4], sum_b[kRms ? 1 : NV][4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (kHoldGamma && (t + i * T) * 8 < a.cols) LoadPairs<float>(a.gamma + (t + i * T) * 8, gamma[kHoldGamma ? i : 0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sum_g[i][j] = 0;
+      if (!kRms) sum_b[i][j] = 0;
+    }
+  }
+  GroupBarrier(T, group);   // the barriers are there
+  uint32_t slot = 0, parity = 0;
+  float next_rstd = 0.0f, next_mean = 0.0f;   // asked for a row ahead, like the row itself
+  if (first < a.rows) {
+    next_rstd = a.rstd[first];
+    if (!kRms) next_mean = a.mean[first];
+  }
+  for (uint64_t row = first; row < a.rows; row += step) {
+    const float rstd = next_rstd, mean = next_mean;
+    if (row + step < a.rows) {
+      next_rstd = a.rstd[row + step];
+      if (!kRms) next_mean = a.mean[row + step];
+    }
+    const f32x2 rstd2 = Splat2(rstd), mean2 = Splat2(-mean);
+    AwaitRow(&bars[slot], parity, a.status);
+    const XT* x = reinterpret_cast<const XT*>(ring + static_cast<size_t>(slot) * slot_bytes);
+    const YT* dy = reinterpret_cast<const YT*>(x + a.cols);
+    f32x2 u[NV][4], d[NV][4], with_u = 0, plain = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * T) * 8;
+      if (c < a.cols) {
+        LoadPairs<XT>(x + c, u[i]);
+        LoadPairs<YT>(dy + c, d[i]);
+        f32x2 g[4];
+        if (!kHoldGamma) LoadPairs<float>(a.gamma + c, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          u[i][j] = Mul2(kRms ? u[i][j] : AddF2(u[i][j], mean2), rstd2);
+          sum_g[i][j] = Fma2(d[i][j], u[i][j], sum_g[i][j]);
+          if (!kRms) sum_b[i][j] = AddF2(sum_b[i][j], d[i][j]);
+          d[i][j] = Mul2(d[i][j], kHoldGamma ? gamma[kHoldGamma ? i : 0][j] : g[j]);
+          with_u = Fma2(d[i][j], u[i][j], with_u);
+          if (!kRms) plain = AddF2(plain, d[i][j]);
+        }
+      }
+    }
+    float2 sum, other;
+    UnpackF2(with_u, &sum.x, &other.x);
+    UnpackF2(plain, &sum.y, &other.y);
+    sum = GroupSum<!kRms>(make_float2(sum.x + other.x, sum.y + other.y), T, group, sums, turn);
+    const f32x2 pull = Splat2(-sum.x * per_col), shift = Splat2(-sum.y * per_col);
+    const XT* add = reinterpret_cast<const XT*>(dy + a.cols);
+    XT* dx = static_cast<XT*>(a.dx) + row * a.x_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * T) * 8;
+      if (c < a.cols) {
+        f32x2 v[4];
+        if (a.addend) LoadPairs<XT>(add + c, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x2 r = Fma2(u[i][j], pull, kRms ? d[i][j] : AddF2(d[i][j], shift));
+          v[j] = a.addend ? Fma2(r, rstd2, v[j]) : Mul2(r, rstd2);
+        }
+        StorePairs<XT>(dx + c, v);
+      }
+    }
+    GroupBarrier(T, group);   // the slot is read
+    if (t == 0 && row + slots * step < a.rows) fill(row + slots * step, slot);
+    if (++slot == slots) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+  float* meet = reinterpret_cast<float*>(dyn);   // [groups][cols]; every copy has been read
+  float* out_g = gridDim.x == 1 ? a.dgamma : a.partials + static_cast<size_t>(blockIdx.x) * a.cols;
+  float* out_b = gridDim.x == 1 ? a.dbeta : a.partials + static_cast<size_t>(gridDim.x + blockIdx.x) * a.cols;
+#pragma unroll
+  for (int which = 0; which < (kRms ? 1 : 2); ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * T) * 8;
+      if (c < a.cols) StorePairs<float>(meet + group * a.cols + c, which ? sum_b[kRms ? 0 : i] : sum_g[i]);
+    }
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+      float s = meet[c];
+      for (uint32_t r = 1; r < groups; ++r) s += meet[r * a.cols + c];
+      (which ? out_b : out_g)[c] = s;
     }
   }
 }
@@ -175,7 +338,7 @@ NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
         }
       }
     }
-    sum = GroupSum(sum, T, group, slots, turn);
+    sum = GroupSum<!kRms>(sum, T, group, slots, turn);
     sum.x *= per_col;
     sum.y *= per_col;
     XT* dx = static_cast<XT*>(a.dx) + row * a.x_stride;
@@ -256,40 +419,90 @@ NormShape ShapeOf(uint32_t cols, bool vec) {
   return n <= 8192 ? NormShape{up((n + 15) / 16), 16} : NormShape{up((n + 31) / 32), 32};
 }
 
-template <typename XT, typename YT, bool kRms, int VEC, int NV>
-cudaError_t Run(const NormArgs& a, uint32_t T, bool backward, uint32_t sms, cudaStream_t s, int* launches) {
-  const uint32_t groups = kNormThreads / T;
-  const uint64_t blocks = (a.rows + groups - 1) / groups;
-  if (!backward) return Next(NormFwdKernel<XT, YT, kRms, VEC, NV>, static_cast<unsigned>(blocks), groups * T, 0, s)(a, T);
-  auto* kernel = NormBwdKernel<XT, YT, kRms, VEC, NV>;
-  const size_t smem = static_cast<size_t>(groups) * a.cols * 4;
-  if (smem > 32 * 1024)   // (the static part counts too)
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)); e != cudaSuccess) return e;
-  uint64_t grid = sms < kNormPartials ? sms : kNormPartials;
-  if (grid > blocks) grid = blocks;
-  if (cudaError_t e = Next(kernel, static_cast<unsigned>(grid), groups * T, smem, s)(a, T); e != cudaSuccess) return e;
+template <bool kRms>
+cudaError_t Fold(const NormArgs& a, uint64_t grid, cudaStream_t s, int* launches) {
   ++*launches;
   if (grid == 1) return cudaSuccess;
   ++*launches;
   return Next(NormFoldKernel, dim3((a.cols + 31) / 32, kRms ? 1 : 2), 1024, 0, s)(a.partials, a.dgamma, a.dbeta, static_cast<uint32_t>(grid), a.cols);
 }
+template <typename K>
+cudaError_t AllowShared(K* kernel, size_t bytes) {   // (the static part counts too)
+  return bytes > 32 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) : cudaSuccess;
+}
+uint64_t Blocks(uint64_t rows, uint32_t groups, uint32_t sms) {
+  const uint64_t blocks = (rows + groups - 1) / groups, most = sms < kNormPartials ? sms : kNormPartials;
+  return blocks < most ? blocks : most;
+}
+
+template <typename XT, typename YT, bool kRms, int NV, uint32_t kThreads>
+cudaError_t RunRing(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s, int* launches) {
+  const size_t row_bytes = static_cast<size_t>(a.cols) * (sizeof(XT) * (a.addend ? 2 : 1) + sizeof(YT));
+  uint32_t groups = kThreads / T;
+  while (groups > 1 && 2 * groups * row_bytes > kRingBytes) --groups;   // two slots to a group, unless it is alone
+  uint32_t slots = static_cast<uint32_t>(kRingBytes / (groups * row_bytes));
+  slots = slots < 1 ? 1 : slots > 8 ? 8 : slots;
+  const size_t smem = groups * slots * (row_bytes + 8);
+  auto* kernel = NormBwdRingKernel<XT, YT, kRms, NV, kThreads>;
+  if (cudaError_t e = AllowShared(kernel, smem); e != cudaSuccess) return e;
+  const uint64_t grid = Blocks(a.rows, groups, sms);
+  if (cudaError_t e = Next(kernel, static_cast<unsigned>(grid), groups * T, smem, s)(a, T, slots); e != cudaSuccess) return e;
+  return Fold<kRms>(a, grid, s, launches);
+}
+
+template <typename XT, typename YT, bool kRms, int VEC, int NV>
+cudaError_t Run(const NormArgs& a, uint32_t T, cudaStream_t s) {
+  const uint32_t groups = kNormThreads / T;
+  return Next(NormFwdKernel<XT, YT, kRms, VEC, NV>, static_cast<unsigned>((a.rows + groups - 1) / groups), groups * T, 0, s)(a, T);
+}
+template <typename XT, typename YT, bool kRms, int NV>
+cudaError_t RunSingles(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s, int* launches) {
+  const uint32_t groups = kNormThreads / T;
+  auto* kernel = NormBwdKernel<XT, YT, kRms, 1, NV>;
+  const size_t smem = static_cast<size_t>(groups) * a.cols * 4;
+  if (cudaError_t e = AllowShared(kernel, smem); e != cudaSuccess) return e;
+  const uint64_t grid = Blocks(a.rows, groups, sms);
+  if (cudaError_t e = Next(kernel, static_cast<unsigned>(grid), groups * T, smem, s)(a, T); e != cudaSuccess) return e;
+  return Fold<kRms>(a, grid, s, launches);
+}
 
 template <typename XT, typename YT, bool kRms>
 cudaError_t Pick(const NormArgs& a, bool backward, uint32_t sms, cudaStream_t s, int* launches) {
   const bool vec = Vec8Able(a, backward);
-  const NormShape shape = ShapeOf(a.cols, vec);
+  const NormShape f = ShapeOf(a.cols, vec);
+  if (vec && backward) {
+    // A warp's row of up to 768 columns, or threads with 16 of wider ones: a row's u and q, the sums and gamma are then in
+    // registers; rms, with one sum, has room for 32, which spreads a row's fixed cost further.  (16384 x 4096 bf16: layer
+    // norm with 32 columns a thread 117 us, spilling, 16 90; rms 16 columns 80, 32 73.)
+    const uint32_t n = a.cols / 8;
+    auto up = [](uint32_t v) { return (v + 31) / 32 * 32; };
+    if (n <= 96) {   // a warp's row
+      if (n <= 32) return RunRing<XT, YT, kRms, 1, 384>(a, 32, sms, s, launches);
+      return n <= 64 ? RunRing<XT, YT, kRms, 2, 384>(a, 32, sms, s, launches) : RunRing<XT, YT, kRms, 3, 384>(a, 32, sms, s, launches);
+    }
+    if (kRms && n <= 1536) return RunRing<XT, YT, kRms, 4, 384>(a, up((n + 3) / 4), sms, s, launches);
+    if (n <= 1024) return RunRing<XT, YT, kRms, 2, 512>(a, up((n + 1) / 2), sms, s, launches);
+    return RunRing<XT, YT, kRms, 4, 512>(a, up((n + 3) / 4), sms, s, launches);
+  }
   if (vec) {
-    switch (shape.nv) {
-      case 1: return Run<XT, YT, kRms, 8, 1>(a, shape.T, backward, sms, s, launches);
-      case 2: return Run<XT, YT, kRms, 8, 2>(a, shape.T, backward, sms, s, launches);
-      case 3: return Run<XT, YT, kRms, 8, 3>(a, shape.T, backward, sms, s, launches);
-      default: return Run<XT, YT, kRms, 8, 4>(a, shape.T, backward, sms, s, launches);
+    switch (f.nv) {
+      case 1: return Run<XT, YT, kRms, 8, 1>(a, f.T, s);
+      case 2: return Run<XT, YT, kRms, 8, 2>(a, f.T, s);
+      case 3: return Run<XT, YT, kRms, 8, 3>(a, f.T, s);
+      default: return Run<XT, YT, kRms, 8, 4>(a, f.T, s);
     }
   }
-  switch (shape.nv) {
-    case 8: return Run<XT, YT, kRms, 1, 8>(a, shape.T, backward, sms, s, launches);
-    case 16: return Run<XT, YT, kRms, 1, 16>(a, shape.T, backward, sms, s, launches);
-    default: return Run<XT, YT, kRms, 1, 32>(a, shape.T, backward, sms, s, launches);
+  if (backward) {
+    switch (f.nv) {
+      case 8: return RunSingles<XT, YT, kRms, 8>(a, f.T, sms, s, launches);
+      case 16: return RunSingles<XT, YT, kRms, 16>(a, f.T, sms, s, launches);
+      default: return RunSingles<XT, YT, kRms, 32>(a, f.T, sms, s, launches);
+    }
+  }
+  switch (f.nv) {
+    case 8: return Run<XT, YT, kRms, 1, 8>(a, f.T, s);
+    case 16: return Run<XT, YT, kRms, 1, 16>(a, f.T, s);
+    default: return Run<XT, YT, kRms, 1, 32>(a, f.T, s);
   }
 }
 

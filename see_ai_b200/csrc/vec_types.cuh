@@ -49,6 +49,11 @@ template <typename T> __device__ __forceinline__ void Unpack2(uint32_t v, float&
   hi = ToF32(b);
 }
 
+template <> __device__ __forceinline__ void Unpack2<Bf16>(uint32_t v, float& lo, float& hi) {
+  lo = __uint_as_float(v << 16);
+  hi = __uint_as_float(v & 0xFFFF0000u);
+}
+
 template <typename T> __device__ __forceinline__ void Load8(const T* p, float* v) {
   const uint4 r = *reinterpret_cast<const uint4*>(p);
   Unpack2<T>(r.x, v[0], v[1]);
