@@ -148,41 +148,62 @@ Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bit
     return std::unexpected(what + ": beta1 and beta2 are from 0 on and below 1");
   if (count && !tensors) return std::unexpected(what + ": tensors is null");
   if (reinterpret_cast<uint64_t>(grad_scale) % 4) return std::unexpected(what + ": grad_scale is not aligned");
-  struct Span { uint64_t begin, end; bool written; };
-  std::vector<Span> spans;
-  spans.reserve(count * 7 + 1);
+  // Seven operands a tensor.  Lists of tensors mostly follow the layout of a few buffers, so each operand's spans are tried in
+  // the list's order first; only where they do not ascend, or two operands' ranges meet, is everything sorted.
+  struct Span { uint64_t begin, end; };
+  constexpr size_t kOperands = 7;
+  static constexpr const char* kNames[kOperands] = {"p", "g", "m", "v", "m_scale", "v_scale", "copy"};
+  const uint64_t state = static_cast<uint64_t>(state_bits) / 8;
+  auto spans_of = [&](const see_adamw_tensor& t, Span (&out)[kOperands]) {
+    const uint64_t scales = state == 1 ? (t.n + k::kAdamBlock - 1) / k::kAdamBlock * 4 : 0;
+    const void* p[kOperands] = {t.p, t.g, t.m, t.v, t.m_scale, t.v_scale, t.copy};
+    const uint64_t bytes[kOperands] = {t.n * 4, t.n * SizeOfType(t.g_type), t.n * state, t.n * state, scales, scales, t.copy ? t.n * 2 : 0};
+    for (size_t o = 0; o < kOperands; ++o) out[o] = {reinterpret_cast<uint64_t>(p[o]), reinterpret_cast<uint64_t>(p[o]) + bytes[o]};
+  };
+  Span range[kOperands + 1];
+  for (Span& r : range) r = {~0ull, 0};
+  bool ascending = true;
   for (uint64_t i = 0; i < count; ++i) {
     const see_adamw_tensor& t = tensors[i];
-    const std::string name = what + ": tensor " + std::to_string(i);
-    if (!IsType(t.g_type) || !IsType(t.copy_type)) return std::unexpected(name + ": unknown type");
-    if (t.flags & ~static_cast<uint32_t>(SEE_ADAMW_NO_DECAY)) return std::unexpected(name + ": unknown flag");
-    if ((t.copy_type == SEE_F32) != (t.copy == nullptr)) return std::unexpected(name + ": a copy has 16 bits, and none is null with type f32");
+    auto refuse = [&](const std::string& why) { return std::unexpected(what + ": tensor " + std::to_string(i) + ": " + why); };
+    if (!IsType(t.g_type) || !IsType(t.copy_type)) return refuse("unknown type");
+    if (t.flags & ~static_cast<uint32_t>(SEE_ADAMW_NO_DECAY)) return refuse("unknown flag");
+    if ((t.copy_type == SEE_F32) != (t.copy == nullptr)) return refuse("a copy has 16 bits, and none is null with type f32");
     if (t.n == 0) continue;
-    if (t.n > (1ull << 42)) return std::unexpected(name + ": more than 2^42 elements");
-    const uint64_t blocks = (t.n + k::kAdamBlock - 1) / k::kAdamBlock, state = state_bits / 8;
-    const struct { const char* name; const void* p; uint64_t bytes, align; bool written; } ops[] = {
-        {"p", t.p, t.n * 4, 4, true},
-        {"g", t.g, t.n * SizeOfType(t.g_type), SizeOfType(t.g_type), false},
-        {"m", t.m, t.n * state, state, true},
-        {"v", t.v, t.n * state, state, true},
-        {"m_scale", t.m_scale, state == 1 ? blocks * 4 : 0, 4, true},
-        {"v_scale", t.v_scale, state == 1 ? blocks * 4 : 0, 4, true},
-        {"copy", t.copy, t.copy ? t.n * 2 : 0, 2, true}};
-    for (const auto& o : ops) {
-      if (o.bytes == 0) continue;
-      const uint64_t at = reinterpret_cast<uint64_t>(o.p);
-      if (!at) return std::unexpected(name + ": " + o.name + " is null");
-      if (at % o.align) return std::unexpected(name + ": " + o.name + " is not aligned");
-      spans.push_back({at, at + o.bytes, o.written});
+    if (t.n > (1ull << 39)) return refuse("more than 2^39 elements");
+    const uint64_t align[kOperands] = {4, SizeOfType(t.g_type), state, state, 4, 4, 2};
+    Span spans[kOperands];
+    spans_of(t, spans);
+    for (size_t o = 0; o < kOperands; ++o) {
+      if (spans[o].begin == spans[o].end) continue;
+      if (!spans[o].begin) return refuse(std::string(kNames[o]) + " is null");
+      if (spans[o].begin % align[o]) return refuse(std::string(kNames[o]) + " is not aligned");
+      ascending = ascending && (range[o].end == 0 || spans[o].begin >= range[o].end);
+      range[o] = {std::min(range[o].begin, spans[o].begin), std::max(range[o].end, spans[o].end)};
     }
   }
-  if (grad_scale) spans.push_back({reinterpret_cast<uint64_t>(grad_scale), reinterpret_cast<uint64_t>(grad_scale) + 4, false});
-  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  if (grad_scale) range[kOperands] = {reinterpret_cast<uint64_t>(grad_scale), reinterpret_cast<uint64_t>(grad_scale) + 4};
+  for (size_t i = 0; i <= kOperands && ascending; ++i)
+    for (size_t j = i + 1; j <= kOperands; ++j)
+      if (range[i].end && range[j].end && range[i].begin < range[j].end && range[j].begin < range[i].end) ascending = false;
+  if (ascending) return {};
+  struct Sorted { Span span; bool written; };
+  std::vector<Sorted> all;
+  all.reserve(count * kOperands + 1);
+  for (uint64_t i = 0; i < count; ++i) {
+    if (tensors[i].n == 0) continue;
+    Span spans[kOperands];
+    spans_of(tensors[i], spans);
+    for (size_t o = 0; o < kOperands; ++o)
+      if (spans[o].begin != spans[o].end) all.push_back({spans[o], o != 1});
+  }
+  if (grad_scale) all.push_back({range[kOperands], false});
+  std::sort(all.begin(), all.end(), [](const Sorted& a, const Sorted& b) { return a.span.begin < b.span.begin; });
   uint64_t any = 0, written = 0;   // how far the spans so far reach
-  for (const Span& s : spans) {
-    if (s.begin < written || (s.written && s.begin < any)) return std::unexpected(what + ": operands overlap");
-    any = std::max(any, s.end);
-    if (s.written) written = std::max(written, s.end);
+  for (const Sorted& s : all) {
+    if (s.span.begin < written || (s.written && s.span.begin < any)) return std::unexpected(what + ": operands overlap");
+    any = std::max(any, s.span.end);
+    if (s.written) written = std::max(written, s.span.end);
   }
   return {};
 }
@@ -206,7 +227,7 @@ Status CudaBackend::AdamWTensors(const see_adamw_tensor* tensors, uint64_t count
   OnDevice on(device_);
   if (!on.ok()) return Check(cudaGetLastError(), "adamw: device");
   int launches = 0;
-  const cudaError_t e = k::AdamWTensors(tensors, count, state_bits, a, grad_scale, sms_, stream_, &launches);
+  const cudaError_t e = k::AdamWTensors(tensors, count, state_bits, a, grad_scale, sms_, d_status_, stream_, &launches);
   counters_.kernel_launches += static_cast<uint64_t>(launches);
   return Check(e, "adamw");
 }

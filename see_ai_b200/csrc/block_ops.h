@@ -42,7 +42,7 @@ struct AdamStepScalars {
   uint32_t phase;   // the step's share of the rounding words
 };
 cudaError_t AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const AdamStepScalars& a,
-                         const float* grad_scale, uint32_t sms, cudaStream_t s, int* launches);
+                         const float* grad_scale, uint32_t sms, DeviceStatus* status, cudaStream_t s, int* launches);
 
 }  // namespace see::k
 

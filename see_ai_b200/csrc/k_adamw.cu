@@ -15,18 +15,21 @@
 // (i phi + t sqrt(2)) mod 1 (phi the golden section), spread evenly over elements and over steps.  A root that is not zero
 // is held as at least the smallest e4m3: a zero would let a later step divide by eps alone.
 //
-// Bound by HBM: 14 bytes an element with 16-bit gradients and moments in 8 bits, 28 in f32.  A warp takes a block of 256
-// elements, eight a lane; a thread block takes eight of them, and finds its tensor by bisection over the table, which the
-// launch carries as a parameter: nothing is uploaded, and a captured launch owns its copy.
+// Bound by HBM: 14 bytes an element with 16-bit gradients and moments in 8 bits, 28 in f32.  A warp takes blocks of 256
+// elements, eight a lane, that follow one another, through a ring of two in shared memory that bulk copies fill; the launch
+// carries the table of tensors as a parameter: nothing is uploaded, and a captured launch owns its copy.
+#include <type_traits>
+
+#include "act_expr.cuh"
 #include "block_ops.h"
 #include "launch.cuh"
+#include "umma_device.cuh"
 #include "vec_types.cuh"
 
 namespace see::k {
 
 namespace {
 
-constexpr uint32_t kAdamWarps = 8;
 constexpr uint32_t kGolden = 0x9E3779B9u;       // 2^32 times the golden section
 constexpr uint32_t kHalfTurn = 0x80000000u;     // between the words of m and of sqrt(v)
 
@@ -37,13 +40,46 @@ struct AdamEntry {
   float *m_scale, *v_scale;
   void* copy;
   uint64_t n;
-  uint8_t g_type, copy_type, decays, wide;   // copy_type SEE_F32: no copy; wide: every address is aligned to its four elements
+  uint8_t g_type, copy_type, decays, wide;   // copy_type SEE_F32: no copy; wide: every address is a multiple of 16
 };
 template <uint32_t kEntries>
 struct AdamTable {
   uint32_t count;
-  uint32_t chunk_end[kEntries];   // chunks (eight blocks of 256) of entries 0 .. i
+  uint32_t block_end[kEntries];   // blocks of 256 of entries 0 .. i
   AdamEntry entry[kEntries];
+};
+
+// A warp's ring: p, m, v and g of a block, gradients as wide as they come.
+template <int kBits>
+struct AdamRing {
+  static constexpr uint32_t kStateBytes = kAdamBlock * kBits / 8;
+  static constexpr uint32_t kM = kAdamBlock * 4, kV = kM + kStateBytes, kG = kV + kStateBytes;   // offsets in a slot
+  static constexpr uint32_t kSlotBytes = kG + kAdamBlock * 4;
+  static constexpr uint32_t kWarps = kBits == 8 ? 32 : 24, kSlots = 2;
+  static constexpr uint32_t kBytes = kWarps * kSlots * (kSlotBytes + 8);
+};
+
+// Where a block of the table's list lies.
+template <uint32_t kEntries>
+struct AdamCursor {
+  uint32_t entry, begin, end;
+  __device__ __forceinline__ void Find(const AdamTable<kEntries>& t, uint32_t block) {
+    uint32_t lo = 0, hi = t.count - 1;   // the first entry that ends behind the block
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (t.block_end[mid] > block) hi = mid;
+      else lo = mid + 1;
+    }
+    entry = lo;
+    begin = lo ? t.block_end[lo - 1] : 0u;
+    end = t.block_end[lo];
+  }
+  __device__ __forceinline__ void MoveTo(const AdamTable<kEntries>& t, uint32_t block) {   // not before the last one
+    while (block >= end) {
+      begin = end;
+      end = t.block_end[++entry];
+    }
+  }
 };
 
 __device__ __forceinline__ void Load4(const void* p, int type, uint64_t i, float* v) {   // i % 4 == 0, aligned
@@ -71,13 +107,48 @@ __device__ __forceinline__ void FromE4m3x2(uint16_t codes, float& lo, float& hi)
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(codes));
   Unpack2<F16>(h, lo, hi);
 }
-// |x| times `factor` as e4m3 without its sign (see above); `word` is the element's.
-__device__ __forceinline__ uint32_t ToE4m3(float magnitude, float factor, uint32_t word) {
-  const float a = magnitude * factor;
-  const bool low = a < 0.015625f;   // below the smallest normal: the distance of codes stays 2^-9
-  const uint32_t bits = __float_as_uint(low ? a + 0.015625f : a) + (word >> 12);
-  const uint32_t code = (bits >> 20) - (low ? 968u : 960u);
-  return code < 126u ? code : 126u;
+// Two values times their block's factor as e4m3, cut as above: the sum's upper 12 bits are the value where e4m3 is normal
+// (whose neighbours are a step of those apart), so that the conversion finds nothing left to round.  kLow: some value may lie
+// below 2^-6, where the distance of codes stays 2^-9 and the sum is taken 2^-6 further out.
+template <bool kLow>
+__device__ __forceinline__ uint32_t ToE4m3x2(f32x2 pair, uint32_t word_a, uint32_t word_b) {
+  auto cut = [](float x, uint32_t word) {
+    const float out = kLow && fabsf(x) < 0.015625f ? copysignf(0.015625f, x) : 0.0f;
+    const float y = kLow ? x + out : x;
+    const float c = __uint_as_float((__float_as_uint(y) + (word >> 12)) & 0xFFF00000u);
+    return kLow ? c - out : c;
+  };
+  float a, b;
+  UnpackF2(pair, &a, &b);
+  uint16_t codes;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(codes) : "f"(cut(b, word_b)), "f"(cut(a, word_a)));
+  return codes;
+}
+// The largest and the smallest magnitude of three; a NaN stays in the largest.
+__device__ __forceinline__ float MaxMagnitude(float a, f32x2 pair) {
+  float x, y, r;
+  UnpackF2(pair, &x, &y);
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float MinMagnitude(float a, f32x2 pair) {
+  float x, y, r;
+  UnpackF2(pair, &x, &y);
+  asm("min.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(x), "f"(y));
+  return r;
+}
+// sqrt(v) by one Newton step on the hardware's reciprocal root: s = v y, s + (v - s s) y / 2, the remainder exact in an FMA.
+// (A call of sqrtf costs three times as much here.)  Zero stays zero; what is not finite becomes NaN.
+__device__ __forceinline__ f32x2 Root2(f32x2 v) {
+  float a, b;
+  UnpackF2(v, &a, &b);
+  auto reciprocal = [](float x) {
+    float y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, 1.17549435e-38f)));
+    return y;
+  };
+  const f32x2 y = PackF2(reciprocal(a), reciprocal(b)), s = Mul2(v, y);
+  return Fma2(Fma2(Mul2(s, Splat2(-1.0f)), s, v), Mul2(y, Splat2(0.5f)), s);
 }
 
 // The largest magnitude's block scale: 0 where it is below 2^-100, NaN where it is not finite (one such element makes the
@@ -90,172 +161,247 @@ __device__ __forceinline__ BlockScale ScaleOf(uint32_t largest_bits) {
   return {1.0f / largest * 448.0f, largest * (1.0f / 448.0f)};
 }
 
-template <int kBits, uint32_t kEntries>
-__global__ void __launch_bounds__(32 * kAdamWarps)
-AdamWTensorsKernel(const __grid_constant__ AdamTable<kEntries> table, const AdamStepScalars a, const float* __restrict__ grad_scale) {
-  AwaitPrevious();
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float gs = grad_scale ? *grad_scale : 1.0f;
-  const uint32_t chunks = table.chunk_end[table.count - 1];
-  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    uint32_t lo = 0, hi = table.count - 1;   // the first entry that ends behind the chunk
-    while (lo < hi) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (table.chunk_end[mid] > chunk) hi = mid;
-      else lo = mid + 1;
-    }
-    const AdamEntry& e = table.entry[lo];
-    const uint64_t block = static_cast<uint64_t>(chunk - (lo ? table.chunk_end[lo - 1] : 0u)) * kAdamWarps + warp;
-    const uint64_t base = block * kAdamBlock;
-    if (base >= e.n) continue;
-    const bool whole = e.wide && base + kAdamBlock <= e.n;
-    // Element j of a lane: four consecutive ones in each half of the block, or single ones 32 apart.
-    auto at = [&](int j) -> uint64_t { return whole ? base + (j >> 2) * 128 + lane * 4 + (j & 3) : base + j * 32 + lane; };
-    float p[8], g[8], m[8], v[8];
-    if (whole) {
+// One block: a whole one that lies in `src`, or the elements that there are, where they lie.  `read` is called once nothing
+// more is read.
+template <int kBits, bool kWhole, typename Read>
+__device__ __forceinline__ void StepBlock(const AdamEntry& e, uint64_t block, const uint8_t* src, const AdamStepScalars& a, float gs,
+                                          uint32_t lane, Read read) {
+  using R = AdamRing<kBits>;
+  const uint64_t base = block * kAdamBlock;
+  [[maybe_unused]] const float m_scale = kBits == 8 ? e.m_scale[block] : 0.0f, v_scale = kBits == 8 ? e.v_scale[block] : 0.0f;
+  // Element j of a lane: four consecutive ones in each half of the block, or single ones 32 apart.
+  auto at = [&](int j) -> uint64_t { return kWhole ? base + (j >> 2) * 128 + lane * 4 + (j & 3) : base + j * 32 + lane; };
+  float p[8], g[8], m[8], v[8];
+  if constexpr (kWhole) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint64_t i = at(4 * h);
-        Load4(e.p, SEE_F32, i, p + 4 * h);
-        Load4(e.g, e.g_type, i, g + 4 * h);
-        if constexpr (kBits == 32) {
-          Load4(e.m, SEE_F32, i, m + 4 * h);
-          Load4(e.v, SEE_F32, i, v + 4 * h);
-        } else {
-          const uint32_t mc = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(e.m) + i);
-          const uint32_t vc = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(e.v) + i);
-          FromE4m3x2(static_cast<uint16_t>(mc), m[4 * h], m[4 * h + 1]);
-          FromE4m3x2(static_cast<uint16_t>(mc >> 16), m[4 * h + 2], m[4 * h + 3]);
-          FromE4m3x2(static_cast<uint16_t>(vc), v[4 * h], v[4 * h + 1]);
-          FromE4m3x2(static_cast<uint16_t>(vc >> 16), v[4 * h + 2], v[4 * h + 3]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint64_t i = at(j);
-        p[j] = g[j] = m[j] = v[j] = 0.0f;
-        if (i < e.n) {
-          p[j] = e.p[i];
-          g[j] = Load1(e.g, e.g_type, i);
-          if constexpr (kBits == 32) {
-            m[j] = static_cast<const float*>(e.m)[i];
-            v[j] = static_cast<const float*>(e.v)[i];
-          } else {
-            float none;
-            FromE4m3x2(static_cast<const uint8_t*>(e.m)[i], m[j], none);
-            FromE4m3x2(static_cast<const uint8_t*>(e.v)[i], v[j], none);
-          }
-        }
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t i = h * 128 + lane * 4;
+      Load4(src, SEE_F32, i, p + 4 * h);
+      Load4(src + R::kG, e.g_type, i, g + 4 * h);
+      if constexpr (kBits == 32) {
+        Load4(src + R::kM, SEE_F32, i, m + 4 * h);
+        Load4(src + R::kV, SEE_F32, i, v + 4 * h);
+      } else {
+        const uint32_t mc = *reinterpret_cast<const uint32_t*>(src + R::kM + i), vc = *reinterpret_cast<const uint32_t*>(src + R::kV + i);
+        FromE4m3x2(static_cast<uint16_t>(mc), m[4 * h], m[4 * h + 1]);
+        FromE4m3x2(static_cast<uint16_t>(mc >> 16), m[4 * h + 2], m[4 * h + 3]);
+        FromE4m3x2(static_cast<uint16_t>(vc), v[4 * h], v[4 * h + 1]);
+        FromE4m3x2(static_cast<uint16_t>(vc >> 16), v[4 * h + 2], v[4 * h + 3]);
       }
     }
-    [[maybe_unused]] const float m_scale = kBits == 8 ? e.m_scale[block] : 0.0f, v_scale = kBits == 8 ? e.v_scale[block] : 0.0f;
-    const float decay = e.decays ? a.weight_decay : 0.0f;
-    [[maybe_unused]] uint32_t m_top = 0, v_top = 0;
+  } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (grad_scale) g[j] *= gs;
-      float size;
-      if constexpr (kBits == 8) {
-        const float root = v[j] * v_scale;
-        m[j] = m[j] * m_scale * a.beta1 + g[j] * a.om_beta1;
-        v[j] = sqrtf(root * root * a.beta2 + g[j] * a.om_beta2 * g[j]);   // from here on the root
-        size = v[j] * a.root_inv_bc2;
-        m_top = max(m_top, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-        v_top = max(v_top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+      const uint64_t i = at(j);
+      p[j] = g[j] = m[j] = v[j] = 0.0f;
+      if (i < e.n) {
+        p[j] = e.p[i];
+        g[j] = Load1(e.g, e.g_type, i);
+        if constexpr (kBits == 32) {
+          m[j] = static_cast<const float*>(e.m)[i];
+          v[j] = static_cast<const float*>(e.v)[i];
+        } else {
+          float none;
+          FromE4m3x2(static_cast<const uint8_t*>(e.m)[i], m[j], none);
+          FromE4m3x2(static_cast<const uint8_t*>(e.v)[i], v[j], none);
+        }
+      }
+    }
+  }
+  read();
+  const float decay = e.decays ? a.weight_decay : 0.0f;
+  [[maybe_unused]] uint32_t mc[4], vc[4];   // two codes each
+  if (gs != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] *= gs;
+  }
+  if constexpr (kBits == 32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = a.beta1 * m[j] + a.om_beta1 * g[j];
+      v[j] = a.beta2 * v[j] + a.om_beta2 * g[j] * g[j];
+      p[j] -= a.lr * (m[j] * a.inv_bc1 / (sqrtf(v[j] * a.inv_bc2) + a.eps) + decay * p[j]);
+    }
+  } else {
+    float m_top = 0.0f, v_top = 0.0f;
+    f32x2 m2[4], v2[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x2 grad = PackF2(g[2 * k], g[2 * k + 1]), root = Mul2(PackF2(v[2 * k], v[2 * k + 1]), Splat2(v_scale));
+      const f32x2 weight = PackF2(p[2 * k], p[2 * k + 1]);
+      m2[k] = AddF2(Mul2(Mul2(PackF2(m[2 * k], m[2 * k + 1]), Splat2(m_scale)), Splat2(a.beta1)), Mul2(grad, Splat2(a.om_beta1)));
+      v2[k] = Root2(AddF2(Mul2(Mul2(root, root), Splat2(a.beta2)), Mul2(Mul2(grad, Splat2(a.om_beta2)), grad)));
+      float size0, size1;
+      UnpackF2(AddF2(Mul2(v2[k], Splat2(a.root_inv_bc2)), Splat2(a.eps)), &size0, &size1);
+      const f32x2 move = Mul2(Mul2(m2[k], Splat2(a.inv_bc1)), PackF2(RcpApprox(size0), RcpApprox(size1)));
+      UnpackF2(Fma2(Fma2(weight, Splat2(decay), move), Splat2(-a.lr), weight), &p[2 * k], &p[2 * k + 1]);
+      m_top = MaxMagnitude(m_top, m2[k]);
+      v_top = MaxMagnitude(v_top, v2[k]);
+    }
+    const BlockScale ms = ScaleOf(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m_top)));
+    const BlockScale vs = ScaleOf(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v_top)));
+    if (lane == 0) {
+      e.m_scale[block] = ms.scale;
+      e.v_scale[block] = vs.scale;
+    }
+    float lowest = 1.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      m2[k] = Mul2(m2[k], Splat2(ms.factor));
+      v2[k] = Mul2(v2[k], Splat2(vs.factor));
+      lowest = MinMagnitude(MinMagnitude(lowest, m2[k]), v2[k]);
+    }
+    const uint32_t word = static_cast<uint32_t>(at(0)) * kGolden + a.phase;
+    auto codes = [&](auto low) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // (how far element j lies behind the lane's first)
+        const uint32_t w0 = word + (kWhole ? (k >> 1) * 128 + (k & 1) * 2 : 64 * k) * kGolden, w1 = w0 + (kWhole ? 1 : 32) * kGolden;
+        mc[k] = ToE4m3x2<low.value>(m2[k], w0, w1);
+        vc[k] = ToE4m3x2<low.value>(v2[k], w0 + kHalfTurn, w1 + kHalfTurn);
+      }
+    };
+    if (lowest >= 0.015625f) {
+      codes(std::false_type{});
+    } else {   // a few blocks in a hundred
+      codes(std::true_type{});
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float x, y;
+        UnpackF2(v2[k], &x, &y);
+        if (x > 0.0f && (vc[k] & 0xFFu) == 0) vc[k] |= 1u;
+        if (y > 0.0f && (vc[k] & 0xFF00u) == 0) vc[k] |= 0x100u;
+      }
+    }
+    if (ms.factor == 0.0f) mc[0] = mc[1] = mc[2] = mc[3] = 0;   // (what is not finite times 0)
+    if (vs.factor == 0.0f) vc[0] = vc[1] = vc[2] = vc[3] = 0;
+  }
+  if constexpr (kWhole) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint64_t i = at(4 * h);
+      const float* q = p + 4 * h;
+      *reinterpret_cast<float4*>(e.p + i) = make_float4(q[0], q[1], q[2], q[3]);
+      if constexpr (kBits == 32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(e.m) + i) = make_float4(m[4 * h], m[4 * h + 1], m[4 * h + 2], m[4 * h + 3]);
+        *reinterpret_cast<float4*>(static_cast<float*>(e.v) + i) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
       } else {
-        m[j] = a.beta1 * m[j] + a.om_beta1 * g[j];
-        v[j] = a.beta2 * v[j] + a.om_beta2 * g[j] * g[j];
-        size = sqrtf(v[j] * a.inv_bc2);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(e.m) + i) = mc[2 * h] | mc[2 * h + 1] << 16;
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(e.v) + i) = vc[2 * h] | vc[2 * h + 1] << 16;
       }
-      p[j] -= a.lr * (m[j] * a.inv_bc1 / (size + a.eps) + decay * p[j]);
-    }
-    uint32_t mc[8], vc[8];
-    if constexpr (kBits == 8) {
-      m_top = __reduce_max_sync(0xFFFFFFFFu, m_top);
-      v_top = __reduce_max_sync(0xFFFFFFFFu, v_top);
-      const BlockScale ms = ScaleOf(m_top), vs = ScaleOf(v_top);
-      if (lane == 0) {
-        e.m_scale[block] = ms.scale;
-        e.v_scale[block] = vs.scale;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t word = static_cast<uint32_t>(at(j)) * kGolden + a.phase;
-        const uint32_t sign = (__float_as_uint(m[j]) >> 31) << 7;
-        mc[j] = ms.factor != 0.0f ? ToE4m3(fabsf(m[j]), ms.factor, word) | (m[j] < 0.0f ? sign : 0u) : 0u;
-        vc[j] = vs.factor != 0.0f ? ToE4m3(v[j], vs.factor, word + kHalfTurn) : 0u;
-        if (vc[j] == 0 && v[j] * vs.factor > 0.0f) vc[j] = 1;
+      if (e.copy_type != SEE_F32) {
+        const bool bf = e.copy_type == SEE_BF16;
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(e.copy) + i) =
+            make_uint2(bf ? Pack2<Bf16>(q[0], q[1]) : Pack2<F16>(q[0], q[1]), bf ? Pack2<Bf16>(q[2], q[3]) : Pack2<F16>(q[2], q[3]));
       }
     }
-    if (whole) {
+  } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint64_t i = at(4 * h);
-        const float* q = p + 4 * h;
-        *reinterpret_cast<float4*>(e.p + i) = make_float4(q[0], q[1], q[2], q[3]);
-        if constexpr (kBits == 32) {
-          *reinterpret_cast<float4*>(static_cast<float*>(e.m) + i) = make_float4(m[4 * h], m[4 * h + 1], m[4 * h + 2], m[4 * h + 3]);
-          *reinterpret_cast<float4*>(static_cast<float*>(e.v) + i) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-        } else {
-          const uint32_t* c = mc + 4 * h;
-          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(e.m) + i) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-          c = vc + 4 * h;
-          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(e.v) + i) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-        }
-        if (e.copy_type != SEE_F32) {
-          const bool bf = e.copy_type == SEE_BF16;
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(e.copy) + i) =
-              make_uint2(bf ? Pack2<Bf16>(q[0], q[1]) : Pack2<F16>(q[0], q[1]), bf ? Pack2<Bf16>(q[2], q[3]) : Pack2<F16>(q[2], q[3]));
-        }
+    for (int j = 0; j < 8; ++j) {
+      const uint64_t i = at(j);
+      if (i >= e.n) continue;
+      e.p[i] = p[j];
+      if constexpr (kBits == 32) {
+        static_cast<float*>(e.m)[i] = m[j];
+        static_cast<float*>(e.v)[i] = v[j];
+      } else {
+        static_cast<uint8_t*>(e.m)[i] = static_cast<uint8_t>(mc[j / 2] >> 8 * (j & 1));
+        static_cast<uint8_t*>(e.v)[i] = static_cast<uint8_t>(vc[j / 2] >> 8 * (j & 1));
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint64_t i = at(j);
-        if (i >= e.n) continue;
-        e.p[i] = p[j];
-        if constexpr (kBits == 32) {
-          static_cast<float*>(e.m)[i] = m[j];
-          static_cast<float*>(e.v)[i] = v[j];
-        } else {
-          static_cast<uint8_t*>(e.m)[i] = static_cast<uint8_t>(mc[j]);
-          static_cast<uint8_t*>(e.v)[i] = static_cast<uint8_t>(vc[j]);
-        }
-        if (e.copy_type == SEE_BF16) static_cast<Bf16*>(e.copy)[i] = FromF32<Bf16>(p[j]);
-        else if (e.copy_type == SEE_F16) static_cast<F16*>(e.copy)[i] = FromF32<F16>(p[j]);
-      }
+      if (e.copy_type == SEE_BF16) static_cast<Bf16*>(e.copy)[i] = FromF32<Bf16>(p[j]);
+      else if (e.copy_type == SEE_F16) static_cast<F16*>(e.copy)[i] = FromF32<F16>(p[j]);
     }
   }
 }
 
 template <int kBits, uint32_t kEntries>
+__global__ void __launch_bounds__(32 * AdamRing<kBits>::kWarps, 1)
+AdamWTensorsKernel(const __grid_constant__ AdamTable<kEntries> table, const AdamStepScalars a, const float* __restrict__ grad_scale,
+                   DeviceStatus* status) {
+  using R = AdamRing<kBits>;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint8_t* ring = dyn + warp * R::kSlots * R::kSlotBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + R::kWarps * R::kSlots * R::kSlotBytes) + warp * R::kSlots;
+  if (lane == 0) {
+    for (uint32_t i = 0; i < R::kSlots; ++i) umma_dev::MbarInit(&bars[i], 1);
+    umma_dev::MbarInitFence();
+  }
+  __syncwarp();
+  AwaitPrevious();
+  // A warp's blocks follow one another; few blocks go to warps of different SMs.
+  const uint32_t blocks = table.block_end[table.count - 1], warps = gridDim.x * R::kWarps, self = warp * gridDim.x + blockIdx.x;
+  const uint32_t each = blocks / warps, rest = blocks % warps;
+  const uint32_t first = self * each + (self < rest ? self : rest), last = first + each + (self < rest ? 1u : 0u);
+  if (first == last) return;
+  AdamCursor<kEntries> now, ahead;
+  now.Find(table, first);
+  ahead = now;
+  auto fill = [&](uint32_t f, uint32_t slot) {   // lane 0; a block that the copies cannot take is read where it lies
+    ahead.MoveTo(table, f);
+    const AdamEntry& e = table.entry[ahead.entry];
+    const uint64_t base = static_cast<uint64_t>(f - ahead.begin) * kAdamBlock;
+    if (!e.wide || base + kAdamBlock > e.n) return;
+    uint8_t* dst = ring + slot * R::kSlotBytes;
+    const uint32_t g_bytes = kAdamBlock * (e.g_type == SEE_F32 ? 4 : 2);
+    umma_dev::MbarExpectTx(&bars[slot], R::kG + g_bytes);
+    umma_dev::BulkLoad(dst, e.p + base, kAdamBlock * 4, &bars[slot]);
+    umma_dev::BulkLoad(dst + R::kM, static_cast<const uint8_t*>(e.m) + base * (kBits / 8), R::kStateBytes, &bars[slot]);
+    umma_dev::BulkLoad(dst + R::kV, static_cast<const uint8_t*>(e.v) + base * (kBits / 8), R::kStateBytes, &bars[slot]);
+    umma_dev::BulkLoad(dst + R::kG, static_cast<const uint8_t*>(e.g) + base * (g_bytes / kAdamBlock), g_bytes, &bars[slot]);
+  };
+  if (lane == 0)
+    for (uint32_t i = 0; i < R::kSlots && first + i < last; ++i) fill(first + i, i);
+  const float gs = grad_scale ? *grad_scale : 1.0f;
+  uint32_t slot = 0, parities = 0;   // a bit for each slot
+  for (uint32_t f = first; f < last; ++f) {
+    now.MoveTo(table, f);
+    const AdamEntry& e = table.entry[now.entry];
+    const uint64_t block = f - now.begin, base = block * kAdamBlock;
+    const bool whole = e.wide && base + kAdamBlock <= e.n;
+    if (whole) {
+      if (!umma_dev::MbarWait(&bars[slot], parities >> slot & 1u)) {   // (the copies always land; but no wait is without end)
+        status->wait_timeout = 1;
+        umma_dev::DrainDelay();
+      }
+      parities ^= 1u << slot;
+    }
+    auto read = [&] {   // the slot may be filled again
+      __syncwarp();
+      if (lane == 0 && f + R::kSlots < last) fill(f + R::kSlots, slot);
+    };
+    if (whole) StepBlock<kBits, true>(e, block, ring + slot * R::kSlotBytes, a, gs, lane, read);
+    else StepBlock<kBits, false>(e, block, nullptr, a, gs, lane, read);
+    slot = slot + 1 < R::kSlots ? slot + 1 : 0;
+  }
+}
+
+template <int kBits, uint32_t kEntries>
 cudaError_t Launch(const see_adamw_tensor* tensors, uint64_t count, const AdamStepScalars& a, const float* grad_scale, uint32_t sms,
-                   cudaStream_t s, int* launches) {
-  constexpr uint64_t kChunk = static_cast<uint64_t>(kAdamBlock) * kAdamWarps;
+                   DeviceStatus* status, cudaStream_t s, int* launches) {
+  using R = AdamRing<kBits>;
+  auto* kernel = AdamWTensorsKernel<kBits, kEntries>;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes); e != cudaSuccess) return e;
   AdamTable<kEntries> table;
   uint64_t next = 0;
   while (next < count) {
     table.count = 0;
-    uint64_t chunks = 0;
+    uint64_t blocks = 0;
     for (; next < count && table.count < kEntries; ++next) {
       const see_adamw_tensor& t = tensors[next];
       if (t.n == 0) continue;
-      const uint64_t more = (t.n + kChunk - 1) / kChunk;
-      if (table.count && chunks + more > 0xFFFFFFFFull) break;
-      auto aligned = [](const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; };
+      const uint64_t more = (t.n + kAdamBlock - 1) / kAdamBlock;
+      if (blocks + more > 0xFFFFFFFFull) break;   // (one tensor alone has fewer)
+      auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
       AdamEntry& e = table.entry[table.count];
       e = {t.p, t.g, t.m, t.v, t.m_scale, t.v_scale, t.copy, t.n, static_cast<uint8_t>(t.g_type), static_cast<uint8_t>(t.copy_type),
            static_cast<uint8_t>((t.flags & SEE_ADAMW_NO_DECAY) == 0), 0};
-      e.wide = aligned(t.p, 16) && aligned(t.g, t.g_type == SEE_F32 ? 16 : 8) && aligned(t.m, kBits == 32 ? 16 : 4) &&
-               aligned(t.v, kBits == 32 ? 16 : 4) && (t.copy_type == SEE_F32 || aligned(t.copy, 8));
-      chunks += more;
-      table.chunk_end[table.count++] = static_cast<uint32_t>(chunks);
+      e.wide = aligned(t.p) && aligned(t.g) && aligned(t.m) && aligned(t.v) && aligned(t.copy);
+      blocks += more;
+      table.block_end[table.count++] = static_cast<uint32_t>(blocks);
     }
     if (!table.count) break;
-    const uint64_t most = static_cast<uint64_t>(sms) * 8;
-    if (cudaError_t e = Next(AdamWTensorsKernel<kBits, kEntries>, static_cast<unsigned>(chunks < most ? chunks : most), 32 * kAdamWarps, 0,
-                             s)(table, a, grad_scale);
+    if (cudaError_t e = Next(kernel, static_cast<unsigned>(blocks < sms ? blocks : sms), 32 * R::kWarps, R::kBytes, s)(table, a, grad_scale, status);
         e != cudaSuccess)
       return e;
     ++*launches;
@@ -266,9 +412,9 @@ cudaError_t Launch(const see_adamw_tensor* tensors, uint64_t count, const AdamSt
 }  // namespace
 
 cudaError_t AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const AdamStepScalars& a,
-                         const float* grad_scale, uint32_t sms, cudaStream_t s, int* launches) {
-  return state_bits == 8 ? Launch<8, 48>(tensors, count, a, grad_scale, sms, s, launches)
-                         : Launch<32, 48>(tensors, count, a, grad_scale, sms, s, launches);
+                         const float* grad_scale, uint32_t sms, DeviceStatus* status, cudaStream_t s, int* launches) {
+  return state_bits == 8 ? Launch<8, 192>(tensors, count, a, grad_scale, sms, status, s, launches)
+                         : Launch<32, 192>(tensors, count, a, grad_scale, sms, status, s, launches);
 }
 
 }  // namespace see::k

@@ -149,11 +149,6 @@ template <typename T> __device__ __forceinline__ void StorePairs(T* p, const f32
 // Each group has `slots` of its own, filled by one thread's bulk copies (a whole row each, counted on the slot's mbarrier)
 // and emptied into registers; a slot is asked to be filled again as soon as the group has read it, so that between 60 and
 // 200 KB are on their way to an SM at any time.
-__device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(umma_dev::SmemAddr(dst)), "l"(src), "r"(bytes), "r"(umma_dev::SmemAddr(bar))
-               : "memory");
-}
 __device__ __forceinline__ void GroupBarrier(uint32_t T, uint32_t group) {
   if (T == 32) __syncwarp();
   else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(T) : "memory");
@@ -185,9 +180,9 @@ NormBwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots
   auto fill = [&](uint64_t row, uint32_t slot) {   // the group's thread 0
     uint8_t* dst = ring + static_cast<size_t>(slot) * slot_bytes;
     umma_dev::MbarExpectTx(&bars[slot], slot_bytes);
-    BulkLoad(dst, static_cast<const XT*>(a.x) + row * a.x_stride, x_bytes, &bars[slot]);
-    BulkLoad(dst + x_bytes, static_cast<const YT*>(a.dy) + row * a.y_stride, y_bytes, &bars[slot]);
-    if (a.addend) BulkLoad(dst + x_bytes + y_bytes, static_cast<const XT*>(a.addend) + row * a.x_stride, x_bytes, &bars[slot]);
+    umma_dev::BulkLoad(dst, static_cast<const XT*>(a.x) + row * a.x_stride, x_bytes, &bars[slot]);
+    umma_dev::BulkLoad(dst + x_bytes, static_cast<const YT*>(a.dy) + row * a.y_stride, y_bytes, &bars[slot]);
+    if (a.addend) umma_dev::BulkLoad(dst + x_bytes + y_bytes, static_cast<const XT*>(a.addend) + row * a.x_stride, x_bytes, &bars[slot]);
   };
   AwaitPrevious();
   if (t == 0)

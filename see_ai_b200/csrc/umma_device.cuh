@@ -91,6 +91,12 @@ __device__ __forceinline__ void TmaLoad4D(void* smem_dst, const CUtensorMap* map
       "r"(y), "r"(z), "r"(w)
       : "memory");
 }
+// `bytes` in a row (a multiple of 16, as both addresses are).
+__device__ __forceinline__ void BulkLoad(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(SmemAddr(smem_dst)), "l"(src), "r"(bytes), "r"(SmemAddr(bar))
+               : "memory");
+}
 // Tile store shared -> global; rows/columns outside the tensor are clipped.
 __device__ __forceinline__ void TmaStore2D(const CUtensorMap* map, const void* smem_src, int32_t x,
                                            int32_t y) {
