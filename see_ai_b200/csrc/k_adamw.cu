@@ -151,14 +151,15 @@ __device__ __forceinline__ f32x2 Root2(f32x2 v) {
   return Fma2(Fma2(Mul2(s, Splat2(-1.0f)), s, v), Mul2(y, Splat2(0.5f)), s);
 }
 
-// The largest magnitude's block scale: 0 where it is below 2^-100, NaN where it is not finite (one such element makes the
-// block's moments NaN: eight bits hold none).
+// The largest magnitude's block scale: 0 where it is below 2^-100, NaN from 2^126 on (a moment that is not finite makes its
+// block's NaN: eight bits hold none).
 struct BlockScale { float factor, scale; };
 __device__ __forceinline__ BlockScale ScaleOf(uint32_t largest_bits) {
   const float largest = __uint_as_float(largest_bits);
-  if (largest_bits >= 0x7F800000u) return {0.0f, __uint_as_float(0x7FC00000u)};
+  if (largest_bits >= 0x7E800000u) return {0.0f, __uint_as_float(0x7FC00000u)};
   if (largest < 7.888609052210118e-31f) return {0.0f, 0.0f};
-  return {1.0f / largest * 448.0f, largest * (1.0f / 448.0f)};
+  const float r = RcpApprox(largest);   // a Newton step makes 1 / largest of it
+  return {__fmaf_rn(__fmaf_rn(-largest, r, 1.0f), r, r) * 448.0f, largest * (1.0f / 448.0f)};
 }
 
 // One block: a whole one that lies in `src`, or the elements that there are, where they lie.  `read` is called once nothing
@@ -227,28 +228,33 @@ __device__ __forceinline__ void StepBlock(const AdamEntry& e, uint64_t block, co
     f32x2 m2[4], v2[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const f32x2 grad = PackF2(g[2 * k], g[2 * k + 1]), root = Mul2(PackF2(v[2 * k], v[2 * k + 1]), Splat2(v_scale));
+      // (One by one: a packed product and the packed sum behind it come out as one operation, and these have two roundings.)
+      float m1[2], v1[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float grad = g[2 * k + j], root = v[2 * k + j] * v_scale;
+        m1[j] = m[2 * k + j] * m_scale * a.beta1 + grad * a.om_beta1;
+        v1[j] = root * root * a.beta2 + grad * a.om_beta2 * grad;
+      }
       const f32x2 weight = PackF2(p[2 * k], p[2 * k + 1]);
-      m2[k] = AddF2(Mul2(Mul2(PackF2(m[2 * k], m[2 * k + 1]), Splat2(m_scale)), Splat2(a.beta1)), Mul2(grad, Splat2(a.om_beta1)));
-      v2[k] = Root2(AddF2(Mul2(Mul2(root, root), Splat2(a.beta2)), Mul2(Mul2(grad, Splat2(a.om_beta2)), grad)));
+      m2[k] = PackF2(m1[0], m1[1]);
+      v2[k] = Root2(PackF2(v1[0], v1[1]));
       float size0, size1;
-      UnpackF2(AddF2(Mul2(v2[k], Splat2(a.root_inv_bc2)), Splat2(a.eps)), &size0, &size1);
+      UnpackF2(Fma2(v2[k], Splat2(a.root_inv_bc2), Splat2(a.eps)), &size0, &size1);
       const f32x2 move = Mul2(Mul2(m2[k], Splat2(a.inv_bc1)), PackF2(RcpApprox(size0), RcpApprox(size1)));
       UnpackF2(Fma2(Fma2(weight, Splat2(decay), move), Splat2(-a.lr), weight), &p[2 * k], &p[2 * k + 1]);
       m_top = MaxMagnitude(m_top, m2[k]);
       v_top = MaxMagnitude(v_top, v2[k]);
     }
-    const BlockScale ms = ScaleOf(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m_top)));
-    const BlockScale vs = ScaleOf(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v_top)));
-    if (lane == 0) {
-      e.m_scale[block] = ms.scale;
-      e.v_scale[block] = vs.scale;
-    }
+    const uint32_t m_bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m_top)), v_bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v_top));
+    const BlockScale mine = ScaleOf(lane & 1 ? v_bits : m_bits);   // (one division for both)
+    const float m_factor = __shfl_sync(0xFFFFFFFFu, mine.factor, 0), v_factor = __shfl_sync(0xFFFFFFFFu, mine.factor, 1);
+    if (lane < 2) (lane ? e.v_scale : e.m_scale)[block] = mine.scale;
     float lowest = 1.0f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      m2[k] = Mul2(m2[k], Splat2(ms.factor));
-      v2[k] = Mul2(v2[k], Splat2(vs.factor));
+      m2[k] = Mul2(m2[k], Splat2(m_factor));
+      v2[k] = Mul2(v2[k], Splat2(v_factor));
       lowest = MinMagnitude(MinMagnitude(lowest, m2[k]), v2[k]);
     }
     const uint32_t word = static_cast<uint32_t>(at(0)) * kGolden + a.phase;
@@ -273,8 +279,8 @@ __device__ __forceinline__ void StepBlock(const AdamEntry& e, uint64_t block, co
         if (y > 0.0f && (vc[k] & 0xFF00u) == 0) vc[k] |= 0x100u;
       }
     }
-    if (ms.factor == 0.0f) mc[0] = mc[1] = mc[2] = mc[3] = 0;   // (what is not finite times 0)
-    if (vs.factor == 0.0f) vc[0] = vc[1] = vc[2] = vc[3] = 0;
+    if (m_factor == 0.0f) mc[0] = mc[1] = mc[2] = mc[3] = 0;   // (what is not finite times 0)
+    if (v_factor == 0.0f) vc[0] = vc[1] = vc[2] = vc[3] = 0;
   }
   if constexpr (kWhole) {
 #pragma unroll
@@ -337,21 +343,32 @@ AdamWTensorsKernel(const __grid_constant__ AdamTable<kEntries> table, const Adam
   AdamCursor<kEntries> now, ahead;
   now.Find(table, first);
   ahead = now;
-  auto fill = [&](uint32_t f, uint32_t slot) {   // lane 0; a block that the copies cannot take is read where it lies
-    ahead.MoveTo(table, f);
+  // Lanes 0 to 3 fill a slot with p, m, v and g: each keeps where its operand of the current tensor lies, so that a fill is a
+  // handful of instructions of the warp.  A block that the copies cannot take is read where it lies.
+  const uint8_t* source = nullptr;
+  uint32_t bytes = 0, total = 0, offset = 0, fillable = 0;   // of a block of mine, of all four; in the slot; whole blocks
+  auto look_up = [&] {
     const AdamEntry& e = table.entry[ahead.entry];
-    const uint64_t base = static_cast<uint64_t>(f - ahead.begin) * kAdamBlock;
-    if (!e.wide || base + kAdamBlock > e.n) return;
-    uint8_t* dst = ring + slot * R::kSlotBytes;
     const uint32_t g_bytes = kAdamBlock * (e.g_type == SEE_F32 ? 4 : 2);
-    umma_dev::MbarExpectTx(&bars[slot], R::kG + g_bytes);
-    umma_dev::BulkLoad(dst, e.p + base, kAdamBlock * 4, &bars[slot]);
-    umma_dev::BulkLoad(dst + R::kM, static_cast<const uint8_t*>(e.m) + base * (kBits / 8), R::kStateBytes, &bars[slot]);
-    umma_dev::BulkLoad(dst + R::kV, static_cast<const uint8_t*>(e.v) + base * (kBits / 8), R::kStateBytes, &bars[slot]);
-    umma_dev::BulkLoad(dst + R::kG, static_cast<const uint8_t*>(e.g) + base * (g_bytes / kAdamBlock), g_bytes, &bars[slot]);
+    const void* mine = lane == 0 ? static_cast<const void*>(e.p) : lane == 1 ? e.m : lane == 2 ? e.v : e.g;
+    source = static_cast<const uint8_t*>(mine);
+    bytes = lane == 0 ? kAdamBlock * 4 : lane < 3 ? R::kStateBytes : g_bytes;
+    offset = lane == 0 ? 0 : lane == 1 ? R::kM : lane == 2 ? R::kV : R::kG;
+    total = R::kG + g_bytes;
+    fillable = e.wide ? static_cast<uint32_t>(e.n / kAdamBlock) : 0;
   };
-  if (lane == 0)
-    for (uint32_t i = 0; i < R::kSlots && first + i < last; ++i) fill(first + i, i);
+  look_up();
+  auto fill = [&](uint32_t f, uint32_t slot) {
+    if (f >= ahead.end) {
+      ahead.MoveTo(table, f);
+      look_up();
+    }
+    const uint32_t block = f - ahead.begin;
+    if (block >= fillable) return;
+    if (lane == 0) umma_dev::MbarExpectTx(&bars[slot], total);
+    if (lane < 4) umma_dev::BulkLoad(ring + slot * R::kSlotBytes + offset, source + static_cast<uint64_t>(block) * bytes, bytes, &bars[slot]);
+  };
+  for (uint32_t i = 0; i < R::kSlots && first + i < last; ++i) fill(first + i, i);
   const float gs = grad_scale ? *grad_scale : 1.0f;
   uint32_t slot = 0, parities = 0;   // a bit for each slot
   for (uint32_t f = first; f < last; ++f) {
@@ -368,7 +385,7 @@ AdamWTensorsKernel(const __grid_constant__ AdamTable<kEntries> table, const Adam
     }
     auto read = [&] {   // the slot may be filled again
       __syncwarp();
-      if (lane == 0 && f + R::kSlots < last) fill(f + R::kSlots, slot);
+      if (f + R::kSlots < last) fill(f + R::kSlots, slot);
     };
     if (whole) StepBlock<kBits, true>(e, block, ring + slot * R::kSlotBytes, a, gs, lane, read);
     else StepBlock<kBits, false>(e, block, nullptr, a, gs, lane, read);
