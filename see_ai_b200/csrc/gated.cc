@@ -53,19 +53,98 @@ Status CheckGated(const std::string& what, see_gated_shape* s) {
 
 uint64_t SlopeBytes(uint64_t rows, uint64_t d_hidden) { return (rows * d_hidden * 2 + 127) / 128 * 128; }
 
-// Width of a pair's accumulator: 256 columns do a third more arithmetic per operand byte, 128 leave fewer pairs idle in the
-// last round.
-uint32_t TileWidth(const uint64_t (&tiles)[2], uint32_t sms) {
-  const uint64_t pairs = std::max<uint64_t>(1, sms / 2);
-  const double wide = static_cast<double>((tiles[0] + pairs - 1) / pairs), narrow = 0.6 * static_cast<double>((tiles[1] + pairs - 1) / pairs);
-  return wide <= narrow ? 256 : 128;
+// The backward pass's problems on `pairs` CTA pairs, which take the tiles, then the parts of cut ones, in turn.  A tile's
+// reduction is cut into parts of up to `length` blocks where that ends the launch sooner: the tiles of the last, unfull round;
+// or all of dx's (few rows leave it few tiles with the longest reduction); or all.  By estimate, in blocks (about 0.28 us): a
+// tile costs two besides its own, a part five, for its sums' way to memory, the fold eight and a third for each part.
+// 4096 x 768 x 2048 59 us / 54; 16 rows of it 25 / 15; 600 x 512 x 1376 21 / 16.
+constexpr uint32_t kMostPairs = 74, kMostParts = 2 * kMostPairs;
+struct Cut { uint32_t whole, parts, first_part; };
+struct BackwardPlan {
+  Cut cut[k::kGatedProblems] = {};
+  uint32_t parts = 0;   // in all
+};
+struct Run { uint64_t count; double cost; };
+// The time of the pair that ends last.
+double Longest(const Run* runs, uint32_t count, uint32_t pairs) {
+  double longest = 0.0;
+  uint64_t at[2 * 2 * k::kGatedProblems], first = 0;
+  for (uint32_t r = 0; r < count; first += runs[r++].count) {
+    at[2 * r] = first % pairs;
+    at[2 * r + 1] = (first + runs[r].count + pairs - 1) % pairs;
+  }
+  for (uint32_t i = 0; i < 2 * count; ++i) {   // the time of a pair changes only where a run begins or ends
+    double time = 0.0;
+    first = 0;
+    for (uint32_t r = 0; r < count; first += runs[r++].count) {
+      const uint64_t behind = (at[i] + pairs - first % pairs) % pairs;
+      if (behind < runs[r].count) time += static_cast<double>((runs[r].count - behind + pairs - 1) / pairs) * runs[r].cost;
+    }
+    longest = std::max(longest, time);
+  }
+  return longest;
 }
+BackwardPlan PlanCuts(const uint64_t* tiles, const uint64_t* blocks, uint32_t count, uint32_t pairs) {
+  uint64_t total = 0, longest = 0;
+  for (uint32_t i = 0; i < count; ++i) {
+    total += tiles[i];
+    longest = std::max(longest, blocks[i]);
+  }
+  BackwardPlan best;
+  double best_time = 1e300;
+  enum { kLastRound, kFirst, kAll };
+  for (int which : {kLastRound, kFirst, kAll})
+    for (uint64_t cuts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      const uint64_t length = (longest + cuts - 1) / cuts;
+      if (cuts > 1 && length < 6) break;
+      BackwardPlan plan;
+      Run runs[2 * k::kGatedProblems];
+      uint64_t full = which == kLastRound ? total / pairs * pairs : 0, parts = 0;
+      for (uint32_t i = 0; i < count; ++i) {
+        uint64_t whole = which == kLastRound ? std::min(tiles[i], full) : which == kFirst && i > 0 ? tiles[i] : 0;
+        full -= std::min(full, whole);
+        const uint64_t each = (blocks[i] + length - 1) / length;
+        if (each <= 1) whole = tiles[i];
+        plan.cut[i] = {static_cast<uint32_t>(whole), static_cast<uint32_t>(std::max<uint64_t>(1, each)), static_cast<uint32_t>(std::min<uint64_t>(parts, kMostParts))};
+        runs[i] = {whole, static_cast<double>(blocks[i]) + 2.0};
+        runs[count + i] = {(tiles[i] - whole) * each, static_cast<double>(blocks[i]) / static_cast<double>(std::max<uint64_t>(1, each)) + 5.0};
+        parts += runs[count + i].count;
+      }
+      if (parts > kMostParts) continue;
+      plan.parts = static_cast<uint32_t>(parts);
+      const double time = Longest(runs, 2 * count, pairs) + (parts ? 8.0 + 0.3 * static_cast<double>(parts) : 0.0);
+      if (time < best_time) {
+        best_time = time;
+        best = plan;
+      }
+    }
+  return best;
+}
+// All that a backward pass over these sizes may ask for.
+BackwardPlan PlanBackward(uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool dx, bool dw, uint32_t pairs) {
+  uint64_t tiles[3], blocks[3];
+  uint32_t count = 0;
+  if (dx) {
+    tiles[count] = static_cast<uint64_t>(Up(rows, 256)) * Up(d_in, 256);
+    blocks[count++] = 2ull * Up(d_hidden, 64);
+  }
+  for (int which = 0; which < 2 && dw; ++which) {
+    tiles[count] = static_cast<uint64_t>(Up(d_in, 256)) * Up(d_hidden, 256);
+    blocks[count++] = Up(rows, 64);
+  }
+  return PlanCuts(tiles, blocks, count, pairs);
+}
+uint64_t PartialBytes(const BackwardPlan& plan) { return plan.parts * 256ull * 256 * 4; }
 
 }  // namespace
 
 uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden) {
   if (d_in == 0 || d_hidden == 0 || d_in % 8 || d_hidden % 8 || d_in > (1u << 20) || d_hidden > (1u << 20) || rows > 0x7FFFFF00ull) return 0;
-  return std::max<uint64_t>(128, 2 * SlopeBytes(rows, d_hidden));
+  if (rows == 0) return 128;
+  uint64_t partials = 0;   // whichever gradients are wanted, on however few SMs
+  for (int want = 1; want < 4; ++want)
+    partials = std::max(partials, PartialBytes(PlanBackward(rows, d_in, d_hidden, want & 1, want & 2, kMostPairs)));
+  return 2 * SlopeBytes(rows, d_hidden) + partials;
 }
 
 Status CheckGatedForward(see_gated_shape* shape, const void* x, const void* w_gate, const void* w_up, const void* hidden, const void* gate,
@@ -122,8 +201,9 @@ Status CudaBackend::GatedForward(const see_gated_shape& given, const void* x, co
   const bool f16 = s.type == SEE_F16;
   k::GatedLaunch l = {};
   k::GatedProblem& p = l.p[0];
-  const uint64_t tiles[2] = {static_cast<uint64_t>(Up(s.rows, 256)) * Up(s.d_hidden, 128), static_cast<uint64_t>(Up(s.rows, 256)) * Up(s.d_hidden, 64)};
-  const uint32_t tn = TileWidth(tiles, sms_);
+  // A pair's accumulator of 128 columns instead of 256 costs nearly as much a block of the reduction (A is read as often), so
+  // it pays only where one round takes the twice as many tiles (600 x 512 x 1376: 7.7 us / 7.1; 4096 x 768 x 2048: 24.4 / 30.6).
+  const uint32_t tn = static_cast<uint64_t>(Up(s.rows, 256)) * Up(s.d_hidden, 64) <= sms_ / 2 ? 128 : 256;
   bool ok = MapOf(&p.a[0], f16, x, s.rows, s.d_in, s.x_stride, 64) && MapOf(&p.b[0], f16, w_gate, s.d_in, s.d_hidden, s.d_hidden, 64) &&
             MapOf(&p.b[1], f16, w_up, s.d_in, s.d_hidden, s.d_hidden, 64) && MapOf(&p.c, f16, hidden, s.rows, s.d_hidden, s.hidden_stride, 32);
   if (gate)
@@ -135,6 +215,8 @@ Status CudaBackend::GatedForward(const see_gated_shape& given, const void* x, co
   p.b_mn = 1;
   p.tiles_m = Up(s.rows, 256);
   p.tiles_n = Up(s.d_hidden, tn / 2);
+  p.whole = p.tiles_m * p.tiles_n;
+  p.parts = 1;
   l.count = 1;
   l.f16 = f16;
   l.act = s.act;
@@ -167,39 +249,50 @@ Status CudaBackend::GatedBackward(const see_gated_shape& given, const void* dhid
   l.f16 = f16;
   l.status = d_status_;
   const uint32_t rows = static_cast<uint32_t>(s.rows), d_in = static_cast<uint32_t>(s.d_in), d_hidden = static_cast<uint32_t>(s.d_hidden);
-  uint64_t tiles[2] = {0, 0};
-  auto problem = [&](uint32_t M, uint32_t N) -> k::GatedProblem& {
+  const uint32_t pairs = std::min(sms_ / 2, kMostPairs);
+  const BackwardPlan plan = PlanBackward(s.rows, s.d_in, s.d_hidden, dx != nullptr, dw_gate != nullptr, pairs);
+  if (2 * SlopeBytes(s.rows, s.d_hidden) + PartialBytes(plan) > workspace_bytes)   // (the query has counted for the most SMs there are)
+    return std::unexpected("cuda: gated backward: the workspace is too small");
+  l.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 2 * SlopeBytes(s.rows, s.d_hidden));
+  auto problem = [&](uint32_t M, uint32_t N, void* out, uint64_t out_stride) -> k::GatedProblem& {
+    const Cut& cut = plan.cut[l.count];
     k::GatedProblem& p = l.p[l.count++];
     p.M = M;
     p.N = N;
     p.tiles_m = Up(M, 256);
-    tiles[0] += static_cast<uint64_t>(p.tiles_m) * Up(N, 256);
-    tiles[1] += static_cast<uint64_t>(p.tiles_m) * Up(N, 128);
+    p.tiles_n = Up(N, 256);
+    p.whole = cut.whole;
+    p.parts = cut.parts;
+    p.first_part = cut.first_part;
+    p.out = out;
+    p.out_stride = out_stride;
     return p;
   };
   bool ok = true;
   if (dx) {   // A: dg, then du, along their rows; B: the weights' rows are dx's columns
-    k::GatedProblem& p = problem(rows, d_in);
+    k::GatedProblem& p = problem(rows, d_in, dx, s.x_stride);
     p.blocks[0] = p.blocks[1] = Up(d_hidden, 64);
     ok = MapOf(&p.a[0], f16, dg, rows, d_hidden, d_hidden, 64) && MapOf(&p.a[1], f16, du, rows, d_hidden, d_hidden, 64) &&
          MapOf(&p.b[0], f16, w_gate, d_in, d_hidden, d_hidden, 64) && MapOf(&p.b[1], f16, w_up, d_in, d_hidden, d_hidden, 64) &&
          MapOf(&p.c, f16, dx, rows, d_in, s.x_stride, 32);
   }
   for (int which = 0; which < 2 && dw_gate && ok; ++which) {   // both operands down their columns
-    k::GatedProblem& p = problem(d_in, d_hidden);
+    k::GatedProblem& p = problem(d_in, d_hidden, which ? dw_up : dw_gate, d_hidden);
     p.a_mn = p.b_mn = 1;
     p.blocks[0] = Up(rows, 64);
     ok = MapOf(&p.a[0], f16, x, rows, d_in, s.x_stride, 64) && MapOf(&p.b[0], f16, which ? du : dg, rows, d_hidden, d_hidden, 64) &&
          MapOf(&p.c, f16, which ? dw_up : dw_gate, d_in, d_hidden, d_hidden, 32);
   }
   if (!ok) return std::unexpected("cuda: gated backward: cuTensorMapEncodeTiled refused an operand layout");
-  const uint32_t tn = TileWidth(tiles, sms_);
-  for (uint32_t i = 0; i < l.count; ++i) l.p[i].tiles_n = Up(l.p[i].N, tn);
   if (auto r = Check(k::GatedSlopes(dhidden, gate, up, dg, du, s.rows, d_hidden, s.hidden_stride, s.act, f16, sms_, stream_), "gated backward"); !r)
     return r;
   ++counters_.kernel_launches;
-  if (auto r = Check(k::GatedProducts(l, false, tn, sms_, stream_), "gated backward"); !r) return r;
+  if (auto r = Check(k::GatedProducts(l, false, 256, 2 * pairs, stream_), "gated backward"); !r) return r;
   ++counters_.kernel_launches;
+  if (plan.parts) {
+    if (auto r = Check(k::GatedFold(l, 256, stream_), "gated backward"); !r) return r;
+    ++counters_.kernel_launches;
+  }
   return {};
 }
 

@@ -21,6 +21,11 @@ struct GatedProblem {
   uint32_t blocks[2];        // of 64 along the reduction, for each operand pair (the second may have none)
   uint32_t a_mn, b_mn;       // 1: MN-major
   uint32_t tiles_m, tiles_n;
+  // Tiles from `whole` on (in the kernel's order) have their reduction cut into `parts`, each its own work: its f32 sums go to
+  // partials, part by part from `first_part` on, and GatedFold adds them.  whole = all tiles: none.
+  uint32_t whole, parts, first_part;
+  void* out;                 // what c maps, for the fold
+  uint64_t out_stride;
 };
 constexpr uint32_t kGatedProblems = 3;
 struct GatedLaunch {
@@ -30,10 +35,14 @@ struct GatedLaunch {
   uint32_t f16;              // operands and outputs: 1 f16, 0 bf16
   int act;
   uint32_t keep;             // gated: gate and up leave too
+  float* partials;           // [part][256 x tn]
   DeviceStatus* status;
 };
-// tn: columns of a pair's accumulator, 256 or 128 (gated: half of them the gate's, half the up projection's).
+// tn: columns of a pair's accumulator, 256, or gated also 128 (half of them the gate's, half the up projection's).
 cudaError_t GatedProducts(const GatedLaunch& l, bool gated, uint32_t tn, uint32_t sms, cudaStream_t s);
+
+// The cut tiles' parts added in order, rounded and stored.
+cudaError_t GatedFold(const GatedLaunch& l, uint32_t tn, cudaStream_t s);
 
 // dg = dh u act'(g), du = dh act(g): rows of `cols` elements (a multiple of 8); dh, g, u `stride` apart, dg, du dense.
 cudaError_t GatedSlopes(const void* dh, const void* g, const void* u, void* dg, void* du, uint64_t rows, uint32_t cols, uint64_t stride,

@@ -32,7 +32,7 @@ constexpr uint32_t kBoxBytes = 64 * 64 * 2;
 constexpr uint32_t kEpiWarps = 8;
 constexpr uint32_t kThreads = 64 + 32 * kEpiWarps;   // warp 0 TMA, warp 1 MMA, then the epilogue warps
 constexpr uint32_t kSlabBytes = 32 * 128;  // 32 rows of 64 16-bit columns
-constexpr uint32_t kSlabs = 2;             // to an epilogue warp
+constexpr uint32_t kSlabs = 1;             // to an epilogue warp
 constexpr uint32_t kBand = 8;              // row tiles that share a column tile's B before the next column tile
 
 template <uint32_t kTN>
@@ -40,7 +40,7 @@ struct Tile {
   static constexpr uint32_t kHalf = kTN / 2;                             // columns of B a CTA loads
   static constexpr uint32_t kABytes = kRows * kBlockK * 2, kBBytes = kHalf * kBlockK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  static constexpr uint32_t kStages = kTN == 256 ? 5 : 6;
+  static constexpr uint32_t kStages = kTN == 256 ? 6 : 8;
   static constexpr uint32_t kSmem = kStages * kStageBytes + kEpiWarps * kSlabs * kSlabBytes + 256 + 1024;
 };
 
@@ -58,18 +58,45 @@ __device__ __forceinline__ bool Wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
-struct At { uint32_t p, m_tile, n_tile; };
+// A work item: a tile, or part `part` of `parts` of its reduction (blocks from, to).  Whole tiles come first.
+struct At { uint32_t p, m_tile, n_tile, part, parts, from, to; };
+__device__ __forceinline__ void TileAt(const GatedProblem& p, uint32_t t, uint32_t& m_tile, uint32_t& n_tile) {
+  const uint32_t per_band = kBand * p.tiles_n, band = t / per_band, within = t - band * per_band, first = band * kBand;
+  const uint32_t height = p.tiles_m - first < kBand ? p.tiles_m - first : kBand;
+  n_tile = within / height;
+  m_tile = first + within - n_tile * height;
+}
 __device__ __forceinline__ At Locate(const GatedLaunch& l, uint32_t t) {
-  uint32_t p = 0;
-  while (p + 1 < l.count && t >= l.p[p].tiles_m * l.p[p].tiles_n) {
-    t -= l.p[p].tiles_m * l.p[p].tiles_n;
-    ++p;
+  At at;
+  at.part = 0;
+  at.parts = 1;
+  at.p = 0;
+  while (at.p < l.count && t >= l.p[at.p].whole) t -= l.p[at.p++].whole;
+  if (at.p == l.count) {   // among the parts
+    at.p = 0;
+    while (true) {
+      const GatedProblem& p = l.p[at.p];
+      const uint32_t items = (p.tiles_m * p.tiles_n - p.whole) * p.parts;
+      if (at.p + 1 == l.count || t < items) break;
+      t -= items;
+      ++at.p;
+    }
+    at.parts = l.p[at.p].parts;
+    at.part = t % at.parts;
+    t = l.p[at.p].whole + t / at.parts;
   }
-  const uint32_t tiles_m = l.p[p].tiles_m, per_band = kBand * l.p[p].tiles_n;
-  const uint32_t band = t / per_band, within = t - band * per_band, first = band * kBand;
-  const uint32_t height = tiles_m - first < kBand ? tiles_m - first : kBand;
-  const uint32_t n = within / height;
-  return {p, first + within - n * height, n};
+  const GatedProblem& p = l.p[at.p];
+  TileAt(p, t, at.m_tile, at.n_tile);
+  const uint32_t blocks = p.blocks[0] + p.blocks[1];
+  at.from = static_cast<uint32_t>(static_cast<uint64_t>(blocks) * at.part / at.parts);
+  at.to = static_cast<uint32_t>(static_cast<uint64_t>(blocks) * (at.part + 1) / at.parts);
+  if (at.parts > 1) at.part += p.first_part + (t - p.whole) * at.parts;   // from here on its place among all parts
+  return at;
+}
+__host__ __device__ inline uint32_t Items(const GatedLaunch& l) {
+  uint32_t n = 0;
+  for (uint32_t p = 0; p < l.count; ++p) n += l.p[p].whole + (l.p[p].tiles_m * l.p[p].tiles_n - l.p[p].whole) * l.p[p].parts;
+  return n;
 }
 
 // 64 columns of this lane's row: the slab's row by 16-byte chunks, as the 128-byte swizzle places them.
@@ -88,9 +115,9 @@ struct SlabRing {
   uint8_t* base;
   uint32_t turn;
   __device__ __forceinline__ uint8_t* Next() {
-    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // (of the lane that commits; none for the others)
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // (of the lane that commits; none for the others)
     __syncwarp();
-    uint8_t* s = base + (turn & 1) * kSlabBytes;
+    uint8_t* s = base;
     ++turn;
     return s;
   }
@@ -167,8 +194,7 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = ClusterCtaRank(), unit = blockIdx.x >> 1, units = gridDim.x >> 1;
-  uint32_t total = 0;
-  for (uint32_t p = 0; p < l.count; ++p) total += l.p[p].tiles_m * l.p[p].tiles_n;
+  const uint32_t total = Items(l);
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < C::kStages; ++s) {
@@ -203,9 +229,9 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
         const GatedProblem& p = l.p[at.p];
         const uint32_t m0 = at.m_tile * 2 * kRows + rank * kRows;
         const uint32_t n0 = kGated ? at.n_tile * C::kHalf : at.n_tile * kTN + rank * C::kHalf;
-        for (uint32_t pair = 0; pair < 2 && ok; ++pair) {
-          const CUtensorMap *ma = &p.a[pair], *mb = kGated ? &p.b[rank] : &p.b[pair];
-          for (uint32_t kb = 0; kb < p.blocks[pair]; ++kb, ++it) {
+        for (uint32_t kb = at.from; kb < at.to; ++kb, ++it) {
+            const uint32_t pair = kb < p.blocks[0] ? 0 : 1;
+            const CUtensorMap *ma = &p.a[pair], *mb = kGated ? &p.b[rank] : &p.b[pair];
             const uint32_t s = it % C::kStages, round = it / C::kStages;
             if (round > 0 && !Wait(&bars->empty[s], (round - 1) & 1)) {
               give_up();
@@ -215,7 +241,7 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
             if (rank == 0) MbarExpectTx(&bars->full[s], 2 * C::kStageBytes);   // both CTAs' bytes
             const uint32_t full = MapToCta(SmemAddr(&bars->full[s]), 0);
             uint8_t* dst = smem + s * C::kStageBytes;
-            const int32_t k0 = static_cast<int32_t>(kb * kBlockK);
+            const int32_t k0 = static_cast<int32_t>((kb - (pair ? p.blocks[0] : 0)) * kBlockK);
 #pragma unroll
             for (uint32_t i = 0; i < kRows / 64; ++i) {
               const int32_t r = static_cast<int32_t>(m0 + 64 * i);
@@ -226,7 +252,6 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
               const int32_t r = static_cast<int32_t>(n0 + 64 * i);
               TmaLoad2DPair(dst + C::kABytes + i * kBoxBytes, mb, full, p.b_mn ? r : k0, p.b_mn ? k0 : r);
             }
-          }
         }
       }
     }
@@ -235,7 +260,8 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
       uint32_t it = 0, lt = 0;
       bool ok = true;
       for (uint32_t t = unit; t < total && ok; t += units, ++lt) {
-        const GatedProblem& p = l.p[Locate(l, t).p];
+        const At at = Locate(l, t);
+        const GatedProblem& p = l.p[at.p];
         const uint32_t idesc = ((1u << 4) | ((kTN >> 3) << 17) | ((2 * kRows >> 4) << 24)) | (l.f16 ? 0u : (1u << 7) | (1u << 10)) |
                                (p.a_mn << 15) | (p.b_mn << 16);
         const uint32_t step_a = p.a_mn ? 2048 / 16 : 2, step_b = p.b_mn ? 2048 / 16 : 2;   // 16 along K, in a descriptor
@@ -245,8 +271,8 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
           break;
         }
         TcFenceAfter();
-        const uint32_t acc = tmem_base + buf * kTN, blocks = p.blocks[0] + p.blocks[1];
-        for (uint32_t kb = 0; kb < blocks; ++kb, ++it) {
+        const uint32_t acc = tmem_base + buf * kTN;
+        for (uint32_t kb = at.from; kb < at.to; ++kb, ++it) {
           const uint32_t s = it % C::kStages, round = it / C::kStages;
           if (!Wait(&bars->full[s], round & 1)) {
             give_up();
@@ -259,7 +285,7 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
           const uint64_t desc_a = MakeSmemDescMn(a_addr, p.a_mn ? kBoxBytes : 16), desc_b = MakeSmemDescMn(b_addr, p.b_mn ? kBoxBytes : 16);
 #pragma unroll
           for (uint32_t k = 0; k < kBlockK / 16; ++k)
-            UmmaBf16Pair(acc, desc_a + step_a * k, desc_b + step_b * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            UmmaBf16Pair(acc, desc_a + step_a * k, desc_b + step_b * k, idesc, kb != at.from || k != 0 ? 1u : 0u);
           UmmaCommitPair(&bars->empty[s], 0);
         }
         UmmaCommitPair(&bars->tmem_full[buf], 0);
@@ -283,7 +309,18 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
       constexpr uint32_t kCols = kGated ? C::kHalf : kTN;   // output columns of the tile, 64 to a slab
       for (uint32_t c = which * 64; c < kCols; c += 128) {
         const uint32_t col = at.n_tile * kCols + c;
-        if (kGated) {
+        if (!kGated && at.parts > 1) {
+          // [4 columns][256 rows][4]: a warp's store is 512 bytes in a row
+          float4* to = reinterpret_cast<float4*>(l.partials + static_cast<size_t>(at.part) * 2 * kRows * kTN) + (c / 4) * 2 * kRows + rank * kRows +
+                       quarter * 32 + lane;
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h) {
+            float v[32];
+            LoadAcc(lanes + c + 32 * h, v);
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) to[(8 * h + i) * 2 * kRows] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        } else if (kGated) {
           if (l.f16) GatedColumns<F16>(ring, l, lanes + c, C::kHalf, col, row, row < p.M && col < p.N);
           else GatedColumns<Bf16>(ring, l, lanes + c, C::kHalf, col, row, row < p.M && col < p.N);
         } else {
@@ -306,6 +343,48 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
     TcFenceAfter();
     TmemFreePair(tmem_base, 2 * kTN);
   }
+}
+
+// 32 rows x 64 columns of a cut tile a block: its parts added in order, turned to rows in shared memory, stored.
+template <typename T>
+__global__ void __launch_bounds__(256)
+GatedFoldKernel(const __grid_constant__ GatedLaunch l, uint32_t tn) {
+  __shared__ float turn[32][65];
+  AwaitPrevious();
+  const uint32_t across = tn / 64, per_tile = 8 * across;   // blocks
+  uint32_t t = blockIdx.x / per_tile, q = 0;
+  const uint32_t within = blockIdx.x - t * per_tile;
+  while (q + 1 < l.count && t >= l.p[q].tiles_m * l.p[q].tiles_n - l.p[q].whole) {
+    t -= l.p[q].tiles_m * l.p[q].tiles_n - l.p[q].whole;
+    ++q;
+  }
+  const GatedProblem& p = l.p[q];
+  uint32_t m_tile, n_tile;
+  TileAt(p, p.whole + t, m_tile, n_tile);
+  const uint32_t r0 = (within / across) * 32, c0 = (within % across) * 64;   // in the tile
+  if (m_tile * 256 + r0 >= p.M || n_tile * tn + c0 >= p.N) return;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const size_t part_floats = 256ull * tn;
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) {
+    const uint32_t c4 = warp + 8 * i;   // four columns of the block's 64
+    const float4* from = reinterpret_cast<const float4*>(l.partials + (p.first_part + static_cast<size_t>(t) * p.parts) * part_floats) +
+                         (c0 / 4 + c4) * 256 + r0 + lane;
+    float4 sum = from[0];
+    for (uint32_t k = 1; k < p.parts; ++k) {
+      const float4 v = from[k * (part_floats / 4)];
+      sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+    }
+    float* to = &turn[lane][c4 * 4];
+    to[0] = sum.x;
+    to[1] = sum.y;
+    to[2] = sum.z;
+    to[3] = sum.w;
+  }
+  __syncthreads();
+  const uint32_t row = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;   // eight columns a thread
+  const uint32_t m = m_tile * 256 + r0 + row, n = n_tile * tn + c0 + c;
+  if (m < p.M && n < p.N) Store8<T>(static_cast<T*>(p.out) + m * p.out_stride + n, &turn[row][c]);
 }
 
 template <typename T, int kAct>
@@ -352,17 +431,22 @@ cudaError_t Run(const GatedLaunch& l, uint32_t sms, cudaStream_t s) {
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<kTN>::kSmem); e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
-  uint64_t tiles = 0;
-  for (uint32_t p = 0; p < l.count; ++p) tiles += static_cast<uint64_t>(l.p[p].tiles_m) * l.p[p].tiles_n;
-  const uint64_t pairs = sms / 2;
+  const uint64_t tiles = Items(l), pairs = sms / 2;
   return Next(kernel, static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)), kThreads, Tile<kTN>::kSmem, s, 2)(l);
 }
 
 }  // namespace
 
 cudaError_t GatedProducts(const GatedLaunch& l, bool gated, uint32_t tn, uint32_t sms, cudaStream_t s) {
-  if (gated) return tn == 256 ? Run<256, true>(l, sms, s) : Run<128, true>(l, sms, s);
-  return tn == 256 ? Run<256, false>(l, sms, s) : Run<128, false>(l, sms, s);
+  if (!gated) return Run<256, false>(l, sms, s);
+  return tn == 256 ? Run<256, true>(l, sms, s) : Run<128, true>(l, sms, s);
+}
+
+cudaError_t GatedFold(const GatedLaunch& l, uint32_t tn, cudaStream_t s) {
+  uint32_t tiles = 0;
+  for (uint32_t p = 0; p < l.count; ++p) tiles += l.p[p].tiles_m * l.p[p].tiles_n - l.p[p].whole;
+  const unsigned grid = tiles * 8 * (tn / 64);
+  return l.f16 ? Next(GatedFoldKernel<F16>, grid, 256, 0, s)(l, tn) : Next(GatedFoldKernel<Bf16>, grid, 256, 0, s)(l, tn);
 }
 
 cudaError_t GatedSlopes(const void* dh, const void* g, const void* u, void* dg, void* du, uint64_t rows, uint32_t cols, uint64_t stride,
