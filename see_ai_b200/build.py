@@ -45,6 +45,7 @@ CU_SOURCES = {
     "k_block_norm.cu": [],
     "k_adamw.cu": ["-fmad=false"],
     "k_gated_umma.cu": [],
+    "k_gated_token.cu": [],
 }
 CC_SOURCES = ["extents.cc", "cuda_backend.cc", "c_api.cc", "umma_gemm.cc", "engine.cc", "exchange.cc", "block_ops.cc", "gated.cc"]
 

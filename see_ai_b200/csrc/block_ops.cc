@@ -78,6 +78,7 @@ Status CudaBackend::NormForward(const see_norm_shape& given, const void* x, cons
   a.y = y;
   a.mean = mean;
   a.rstd = rstd;
+  a.status = d_status_;
   OnDevice on(device_);
   if (!on.ok()) return Check(cudaGetLastError(), "norm forward: device");
   if (auto r = Check(k::NormForward(a, sms_, stream_), "norm forward"); !r) return r;

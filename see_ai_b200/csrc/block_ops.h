@@ -16,7 +16,7 @@ namespace see::k {
 
 // ---- norm (k_block_norm.cu) ------------------------------------------------
 constexpr uint32_t kNormMaxCols = 16384;      // a row is held in the registers of one block
-constexpr uint32_t kNormPartials = 296;       // most rows of partial sums of the weights' gradients
+constexpr uint32_t kNormPartials = 148;       // most rows of partial sums of the weights' gradients
 struct NormArgs {
   const void *x = nullptr, *dy = nullptr, *addend = nullptr;
   const float *gamma = nullptr, *beta = nullptr;

@@ -197,6 +197,12 @@ Status CudaBackend::GatedForward(const see_gated_shape& given, const void* x, co
   if (s.rows == 0) return {};
   OnDevice on(device_);
   if (!on.ok()) return Check(cudaGetLastError(), "gated forward: device");
+  if (k::GatedTokenTakes(s.rows, s.d_in)) {
+    const k::GatedTokenArgs a = {x, w_gate, w_up, hidden, gate, up, static_cast<uint32_t>(s.d_in), static_cast<uint32_t>(s.d_hidden), s.act};
+    if (auto r = Check(k::GatedToken(a, s.type == SEE_F16, sms_, stream_), "gated forward"); !r) return r;
+    ++counters_.kernel_launches;
+    return {};
+  }
   if (!Encoder()) return std::unexpected("cuda: gated forward: the driver does not provide cuTensorMapEncodeTiled");
   const bool f16 = s.type == SEE_F16;
   k::GatedLaunch l = {};

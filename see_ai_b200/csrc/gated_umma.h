@@ -1,4 +1,4 @@
-// Interface between the tensor-core kernel of the gated feed-forward block (k_gated_umma.cu) and its host side (gated.cc).
+// Interface between the kernels of the gated feed-forward block (k_gated_umma.cu, k_gated_token.cu) and their host side (gated.cc).
 #ifndef SEE_CUDA_GATED_UMMA_H_
 #define SEE_CUDA_GATED_UMMA_H_
 
@@ -47,6 +47,16 @@ cudaError_t GatedFold(const GatedLaunch& l, uint32_t tn, cudaStream_t s);
 // dg = dh u act'(g), du = dh act(g): rows of `cols` elements (a multiple of 8); dh, g, u `stride` apart, dg, du dense.
 cudaError_t GatedSlopes(const void* dh, const void* g, const void* u, void* dg, void* du, uint64_t rows, uint32_t cols, uint64_t stride,
                         int act, bool f16, uint32_t sms, cudaStream_t s);
+
+// The forward pass of one row (k_gated_token.cu).
+struct GatedTokenArgs {
+  const void *x, *w_gate, *w_up;
+  void *hidden, *gate, *up;   // gate and up null: not kept
+  uint32_t d_in, d_hidden;
+  int act;
+};
+bool GatedTokenTakes(uint64_t rows, uint64_t d_in);
+cudaError_t GatedToken(const GatedTokenArgs& a, bool f16, uint32_t sms, cudaStream_t s);
 
 }  // namespace see::k
 

@@ -3,11 +3,11 @@
 //   y = u gamma + beta,   dx = rstd (q - <q> - u <q u>) (+ addend),   dgamma = sum over rows of dy u,   dbeta = of dy
 // (rms: neither beta nor <q>).  Bound by HBM: each matrix is read or written once.
 //
-// A row belongs to a group of T threads (a multiple of 32), which hold it in registers, eight consecutive columns at a
-// time where widths, strides and addresses allow 16-byte accesses and single columns T apart otherwise; a block has as
-// many groups as fit into 512 threads.  A thread has the same columns in every row, so that the backward pass sums dgamma
-// and dbeta over a block's rows in registers; the groups meet in shared memory, the blocks (at most two to an SM) in
-// NormFoldKernel, both in an order that the sizes alone fix.
+// A row belongs to a group of T threads (a multiple of 32), which hold it in registers, four or eight consecutive columns at a
+// time where widths, strides and addresses allow 16-byte accesses and single columns T apart otherwise; a block has several
+// groups.  Rows reach them through a ring in shared memory, or, single columns and few rows, directly.  A thread has the same
+// columns in every row, so that the backward pass sums dgamma and dbeta over a block's rows in registers; the groups meet in
+// shared memory, the blocks (one to an SM) in NormFoldKernel, both in an order that the sizes alone fix.
 //
 // All sums are f32.  The forward pass takes the mean twice: the second pass over the registers sums the deviations from
 // the first result, which corrects it, beside their squares, so rows far from zero lose nothing to cancellation.
@@ -22,6 +22,7 @@ namespace see::k {
 namespace {
 
 constexpr uint32_t kNormThreads = 512;
+constexpr uint32_t kWideThreads = 768;
 constexpr size_t kRingBytes = 200 * 1024;   // of a block
 
 template <bool kBoth>
@@ -37,7 +38,7 @@ __device__ __forceinline__ float2 WarpSum(float2 v) {
 // The sums of a group's T threads, in all of them.  `slots`: two sets of 16 per block, used in turn, so that one barrier
 // a sum is enough: who writes a set again has passed the barrier that the readers of its last use arrived at after it.
 template <bool kBoth>   // or v.x alone
-__device__ __forceinline__ float2 GroupSum(float2 v, uint32_t T, uint32_t group, float2 (*slots)[kNormThreads / 32], uint32_t& turn) {
+__device__ __forceinline__ float2 GroupSum(float2 v, uint32_t T, uint32_t group, float2 (*slots)[kWideThreads / 32], uint32_t& turn) {
   v = WarpSum<kBoth>(v);
   if (T == 32) return v;
   float2* set = slots[turn] + group * (T / 32);
@@ -50,6 +51,14 @@ __device__ __forceinline__ float2 GroupSum(float2 v, uint32_t T, uint32_t group,
     if (kBoth) sum.y += set[w].y;
   }
   return sum;
+}
+
+// The sums of the deviations from `mean` and of their squares correct it and give the variance.
+__device__ __forceinline__ void CorrectMean(float2 sum, float per_col, float& mean, float& var) {
+  const float shift = sum.x * per_col;
+  if (isfinite(shift)) mean += shift;
+  var = fmaxf(sum.y * per_col - shift * shift, 0.0f);
+  if (!isfinite(sum.y)) var = sum.y;   // (fmaxf drops a NaN)
 }
 
 template <typename T, int VEC>
@@ -66,7 +75,7 @@ __device__ __forceinline__ void StoreCols(T* p, const float* v) {
 template <typename XT, typename YT, bool kRms, int VEC, int NV>
 __global__ void __launch_bounds__(kNormThreads)
 NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
-  __shared__ float2 slots[2][kNormThreads / 32];
+  __shared__ float2 slots[2][kWideThreads / 32];
   AwaitPrevious();
   const uint32_t group = threadIdx.x / T, t = threadIdx.x - group * T;
   const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (blockDim.x / T) + group;
@@ -106,10 +115,7 @@ NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
         }
       }
     sum = GroupSum<true>(sum, T, group, slots, turn);
-    const float shift = sum.x * per_col;
-    if (isfinite(shift)) mean += shift;
-    var = fmaxf(sum.y * per_col - shift * shift, 0.0f);
-    if (!isfinite(sum.y)) var = sum.y;   // (fmaxf drops a NaN)
+    CorrectMean(sum, per_col, mean, var);
   }
   const float rstd = 1.0f / sqrtf(var + a.eps);
   if (t == 0) {
@@ -145,6 +151,28 @@ template <typename T> __device__ __forceinline__ void StorePairs(T* p, const f32
   Store8<T>(p, f);
 }
 
+// Four columns as two pairs: where gamma and beta lie in shared memory beside the rows, a warp's accesses are then whole runs.
+template <typename T> __device__ __forceinline__ void LoadFour(const T* p, f32x2 (&v)[2]) {
+  float f[4];
+  if constexpr (sizeof(T) == 4) {
+    const float4 r = *reinterpret_cast<const float4*>(p);
+    f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w;
+  } else {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    Unpack2<T>(r.x, f[0], f[1]);
+    Unpack2<T>(r.y, f[2], f[3]);
+  }
+  v[0] = PackF2(f[0], f[1]);
+  v[1] = PackF2(f[2], f[3]);
+}
+template <typename T> __device__ __forceinline__ void StoreFour(T* p, const f32x2 (&v)[2]) {
+  float f[4];
+  UnpackF2(v[0], &f[0], &f[1]);
+  UnpackF2(v[1], &f[2], &f[3]);
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(Pack2<T>(f[0], f[1]), Pack2<T>(f[2], f[3]));
+}
+
 // ---- rows through a ring in shared memory -----------------------------------------------
 // Each group has `slots` of its own, filled by one thread's bulk copies (a whole row each, counted on the slot's mbarrier)
 // and emptied into registers; a slot is asked to be filled again as soon as the group has read it, so that between 60 and
@@ -161,12 +189,123 @@ __device__ __forceinline__ void AwaitRow(uint64_t* bar, uint32_t parity, DeviceS
   umma_dev::DrainDelay();
 }
 
+// The forward pass of more than two rows to a group.  NV: times four columns to a thread.  Up to 768 columns a row is a warp's
+// and gamma and beta stay in registers (kHold); of wider ones they lie in shared memory, which leaves registers for half as many
+// threads again.  Read from global memory for every row, as NormFwdKernel does, they are twice an f32 row's bytes.  NormFwdKernel
+// / this, us: 32768 x 768 f32 to bf16 32 / 26.6, 32768 x 1024 40 / 36, 16384 x 4096 bf16 101 / 66, rms 58 / 48.
+template <typename XT, typename YT, bool kRms, int NV, bool kHold>
+__global__ void __launch_bounds__(kHold ? kNormThreads : kWideThreads, 1)
+NormFwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots) {
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ float2 sums[2][kWideThreads / 32];
+  const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T, row_bytes = a.cols * sizeof(XT);
+  uint8_t* ring = dyn + static_cast<size_t>(group) * slots * row_bytes;
+  float* weights = reinterpret_cast<float*>(dyn + static_cast<size_t>(groups) * slots * row_bytes);   // gamma, beta
+  uint64_t* bars = reinterpret_cast<uint64_t*>(weights + (kHold ? 0 : (kRms ? 1 : 2) * a.cols)) + group * slots;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups + group, step = static_cast<uint64_t>(gridDim.x) * groups;
+  if (t == 0) {
+    for (uint32_t i = 0; i < slots; ++i) umma_dev::MbarInit(&bars[i], 1);
+    umma_dev::MbarInitFence();
+  }
+  auto fill = [&](uint64_t row, uint32_t slot) {   // the group's thread 0
+    umma_dev::MbarExpectTx(&bars[slot], row_bytes);
+    umma_dev::BulkLoad(ring + static_cast<size_t>(slot) * row_bytes, static_cast<const XT*>(a.x) + row * a.x_stride, row_bytes, &bars[slot]);
+  };
+  AwaitPrevious();
+  if (t == 0)
+    for (uint32_t i = 0; i < slots && first + i * step < a.rows; ++i) fill(first + i * step, i);
+  f32x2 gamma[kHold ? NV : 1][2], beta[kHold && !kRms ? NV : 1][2];
+  if constexpr (kHold) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((t + i * T) * 4 < a.cols) {
+        LoadFour(a.gamma + (t + i * T) * 4, gamma[i]);
+        if (!kRms) LoadFour(a.beta + (t + i * T) * 4, beta[kRms ? 0 : i]);
+      }
+  } else {
+    for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+      weights[c] = a.gamma[c];
+      if (!kRms) weights[a.cols + c] = a.beta[c];
+    }
+  }
+  __syncthreads();
+  const float per_col = 1.0f / static_cast<float>(a.cols);
+  uint32_t turn = 0, slot = 0, parity = 0;
+  for (uint64_t row = first; row < a.rows; row += step) {
+    AwaitRow(&bars[slot], parity, a.status);
+    const XT* x = reinterpret_cast<const XT*>(ring + static_cast<size_t>(slot) * row_bytes);
+    f32x2 v[NV][2], total = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * T) * 4;
+      if (c < a.cols) {
+        LoadFour(x + c, v[i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) total = kRms ? Fma2(v[i][j], v[i][j], total) : AddF2(total, v[i][j]);
+      }
+    }
+    float2 sum, other;
+    UnpackF2(total, &sum.x, &other.x);
+    sum = GroupSum<false>(make_float2(sum.x + other.x, 0.0f), T, group, sums, turn);
+    if (T == 32) __syncwarp();   // (a wider group has met at the sum's barrier: the slot is read)
+    if (t == 0 && row + slots * step < a.rows) fill(row + slots * step, slot);
+    if (++slot == slots) {
+      slot = 0;
+      parity ^= 1;
+    }
+    float mean = 0.0f, var = sum.x * per_col;
+    if constexpr (!kRms) {
+      mean = sum.x * per_col;
+      const f32x2 away = Splat2(-mean);
+      f32x2 linear = 0, square = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((t + i * T) * 4 < a.cols) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const f32x2 d = AddF2(v[i][j], away);
+            linear = AddF2(linear, d);
+            square = Fma2(d, d, square);
+          }
+        }
+      UnpackF2(linear, &sum.x, &other.x);
+      UnpackF2(square, &sum.y, &other.y);
+      sum = GroupSum<true>(make_float2(sum.x + other.x, sum.y + other.y), T, group, sums, turn);
+      CorrectMean(sum, per_col, mean, var);
+    }
+    const float rstd = 1.0f / sqrtf(var + a.eps);
+    if (t == 0) {
+      a.rstd[row] = rstd;
+      if (!kRms) a.mean[row] = mean;
+    }
+    const f32x2 away = Splat2(-mean), rstd2 = Splat2(rstd);
+    YT* y = static_cast<YT*>(a.y) + row * a.y_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * T) * 4;
+      if (c < a.cols) {
+        f32x2 g[2], b[2];
+        if (!kHold) {
+          LoadFour(weights + c, g);
+          if (!kRms) LoadFour(weights + a.cols + c, b);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const f32x2 unit = Mul2(kRms ? v[i][j] : AddF2(v[i][j], away), rstd2), by = kHold ? gamma[kHold ? i : 0][j] : g[j];
+          v[i][j] = kRms ? Mul2(unit, by) : Fma2(unit, by, kHold ? beta[kHold && !kRms ? i : 0][j] : b[j]);
+        }
+        StoreFour(y + c, v[i]);
+      }
+    }
+  }
+}
+
 template <typename XT, typename YT, bool kRms, int NV, uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads, 1)
 NormBwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots) {
   constexpr bool kHoldGamma = kThreads < 512 || NV <= 2;   // in registers, as far as they go
   extern __shared__ __align__(128) uint8_t dyn[];
-  __shared__ float2 sums[2][kNormThreads / 32];
+  __shared__ float2 sums[2][kWideThreads / 32];
   const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
   const uint32_t x_bytes = a.cols * sizeof(XT), y_bytes = a.cols * sizeof(YT);
   const uint32_t slot_bytes = x_bytes + y_bytes + (a.addend ? x_bytes : 0);
@@ -289,7 +428,7 @@ template <typename XT, typename YT, bool kRms, int VEC, int NV>
 __global__ void __launch_bounds__(kNormThreads, 1)
 NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
   extern __shared__ float meet[];   // [groups][cols]
-  __shared__ float2 slots[2][kNormThreads / 32];
+  __shared__ float2 slots[2][kWideThreads / 32];
   AwaitPrevious();
   const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
   const float per_col = 1.0f / static_cast<float>(a.cols);
@@ -445,6 +584,19 @@ cudaError_t RunRing(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s,
   return Fold<kRms>(a, grid, s, launches);
 }
 
+template <typename XT, typename YT, bool kRms, int NV, bool kHold>
+cudaError_t RunFwdRing(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s) {
+  const size_t row_bytes = static_cast<size_t>(a.cols) * sizeof(XT), weights = kHold ? 0 : a.cols * (kRms ? 4 : 8);
+  uint32_t groups = (kHold ? kNormThreads : kWideThreads) / T;
+  while (groups > 1 && groups * row_bytes > kRingBytes - weights) --groups;
+  uint32_t slots = static_cast<uint32_t>((kRingBytes - weights) / (groups * row_bytes));   // (one at least, up to 8192 columns)
+  slots = slots > 8 ? 8 : slots;
+  const size_t smem = groups * slots * (row_bytes + 8) + weights;
+  auto* kernel = NormFwdRingKernel<XT, YT, kRms, NV, kHold>;
+  if (cudaError_t e = AllowShared(kernel, smem); e != cudaSuccess) return e;
+  return Next(kernel, static_cast<unsigned>(Blocks(a.rows, groups, sms)), groups * T, smem, s)(a, T, slots);
+}
+
 template <typename XT, typename YT, bool kRms, int VEC, int NV>
 cudaError_t Run(const NormArgs& a, uint32_t T, cudaStream_t s) {
   const uint32_t groups = kNormThreads / T;
@@ -478,6 +630,15 @@ cudaError_t Pick(const NormArgs& a, bool backward, uint32_t sms, cudaStream_t s,
     if (kRms && n <= 1536) return RunRing<XT, YT, kRms, 4, 384>(a, up((n + 3) / 4), sms, s, launches);
     if (n <= 1024) return RunRing<XT, YT, kRms, 2, 512>(a, up((n + 1) / 2), sms, s, launches);
     return RunRing<XT, YT, kRms, 4, 512>(a, up((n + 3) / 4), sms, s, launches);
+  }
+  if (vec && a.cols <= 8192) {   // (two slots to a group of the widest)
+    const uint32_t n = a.cols / 4, T = n <= 256 ? 32 : (n + 255) / 256 * 32;
+    if (a.rows > 2ull * (kNormThreads / T) * sms) {
+      if (n <= 64) return RunFwdRing<XT, YT, kRms, 2, true>(a, T, sms, s);
+      if (n <= 128) return RunFwdRing<XT, YT, kRms, 4, true>(a, T, sms, s);
+      if (n <= 192) return RunFwdRing<XT, YT, kRms, 6, true>(a, T, sms, s);
+      return RunFwdRing<XT, YT, kRms, 8, false>(a, T, sms, s);
+    }
   }
   if (vec) {
     switch (f.nv) {

@@ -80,7 +80,8 @@ def check_forward(kind, x, gamma, beta, eps, yt, y, mean, rstd):
 @pytest.mark.parametrize("xt,yt", PAIRS)
 @pytest.mark.parametrize("kind", [B.NORM_LAYER, B.NORM_RMS])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 768), (3, 7), (17, 33), (257, 256), (64, 1000), (33, 1029), (5, 4096), (9, 4104),
-                                       (2, 8200), (3, 12001), (2, 16384), (1, 16383), (700, 64)])
+                                       (2, 8200), (3, 12001), (2, 16384), (1, 16383), (700, 64), (5000, 64), (4800, 256),
+                                       (5001, 768), (7100, 1000), (4737, 1024), (2500, 1544), (1200, 4096), (700, 8192)])
 def test_forward(be, kind, rows, cols, xt, yt):
     torch.manual_seed(rows * 31 + cols)
     x = (torch.randn(rows, cols, device="cuda") * 2 + 0.5).to(DTYPES[xt])
