@@ -9,8 +9,11 @@
 // columns in every row, so that the backward pass sums dgamma and dbeta over a block's rows in registers; the groups meet in
 // shared memory, the blocks (one to an SM) in NormFoldKernel, both in an order that the sizes alone fix.
 //
-// All sums are f32.  The forward pass takes the mean twice: the second pass over the registers sums the deviations from
-// the first result, which corrects it, beside their squares, so rows far from zero lose nothing to cancellation.
+// Sums are f32, but for the mean: the threads' sums are added in double.  A thread's share is summed plainly where it has 16 bits
+// (a few dozen values of 8 or 11 fit); in f32, with what each addition rounds away in NormFwdKernel, where it costs nothing
+// beside the latency, and corrected by the average deviation from the first result in NormFwdRingKernel, where it would (26.6 us
+// to 31.5 at 32768 x 768).  The variance is the average square of the deviations, a second pass over the registers, so rows far
+// from zero lose nothing to cancellation.
 #include "act_expr.cuh"
 #include "block_ops.h"
 #include "launch.cuh"
@@ -53,12 +56,25 @@ __device__ __forceinline__ float2 GroupSum(float2 v, uint32_t T, uint32_t group,
   return sum;
 }
 
-// The sums of the deviations from `mean` and of their squares correct it and give the variance.
-__device__ __forceinline__ void CorrectMean(float2 sum, float per_col, float& mean, float& var) {
-  const float shift = sum.x * per_col;
-  if (isfinite(shift)) mean += shift;
-  var = fmaxf(sum.y * per_col - shift * shift, 0.0f);
-  if (!isfinite(sum.y)) var = sum.y;   // (fmaxf drops a NaN)
+// The same of one double.
+__device__ __forceinline__ double GroupSum(double v, uint32_t T, uint32_t group, float2 (*slots)[kWideThreads / 32], uint32_t& turn) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  if (T == 32) return v;
+  double* set = reinterpret_cast<double*>(slots[turn]) + group * (T / 32);
+  turn ^= 1;
+  if ((threadIdx.x & 31) == 0) set[(threadIdx.x - group * T) >> 5] = v;
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(T) : "memory");
+  double sum = set[0];
+  for (uint32_t w = 1; w < T / 32; ++w) sum += set[w];
+  return sum;
+}
+
+// sum + x into sum, what that rounds away into rest (Knuth's TwoSum: no order of magnitudes asked for).
+__device__ __forceinline__ void AddExactly(float& sum, float& rest, float x) {
+  const float s = sum + x, z = s - sum;
+  rest += (sum - (s - z)) + (x - z);
+  sum = s;
 }
 
 template <typename T, int VEC>
@@ -75,15 +91,15 @@ __device__ __forceinline__ void StoreCols(T* p, const float* v) {
 template <typename XT, typename YT, bool kRms, int VEC, int NV>
 __global__ void __launch_bounds__(kNormThreads)
 NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
-  __shared__ float2 slots[2][kWideThreads / 32];
+  __shared__ __align__(8) float2 slots[2][kWideThreads / 32];
   AwaitPrevious();
   const uint32_t group = threadIdx.x / T, t = threadIdx.x - group * T;
   const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (blockDim.x / T) + group;
   if (row >= a.rows) return;
   const XT* x = static_cast<const XT*>(a.x) + row * a.x_stride;
   uint32_t turn = 0;
-  float v[NV][VEC];
-  float2 sum = make_float2(0.0f, 0.0f);
+  float v[NV][VEC], total = 0.0f;
+  [[maybe_unused]] float rest = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint32_t c = (t + i * T) * VEC;
@@ -94,29 +110,29 @@ NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
       for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
     }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum.x += kRms ? v[i][j] * v[i][j] : v[i][j];
+    for (int j = 0; j < VEC; ++j) {
+      if (kRms) total += v[i][j] * v[i][j];
+      else if (sizeof(XT) == 4) AddExactly(total, rest, v[i][j]);
+      else total += v[i][j];
+    }
   }
-  sum = GroupSum<false>(sum, T, group, slots, turn);
   const float per_col = 1.0f / static_cast<float>(a.cols);
-  float mean = 0.0f, var;
-  if constexpr (kRms) {
-    var = sum.x * per_col;
-  } else {
-    mean = sum.x * per_col;
-    sum = make_float2(0.0f, 0.0f);
+  float mean = 0.0f;
+  if constexpr (!kRms) {
+    const double share = isfinite(rest) ? static_cast<double>(total) + static_cast<double>(rest) : static_cast<double>(total);
+    mean = static_cast<float>(GroupSum(share, T, group, slots, turn) / static_cast<double>(a.cols));
+    total = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((t + i * T) * VEC < a.cols) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float d = v[i][j] - mean;
-          sum.x += d;
-          sum.y += d * d;
+          total += d * d;
         }
       }
-    sum = GroupSum<true>(sum, T, group, slots, turn);
-    CorrectMean(sum, per_col, mean, var);
   }
+  const float var = GroupSum<false>(make_float2(total, 0.0f), T, group, slots, turn).x * per_col;
   const float rstd = 1.0f / sqrtf(var + a.eps);
   if (t == 0) {
     a.rstd[row] = rstd;
@@ -230,6 +246,7 @@ NormFwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots
   }
   __syncthreads();
   const float per_col = 1.0f / static_cast<float>(a.cols);
+  [[maybe_unused]] const double per_col_wide = 1.0 / static_cast<double>(a.cols);
   uint32_t turn = 0, slot = 0, parity = 0;
   for (uint64_t row = first; row < a.rows; row += step) {
     AwaitRow(&bars[slot], parity, a.status);
@@ -244,34 +261,46 @@ NormFwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots
         for (int j = 0; j < 2; ++j) total = kRms ? Fma2(v[i][j], v[i][j], total) : AddF2(total, v[i][j]);
       }
     }
-    float2 sum, other;
-    UnpackF2(total, &sum.x, &other.x);
-    sum = GroupSum<false>(make_float2(sum.x + other.x, 0.0f), T, group, sums, turn);
+    float one, other;
+    UnpackF2(total, &one, &other);
+    float mean = 0.0f, var;
+    if constexpr (kRms) {
+      var = GroupSum<false>(make_float2(one + other, 0.0f), T, group, sums, turn).x * per_col;
+    } else {
+      mean = static_cast<float>(GroupSum(static_cast<double>(one) + static_cast<double>(other), T, group, sums, turn) * per_col_wide);
+    }
     if (T == 32) __syncwarp();   // (a wider group has met at the sum's barrier: the slot is read)
     if (t == 0 && row + slots * step < a.rows) fill(row + slots * step, slot);
     if (++slot == slots) {
       slot = 0;
       parity ^= 1;
     }
-    float mean = 0.0f, var = sum.x * per_col;
     if constexpr (!kRms) {
-      mean = sum.x * per_col;
+      constexpr bool kCorrect = sizeof(XT) == 4;
       const f32x2 away = Splat2(-mean);
-      f32x2 linear = 0, square = 0;
+      f32x2 linear = 0;
+      total = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if ((t + i * T) * 4 < a.cols) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const f32x2 d = AddF2(v[i][j], away);
-            linear = AddF2(linear, d);
-            square = Fma2(d, d, square);
+            if (kCorrect) linear = AddF2(linear, d);
+            total = Fma2(d, d, total);
           }
         }
-      UnpackF2(linear, &sum.x, &other.x);
-      UnpackF2(square, &sum.y, &other.y);
-      sum = GroupSum<true>(make_float2(sum.x + other.x, sum.y + other.y), T, group, sums, turn);
-      CorrectMean(sum, per_col, mean, var);
+      float2 sum = make_float2(0.0f, 0.0f);
+      if (kCorrect) {
+        UnpackF2(linear, &one, &other);
+        sum.x = one + other;
+      }
+      UnpackF2(total, &one, &other);
+      sum.y = one + other;
+      if (!kCorrect) sum.x = sum.y;
+      sum = GroupSum<kCorrect>(sum, T, group, sums, turn);
+      var = (kCorrect ? sum.y : sum.x) * per_col;
+      if (kCorrect && isfinite(sum.x)) mean += sum.x * per_col;   // (which moves the average square by its own square: nothing)
     }
     const float rstd = 1.0f / sqrtf(var + a.eps);
     if (t == 0) {
