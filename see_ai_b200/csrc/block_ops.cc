@@ -13,17 +13,17 @@ namespace see {
 namespace {
 
 // Shape checks common to both directions; fills the strides.
-Status CheckNorm(const std::string& what, see_norm_shape* s) {
-  if (s->kind != SEE_NORM_LAYER && s->kind != SEE_NORM_RMS) return std::unexpected(what + ": unknown kind");
+Status CheckNorm(const char* what, see_norm_shape* s) {
+  if (s->kind != SEE_NORM_LAYER && s->kind != SEE_NORM_RMS) return std::unexpected(std::string(what) + ": unknown kind");
   if (!IsType(s->x_type) || !IsType(s->y_type) || (s->x_type != s->y_type && s->x_type != SEE_F32))
-    return std::unexpected(what + ": x_type and y_type are equal, or x_type is f32");
-  if (!(s->eps >= 0.0f) || !std::isfinite(s->eps)) return std::unexpected(what + ": eps is not a finite number from 0 on");
-  if (s->cols == 0 || s->cols > k::kNormMaxCols) return std::unexpected(what + ": 1 to 16384 columns");
-  if (s->rows > 0x7FFFFFFFull) return std::unexpected(what + ": more than 2^31 - 1 rows");
+    return std::unexpected(std::string(what) + ": x_type and y_type are equal, or x_type is f32");
+  if (!(s->eps >= 0.0f) || !std::isfinite(s->eps)) return std::unexpected(std::string(what) + ": eps is not a finite number from 0 on");
+  if (s->cols == 0 || s->cols > k::kNormMaxCols) return std::unexpected(std::string(what) + ": 1 to 16384 columns");
+  if (s->rows > 0x7FFFFFFFull) return std::unexpected(std::string(what) + ": more than 2^31 - 1 rows");
   if (s->x_stride == 0) s->x_stride = s->cols;
   if (s->y_stride == 0) s->y_stride = s->cols;
   if (s->x_stride < s->cols || s->y_stride < s->cols || s->x_stride > (1ull << 40) || s->y_stride > (1ull << 40))
-    return std::unexpected(what + ": a stride is smaller than a row, or over 2^40");
+    return std::unexpected(std::string(what) + ": a stride is smaller than a row, or over 2^40");
   return {};
 }
 
@@ -49,21 +49,21 @@ uint64_t NormBackwardWorkspace(uint64_t rows, uint64_t cols) {
 
 Status CheckNormForward(see_norm_shape* shape, const void* x, const float* gamma, const float* beta, const void* y, const float* mean,
                         const float* rstd) {
-  const std::string what = "cuda: norm forward";
+  const char* const what = "cuda: norm forward";
   if (auto r = CheckNorm(what, shape); !r) return r;
   const see_norm_shape& s = *shape;
   const bool layer = s.kind == SEE_NORM_LAYER;
-  if (!layer && (beta || mean)) return std::unexpected(what + ": rms has neither beta nor mean");
+  if (!layer && (beta || mean)) return std::unexpected(std::string(what) + ": rms has neither beta nor mean");
   const uint64_t xs = SizeOfType(s.x_type), ys = SizeOfType(s.y_type);
-  std::vector<Operand> ops = {{"x", x, s.rows, s.cols * xs, s.x_stride * xs, xs, false},
+  Operands ops = {{"x", x, s.rows, s.cols * xs, s.x_stride * xs, xs, false},
                               {"y", y, s.rows, s.cols * ys, s.y_stride * ys, ys, true},
                               Vector("gamma", gamma, s.cols * 4, 4, false),
                               Vector("rstd", rstd, s.rows * 4, 4, true)};
   if (layer) {
-    ops.push_back(Vector("beta", beta, s.cols * 4, 4, false));
-    ops.push_back(Vector("mean", mean, s.rows * 4, 4, true));
+    ops.Add(Vector("beta", beta, s.cols * 4, 4, false));
+    ops.Add(Vector("mean", mean, s.rows * 4, 4, true));
   }
-  return CheckOperands(what, ops);
+  return ops.Check(what);
 }
 
 Status CudaBackend::NormForward(const see_norm_shape& given, const void* x, const float* gamma, const float* beta, void* y, float* mean,
@@ -89,26 +89,26 @@ Status CudaBackend::NormForward(const see_norm_shape& given, const void* x, cons
 Status CheckNormBackward(see_norm_shape* shape, const void* dy, const void* x, const float* gamma, const float* mean, const float* rstd,
                          const void* addend, const void* dx, const float* dgamma, const float* dbeta, const void* workspace,
                          uint64_t workspace_bytes) {
-  const std::string what = "cuda: norm backward";
+  const char* const what = "cuda: norm backward";
   if (auto r = CheckNorm(what, shape); !r) return r;
   const see_norm_shape& s = *shape;
   const bool layer = s.kind == SEE_NORM_LAYER;
-  if (!layer && (dbeta || mean)) return std::unexpected(what + ": rms has neither mean nor dbeta");
-  if (workspace_bytes < NormBackwardWorkspace(s.rows, s.cols)) return std::unexpected(what + ": the workspace is too small");
+  if (!layer && (dbeta || mean)) return std::unexpected(std::string(what) + ": rms has neither mean nor dbeta");
+  if (workspace_bytes < NormBackwardWorkspace(s.rows, s.cols)) return std::unexpected(std::string(what) + ": the workspace is too small");
   const uint64_t xs = SizeOfType(s.x_type), ys = SizeOfType(s.y_type);
-  std::vector<Operand> ops = {{"dy", dy, s.rows, s.cols * ys, s.y_stride * ys, ys, false},
+  Operands ops = {{"dy", dy, s.rows, s.cols * ys, s.y_stride * ys, ys, false},
                               {"x", x, s.rows, s.cols * xs, s.x_stride * xs, xs, false},
                               {"dx", dx, s.rows, s.cols * xs, s.x_stride * xs, xs, true},
                               Vector("gamma", gamma, s.cols * 4, 4, false),
                               Vector("rstd", rstd, s.rows * 4, 4, false),
                               Vector("dgamma", dgamma, s.cols * 4, 4, true),
                               Vector("workspace", workspace, workspace_bytes, 16, true)};
-  if (addend) ops.push_back({"addend", addend, s.rows, s.cols * xs, s.x_stride * xs, xs, false});
+  if (addend) ops.Add({"addend", addend, s.rows, s.cols * xs, s.x_stride * xs, xs, false});
   if (layer) {
-    ops.push_back(Vector("mean", mean, s.rows * 4, 4, false));
-    ops.push_back(Vector("dbeta", dbeta, s.cols * 4, 4, true));
+    ops.Add(Vector("mean", mean, s.rows * 4, 4, false));
+    ops.Add(Vector("dbeta", dbeta, s.cols * 4, 4, true));
   }
-  return CheckOperands(what, ops);
+  return ops.Check(what);
 }
 
 Status CudaBackend::NormBackward(const see_norm_shape& given, const void* dy, const void* x, const float* gamma, const float* mean,
@@ -142,13 +142,13 @@ Status CudaBackend::NormBackward(const see_norm_shape& given, const void* dy, co
 }
 
 Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale) {
-  const std::string what = "cuda: adamw";
-  if (state_bits != 8 && state_bits != 32) return std::unexpected(what + ": moments have 8 or 32 bits");
-  if (params.step == 0) return std::unexpected(what + ": steps count from 1");
+  const char* const what = "cuda: adamw";
+  if (state_bits != 8 && state_bits != 32) return std::unexpected(std::string(what) + ": moments have 8 or 32 bits");
+  if (params.step == 0) return std::unexpected(std::string(what) + ": steps count from 1");
   if (!(params.beta1 >= 0.0f && params.beta1 < 1.0f && params.beta2 >= 0.0f && params.beta2 < 1.0f))
-    return std::unexpected(what + ": beta1 and beta2 are from 0 on and below 1");
-  if (count && !tensors) return std::unexpected(what + ": tensors is null");
-  if (reinterpret_cast<uint64_t>(grad_scale) % 4) return std::unexpected(what + ": grad_scale is not aligned");
+    return std::unexpected(std::string(what) + ": beta1 and beta2 are from 0 on and below 1");
+  if (count && !tensors) return std::unexpected(std::string(what) + ": tensors is null");
+  if (reinterpret_cast<uint64_t>(grad_scale) % 4) return std::unexpected(std::string(what) + ": grad_scale is not aligned");
   // Seven operands a tensor.  Lists of tensors mostly follow the layout of a few buffers, so each operand's spans are tried in
   // the list's order first; only where they do not ascend, or two operands' ranges meet, is everything sorted.
   struct Span { uint64_t begin, end; };
@@ -166,7 +166,7 @@ Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bit
   bool ascending = true;
   for (uint64_t i = 0; i < count; ++i) {
     const see_adamw_tensor& t = tensors[i];
-    auto refuse = [&](const std::string& why) { return std::unexpected(what + ": tensor " + std::to_string(i) + ": " + why); };
+    auto refuse = [&](const std::string& why) { return std::unexpected(std::string(what) + ": tensor " + std::to_string(i) + ": " + why); };
     if (!IsType(t.g_type) || !IsType(t.copy_type)) return refuse("unknown type");
     if (t.flags & ~static_cast<uint32_t>(SEE_ADAMW_NO_DECAY)) return refuse("unknown flag");
     if ((t.copy_type == SEE_F32) != (t.copy == nullptr)) return refuse("a copy has 16 bits, and none is null with type f32");
@@ -202,7 +202,7 @@ Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bit
   std::sort(all.begin(), all.end(), [](const Sorted& a, const Sorted& b) { return a.span.begin < b.span.begin; });
   uint64_t any = 0, written = 0;   // how far the spans so far reach
   for (const Sorted& s : all) {
-    if (s.span.begin < written || (s.written && s.span.begin < any)) return std::unexpected(what + ": operands overlap");
+    if (s.span.begin < written || (s.written && s.span.begin < any)) return std::unexpected(std::string(what) + ": operands overlap");
     any = std::max(any, s.span.end);
     if (s.written) written = std::max(written, s.span.end);
   }

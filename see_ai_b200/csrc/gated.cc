@@ -34,20 +34,20 @@ bool MapOf(CUtensorMap* map, bool f16, const void* base, uint64_t rows, uint64_t
 
 uint32_t Up(uint64_t n, uint64_t by) { return static_cast<uint32_t>((n + by - 1) / by); }
 
-Status CheckGated(const std::string& what, see_gated_shape* s) {
-  if (s->type != SEE_BF16 && s->type != SEE_F16) return std::unexpected(what + ": the type is bf16 or f16");
-  if (s->act != SEE_ACT_RELU && s->act != SEE_ACT_GELU && s->act != SEE_ACT_SILU) return std::unexpected(what + ": unknown activation");
+Status CheckGated(const char* what, see_gated_shape* s) {
+  if (s->type != SEE_BF16 && s->type != SEE_F16) return std::unexpected(std::string(what) + ": the type is bf16 or f16");
+  if (s->act != SEE_ACT_RELU && s->act != SEE_ACT_GELU && s->act != SEE_ACT_SILU) return std::unexpected(std::string(what) + ": unknown activation");
   if (s->d_in == 0 || s->d_hidden == 0 || s->d_in % 8 || s->d_hidden % 8 || s->d_in > (1u << 20) || s->d_hidden > (1u << 20))
-    return std::unexpected(what + ": d_in and d_hidden are multiples of 8 from 8 to 2^20");
-  if (s->rows > 0x7FFFFF00ull) return std::unexpected(what + ": more than 2^31 - 256 rows");
+    return std::unexpected(std::string(what) + ": d_in and d_hidden are multiples of 8 from 8 to 2^20");
+  if (s->rows > 0x7FFFFF00ull) return std::unexpected(std::string(what) + ": more than 2^31 - 256 rows");
   if (s->x_stride == 0) s->x_stride = s->d_in;
   if (s->hidden_stride == 0) s->hidden_stride = s->d_hidden;
   if (s->x_stride < s->d_in || s->hidden_stride < s->d_hidden || s->x_stride % 8 || s->hidden_stride % 8 || s->x_stride > (1ull << 36) ||
       s->hidden_stride > (1ull << 36))
-    return std::unexpected(what + ": a stride is smaller than a row, not a multiple of 8, or over 2^36");
+    return std::unexpected(std::string(what) + ": a stride is smaller than a row, not a multiple of 8, or over 2^36");
   // (the tiles of any product are numbered in 32 bits)
   if ((s->rows / 256 + 1) * (s->d_hidden / 64 + 1) > 0x7FFFFFFFull || (s->rows / 256 + 1) * (s->d_in / 128 + 1) > 0x7FFFFFFFull)
-    return std::unexpected(what + ": too many rows for these widths");
+    return std::unexpected(std::string(what) + ": too many rows for these widths");
   return {};
 }
 
@@ -65,20 +65,24 @@ struct BackwardPlan {
   uint32_t parts = 0;   // in all
 };
 struct Run { uint64_t count; double cost; };
-// The time of the pair that ends last.
+// The time of the pair that ends last: it changes from pair to pair only where a run of equal items begins or ends.
 double Longest(const Run* runs, uint32_t count, uint32_t pairs) {
-  double longest = 0.0;
-  uint64_t at[2 * 2 * k::kGatedProblems], first = 0;
+  uint32_t begin[2 * k::kGatedProblems], rest[2 * k::kGatedProblems];   // of a run: its first pair, items behind full rounds
+  double full = 0.0, longest = 0.0;
+  uint64_t first = 0;
   for (uint32_t r = 0; r < count; first += runs[r++].count) {
-    at[2 * r] = first % pairs;
-    at[2 * r + 1] = (first + runs[r].count + pairs - 1) % pairs;
+    const uint64_t rounds = runs[r].count / pairs;
+    begin[r] = static_cast<uint32_t>(first % pairs);
+    rest[r] = static_cast<uint32_t>(runs[r].count - rounds * pairs);
+    full += static_cast<double>(rounds) * runs[r].cost;
   }
-  for (uint32_t i = 0; i < 2 * count; ++i) {   // the time of a pair changes only where a run begins or ends
-    double time = 0.0;
-    first = 0;
-    for (uint32_t r = 0; r < count; first += runs[r++].count) {
-      const uint64_t behind = (at[i] + pairs - first % pairs) % pairs;
-      if (behind < runs[r].count) time += static_cast<double>((runs[r].count - behind + pairs - 1) / pairs) * runs[r].cost;
+  for (uint32_t i = 0; i < 2 * count; ++i) {
+    uint32_t pair = begin[i / 2] + (i & 1 ? rest[i / 2] + pairs - 1 : 0);
+    while (pair >= pairs) pair -= pairs;
+    double time = full;
+    for (uint32_t r = 0; r < count; ++r) {
+      const uint32_t behind = pair >= begin[r] ? pair - begin[r] : pair + pairs - begin[r];
+      if (behind < rest[r]) time += runs[r].cost;
     }
     longest = std::max(longest, time);
   }
@@ -149,45 +153,45 @@ uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden)
 
 Status CheckGatedForward(see_gated_shape* shape, const void* x, const void* w_gate, const void* w_up, const void* hidden, const void* gate,
                          const void* up) {
-  const std::string what = "cuda: gated forward";
+  const char* const what = "cuda: gated forward";
   if (auto r = CheckGated(what, shape); !r) return r;
   const see_gated_shape& s = *shape;
-  if (!gate != !up) return std::unexpected(what + ": gate and up are kept together or not at all");
+  if (!gate != !up) return std::unexpected(std::string(what) + ": gate and up are kept together or not at all");
   const uint64_t weights = s.d_in * s.d_hidden * 2, width = s.d_hidden * 2, pitch = s.hidden_stride * 2;
-  std::vector<Operand> ops = {{"x", x, s.rows, s.d_in * 2, s.x_stride * 2, 16, false},
+  Operands ops = {{"x", x, s.rows, s.d_in * 2, s.x_stride * 2, 16, false},
                               Vector("w_gate", w_gate, weights, 16, false),
                               Vector("w_up", w_up, weights, 16, false),
                               {"hidden", hidden, s.rows, width, pitch, 16, true}};
   if (gate) {
-    ops.push_back({"gate", gate, s.rows, width, pitch, 16, true});
-    ops.push_back({"up", up, s.rows, width, pitch, 16, true});
+    ops.Add({"gate", gate, s.rows, width, pitch, 16, true});
+    ops.Add({"up", up, s.rows, width, pitch, 16, true});
   }
-  return CheckOperands(what, ops);
+  return ops.Check(what);
 }
 
 Status CheckGatedBackward(see_gated_shape* shape, const void* dhidden, const void* x, const void* w_gate, const void* w_up,
                           const void* gate, const void* up, const void* dx, const void* dw_gate, const void* dw_up, const void* workspace,
                           uint64_t workspace_bytes) {
-  const std::string what = "cuda: gated backward";
+  const char* const what = "cuda: gated backward";
   if (auto r = CheckGated(what, shape); !r) return r;
   const see_gated_shape& s = *shape;
-  if (!dw_gate != !dw_up) return std::unexpected(what + ": dw_gate and dw_up are wanted together or not at all");
-  if (!dx && !dw_gate) return std::unexpected(what + ": no output is wanted");
-  if (workspace_bytes < GatedBackwardWorkspace(s.rows, s.d_in, s.d_hidden)) return std::unexpected(what + ": the workspace is too small");
+  if (!dw_gate != !dw_up) return std::unexpected(std::string(what) + ": dw_gate and dw_up are wanted together or not at all");
+  if (!dx && !dw_gate) return std::unexpected(std::string(what) + ": no output is wanted");
+  if (workspace_bytes < std::max<uint64_t>(128, 2 * SlopeBytes(s.rows, s.d_hidden))) return std::unexpected(std::string(what) + ": the workspace is too small");
   const uint64_t weights = s.d_in * s.d_hidden * 2, width = s.d_hidden * 2, pitch = s.hidden_stride * 2;
-  std::vector<Operand> ops = {{"dhidden", dhidden, s.rows, width, pitch, 16, false},
+  Operands ops = {{"dhidden", dhidden, s.rows, width, pitch, 16, false},
                               {"x", x, s.rows, s.d_in * 2, s.x_stride * 2, 16, false},
                               Vector("w_gate", w_gate, weights, 16, false),
                               Vector("w_up", w_up, weights, 16, false),
                               {"gate", gate, s.rows, width, pitch, 16, false},
                               {"up", up, s.rows, width, pitch, 16, false},
                               Vector("workspace", workspace, workspace_bytes, 128, true)};
-  if (dx) ops.push_back({"dx", dx, s.rows, s.d_in * 2, s.x_stride * 2, 16, true});
+  if (dx) ops.Add({"dx", dx, s.rows, s.d_in * 2, s.x_stride * 2, 16, true});
   if (dw_gate) {
-    ops.push_back(Vector("dw_gate", dw_gate, weights, 16, true));
-    ops.push_back(Vector("dw_up", dw_up, weights, 16, true));
+    ops.Add(Vector("dw_gate", dw_gate, weights, 16, true));
+    ops.Add(Vector("dw_up", dw_up, weights, 16, true));
   }
-  return CheckOperands(what, ops);
+  return ops.Check(what);
 }
 
 Status CudaBackend::GatedForward(const see_gated_shape& given, const void* x, const void* w_gate, const void* w_up, void* hidden, void* gate,
@@ -257,7 +261,7 @@ Status CudaBackend::GatedBackward(const see_gated_shape& given, const void* dhid
   const uint32_t rows = static_cast<uint32_t>(s.rows), d_in = static_cast<uint32_t>(s.d_in), d_hidden = static_cast<uint32_t>(s.d_hidden);
   const uint32_t pairs = std::min(sms_ / 2, kMostPairs);
   const BackwardPlan plan = PlanBackward(s.rows, s.d_in, s.d_hidden, dx != nullptr, dw_gate != nullptr, pairs);
-  if (2 * SlopeBytes(s.rows, s.d_hidden) + PartialBytes(plan) > workspace_bytes)   // (the query has counted for the most SMs there are)
+  if (2 * SlopeBytes(s.rows, s.d_hidden) + PartialBytes(plan) > workspace_bytes)
     return std::unexpected("cuda: gated backward: the workspace is too small");
   l.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 2 * SlopeBytes(s.rows, s.d_hidden));
   auto problem = [&](uint32_t M, uint32_t N, void* out, uint64_t out_stride) -> k::GatedProblem& {

@@ -18,6 +18,7 @@
 // Bound by HBM: 14 bytes an element with 16-bit gradients and moments in 8 bits, 28 in f32.  A warp takes blocks of 256
 // elements, eight a lane, that follow one another, through a ring of two in shared memory that bulk copies fill; the launch
 // carries the table of tensors as a parameter: nothing is uploaded, and a captured launch owns its copy.
+#include <atomic>
 #include <type_traits>
 
 #include "act_expr.cuh"
@@ -401,7 +402,14 @@ cudaError_t Launch(const see_adamw_tensor* tensors, uint64_t count, const AdamSt
                    DeviceStatus* status, cudaStream_t s, int* launches) {
   using R = AdamRing<kBits>;
   auto* kernel = AdamWTensorsKernel<kBits, kEntries>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes); e != cudaSuccess) return e;
+  // The shared-memory limit is a device's: one flag for each.
+  static std::atomic<bool> configured[64] = {};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes); e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
   AdamTable<kEntries> table;
   uint64_t next = 0;
   while (next < count) {

@@ -14,6 +14,8 @@
 // beside the latency, and corrected by the average deviation from the first result in NormFwdRingKernel, where it would (26.6 us
 // to 31.5 at 32768 x 768).  The variance is the average square of the deviations, a second pass over the registers, so rows far
 // from zero lose nothing to cancellation.
+#include <atomic>
+
 #include "act_expr.cuh"
 #include "block_ops.h"
 #include "launch.cuh"
@@ -26,7 +28,7 @@ namespace {
 
 constexpr uint32_t kNormThreads = 512;
 constexpr uint32_t kWideThreads = 768;
-constexpr size_t kRingBytes = 200 * 1024;   // of a block
+constexpr size_t kRingBytes = 200 * 1024, kMostShared = 224 * 1024;   // of a block
 
 template <bool kBoth>
 __device__ __forceinline__ float2 WarpSum(float2 v) {
@@ -589,9 +591,20 @@ cudaError_t Fold(const NormArgs& a, uint64_t grid, cudaStream_t s, int* launches
   ++*launches;
   return Next(NormFoldKernel, dim3((a.cols + 31) / 32, kRms ? 1 : 2), 1024, 0, s)(a.partials, a.dgamma, a.dbeta, static_cast<uint32_t>(grid), a.cols);
 }
-template <typename K>
-cudaError_t AllowShared(K* kernel, size_t bytes) {   // (the static part counts too)
-  return bytes > 32 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) : cudaSuccess;
+// A kernel's limit of shared memory is a device's: what has been granted is remembered for each (the call takes the driver a
+// microsecond or two).
+template <auto kKernel>
+cudaError_t AllowShared(size_t bytes) {
+  if (bytes <= 32 * 1024) return cudaSuccess;   // (the static part counts too)
+  static std::atomic<size_t> granted[64] = {};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && granted[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  // (grants only grow: the most that any call asks for)
+  if (cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostShared)); e != cudaSuccess)
+    return e;
+  if (dev >= 0 && dev < 64) granted[dev].store(kMostShared, std::memory_order_release);
+  return cudaSuccess;
 }
 uint64_t Blocks(uint64_t rows, uint32_t groups, uint32_t sms) {
   const uint64_t blocks = (rows + groups - 1) / groups, most = sms < kNormPartials ? sms : kNormPartials;
@@ -606,8 +619,8 @@ cudaError_t RunRing(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s,
   uint32_t slots = static_cast<uint32_t>(kRingBytes / (groups * row_bytes));
   slots = slots < 1 ? 1 : slots > 8 ? 8 : slots;
   const size_t smem = groups * slots * (row_bytes + 8);
-  auto* kernel = NormBwdRingKernel<XT, YT, kRms, NV, kThreads>;
-  if (cudaError_t e = AllowShared(kernel, smem); e != cudaSuccess) return e;
+  constexpr auto* kernel = NormBwdRingKernel<XT, YT, kRms, NV, kThreads>;
+  if (cudaError_t e = AllowShared<kernel>(smem); e != cudaSuccess) return e;
   const uint64_t grid = Blocks(a.rows, groups, sms);
   if (cudaError_t e = Next(kernel, static_cast<unsigned>(grid), groups * T, smem, s)(a, T, slots); e != cudaSuccess) return e;
   return Fold<kRms>(a, grid, s, launches);
@@ -621,8 +634,8 @@ cudaError_t RunFwdRing(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t
   uint32_t slots = static_cast<uint32_t>((kRingBytes - weights) / (groups * row_bytes));   // (one at least, up to 8192 columns)
   slots = slots > 8 ? 8 : slots;
   const size_t smem = groups * slots * (row_bytes + 8) + weights;
-  auto* kernel = NormFwdRingKernel<XT, YT, kRms, NV, kHold>;
-  if (cudaError_t e = AllowShared(kernel, smem); e != cudaSuccess) return e;
+  constexpr auto* kernel = NormFwdRingKernel<XT, YT, kRms, NV, kHold>;
+  if (cudaError_t e = AllowShared<kernel>(smem); e != cudaSuccess) return e;
   return Next(kernel, static_cast<unsigned>(Blocks(a.rows, groups, sms)), groups * T, smem, s)(a, T, slots);
 }
 
@@ -634,9 +647,9 @@ cudaError_t Run(const NormArgs& a, uint32_t T, cudaStream_t s) {
 template <typename XT, typename YT, bool kRms, int NV>
 cudaError_t RunSingles(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s, int* launches) {
   const uint32_t groups = kNormThreads / T;
-  auto* kernel = NormBwdKernel<XT, YT, kRms, 1, NV>;
+  constexpr auto* kernel = NormBwdKernel<XT, YT, kRms, 1, NV>;
   const size_t smem = static_cast<size_t>(groups) * a.cols * 4;
-  if (cudaError_t e = AllowShared(kernel, smem); e != cudaSuccess) return e;
+  if (cudaError_t e = AllowShared<kernel>(smem); e != cudaSuccess) return e;
   const uint64_t grid = Blocks(a.rows, groups, sms);
   if (cudaError_t e = Next(kernel, static_cast<unsigned>(grid), groups * T, smem, s)(a, T); e != cudaSuccess) return e;
   return Fold<kRms>(a, grid, s, launches);

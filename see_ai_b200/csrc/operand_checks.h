@@ -6,8 +6,8 @@
 
 #include <cstdint>
 #include <expected>
+#include <initializer_list>
 #include <string>
-#include <vector>
 
 #include "../../include/see_cuda.h"
 
@@ -58,21 +58,35 @@ inline bool Overlap(const Operand& a, const Operand& b) {
   return true;
 }
 
-// Null, misaligned, too large, or overlapping something that is written.
-inline Status CheckOperands(const std::string& what, const std::vector<Operand>& ops) {
-  for (const Operand& o : ops) {
-    if (!o.p) return std::unexpected(what + ": " + o.name + " is null");
-    if (o.begin() % o.align) return std::unexpected(what + ": " + o.name + " is not aligned");
-    uint64_t span;
-    if (__builtin_mul_overflow(o.rows, o.pitch, &span) || span > (1ull << 56) || o.width > (1ull << 56) || o.begin() > (1ull << 57))
-      return std::unexpected(what + ": " + o.name + " is too large");
+// A call's operands, without allocation: these checks are part of calls of a few microseconds.
+class Operands {
+ public:
+  Operands(std::initializer_list<Operand> list) {
+    for (const Operand& o : list) Add(o);
   }
-  for (size_t i = 0; i < ops.size(); ++i)
-    for (size_t j = i + 1; j < ops.size(); ++j)
-      if ((ops[i].written || ops[j].written) && Overlap(ops[i], ops[j]))
-        return std::unexpected(what + ": " + ops[i].name + " and " + ops[j].name + " overlap");
-  return {};
-}
+  void Add(const Operand& o) { ops_[count_++] = o; }
+  // Null, misaligned, too large, or overlapping something that is written.
+  Status Check(const char* what) const {
+    auto refuse = [what](const std::string& why) { return std::unexpected(std::string(what) + ": " + why); };
+    for (size_t i = 0; i < count_; ++i) {
+      const Operand& o = ops_[i];
+      if (!o.p) return refuse(std::string(o.name) + " is null");
+      if (o.begin() % o.align) return refuse(std::string(o.name) + " is not aligned");
+      uint64_t span;
+      if (__builtin_mul_overflow(o.rows, o.pitch, &span) || span > (1ull << 56) || o.width > (1ull << 56) || o.begin() > (1ull << 57))
+        return refuse(std::string(o.name) + " is too large");
+    }
+    for (size_t i = 0; i < count_; ++i)
+      for (size_t j = i + 1; j < count_; ++j)
+        if ((ops_[i].written || ops_[j].written) && Overlap(ops_[i], ops_[j]))
+          return refuse(std::string(ops_[i].name) + " and " + ops_[j].name + " overlap");
+    return {};
+  }
+
+ private:
+  Operand ops_[12];
+  size_t count_ = 0;
+};
 
 }  // namespace see
 
