@@ -15,9 +15,12 @@
 // (i phi + t sqrt(2)) mod 1 (phi the golden section), spread evenly over elements and over steps.  A root that is not zero
 // is held as at least the smallest e4m3: a zero would let a later step divide by eps alone.
 //
-// Bound by HBM: 14 bytes an element with 16-bit gradients and moments in 8 bits, 28 in f32.  A warp takes blocks of 256
-// elements, eight a lane, that follow one another, through a ring of two in shared memory that bulk copies fill; the launch
-// carries the table of tensors as a parameter: nothing is uploaded, and a captured launch owns its copy.
+// Bound by HBM: 14 bytes an element with 16-bit gradients and moments in 8 bits (16 with a 16-bit copy), 28 in f32.  A warp
+// takes blocks of 256 elements, eight a lane, through a ring of two in shared memory that bulk copies fill: the loads of a step
+// straight into registers left half of the bandwidth unused (587 us of 110 million weights, 304 now: 5.8 TB/s).  Of the
+// instructions, which came next, the roots, quotients and conversions went to the hardware's approximations with a Newton step,
+// and to two elements at once.  The launch carries the table of tensors as a parameter: nothing is uploaded, and a captured
+// launch owns its copy.
 #include <atomic>
 #include <type_traits>
 
@@ -56,7 +59,8 @@ struct AdamRing {
   static constexpr uint32_t kStateBytes = kAdamBlock * kBits / 8;
   static constexpr uint32_t kM = kAdamBlock * 4, kV = kM + kStateBytes, kG = kV + kStateBytes;   // offsets in a slot
   static constexpr uint32_t kSlotBytes = kG + kAdamBlock * 4;
-  static constexpr uint32_t kWarps = kBits == 8 ? 32 : 24, kSlots = 2;
+  // 110 million weights with moments in 8 bits, us: 20 warps 320, 22 310, 23 304, 24 322, 28 337, 32 383.
+  static constexpr uint32_t kWarps = kBits == 8 ? 23 : 24, kSlots = 2;
   static constexpr uint32_t kBytes = kWarps * kSlots * (kSlotBytes + 8);
 };
 
@@ -167,10 +171,9 @@ __device__ __forceinline__ BlockScale ScaleOf(uint32_t largest_bits) {
 // more is read.
 template <int kBits, bool kWhole, typename Read>
 __device__ __forceinline__ void StepBlock(const AdamEntry& e, uint64_t block, const uint8_t* src, const AdamStepScalars& a, float gs,
-                                          uint32_t lane, Read read) {
+                                          uint32_t lane, [[maybe_unused]] float m_scale, [[maybe_unused]] float v_scale, Read read) {
   using R = AdamRing<kBits>;
   const uint64_t base = block * kAdamBlock;
-  [[maybe_unused]] const float m_scale = kBits == 8 ? e.m_scale[block] : 0.0f, v_scale = kBits == 8 ? e.v_scale[block] : 0.0f;
   // Element j of a lane: four consecutive ones in each half of the block, or single ones 32 apart.
   auto at = [&](int j) -> uint64_t { return kWhole ? base + (j >> 2) * 128 + lane * 4 + (j & 3) : base + j * 32 + lane; };
   float p[8], g[8], m[8], v[8];
@@ -297,9 +300,9 @@ __device__ __forceinline__ void StepBlock(const AdamEntry& e, uint64_t block, co
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(e.v) + i) = vc[2 * h] | vc[2 * h + 1] << 16;
       }
       if (e.copy_type != SEE_F32) {
-        const bool bf = e.copy_type == SEE_BF16;
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(e.copy) + i) =
-            make_uint2(bf ? Pack2<Bf16>(q[0], q[1]) : Pack2<F16>(q[0], q[1]), bf ? Pack2<Bf16>(q[2], q[3]) : Pack2<F16>(q[2], q[3]));
+        uint2* to = reinterpret_cast<uint2*>(static_cast<uint16_t*>(e.copy) + i);
+        if (e.copy_type == SEE_BF16) *to = make_uint2(Pack2<Bf16>(q[0], q[1]), Pack2<Bf16>(q[2], q[3]));
+        else *to = make_uint2(Pack2<F16>(q[0], q[1]), Pack2<F16>(q[2], q[3]));
       }
     }
   } else {
@@ -336,41 +339,51 @@ AdamWTensorsKernel(const __grid_constant__ AdamTable<kEntries> table, const Adam
   }
   __syncwarp();
   AwaitPrevious();
-  // All warps sweep the list together, a thread block's warps side by side: what is under way at one time lies together in
-  // memory (110 million weights: 329 us, with a range of the list to each warp 347).  A list that one sweep covers is spread over
-  // the SMs instead.
-  const uint32_t blocks = table.block_end[table.count - 1], warps = gridDim.x * R::kWarps;
-  const uint32_t first = blocks > warps ? blockIdx.x * R::kWarps + warp : warp * gridDim.x + blockIdx.x;
-  if (first >= blocks) return;
+  // A thread block's warps sweep its range of the list side by side (a range to each warp, or one sweep of all, 330 to 350 us); a
+  // list that one sweep of all covers is spread over the SMs instead.
+  const uint32_t blocks = table.block_end[table.count - 1], all = gridDim.x * R::kWarps;
+  const uint32_t each = blocks / gridDim.x, rest = blocks % gridDim.x, begin = blockIdx.x * each + min(blockIdx.x, rest);
+  const uint32_t end = blocks > all ? begin + each + (blockIdx.x < rest) : blocks, warps = blocks > all ? R::kWarps : all;
+  const uint32_t first = blocks > all ? begin + warp : warp * gridDim.x + blockIdx.x;
+  if (first >= end) return;
   AdamCursor<kEntries> now, ahead;
   now.Find(table, first);
   ahead = now;
-  // Lanes 0 to 3 fill a slot with p, m, v and g: each keeps where its operand of the current tensor lies, so that a fill is a
-  // handful of instructions of the warp.  A block that the copies cannot take is read where it lies.
+  // Lanes 0 to 3 fill a slot with p, m, v and g, lanes 4 and 5 ask for the block's two scales: each keeps where its operand of the
+  // current tensor lies, so that a fill is a handful of instructions of the warp.  A block that the copies cannot take is read
+  // where it lies.
   const uint8_t* source = nullptr;
-  uint32_t bytes = 0, total = 0, offset = 0, fillable = 0;   // of a block of mine, of all four; in the slot; whole blocks
+  uint32_t bytes = 0, total = 0, offset = 0, fillable = 0;   // of a block of mine, of the first four; in the slot; whole blocks
   auto look_up = [&] {
     const AdamEntry& e = table.entry[ahead.entry];
     const uint32_t g_bytes = kAdamBlock * (e.g_type == SEE_F32 ? 4 : 2);
-    const void* mine = lane == 0 ? static_cast<const void*>(e.p) : lane == 1 ? e.m : lane == 2 ? e.v : e.g;
-    source = static_cast<const uint8_t*>(mine);
-    bytes = lane == 0 ? kAdamBlock * 4 : lane < 3 ? R::kStateBytes : g_bytes;
-    offset = lane == 0 ? 0 : lane == 1 ? R::kM : lane == 2 ? R::kV : R::kG;
+    const void* const operands[6] = {e.p, e.m, e.v, e.g, e.m_scale, e.v_scale};
+    const uint32_t sizes[6] = {kAdamBlock * 4, R::kStateBytes, R::kStateBytes, g_bytes, 4, 4}, offsets[6] = {0, R::kM, R::kV, R::kG, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 6; ++i)
+      if (lane == i) {
+        source = static_cast<const uint8_t*>(operands[i]);
+        bytes = sizes[i];
+        offset = offsets[i];
+      }
     total = R::kG + g_bytes;
     fillable = e.wide ? static_cast<uint32_t>(e.n / kAdamBlock) : 0;
   };
   look_up();
+  static_assert(R::kSlots == 2);
+  [[maybe_unused]] float scale0 = 0.0f, scale1 = 0.0f;   // of the block in either slot: m's in lane 4, v's in lane 5
   auto fill = [&](uint32_t f, uint32_t slot) {
     if (f >= ahead.end) {
       ahead.MoveTo(table, f);
       look_up();
     }
     const uint32_t block = f - ahead.begin;
+    if (kBits == 8 && (lane == 4 || lane == 5)) (slot ? scale1 : scale0) = *reinterpret_cast<const float*>(source + static_cast<uint64_t>(block) * 4);
     if (block >= fillable) return;
     if (lane == 0) umma_dev::MbarExpectTx(&bars[slot], total);
     if (lane < 4) umma_dev::BulkLoad(ring + slot * R::kSlotBytes + offset, source + static_cast<uint64_t>(block) * bytes, bytes, &bars[slot]);
   };
-  const uint32_t count = (blocks - first + warps - 1) / warps;   // mine
+  const uint32_t count = (end - first + warps - 1) / warps;   // mine
   for (uint32_t i = 0; i < R::kSlots && i < count; ++i) fill(first + i * warps, i);
   const float gs = grad_scale ? *grad_scale : 1.0f;
   uint32_t slot = 0, parities = 0;   // a bit for each slot
@@ -391,8 +404,9 @@ AdamWTensorsKernel(const __grid_constant__ AdamTable<kEntries> table, const Adam
       __syncwarp();
       if (i + R::kSlots < count) fill(f + R::kSlots * warps, slot);
     };
-    if (whole) StepBlock<kBits, true>(e, block, ring + slot * R::kSlotBytes, a, gs, lane, read);
-    else StepBlock<kBits, false>(e, block, nullptr, a, gs, lane, read);
+    const float scale = slot ? scale1 : scale0, m_scale = __shfl_sync(0xFFFFFFFFu, scale, 4), v_scale = __shfl_sync(0xFFFFFFFFu, scale, 5);
+    if (whole) StepBlock<kBits, true>(e, block, ring + slot * R::kSlotBytes, a, gs, lane, m_scale, v_scale, read);
+    else StepBlock<kBits, false>(e, block, nullptr, a, gs, lane, m_scale, v_scale, read);
     slot = slot + 1 < R::kSlots ? slot + 1 : 0;
   }
 }
