@@ -246,14 +246,14 @@ int see_cuda_gated_backward(see_cuda_backend* h, const see_gated_shape* shape, c
                             const void* w_gate, const void* w_up, const void* gate, const void* up, void* dx,
                             void* dw_gate, void* dw_up, void* workspace, uint64_t workspace_bytes);
 
-/* One AdamW step over `count` tensors of n elements each, in the kAdamWStep instruction's expression.  p: f32 weights.
+/* One AdamW step over `count` tensors of n elements (up to 2^38) each, in the kAdamWStep instruction's expression.  p: f32 weights.
  * g: their gradients.  copy: the new weights in 16 bits (copy_type SEE_BF16 or SEE_F16), or NULL with copy_type SEE_F32.
  * state_bits 32: m, v f32 moments.  state_bits 8: m and v are e4m3 (one byte an element), v holding the ROOT of the second
  * moment; m_scale, v_scale: an f32 for each block of SEE_ADAMW_BLOCK elements (the last may be short), whose product with
  * an element is its value.  All zero bytes are the state before the first step.  A moment that is not finite makes its
  * block's NaN.  The 8-bit rounding cuts at a point that depends on element and params->step alone.
  * flags: SEE_ADAMW_NO_DECAY: weight decay 0.  grad_scale: an f32 that every gradient is multiplied by first, or NULL.
- * `tensors` and `params` are HOST memory and are read before the call returns.  p, m, v, the scales and copy of all
+ * `tensors` and `params` are HOST memory and are read before the call returns (a captured call keeps their values, the step too).  p, m, v, the scales and copy of all
  * tensors are written and may not overlap. */
 enum { SEE_ADAMW_BLOCK = 256 };
 enum { SEE_ADAMW_NO_DECAY = 1 };

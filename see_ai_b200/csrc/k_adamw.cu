@@ -433,7 +433,7 @@ cudaError_t Launch(const see_adamw_tensor* tensors, uint64_t count, const AdamSt
       const see_adamw_tensor& t = tensors[next];
       if (t.n == 0) continue;
       const uint64_t more = (t.n + kAdamBlock - 1) / kAdamBlock;
-      if (blocks + more > 0xFFFFFFFFull) break;   // (one tensor alone has fewer)
+      if (blocks + more > 0x7FFFFFFFull) break;   // (one tensor alone has at most half as many)
       auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
       AdamEntry& e = table.entry[table.count];
       e = {t.p, t.g, t.m, t.v, t.m_scale, t.v_scale, t.copy, t.n, static_cast<uint8_t>(t.g_type), static_cast<uint8_t>(t.copy_type),

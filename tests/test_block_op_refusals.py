@@ -32,7 +32,7 @@ EXPECTED = {
     "adamw": None, "adamw 32": None, "adamw bits": "8 or 32 bits", "adamw step": "count from 1", "adamw beta": "beta1 and beta2",
     "adamw g_type": "tensor 1: unknown type", "adamw copy": "tensor 1: a copy", "adamw no copy": None, "adamw flag": "tensor 2: unknown flag",
     "adamw null": "tensor 2: v is null", "adamw scale null": "tensor 0: m_scale is null", "adamw aligned": "tensor 0: p is not aligned",
-    "adamw large": "2^39", "adamw twice": "overlap", "adamw into": "overlap", "adamw p over g": "overlap", "adamw same g": None,
+    "adamw large": "2^38", "adamw twice": "overlap", "adamw into": "overlap", "adamw p over g": "overlap", "adamw same g": None,
     "adamw descending": None, "adamw interleaved": None, "adamw scale in p": "overlap", "adamw scale": None,
     "adamw scale aligned": "grad_scale is not aligned", "adamw empty tensor": None, "adamw none": None, "adamw no table": "tensors is null",
     "handle": None, "handle gated": None, "handle adamw": None,
