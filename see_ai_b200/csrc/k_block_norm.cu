@@ -1,7 +1,9 @@
 // Layer norm and root-mean-square norm of rows in f32, bf16 or f16, and their backward pass with the gradients of the
 // weights.  With u = (x - mean) rstd (rms: mean = 0), q = dy gamma and <.> a row's average:
 //   y = u gamma + beta,   dx = rstd (q - <q> - u <q u>) (+ addend),   dgamma = sum over rows of dy u,   dbeta = of dy
-// (rms: neither beta nor <q>).  Bound by HBM: each matrix is read or written once.
+// (rms: neither beta nor <q>).  Bound by HBM: each matrix is read or written once.  Layer norm of 32768 x 768, f32 and bf16,
+// backward with an addend: 61 us, 5.8 TB/s (loads straight into registers: 84); forward 27 us, 5.6 TB/s.  16384 x 4096 in bf16
+// backward: rms 72 us, 5.6 TB/s; layer 90 us, 4.5, short of issue slots beside a row's three barriers.
 //
 // A row belongs to a group of T threads (a multiple of 32), which hold it in registers, four or eight consecutive columns at a
 // time where widths, strides and addresses allow 16-byte accesses and single columns T apart otherwise; a block has several

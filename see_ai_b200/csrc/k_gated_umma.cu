@@ -6,12 +6,18 @@
 // receives its 128 rows.  Forward: the even CTA's half of B is the gate's columns and the odd one's the up projection's, so
 // one MMA makes both, and column j's two factors lie kTN / 2 columns apart in one thread's lane: the activation and the
 // product need no exchange.  The accumulator is double-buffered: a tile's epilogue (eight warps) runs under the next one's
-// products.
+// products.  (Sixteen warps with slabs of 32 columns: 32768 x 768 x 2048 177 us / 219, for rows of 64 bytes leave worse.)
 //
 // No operand is ever transposed or copied: x, the weights [d_in, d_hidden] and dg, du lie as the caller has them, and a box of
 // 64 x 64 elements under the 128-byte swizzle is a K-major operand where the reduction runs along its rows and an MN-major one
 // where it runs down its columns (one descriptor bit).  x is K-major forward and MN-major for dW; the weights are MN-major
 // forward and K-major for dx.
+//
+// Bound by the tensor pipe: 256 x 256 x 64 of a pair are 512 cycles.  4096 x 4096 x 4096 forward, gate and up kept: 191 us,
+// 1440 TFLOP/s where cuBLAS did one of the two products at 1230 on the same board; busy 66 to 75 % of a launch's cycles under the
+// profiler.  With d_in = 768 a tile's products (6100 cycles) are shorter than its three stores: 32768 x 768 x 2048 177 us, 152
+// without gate and up.  dg and du are rounded to the operands' 16 bits between the passes, as the products take them: half a step
+// of each term, which leaves dx and dW 1.4 times one rounding's error.
 #include <atomic>
 
 #include "gated_act.cuh"
