@@ -145,7 +145,7 @@ uint64_t PartialBytes(const BackwardPlan& plan) { return plan.parts * 256ull * 2
 uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden) {
   if (d_in == 0 || d_hidden == 0 || d_in % 8 || d_hidden % 8 || d_in > (1u << 20) || d_hidden > (1u << 20) || rows > 0x7FFFFF00ull) return 0;
   if (rows == 0) return 128;
-  uint64_t partials = 0;   // whichever gradients are wanted, on however few SMs
+  uint64_t partials = 0;   // whichever gradients are wanted, on 148 SMs
   for (int want = 1; want < 4; ++want)
     partials = std::max(partials, PartialBytes(PlanBackward(rows, d_in, d_hidden, want & 1, want & 2, kMostPairs)));
   return 2 * SlopeBytes(rows, d_hidden) + partials;

@@ -14,7 +14,7 @@
 // forward and K-major for dx.
 //
 // Bound by the tensor pipe: 256 x 256 x 64 of a pair are 512 cycles.  4096 x 4096 x 4096 forward, gate and up kept: 191 us,
-// 1440 TFLOP/s where cuBLAS did one of the two products at 1230 on the same board; busy 66 to 75 % of a launch's cycles under the
+// 1440 TFLOP/s, where the library's product did one of the two at 1230 on the same board; busy 66 to 75 % of a launch's cycles under the
 // profiler.  With d_in = 768 a tile's products (6100 cycles) are shorter than its three stores: 32768 x 768 x 2048 177 us, 152
 // without gate and up.  dg and du are rounded to the operands' 16 bits between the passes, as the products take them: half a step
 // of each term, which leaves dx and dW 1.4 times one rounding's error.
