@@ -456,6 +456,149 @@ NormBwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots
   }
 }
 
+// ---- rows of any width and alignment through the ring ----------------------------------------
+// A bulk copy begins and ends on 16 bytes: a row is copied with what lies beside it up to there, which for all but the first and
+// the last row (or rows, where they are shorter than that) lies within the matrix, its neighbours' ends or what is between them,
+// and is used from where it begins.  The others are copied element by element.  Threads then take single columns, T apart.
+// Straight into registers / so, us: 30000 x 1029 f32 155 / 144, bf16 295 / 127; 8000 x 5003 f32 and bf16 566 / 215;
+// 40373 x 55 f32 and f16 with an addend 34 / 23.
+template <typename T>
+struct OddRow {
+  const uint8_t* from;   // 16-byte aligned, at most 15 bytes before the row
+  uint32_t skip, bytes;  // ... in front of it; to copy, a multiple of 16
+  __device__ __forceinline__ OddRow(const void* base, uint64_t row, uint64_t stride, uint32_t cols) {
+    const uint64_t at = reinterpret_cast<uint64_t>(static_cast<const T*>(base) + row * stride);
+    skip = static_cast<uint32_t>(at & 15);
+    from = reinterpret_cast<const uint8_t*>(at - skip);
+    bytes = (skip + cols * static_cast<uint32_t>(sizeof(T)) + 15) & ~15u;
+  }
+};
+template <typename T> __host__ __device__ constexpr uint32_t OddSlot(uint32_t cols) { return (cols * sizeof(T) + 45) / 16 * 16; }
+
+// Element-wise, by the whole group; the caller synchronises.
+template <typename T>
+__device__ __forceinline__ void CopyRow(uint8_t* slot, const void* base, uint64_t row, uint64_t stride, uint32_t cols, uint32_t t, uint32_t threads) {
+  const T* from = static_cast<const T*>(base) + row * stride;
+  T* to = reinterpret_cast<T*>(slot + (reinterpret_cast<uint64_t>(from) & 15));
+  for (uint32_t c = t; c < cols; c += threads) to[c] = from[c];
+}
+
+// NV single columns a thread.
+template <typename XT, typename YT, bool kRms, int NV>
+__global__ void __launch_bounds__(kNormThreads, 1)
+NormBwdOddKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots) {
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ float2 sums[2][kWideThreads / 32];
+  const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
+  const uint32_t x_slot = OddSlot<XT>(a.cols), y_slot = OddSlot<YT>(a.cols), slot_bytes = x_slot + y_slot + (a.addend ? x_slot : 0);
+  uint8_t* ring = dyn + static_cast<size_t>(group) * slots * slot_bytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + static_cast<size_t>(groups) * slots * slot_bytes) + group * slots;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * groups + group, step = static_cast<uint64_t>(gridDim.x) * groups;
+  if (t == 0) {
+    for (uint32_t i = 0; i < slots; ++i) umma_dev::MbarInit(&bars[i], 1);
+    umma_dev::MbarInitFence();
+  }
+  // Rows with 16 bytes of the matrix on either side.
+  const uint64_t narrow = min(a.x_stride * sizeof(XT), a.y_stride * sizeof(YT)), edge = (15 + narrow) / narrow;
+  auto inner = [&](uint64_t row) { return row >= edge && row + edge < a.rows; };
+  auto fill = [&](uint64_t row, uint32_t slot) {   // the group's thread 0
+    if (!inner(row)) return;
+    umma_dev::FenceProxyAsync();   // (an edge row's elements may have been written there)
+    uint8_t* dst = ring + static_cast<size_t>(slot) * slot_bytes;
+    const OddRow<XT> x(a.x, row, a.x_stride, a.cols);
+    const OddRow<YT> dy(a.dy, row, a.y_stride, a.cols);
+    const OddRow<XT> add(a.addend, row, a.x_stride, a.cols);
+    umma_dev::MbarExpectTx(&bars[slot], x.bytes + dy.bytes + (a.addend ? add.bytes : 0));
+    umma_dev::BulkLoad(dst, x.from, x.bytes, &bars[slot]);
+    umma_dev::BulkLoad(dst + x_slot, dy.from, dy.bytes, &bars[slot]);
+    if (a.addend) umma_dev::BulkLoad(dst + x_slot + y_slot, add.from, add.bytes, &bars[slot]);
+  };
+  AwaitPrevious();
+  if (t == 0)
+    for (uint32_t i = 0; i < slots && first + i * step < a.rows; ++i) fill(first + i * step, i);
+  float gamma[NV], sum_g[NV], sum_b[kRms ? 1 : NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    gamma[i] = t + i * T < a.cols ? a.gamma[t + i * T] : 0.0f;
+    sum_g[i] = 0.0f;
+    if (!kRms) sum_b[i] = 0.0f;
+  }
+  GroupBarrier(T, group);   // the barriers are there
+  const float per_col = 1.0f / static_cast<float>(a.cols);
+  uint32_t turn = 0, slot = 0, parities = 0;   // a bit for each slot, of the copies that went through it
+  float next_rstd = 0.0f, next_mean = 0.0f;
+  if (first < a.rows) {
+    next_rstd = a.rstd[first];
+    if (!kRms) next_mean = a.mean[first];
+  }
+  for (uint64_t row = first; row < a.rows; row += step) {
+    const float rstd = next_rstd, mean = next_mean;
+    if (row + step < a.rows) {
+      next_rstd = a.rstd[row + step];
+      if (!kRms) next_mean = a.mean[row + step];
+    }
+    uint8_t* at = ring + static_cast<size_t>(slot) * slot_bytes;
+    if (inner(row)) {
+      AwaitRow(&bars[slot], parities >> slot & 1u, a.status);
+      parities ^= 1u << slot;
+    } else {
+      CopyRow<XT>(at, a.x, row, a.x_stride, a.cols, t, T);
+      CopyRow<YT>(at + x_slot, a.dy, row, a.y_stride, a.cols, t, T);
+      if (a.addend) CopyRow<XT>(at + x_slot + y_slot, a.addend, row, a.x_stride, a.cols, t, T);
+      GroupBarrier(T, group);
+    }
+    const XT* x = reinterpret_cast<const XT*>(at + OddRow<XT>(a.x, row, a.x_stride, a.cols).skip);
+    const YT* dy = reinterpret_cast<const YT*>(at + x_slot + OddRow<YT>(a.dy, row, a.y_stride, a.cols).skip);
+    const XT* add = reinterpret_cast<const XT*>(at + x_slot + y_slot + OddRow<XT>(a.addend, row, a.x_stride, a.cols).skip);
+    float u[NV], d[NV];
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = t + i * T;
+      if (c < a.cols) {
+        u[i] = (ToF32(x[c]) - mean) * rstd;
+        const float dv = ToF32(dy[c]);
+        sum_g[i] += dv * u[i];
+        if (!kRms) sum_b[i] += dv;
+        d[i] = dv * gamma[i];
+        sum.x += d[i] * u[i];
+        if (!kRms) sum.y += d[i];
+      }
+    }
+    sum = GroupSum<!kRms>(sum, T, group, sums, turn);
+    sum.x *= per_col;
+    sum.y *= per_col;
+    XT* dx = static_cast<XT*>(a.dx) + row * a.x_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = t + i * T;
+      if (c < a.cols) {
+        const float r = rstd * (kRms ? d[i] - u[i] * sum.x : d[i] - sum.y - u[i] * sum.x);
+        dx[c] = FromF32<XT>(a.addend ? r + ToF32(add[c]) : r);
+      }
+    }
+    GroupBarrier(T, group);   // the slot is read
+    if (t == 0 && row + slots * step < a.rows) fill(row + slots * step, slot);
+    if (++slot == slots) slot = 0;
+  }
+  float* meet = reinterpret_cast<float*>(dyn);   // [groups][cols]; every copy has been read
+  float* out_g = gridDim.x == 1 ? a.dgamma : a.partials + static_cast<size_t>(blockIdx.x) * a.cols;
+  float* out_b = gridDim.x == 1 ? a.dbeta : a.partials + static_cast<size_t>(gridDim.x + blockIdx.x) * a.cols;
+#pragma unroll
+  for (int which = 0; which < (kRms ? 1 : 2); ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (t + i * T < a.cols) meet[group * a.cols + t + i * T] = which ? sum_b[kRms ? 0 : i] : sum_g[i];
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+      float s = meet[c];
+      for (uint32_t r = 1; r < groups; ++r) s += meet[r * a.cols + c];
+      (which ? out_b : out_g)[c] = s;
+    }
+  }
+}
+
 // One row of partial sums a block; a lone block writes the gradients themselves.
 template <typename XT, typename YT, bool kRms, int VEC, int NV>
 __global__ void __launch_bounds__(kNormThreads, 1)
@@ -647,6 +790,21 @@ cudaError_t Run(const NormArgs& a, uint32_t T, cudaStream_t s) {
   return Next(NormFwdKernel<XT, YT, kRms, VEC, NV>, static_cast<unsigned>((a.rows + groups - 1) / groups), groups * T, 0, s)(a, T);
 }
 template <typename XT, typename YT, bool kRms, int NV>
+cudaError_t RunOdd(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s, int* launches) {
+  const size_t slot_bytes = OddSlot<XT>(a.cols) * (a.addend ? 2 : 1) + OddSlot<YT>(a.cols);
+  uint32_t groups = kNormThreads / T;
+  while (groups > 1 && 2 * groups * slot_bytes > kRingBytes) --groups;   // two slots to a group, unless it is alone
+  uint32_t slots = static_cast<uint32_t>(kRingBytes / (groups * slot_bytes));
+  slots = slots < 1 ? 1 : slots > 8 ? 8 : slots;
+  const size_t smem = groups * slots * (slot_bytes + 8);
+  constexpr auto* kernel = NormBwdOddKernel<XT, YT, kRms, NV>;
+  if (cudaError_t e = AllowShared<kernel>(smem); e != cudaSuccess) return e;
+  const uint64_t grid = Blocks(a.rows, groups, sms);
+  if (cudaError_t e = Next(kernel, static_cast<unsigned>(grid), groups * T, smem, s)(a, T, slots); e != cudaSuccess) return e;
+  return Fold<kRms>(a, grid, s, launches);
+}
+
+template <typename XT, typename YT, bool kRms, int NV>
 cudaError_t RunSingles(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s, int* launches) {
   const uint32_t groups = kNormThreads / T;
   constexpr auto* kernel = NormBwdKernel<XT, YT, kRms, 1, NV>;
@@ -693,11 +851,18 @@ cudaError_t Pick(const NormArgs& a, bool backward, uint32_t sms, cudaStream_t s,
     }
   }
   if (backward) {
-    switch (f.nv) {
-      case 8: return RunSingles<XT, YT, kRms, 8>(a, f.T, sms, s, launches);
-      case 16: return RunSingles<XT, YT, kRms, 16>(a, f.T, sms, s, launches);
-      default: return RunSingles<XT, YT, kRms, 32>(a, f.T, sms, s, launches);
+    // Few rows are over before a ring pays (777 x 1029: 8.6 us straight into registers, 14.9), and the widest have no room for one.
+    if (a.cols > 8192 || a.rows <= 4ull * sms * (kNormThreads / f.T)) {
+      switch (f.nv) {
+        case 8: return RunSingles<XT, YT, kRms, 8>(a, f.T, sms, s, launches);
+        case 16: return RunSingles<XT, YT, kRms, 16>(a, f.T, sms, s, launches);
+        default: return RunSingles<XT, YT, kRms, 32>(a, f.T, sms, s, launches);
+      }
     }
+    const uint32_t T = a.cols <= 512 ? 32 : (a.cols + 511) / 512 * 32, each = (a.cols + T - 1) / T;
+    if (each <= 2) return RunOdd<XT, YT, kRms, 2>(a, T, sms, s, launches);
+    if (each <= 4) return RunOdd<XT, YT, kRms, 4>(a, T, sms, s, launches);
+    return each <= 8 ? RunOdd<XT, YT, kRms, 8>(a, T, sms, s, launches) : RunOdd<XT, YT, kRms, 16>(a, T, sms, s, launches);
   }
   switch (f.nv) {
     case 8: return Run<XT, YT, kRms, 1, 8>(a, f.T, s);

@@ -135,7 +135,8 @@ def stats(kind, x, eps=1e-5):
 @pytest.mark.parametrize("rows,cols,add", [(1, 1, True), (1, 768, False), (3, 7, True), (17, 33, False), (2500, 256, True),
                                            (4097, 768, True), (640, 1000, True), (777, 1029, True), (333, 4096, False),
                                            (9, 4104, True), (20, 8200, False), (3, 12001, True), (302, 16384, True),
-                                           (155, 16383, False), (700, 64, False)])
+                                           (155, 16383, False), (700, 64, False), (9600, 1, True), (9500, 3, False),
+                                           (9501, 55, True), (6000, 333, True), (2400, 1029, False), (700, 5003, True), (593, 8191, True)])
 def test_backward(be, kind, rows, cols, add, xt, yt):
     torch.manual_seed(rows * 31 + cols)
     x = (torch.randn(rows, cols, device="cuda") * 2 + 0.5).to(DTYPES[xt])
@@ -259,3 +260,26 @@ def test_captured_and_replayed_on_another_stream(be):
             o.zero_()
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("cols,x_stride,y_stride,offset", [(33, 37, 41, 1), (3, 3, 5, 1), (250, 251, 250, 3)])
+def test_odd_rows_in_wider_buffers(be, cols, x_stride, y_stride, offset):
+    """Many rows of odd widths, strides and addresses: copied with what lies beside them, which neither shows nor changes."""
+    torch.manual_seed(9)
+    rows = 9601
+    def strided(stride, value):
+        buf = torch.full(((rows - 1) * stride + cols + offset,), value, device="cuda", dtype=torch.bfloat16)
+        return buf, torch.as_strided(buf, (rows, cols), (stride, 1), offset)
+    xbuf, x = strided(x_stride, float("nan"))
+    x.copy_(torch.randn(rows, cols))
+    _, dy = strided(y_stride, float("nan"))
+    dy.copy_(torch.randn(rows, cols))
+    _, add = strided(x_stride, float("nan"))
+    add.copy_(torch.randn(rows, cols))
+    dxbuf, dx = strided(x_stride, -3.0)
+    gamma = 1 + 0.1 * torch.randn(cols, device="cuda")
+    mean, rstd = stats(B.NORM_LAYER, x)
+    out = backward(be, B.NORM_LAYER, dy, x, gamma, mean, rstd, add, dx)
+    check_backward(B.NORM_LAYER, dy, x, gamma, mean, rstd, add, *out)
+    dx.fill_(-3.0)
+    assert (dxbuf == -3.0).all()
