@@ -81,7 +81,8 @@ def check_forward(kind, x, gamma, beta, eps, yt, y, mean, rstd):
 @pytest.mark.parametrize("kind", [B.NORM_LAYER, B.NORM_RMS])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 768), (3, 7), (17, 33), (257, 256), (64, 1000), (33, 1029), (5, 4096), (9, 4104),
                                        (2, 8200), (3, 12001), (2, 16384), (1, 16383), (700, 64), (5000, 64), (4800, 256),
-                                       (5001, 768), (7100, 1000), (4737, 1024), (2500, 1544), (1200, 4096), (700, 8192)])
+                                       (5001, 768), (7100, 1000), (4737, 1024), (2500, 1544), (1200, 4096), (700, 8192), (9600, 1), (9500, 3),
+                                       (9501, 55), (6000, 333), (2400, 1029), (700, 5003), (593, 8191)])
 def test_forward(be, kind, rows, cols, xt, yt):
     torch.manual_seed(rows * 31 + cols)
     x = (torch.randn(rows, cols, device="cuda") * 2 + 0.5).to(DTYPES[xt])
@@ -283,3 +284,8 @@ def test_odd_rows_in_wider_buffers(be, cols, x_stride, y_stride, offset):
     check_backward(B.NORM_LAYER, dy, x, gamma, mean, rstd, add, *out)
     dx.fill_(-3.0)
     assert (dxbuf == -3.0).all()
+    ybuf, y = strided(y_stride, -3.0)
+    beta = torch.randn(cols, device="cuda")
+    check_forward(B.NORM_LAYER, x, gamma, beta, 1e-5, "bf16", *forward(be, B.NORM_LAYER, x, gamma, beta, 1e-5, "bf16", y))
+    y.fill_(-3.0)
+    assert (ybuf == -3.0).all()
