@@ -95,8 +95,8 @@ __device__ __forceinline__ void StoreCols(T* p, const float* v) {
 template <typename XT, typename YT, bool kRms, int VEC, int NV>
 __global__ void __launch_bounds__(kNormThreads)
 NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
-  __shared__ __align__(8) float2 slots[2][kWideThreads / 32];
   AwaitPrevious();
+  __shared__ __align__(8) float2 slots[2][kWideThreads / 32];
   const uint32_t group = threadIdx.x / T, t = threadIdx.x - group * T;
   const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (blockDim.x / T) + group;
   if (row >= a.rows) return;
@@ -689,9 +689,9 @@ NormFwdOddKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots)
 template <typename XT, typename YT, bool kRms, int VEC, int NV>
 __global__ void __launch_bounds__(kNormThreads, 1)
 NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
+  AwaitPrevious();
   extern __shared__ float meet[];   // [groups][cols]
   __shared__ float2 slots[2][kWideThreads / 32];
-  AwaitPrevious();
   const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
   const float per_col = 1.0f / static_cast<float>(a.cols);
   uint32_t turn = 0;
@@ -778,8 +778,8 @@ NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
 // The blocks' partial sums of 32 columns: warp w of a block adds rows w, w + 32, ...; then the warps' sums in order.
 __global__ void __launch_bounds__(1024)
 NormFoldKernel(const float* __restrict__ partials, float* __restrict__ dgamma, float* __restrict__ dbeta, uint32_t blocks, uint32_t cols) {
-  __shared__ float meet[32][33];
   AwaitPrevious();
+  __shared__ float meet[32][33];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   const float* p = partials + static_cast<size_t>(blockIdx.y) * blocks * cols;
   float s = 0.0f;

@@ -40,12 +40,12 @@ __device__ __forceinline__ float PeerFloat(const float* p, uint32_t rank) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 GatedTokenKernel(const GatedTokenArgs a, uint32_t columns) {
+  AwaitPrevious();
   extern __shared__ __align__(16) float token[];
   const uint32_t rank = umma_dev::ClusterCtaRank(), first_col = (blockIdx.x / kCluster) * columns;
   const uint32_t lanes = columns / 8, groups = kThreads / lanes, group = threadIdx.x / lanes, col = (threadIdx.x - group * lanes) * 8;
   const uint32_t share = (a.d_in + kCluster - 1) / kCluster, from = min(rank * share, a.d_in), depth = min(share, a.d_in - from);
   float* sums = token + share;
-  AwaitPrevious();
   const bool inside = first_col + col < a.d_hidden;
   const size_t at = static_cast<size_t>(from) * a.d_hidden + first_col + col;
   const T *wg = static_cast<const T*>(a.w_gate) + at, *wu = static_cast<const T*>(a.w_up) + at;

@@ -355,8 +355,8 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 GatedFoldKernel(const __grid_constant__ GatedLaunch l, uint32_t tn) {
-  __shared__ float turn[32][65];
   AwaitPrevious();
+  __shared__ float turn[32][65];
   const uint32_t across = tn / 64, per_tile = 8 * across;   // blocks
   uint32_t t = blockIdx.x / per_tile, q = 0;
   const uint32_t within = blockIdx.x - t * per_tile;
