@@ -38,7 +38,6 @@ constexpr uint32_t kBoxBytes = 64 * 64 * 2;
 constexpr uint32_t kEpiWarps = 8;
 constexpr uint32_t kThreads = 64 + 32 * kEpiWarps;   // warp 0 TMA, warp 1 MMA, then the epilogue warps
 constexpr uint32_t kSlabBytes = 32 * 128;  // 32 rows of 64 16-bit columns
-constexpr uint32_t kSlabs = 1;             // to an epilogue warp
 constexpr uint32_t kBand = 8;              // row tiles that share a column tile's B before the next column tile
 
 template <uint32_t kTN>
@@ -47,7 +46,7 @@ struct Tile {
   static constexpr uint32_t kABytes = kRows * kBlockK * 2, kBBytes = kHalf * kBlockK * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
   static constexpr uint32_t kStages = kTN == 256 ? 6 : 8;
-  static constexpr uint32_t kSmem = kStages * kStageBytes + kEpiWarps * kSlabs * kSlabBytes + 256 + 1024;
+  static constexpr uint32_t kSmem = kStages * kStageBytes + kEpiWarps * kSlabBytes + 256 + 1024;
 };
 
 struct __align__(8) Barriers {
@@ -116,22 +115,20 @@ __device__ __forceinline__ void PutHalfSlab(uint8_t* slab, uint32_t lane, uint32
   }
 }
 
-// An epilogue warp's two slabs, used in turn: a slab is written again once the store before the last has read it.
-struct SlabRing {
+// An epilogue warp's slab, written again once the store before has read it (a second slab each took the ring's sixth stage:
+// 32768 x 768 x 2048 185 us, 177 with the stage).
+struct Slab {
   uint8_t* base;
-  uint32_t turn;
-  __device__ __forceinline__ uint8_t* Next() {
+  __device__ __forceinline__ uint8_t* Await() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // (of the lane that commits; none for the others)
     __syncwarp();
-    uint8_t* s = base;
-    ++turn;
-    return s;
+    return base;
   }
-  __device__ __forceinline__ void Store(const CUtensorMap* map, uint8_t* slab, uint32_t col, uint32_t row, bool inside) {
+  __device__ __forceinline__ void Store(const CUtensorMap* map, uint32_t col, uint32_t row, bool inside) {
     FenceProxyAsync();
     __syncwarp();
     if ((threadIdx.x & 31) == 0) {
-      if (inside) TmaStore2D(map, slab, static_cast<int32_t>(col), static_cast<int32_t>(row));
+      if (inside) TmaStore2D(map, base, static_cast<int32_t>(col), static_cast<int32_t>(row));
       TmaStoreCommit();
     }
   }
@@ -146,24 +143,24 @@ __device__ __forceinline__ void LoadAcc(uint32_t taddr, float (&v)[32]) {
 }
 
 template <typename T>
-__device__ __forceinline__ void PlainSlab(SlabRing& ring, const CUtensorMap* map, uint32_t taddr, uint32_t col, uint32_t row, bool inside) {
+__device__ __forceinline__ void PlainSlab(Slab& out, const CUtensorMap* map, uint32_t taddr, uint32_t col, uint32_t row, bool inside) {
   const uint32_t lane = threadIdx.x & 31;
-  uint8_t* slab = ring.Next();
+  uint8_t* slab = out.Await();
 #pragma unroll
   for (uint32_t h = 0; h < 2; ++h) {
     float v[32];
     LoadAcc(taddr + 32 * h, v);
     PutHalfSlab<T>(slab, lane, h, v);
   }
-  ring.Store(map, slab, col, row, inside);
+  out.Store(map, col, row, inside);
 }
 
 // hidden = act(gate) up of 64 columns, from accumulators `apart` columns apart.
 template <typename T, int kAct>
-__device__ __forceinline__ void HiddenSlab(SlabRing& ring, const CUtensorMap* map, uint32_t taddr, uint32_t apart, uint32_t col, uint32_t row,
+__device__ __forceinline__ void HiddenSlab(Slab& out, const CUtensorMap* map, uint32_t taddr, uint32_t apart, uint32_t col, uint32_t row,
                                            bool inside) {
   const uint32_t lane = threadIdx.x & 31;
-  uint8_t* slab = ring.Next();
+  uint8_t* slab = out.Await();
 #pragma unroll
   for (uint32_t h = 0; h < 2; ++h) {
     float g[32], u[32];
@@ -173,18 +170,18 @@ __device__ __forceinline__ void HiddenSlab(SlabRing& ring, const CUtensorMap* ma
     for (int i = 0; i < 32; ++i) g[i] = GatedAct<kAct>(g[i]) * u[i];
     PutHalfSlab<T>(slab, lane, h, g);
   }
-  ring.Store(map, slab, col, row, inside);
+  out.Store(map, col, row, inside);
 }
 
 template <typename T>
-__device__ __forceinline__ void GatedColumns(SlabRing& ring, const GatedLaunch& l, uint32_t taddr, uint32_t apart, uint32_t col, uint32_t row,
+__device__ __forceinline__ void GatedColumns(Slab& out, const GatedLaunch& l, uint32_t taddr, uint32_t apart, uint32_t col, uint32_t row,
                                              bool inside) {
-  if (l.act == kActSilu) HiddenSlab<T, kActSilu>(ring, &l.p[0].c, taddr, apart, col, row, inside);
-  else if (l.act == kActGelu) HiddenSlab<T, kActGelu>(ring, &l.p[0].c, taddr, apart, col, row, inside);
-  else HiddenSlab<T, kActRelu>(ring, &l.p[0].c, taddr, apart, col, row, inside);
+  if (l.act == kActSilu) HiddenSlab<T, kActSilu>(out, &l.p[0].c, taddr, apart, col, row, inside);
+  else if (l.act == kActGelu) HiddenSlab<T, kActGelu>(out, &l.p[0].c, taddr, apart, col, row, inside);
+  else HiddenSlab<T, kActRelu>(out, &l.p[0].c, taddr, apart, col, row, inside);
   if (l.keep) {
-    PlainSlab<T>(ring, &l.gate, taddr, col, row, inside);
-    PlainSlab<T>(ring, &l.up, taddr + apart, col, row, inside);
+    PlainSlab<T>(out, &l.gate, taddr, col, row, inside);
+    PlainSlab<T>(out, &l.up, taddr + apart, col, row, inside);
   }
 }
 
@@ -195,7 +192,7 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (SmemAddr(smem_raw) & 1023u)) & 1023u);
   uint8_t* slabs = smem + C::kStages * C::kStageBytes;
-  Barriers* bars = reinterpret_cast<Barriers*>(slabs + kEpiWarps * kSlabs * kSlabBytes);
+  Barriers* bars = reinterpret_cast<Barriers*>(slabs + kEpiWarps * kSlabBytes);
   static_assert(sizeof(Barriers) <= 256);
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -236,28 +233,28 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
         const uint32_t m0 = at.m_tile * 2 * kRows + rank * kRows;
         const uint32_t n0 = kGated ? at.n_tile * C::kHalf : at.n_tile * kTN + rank * C::kHalf;
         for (uint32_t kb = at.from; kb < at.to; ++kb, ++it) {
-            const uint32_t pair = kb < p.blocks[0] ? 0 : 1;
-            const CUtensorMap *ma = &p.a[pair], *mb = kGated ? &p.b[rank] : &p.b[pair];
-            const uint32_t s = it % C::kStages, round = it / C::kStages;
-            if (round > 0 && !Wait(&bars->empty[s], (round - 1) & 1)) {
-              give_up();
-              ok = false;
-              break;
-            }
-            if (rank == 0) MbarExpectTx(&bars->full[s], 2 * C::kStageBytes);   // both CTAs' bytes
-            const uint32_t full = MapToCta(SmemAddr(&bars->full[s]), 0);
-            uint8_t* dst = smem + s * C::kStageBytes;
-            const int32_t k0 = static_cast<int32_t>((kb - (pair ? p.blocks[0] : 0)) * kBlockK);
+          const uint32_t pair = kb < p.blocks[0] ? 0 : 1;
+          const CUtensorMap *ma = &p.a[pair], *mb = kGated ? &p.b[rank] : &p.b[pair];
+          const uint32_t s = it % C::kStages, round = it / C::kStages;
+          if (round > 0 && !Wait(&bars->empty[s], (round - 1) & 1)) {
+            give_up();
+            ok = false;
+            break;
+          }
+          if (rank == 0) MbarExpectTx(&bars->full[s], 2 * C::kStageBytes);   // both CTAs' bytes
+          const uint32_t full = MapToCta(SmemAddr(&bars->full[s]), 0);
+          uint8_t* dst = smem + s * C::kStageBytes;
+          const int32_t k0 = static_cast<int32_t>((kb - (pair ? p.blocks[0] : 0)) * kBlockK);
 #pragma unroll
-            for (uint32_t i = 0; i < kRows / 64; ++i) {
-              const int32_t r = static_cast<int32_t>(m0 + 64 * i);
-              TmaLoad2DPair(dst + i * kBoxBytes, ma, full, p.a_mn ? r : k0, p.a_mn ? k0 : r);
-            }
+          for (uint32_t i = 0; i < kRows / 64; ++i) {
+            const int32_t r = static_cast<int32_t>(m0 + 64 * i);
+            TmaLoad2DPair(dst + i * kBoxBytes, ma, full, p.a_mn ? r : k0, p.a_mn ? k0 : r);
+          }
 #pragma unroll
-            for (uint32_t i = 0; i < C::kHalf / 64; ++i) {
-              const int32_t r = static_cast<int32_t>(n0 + 64 * i);
-              TmaLoad2DPair(dst + C::kABytes + i * kBoxBytes, mb, full, p.b_mn ? r : k0, p.b_mn ? k0 : r);
-            }
+          for (uint32_t i = 0; i < C::kHalf / 64; ++i) {
+            const int32_t r = static_cast<int32_t>(n0 + 64 * i);
+            TmaLoad2DPair(dst + C::kABytes + i * kBoxBytes, mb, full, p.b_mn ? r : k0, p.b_mn ? k0 : r);
+          }
         }
       }
     }
@@ -299,7 +296,7 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
     }
   } else {   // ---- epilogue: TMEM lane quarter = warp % 4; the two warps of a quarter share the columns
     const uint32_t quarter = warp & 3, which = (warp - 2) >> 2;
-    SlabRing ring{slabs + (warp - 2) * kSlabs * kSlabBytes, 0};
+    Slab slab{slabs + (warp - 2) * kSlabBytes};
     uint32_t lt = 0;
     for (uint32_t t = unit; t < total; t += units, ++lt) {
       const uint32_t buf = lt & 1, use = lt >> 1;
@@ -327,11 +324,11 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
             for (uint32_t i = 0; i < 8; ++i) to[(8 * h + i) * 2 * kRows] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
           }
         } else if (kGated) {
-          if (l.f16) GatedColumns<F16>(ring, l, lanes + c, C::kHalf, col, row, row < p.M && col < p.N);
-          else GatedColumns<Bf16>(ring, l, lanes + c, C::kHalf, col, row, row < p.M && col < p.N);
+          if (l.f16) GatedColumns<F16>(slab, l, lanes + c, C::kHalf, col, row, row < p.M && col < p.N);
+          else GatedColumns<Bf16>(slab, l, lanes + c, C::kHalf, col, row, row < p.M && col < p.N);
         } else {
-          if (l.f16) PlainSlab<F16>(ring, &p.c, lanes + c, col, row, row < p.M && col < p.N);
-          else PlainSlab<Bf16>(ring, &p.c, lanes + c, col, row, row < p.M && col < p.N);
+          if (l.f16) PlainSlab<F16>(slab, &p.c, lanes + c, col, row, row < p.M && col < p.N);
+          else PlainSlab<Bf16>(slab, &p.c, lanes + c, col, row, row < p.M && col < p.N);
         }
       }
       TcFenceBefore();
