@@ -67,6 +67,7 @@ int see_cuda_begin_range(see_cuda_backend* h, const void* instructions, uint64_t
                          uint64_t begin, uint64_t end);
 int see_cuda_execute(see_cuda_backend* h, const void* instruction, const see_step_params* params);
 int see_cuda_end_range(see_cuda_backend* h);
+/* Waits for the handle's stream and reports what its kernels raised since the last flush, whether or not a plan is bound. */
 int see_cuda_flush(see_cuda_backend* h);
 
 /* Convenience over the three calls above: BeginRange, Execute each of

@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "operand_checks.h"
 #include "umma_gemm.h"
 
 namespace see {
@@ -1884,8 +1885,16 @@ const k::Shadow* CudaBackend::ShadowFor(uint64_t out_ref, uint64_t elems) const 
   return &cur_shadow_;
 }
 
+Status CudaBackend::Flush() {
+  if (d_arena_) return FlushWith({});
+  // No plan is bound: the operators on caller memory raise the same status words, and leave the current device as it was.
+  OnDevice on(device_);
+  if (!on.ok()) return Check(cudaGetLastError(), "flush: device");
+  return FlushWith({});
+}
+
 Status CudaBackend::FlushWith(std::initializer_list<k::PublishItem> items, uint32_t* out) {
-  if (!d_arena_) return {};
+  if (!d_arena_ && items.size()) return {};   // (the items are a bound plan's)
   cudaSetDevice(device_);
   // Strict coherence: every range written since the last flush comes back.  Scattered over at most kFlushStaging bytes
   // they come as ONE copy of the whole span into pinned memory, and the host takes just the written ranges from there (a

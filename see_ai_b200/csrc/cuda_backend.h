@@ -115,7 +115,7 @@ class CudaBackend {
   }
   void BeginRange(std::span<const Instruction> program, size_t begin, size_t end);
   void EndRange();
-  Status Flush() { return FlushWith({}); }
+  Status Flush();
   // Flush, and read `items` (device words, at most kPublishWords in all) into `out` on the way: one launch and one wait.
   static constexpr uint32_t kPublishWords = 48;
   Status FlushWith(std::initializer_list<k::PublishItem> items, uint32_t* out = nullptr);
@@ -259,6 +259,7 @@ class CudaBackend {
   StepParams last_params_{};
   bool scalars_valid_ = false;
   bool capturing_ = false;
+  friend struct DeviceStatusAccess;  // tests set the device's status words from the host
   uint32_t* h_published_ = nullptr;  // pinned: the status words, then what a FlushWith asked for
   uint8_t* h_flush_ = nullptr;       // pinned staging of a strict flush's downloads (from a strict Bind on)
   uint64_t flush_capacity_ = 0;
