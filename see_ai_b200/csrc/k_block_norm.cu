@@ -14,8 +14,9 @@
 // Sums are f32, but for the mean: the threads' sums are added in double.  A thread's share is summed plainly where it has 16 bits
 // (a few dozen values of 8 or 11 fit); in f32, with what each addition rounds away in NormFwdKernel, where it costs nothing
 // beside the latency, and corrected by the average deviation from the first result in NormFwdRingKernel, where it would (26.6 us
-// to 31.5 at 32768 x 768).  The variance is the average square of the deviations, a second pass over the registers, so rows far
-// from zero lose nothing to cancellation.
+// to 31.5 at 32768 x 768).  The variance is the average square of the deviations, a second pass over the registers, less the
+// square of what that mean is off (its rounding; in the ring kernels the average deviation): beside a small eps that would show in
+// rows far from zero, whose squares a sum of x^2 would lose altogether.
 #include <atomic>
 
 #include "act_expr.cuh"
@@ -81,6 +82,12 @@ __device__ __forceinline__ void AddExactly(float& sum, float& rest, float x) {
   sum = s;
 }
 
+// The variance, from the average square of deviations from a mean that is off by `off`, their own average.  (What is not finite stays.)
+__device__ __forceinline__ float Variance(float square, float off) {
+  const float less = square - off * off;
+  return !isfinite(off * off) ? square : less < 0.0f ? 0.0f : less;
+}
+
 template <typename T, int VEC>
 __device__ __forceinline__ void LoadCols(const T* p, float* v) {
   if constexpr (VEC == 8) Load8<T>(p, v);
@@ -122,9 +129,12 @@ NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
   }
   const float per_col = 1.0f / static_cast<float>(a.cols);
   float mean = 0.0f;
+  [[maybe_unused]] float off = 0.0f;
   if constexpr (!kRms) {
     const double share = isfinite(rest) ? static_cast<double>(total) + static_cast<double>(rest) : static_cast<double>(total);
-    mean = static_cast<float>(GroupSum(share, T, group, slots, turn) / static_cast<double>(a.cols));
+    const double wide = GroupSum(share, T, group, slots, turn) / static_cast<double>(a.cols);
+    mean = static_cast<float>(wide);
+    off = static_cast<float>(wide - static_cast<double>(mean));
     total = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -136,7 +146,7 @@ NormFwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
         }
       }
   }
-  const float var = GroupSum<false>(make_float2(total, 0.0f), T, group, slots, turn).x * per_col;
+  const float square = GroupSum<false>(make_float2(total, 0.0f), T, group, slots, turn).x * per_col, var = kRms ? square : Variance(square, off);
   const float rstd = 1.0f / sqrtf(var + a.eps);
   if (t == 0) {
     a.rstd[row] = rstd;
@@ -303,8 +313,13 @@ NormFwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots
       sum.y = one + other;
       if (!kCorrect) sum.x = sum.y;
       sum = GroupSum<kCorrect>(sum, T, group, sums, turn);
-      var = (kCorrect ? sum.y : sum.x) * per_col;
-      if (kCorrect && isfinite(sum.x)) mean += sum.x * per_col;   // (which moves the average square by its own square: nothing)
+      if (kCorrect) {
+        sum.x *= per_col;
+        var = Variance(sum.y * per_col, sum.x);
+        if (isfinite(sum.x)) mean += sum.x;
+      } else {
+        var = sum.x * per_col;   // (a few dozen values of 8 or 11 bits: the mean has its own rounding alone)
+      }
     }
     const float rstd = 1.0f / sqrtf(var + a.eps);
     if (t == 0) {
@@ -669,8 +684,9 @@ NormFwdOddKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots)
           sum.y += d * d;
         }
       sum = GroupSum<true>(sum, T, group, sums, turn);
-      var = sum.y * per_col;
-      if (isfinite(sum.x)) mean += sum.x * per_col;
+      sum.x *= per_col;
+      var = Variance(sum.y * per_col, sum.x);
+      if (isfinite(sum.x)) mean += sum.x;
     }
     const float rstd = 1.0f / sqrtf(var + a.eps);
     if (t == 0) {
