@@ -200,7 +200,8 @@ const char* see_cuda_static_last_error(void);
  * can be captured into a CUDA graph after a first call of its kind.  Calls share no memory but what they are given:
  * calls that can overlap on the GPU need workspaces of their own.  A call that is refused (SEE_ERROR: a null, misaligned
  * or overlapping operand, a size outside the stated range, a workspace too small) enqueues nothing.  Outputs may not
- * overlap inputs or one another; two matrices may lie side by side in the rows of one buffer (equal strides). */
+ * overlap inputs or one another; two matrices may lie side by side in the rows of one buffer (equal strides).  With zero
+ * rows an operand of rows covers no bytes, and its address may be anything, NULL too. */
 enum { SEE_F32 = 0, SEE_BF16 = 1, SEE_F16 = 2 };        /* element types */
 enum { SEE_NORM_LAYER = 0, SEE_NORM_RMS = 1 };
 enum { SEE_ACT_RELU = 1, SEE_ACT_GELU = 2, SEE_ACT_SILU = 3 };   /* GELU: the tanh form, as in the plans */

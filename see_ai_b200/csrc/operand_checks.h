@@ -70,6 +70,7 @@ class Operands {
     auto refuse = [what](const std::string& why) { return std::unexpected(std::string(what) + ": " + why); };
     for (size_t i = 0; i < count_; ++i) {
       const Operand& o = ops_[i];
+      if (o.rows == 0) continue;   // (no bytes: an empty allocation has no address)
       if (!o.p) return refuse(std::string(o.name) + " is null");
       if (o.begin() % o.align) return refuse(std::string(o.name) + " is not aligned");
       uint64_t span;
