@@ -169,8 +169,8 @@ Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bit
     auto refuse = [&](const std::string& why) { return std::unexpected(std::string(what) + ": tensor " + std::to_string(i) + ": " + why); };
     if (!IsType(t.g_type) || !IsType(t.copy_type)) return refuse("unknown type");
     if (t.flags & ~static_cast<uint32_t>(SEE_ADAMW_NO_DECAY)) return refuse("unknown flag");
+    if (t.n == 0) continue;   // (empty allocations have no address, the copy's neither)
     if ((t.copy_type == SEE_F32) != (t.copy == nullptr)) return refuse("a copy has 16 bits, and none is null with type f32");
-    if (t.n == 0) continue;
     if (t.n > (1ull << 38)) return refuse("more than 2^38 elements");
     const uint64_t align[kOperands] = {4, SizeOfType(t.g_type), state, state, 4, 4, 2};
     Span spans[kOperands];

@@ -48,5 +48,17 @@ int main() {
   Say("gated back weights", see::CheckGatedBackward(&g, nullptr, nullptr, nullptr, wu, nullptr, nullptr, nullptr, dwg, dwu, work, 128));
   g.rows = 1;
   Say("gated one row", see::CheckGatedForward(&g, At(7), wg, wu, nullptr, nullptr, nullptr));
+
+  see::StepParams params;
+  params.step = 1;
+  see_adamw_tensor t{nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, SEE_BF16, SEE_BF16, 0, 0};
+  Say("adamw", see::CheckAdamW(&t, 1, 8, params, nullptr));
+  t.copy = At(1, 1);
+  t.copy_type = SEE_F32;
+  Say("adamw copy", see::CheckAdamW(&t, 1, 8, params, nullptr));
+  t.copy_type = 3;
+  Say("adamw type", see::CheckAdamW(&t, 1, 8, params, nullptr));
+  t = {At<float>(1), At(2), At(3), At(4), At<float>(5), At<float>(6), nullptr, 1, SEE_BF16, SEE_BF16, 0, 0};
+  Say("adamw one element", see::CheckAdamW(&t, 1, 8, params, nullptr));
   return 0;
 }

@@ -18,6 +18,7 @@ EXPECTED = {
     "norm back no bytes": "workspace is too small", "rms": None, "rms back": None, "norm one row": "x is null",
     "gated": None, "gated weights": "w_up is null", "gated back": None, "gated back half": "together", "gated back nothing": "no output",
     "gated back dx": None, "gated back weights": "w_gate is null", "gated one row": "hidden is null",
+    "adamw": None, "adamw copy": None, "adamw type": "unknown type", "adamw one element": "a copy has 16 bits",
 }
 
 
@@ -62,5 +63,11 @@ def test_tensors_without_rows():
     be.gated_forward(0, d, f, x, wg.data_ptr(), wu.data_ptr(), h, h, h)
     be.gated_backward(0, d, f, h, x, wg.data_ptr(), wu.data_ptr(), h, h, x, dwg.data_ptr(), dwu.data_ptr(), work.data_ptr(), work.numel())
     assert (dwg == 0).all() and (dwu == 0).all()
+    rest = {k: torch.ones(300, device="cuda") for k in ("p", "g", "m", "v")}
+    copy = torch.empty(300, device="cuda", dtype=torch.bfloat16)
+    table = B.adamw_tensors([dict(p=none(0), g=none(0), m=none(0), v=none(0), copy=none(0, t=torch.bfloat16), n=0, copy_type=B.BF16),
+                             dict({k: v.data_ptr() for k, v in rest.items()}, copy=copy.data_ptr(), n=300, copy_type=B.BF16)])
+    be.adamw_step(table, B.StepParams(1e-3, 0.9, 0.999, 1e-8, 0.0, 0, 1))
+    assert (rest["p"] != 1).all() and torch.equal(copy, rest["p"].bfloat16())
     torch.cuda.synchronize()
     be.close()
