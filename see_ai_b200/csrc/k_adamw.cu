@@ -143,13 +143,18 @@ __device__ __forceinline__ float MinMagnitude(float a, f32x2 pair) {
   return r;
 }
 // sqrt(v) by one Newton step on the hardware's reciprocal root: s = v y, s + (v - s s) y / 2, the remainder exact in an FMA.
-// (A call of sqrtf costs three times as much here.)  Zero stays zero; what is not finite becomes NaN.
+// (A call of sqrtf costs three times as much here.)  Zero stays zero; what is not finite becomes NaN.  kTiny: some value may lie
+// below the smallest normal, whose reciprocal root takes three instructions more; the remainder, a multiple of 2^-149, is then
+// off by at most half of that, 2^-23 of the root from 2^-128 on, and nothing below, where the first s is as good.
+constexpr float kSmallestNormal = 1.17549435e-38f;
+template <bool kTiny>
 __device__ __forceinline__ f32x2 Root2(f32x2 v) {
   float a, b;
   UnpackF2(v, &a, &b);
   auto reciprocal = [](float x) {
     float y;
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, 1.17549435e-38f)));
+    if constexpr (kTiny) asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, 1.4e-45f)));
+    else asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, kSmallestNormal)));
     return y;
   };
   const f32x2 y = PackF2(reciprocal(a), reciprocal(b)), s = Mul2(v, y);
@@ -228,7 +233,7 @@ __device__ __forceinline__ void StepBlock(const AdamEntry& e, uint64_t block, co
       p[j] -= a.lr * (m[j] * a.inv_bc1 / (sqrtf(v[j] * a.inv_bc2) + a.eps) + decay * p[j]);
     }
   } else {
-    float m_top = 0.0f, v_top = 0.0f;
+    float m_top = 0.0f, v_top = 0.0f, v_least = 1.0f;
     f32x2 m2[4], v2[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -240,9 +245,19 @@ __device__ __forceinline__ void StepBlock(const AdamEntry& e, uint64_t block, co
         m1[j] = m[2 * k + j] * m_scale * a.beta1 + grad * a.om_beta1;
         v1[j] = root * root * a.beta2 + grad * a.om_beta2 * grad;
       }
-      const f32x2 weight = PackF2(p[2 * k], p[2 * k + 1]);
       m2[k] = PackF2(m1[0], m1[1]);
-      v2[k] = Root2(PackF2(v1[0], v1[1]));
+      v2[k] = PackF2(v1[0], v1[1]);
+      v_least = MinMagnitude(v_least, v2[k]);
+    }
+    auto roots = [&](auto tiny) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v2[k] = Root2<tiny.value>(v2[k]);
+    };
+    if (v_least >= kSmallestNormal) roots(std::false_type{});
+    else roots(std::true_type{});
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x2 weight = PackF2(p[2 * k], p[2 * k + 1]);
       float size0, size1;
       UnpackF2(Fma2(v2[k], Splat2(a.root_inv_bc2), Splat2(a.eps)), &size0, &size1);
       const f32x2 move = Mul2(Mul2(m2[k], Splat2(a.inv_bc1)), PackF2(RcpApprox(size0), RcpApprox(size1)));
