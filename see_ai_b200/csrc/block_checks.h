@@ -9,6 +9,8 @@ namespace see {
 // Bytes for any shape of these sizes, whatever its types and alignment (0: sizes outside the range).
 uint64_t NormBackwardWorkspace(uint64_t rows, uint64_t cols);
 uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden);
+// What a call for these gradients uses of it on a device of `sms`.
+uint64_t GatedBackwardUses(uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool dx, bool dw, uint32_t sms);
 
 // What see_cuda.h says a call refuses, without a device.  The shapes' strides of 0 are filled in.
 Status CheckNormForward(see_norm_shape* shape, const void* x, const float* gamma, const float* beta, const void* y, const float* mean,

@@ -88,7 +88,7 @@ double Longest(const Run* runs, uint32_t count, uint32_t pairs) {
   }
   return longest;
 }
-BackwardPlan PlanCuts(const uint64_t* tiles, const uint64_t* blocks, uint32_t count, uint32_t pairs) {
+BackwardPlan PlanCuts(const uint64_t* tiles, const uint64_t* blocks, uint32_t count, uint32_t pairs, uint32_t most_parts) {
   uint64_t total = 0, longest = 0;
   for (uint32_t i = 0; i < count; ++i) {
     total += tiles[i];
@@ -114,7 +114,7 @@ BackwardPlan PlanCuts(const uint64_t* tiles, const uint64_t* blocks, uint32_t co
         runs[count + i] = {(tiles[i] - whole) * each, static_cast<double>(blocks[i]) / static_cast<double>(std::max<uint64_t>(1, each)) + 5.0};
         parts += runs[count + i].count;
       }
-      if (parts > kMostParts) continue;
+      if (parts > most_parts) continue;
       plan.parts = static_cast<uint32_t>(parts);
       const double time = Longest(runs, 2 * count, pairs) + (parts ? 8.0 + 0.3 * static_cast<double>(parts) : 0.0);
       if (time < best_time) {
@@ -124,8 +124,7 @@ BackwardPlan PlanCuts(const uint64_t* tiles, const uint64_t* blocks, uint32_t co
     }
   return best;
 }
-// All that a backward pass over these sizes may ask for.
-BackwardPlan PlanBackward(uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool dx, bool dw, uint32_t pairs) {
+BackwardPlan PlanOn(uint32_t pairs, uint32_t most_parts, uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool dx, bool dw) {
   uint64_t tiles[3], blocks[3];
   uint32_t count = 0;
   if (dx) {
@@ -136,19 +135,32 @@ BackwardPlan PlanBackward(uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool 
     tiles[count] = static_cast<uint64_t>(Up(d_in, 256)) * Up(d_hidden, 256);
     blocks[count++] = Up(rows, 64);
   }
-  return PlanCuts(tiles, blocks, count, pairs);
+  return PlanCuts(tiles, blocks, count, pairs, most_parts);
 }
-uint64_t PartialBytes(const BackwardPlan& plan) { return plan.parts * 256ull * 256 * 4; }
+// The parts that a workspace has room for, whichever gradients are wanted: what 148 SMs take.  (Another number of pairs ends its
+// rounds elsewhere, and might do with more.)
+uint32_t PartsReserved(uint64_t rows, uint64_t d_in, uint64_t d_hidden) {
+  uint32_t parts = 0;
+  for (int want = 1; want < 4; ++want) parts = std::max(parts, PlanOn(kMostPairs, kMostParts, rows, d_in, d_hidden, want & 1, want & 2).parts);
+  return parts;
+}
+BackwardPlan PlanBackward(uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool dx, bool dw, uint32_t pairs) {
+  const uint32_t most = pairs == kMostPairs ? kMostParts : PartsReserved(rows, d_in, d_hidden);
+  return PlanOn(pairs, most, rows, d_in, d_hidden, dx, dw);
+}
+uint64_t PartialBytes(uint32_t parts) { return parts * 256ull * 256 * 4; }
+uint32_t PairsOf(uint32_t sms) { return std::min(sms / 2, kMostPairs); }
 
 }  // namespace
 
 uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden) {
   if (d_in == 0 || d_hidden == 0 || d_in % 8 || d_hidden % 8 || d_in > (1u << 20) || d_hidden > (1u << 20) || rows > 0x7FFFFF00ull) return 0;
   if (rows == 0) return 128;
-  uint64_t partials = 0;   // whichever gradients are wanted, on 148 SMs
-  for (int want = 1; want < 4; ++want)
-    partials = std::max(partials, PartialBytes(PlanBackward(rows, d_in, d_hidden, want & 1, want & 2, kMostPairs)));
-  return 2 * SlopeBytes(rows, d_hidden) + partials;
+  return 2 * SlopeBytes(rows, d_hidden) + PartialBytes(PartsReserved(rows, d_in, d_hidden));
+}
+
+uint64_t GatedBackwardUses(uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool dx, bool dw, uint32_t sms) {
+  return 2 * SlopeBytes(rows, d_hidden) + PartialBytes(PlanBackward(rows, d_in, d_hidden, dx, dw, PairsOf(sms)).parts);
 }
 
 Status CheckGatedForward(see_gated_shape* shape, const void* x, const void* w_gate, const void* w_up, const void* hidden, const void* gate,
@@ -259,9 +271,9 @@ Status CudaBackend::GatedBackward(const see_gated_shape& given, const void* dhid
   l.f16 = f16;
   l.status = d_status_;
   const uint32_t rows = static_cast<uint32_t>(s.rows), d_in = static_cast<uint32_t>(s.d_in), d_hidden = static_cast<uint32_t>(s.d_hidden);
-  const uint32_t pairs = std::min(sms_ / 2, kMostPairs);
+  const uint32_t pairs = PairsOf(sms_);
   const BackwardPlan plan = PlanBackward(s.rows, s.d_in, s.d_hidden, dx != nullptr, dw_gate != nullptr, pairs);
-  if (2 * SlopeBytes(s.rows, s.d_hidden) + PartialBytes(plan) > workspace_bytes)
+  if (2 * SlopeBytes(s.rows, s.d_hidden) + PartialBytes(plan.parts) > workspace_bytes)
     return std::unexpected("cuda: gated backward: the workspace is too small");
   l.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 2 * SlopeBytes(s.rows, s.d_hidden));
   auto problem = [&](uint32_t M, uint32_t N, void* out, uint64_t out_stride) -> k::GatedProblem& {
