@@ -312,7 +312,7 @@ Status CudaBackend::GatedBackward(const see_gated_shape& given, const void* dhid
   if (auto r = Check(k::GatedProducts(l, false, 256, 2 * pairs, stream_), "gated backward"); !r) return r;
   ++counters_.kernel_launches;
   if (plan.parts) {
-    if (auto r = Check(k::GatedFold(l, 256, stream_), "gated backward"); !r) return r;
+    if (auto r = Check(k::GatedFold(l, stream_), "gated backward"); !r) return r;
     ++counters_.kernel_launches;
   }
   return {};

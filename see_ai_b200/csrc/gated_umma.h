@@ -35,14 +35,14 @@ struct GatedLaunch {
   uint32_t f16;              // operands and outputs: 1 f16, 0 bf16
   int act;
   uint32_t keep;             // gated: gate and up leave too
-  float* partials;           // [part][256 x tn]
+  float* partials;           // [part][256 x 256]
   DeviceStatus* status;
 };
 // tn: columns of a pair's accumulator, 256, or gated also 128 (half of them the gate's, half the up projection's).
 cudaError_t GatedProducts(const GatedLaunch& l, bool gated, uint32_t tn, uint32_t sms, cudaStream_t s);
 
 // The cut tiles' parts added in order, rounded and stored.
-cudaError_t GatedFold(const GatedLaunch& l, uint32_t tn, cudaStream_t s);
+cudaError_t GatedFold(const GatedLaunch& l, cudaStream_t s);
 
 // dg = dh u act'(g), du = dh act(g): rows of `cols` elements (a multiple of 8); dh, g, u `stride` apart, dg, du dense.
 cudaError_t GatedSlopes(const void* dh, const void* g, const void* u, void* dg, void* du, uint64_t rows, uint32_t cols, uint64_t stride,

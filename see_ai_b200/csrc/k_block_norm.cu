@@ -701,8 +701,8 @@ NormFwdOddKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots)
   }
 }
 
-// One row of partial sums a block; a lone block writes the gradients themselves.
-template <typename XT, typename YT, bool kRms, int VEC, int NV>
+// Single columns, T apart, straight into registers.  One row of partial sums a block; a lone block writes the gradients themselves.
+template <typename XT, typename YT, bool kRms, int NV>
 __global__ void __launch_bounds__(kNormThreads, 1)
 NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
   AwaitPrevious();
@@ -711,43 +711,36 @@ NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
   const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
   const float per_col = 1.0f / static_cast<float>(a.cols);
   uint32_t turn = 0;
-  float sum_g[NV][VEC], sum_b[kRms ? 1 : NV][VEC];
+  float sum_g[NV], sum_b[kRms ? 1 : NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      sum_g[i][j] = 0.0f;
-      if (!kRms) sum_b[i][j] = 0.0f;
-    }
+  for (int i = 0; i < NV; ++i) {
+    sum_g[i] = 0.0f;
+    if (!kRms) sum_b[i] = 0.0f;
+  }
   for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * groups + group; row < a.rows; row += static_cast<uint64_t>(gridDim.x) * groups) {
     const XT* x = static_cast<const XT*>(a.x) + row * a.x_stride;
     const YT* dy = static_cast<const YT*>(a.dy) + row * a.y_stride;
-    float u[NV][VEC], d[NV][VEC];
+    float u[NV], d[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t c = (t + i * T) * VEC;
+      const uint32_t c = t + i * T;
       if (c < a.cols) {
-        LoadCols<XT, VEC>(x + c, u[i]);
-        LoadCols<YT, VEC>(dy + c, d[i]);
+        u[i] = ToF32(x[c]);
+        d[i] = ToF32(dy[c]);
       }
     }
     const float rstd = a.rstd[row], mean = kRms ? 0.0f : a.mean[row];
     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t c = (t + i * T) * VEC;
+      const uint32_t c = t + i * T;
       if (c < a.cols) {
-        float g[VEC];
-        LoadCols<float, VEC>(a.gamma + c, g);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          u[i][j] = (u[i][j] - mean) * rstd;
-          sum_g[i][j] += d[i][j] * u[i][j];
-          if (!kRms) sum_b[i][j] += d[i][j];
-          d[i][j] *= g[j];
-          sum.x += d[i][j] * u[i][j];
-          if (!kRms) sum.y += d[i][j];
-        }
+        u[i] = (u[i] - mean) * rstd;
+        sum_g[i] += d[i] * u[i];
+        if (!kRms) sum_b[i] += d[i];
+        d[i] *= a.gamma[c];
+        sum.x += d[i] * u[i];
+        if (!kRms) sum.y += d[i];
       }
     }
     sum = GroupSum<!kRms>(sum, T, group, slots, turn);
@@ -756,16 +749,10 @@ NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
     XT* dx = static_cast<XT*>(a.dx) + row * a.x_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t c = (t + i * T) * VEC;
+      const uint32_t c = t + i * T;
       if (c < a.cols) {
-        float v[VEC];
-        if (a.addend) LoadCols<XT, VEC>(static_cast<const XT*>(a.addend) + row * a.x_stride + c, v);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float r = rstd * (kRms ? d[i][j] - u[i][j] * sum.x : d[i][j] - sum.y - u[i][j] * sum.x);
-          v[j] = a.addend ? r + v[j] : r;
-        }
-        StoreCols<XT, VEC>(dx + c, v);
+        const float r = rstd * (kRms ? d[i] - u[i] * sum.x : d[i] - sum.y - u[i] * sum.x);
+        dx[c] = FromF32<XT>(a.addend ? r + ToF32(static_cast<const XT*>(a.addend)[row * a.x_stride + c]) : r);
       }
     }
   }
@@ -775,13 +762,8 @@ NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
   for (int which = 0; which < (kRms ? 1 : 2); ++which) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t c = (t + i * T) * VEC;
-      if (c < a.cols) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) meet[group * a.cols + c + j] = which ? sum_b[kRms ? 0 : i][j] : sum_g[i][j];
-      }
-    }
+    for (int i = 0; i < NV; ++i)
+      if (t + i * T < a.cols) meet[group * a.cols + t + i * T] = which ? sum_b[kRms ? 0 : i] : sum_g[i];
     __syncthreads();
     for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
       float s = meet[c];
@@ -922,7 +904,7 @@ cudaError_t RunOdd(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s, 
 template <typename XT, typename YT, bool kRms, int NV>
 cudaError_t RunSingles(const NormArgs& a, uint32_t T, uint32_t sms, cudaStream_t s, int* launches) {
   const uint32_t groups = kNormThreads / T;
-  constexpr auto* kernel = NormBwdKernel<XT, YT, kRms, 1, NV>;
+  constexpr auto* kernel = NormBwdKernel<XT, YT, kRms, NV>;
   const size_t smem = static_cast<size_t>(groups) * a.cols * 4;
   if (cudaError_t e = AllowShared<kernel>(smem); e != cudaSuccess) return e;
   const uint64_t grid = Blocks(a.rows, groups, sms);

@@ -348,13 +348,14 @@ GatedProductsKernel(const __grid_constant__ GatedLaunch l) {
   }
 }
 
+constexpr uint32_t kFoldTN = 256;   // (cuts are the backward pass's, whose tiles have no other width)
 // 32 rows x 64 columns of a cut tile a block: its parts added in order, turned to rows in shared memory, stored.
 template <typename T>
 __global__ void __launch_bounds__(256)
-GatedFoldKernel(const __grid_constant__ GatedLaunch l, uint32_t tn) {
+GatedFoldKernel(const __grid_constant__ GatedLaunch l) {
   AwaitPrevious();
   __shared__ float turn[32][65];
-  const uint32_t across = tn / 64, per_tile = 8 * across;   // blocks
+  constexpr uint32_t across = kFoldTN / 64, per_tile = 8 * across;   // blocks
   uint32_t t = blockIdx.x / per_tile, q = 0;
   const uint32_t within = blockIdx.x - t * per_tile;
   while (q + 1 < l.count && t >= l.p[q].tiles_m * l.p[q].tiles_n - l.p[q].whole) {
@@ -365,9 +366,9 @@ GatedFoldKernel(const __grid_constant__ GatedLaunch l, uint32_t tn) {
   uint32_t m_tile, n_tile;
   TileAt(p, p.whole + t, m_tile, n_tile);
   const uint32_t r0 = (within / across) * 32, c0 = (within % across) * 64;   // in the tile
-  if (m_tile * 256 + r0 >= p.M || n_tile * tn + c0 >= p.N) return;
+  if (m_tile * 256 + r0 >= p.M || n_tile * kFoldTN + c0 >= p.N) return;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const size_t part_floats = 256ull * tn;
+  constexpr size_t part_floats = 256ull * kFoldTN;
 #pragma unroll
   for (uint32_t i = 0; i < 2; ++i) {
     const uint32_t c4 = warp + 8 * i;   // four columns of the block's 64
@@ -386,7 +387,7 @@ GatedFoldKernel(const __grid_constant__ GatedLaunch l, uint32_t tn) {
   }
   __syncthreads();
   const uint32_t row = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;   // eight columns a thread
-  const uint32_t m = m_tile * 256 + r0 + row, n = n_tile * tn + c0 + c;
+  const uint32_t m = m_tile * 256 + r0 + row, n = n_tile * kFoldTN + c0 + c;
   if (m < p.M && n < p.N) Store8<T>(static_cast<T*>(p.out) + m * p.out_stride + n, &turn[row][c]);
 }
 
@@ -445,11 +446,11 @@ cudaError_t GatedProducts(const GatedLaunch& l, bool gated, uint32_t tn, uint32_
   return tn == 256 ? Run<256, true>(l, sms, s) : Run<128, true>(l, sms, s);
 }
 
-cudaError_t GatedFold(const GatedLaunch& l, uint32_t tn, cudaStream_t s) {
+cudaError_t GatedFold(const GatedLaunch& l, cudaStream_t s) {
   uint32_t tiles = 0;
   for (uint32_t p = 0; p < l.count; ++p) tiles += l.p[p].tiles_m * l.p[p].tiles_n - l.p[p].whole;
-  const unsigned grid = tiles * 8 * (tn / 64);
-  return l.f16 ? Next(GatedFoldKernel<F16>, grid, 256, 0, s)(l, tn) : Next(GatedFoldKernel<Bf16>, grid, 256, 0, s)(l, tn);
+  const unsigned grid = tiles * 8 * (kFoldTN / 64);
+  return l.f16 ? Next(GatedFoldKernel<F16>, grid, 256, 0, s)(l) : Next(GatedFoldKernel<Bf16>, grid, 256, 0, s)(l);
 }
 
 cudaError_t GatedSlopes(const void* dh, const void* g, const void* u, void* dg, void* du, uint64_t rows, uint32_t cols, uint64_t stride,
