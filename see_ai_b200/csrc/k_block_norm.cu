@@ -751,8 +751,10 @@ NormBwdKernel(const __grid_constant__ NormArgs a, uint32_t T) {
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = t + i * T;
       if (c < a.cols) {
+        float v;
+        if (a.addend) v = ToF32(static_cast<const XT*>(a.addend)[row * a.x_stride + c]);
         const float r = rstd * (kRms ? d[i] - u[i] * sum.x : d[i] - sum.y - u[i] * sum.x);
-        dx[c] = FromF32<XT>(a.addend ? r + ToF32(static_cast<const XT*>(a.addend)[row * a.x_stride + c]) : r);
+        dx[c] = FromF32<XT>(a.addend ? r + v : r);
       }
     }
   }
