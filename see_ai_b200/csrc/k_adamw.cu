@@ -143,8 +143,8 @@ __device__ __forceinline__ float MinMagnitude(float a, f32x2 pair) {
   return r;
 }
 // sqrt(v) by one Newton step on the hardware's reciprocal root: s = v y, s + (v - s s) y / 2, the remainder exact in an FMA.
-// (A call of sqrtf costs three times as much here.)  Zero stays zero; what is not finite becomes NaN.  kTiny: some value may lie
-// below the smallest normal, whose reciprocal root takes three instructions more; the remainder, a multiple of 2^-149, is then
+// (A call of sqrtf costs three times as much here.)  Zero stays zero; what is not finite becomes NaN.  kTiny: some value may be
+// zero or lie below the smallest normal, whose reciprocal root takes three instructions more; the remainder, a multiple of 2^-149, is then
 // off by at most half of that, 2^-23 of the root from 2^-128 on, and nothing below, where the first s is as good.
 constexpr float kSmallestNormal = 1.17549435e-38f;
 template <bool kTiny>
@@ -154,7 +154,7 @@ __device__ __forceinline__ f32x2 Root2(f32x2 v) {
   auto reciprocal = [](float x) {
     float y;
     if constexpr (kTiny) asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, 1.4e-45f)));
-    else asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, kSmallestNormal)));
+    else asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
   };
   const f32x2 y = PackF2(reciprocal(a), reciprocal(b)), s = Mul2(v, y);
