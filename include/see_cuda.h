@@ -220,7 +220,8 @@ typedef struct see_norm_shape {
 int see_cuda_norm_forward(see_cuda_backend* h, const see_norm_shape* shape, const void* x, const float* gamma,
                           const float* beta, void* y, float* mean, float* rstd);
 /* dx (plus addend, unless NULL: the gradient that reaches x past the norm), dgamma [cols] and, layer, dbeta [cols]: f32
- * sums over all rows, in an order that the sizes alone fix (zero rows: zeros).  Rms: mean and dbeta are NULL.
+ * sums over all rows (zero rows: zeros).  The same call has the same bits; the sums' order goes by sizes, types, strides, the
+ * addresses' alignment, whether there is an addend and the device's number of SMs.  Rms: mean and dbeta are NULL.
  * workspace: at least see_cuda_norm_backward_workspace(rows, cols) bytes, 16-byte aligned. */
 uint64_t see_cuda_norm_backward_workspace(uint64_t rows, uint64_t cols);
 int see_cuda_norm_backward(see_cuda_backend* h, const see_norm_shape* shape, const void* dy, const void* x,
@@ -240,15 +241,17 @@ int see_cuda_gated_forward(see_cuda_backend* h, const see_gated_shape* shape, co
                            const void* w_up, void* hidden, void* gate, void* up);
 /* From dhidden and what the forward pass kept: dgate = dhidden up act'(gate) and dup = dhidden act(gate), rounded to the
  * type as the products' operands (in f16 a gradient beyond 65504 overflows: scale the loss), then
- * dx = dgate w_gate^T + dup w_up^T, dw_gate = x^T dgate, dw_up = x^T dup, sums in f32 and in an order that the sizes alone
- * fix (zero rows: zeros).  dx, or dw_gate and dw_up together, may be NULL: not wanted.  workspace: at least
+ * dx = dgate w_gate^T + dup w_up^T, dw_gate = x^T dgate, dw_up = x^T dup, sums in f32 (zero rows: zeros).  The same call has
+ * the same bits; the sums' order goes by the sizes, by which gradients are wanted and by the device's number of SMs.  dx, or
+ * dw_gate and dw_up together, may be NULL: not wanted.  workspace: at least
  * see_cuda_gated_backward_workspace(rows, d_in, d_hidden) bytes, 128-byte aligned. */
 uint64_t see_cuda_gated_backward_workspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden);
 int see_cuda_gated_backward(see_cuda_backend* h, const see_gated_shape* shape, const void* dhidden, const void* x,
                             const void* w_gate, const void* w_up, const void* gate, const void* up, void* dx,
                             void* dw_gate, void* dw_up, void* workspace, uint64_t workspace_bytes);
 
-/* One AdamW step over `count` tensors of n elements (up to 2^38) each, in the kAdamWStep instruction's expression.  p: f32 weights.
+/* One AdamW step over `count` tensors of n elements (up to 2^38) each, in the kAdamWStep instruction's expression; a tensor of no
+ * elements is passed over, whatever its addresses.  p: f32 weights.
  * g: their gradients.  copy: the new weights in 16 bits (copy_type SEE_BF16 or SEE_F16), or NULL with copy_type SEE_F32.
  * state_bits 32: m, v f32 moments.  state_bits 8: m and v are e4m3 (one byte an element), v holding the ROOT of the second
  * moment; m_scale, v_scale: an f32 for each block of SEE_ADAMW_BLOCK elements (the last may be short), whose product with

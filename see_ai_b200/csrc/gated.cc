@@ -57,7 +57,7 @@ uint64_t SlopeBytes(uint64_t rows, uint64_t d_hidden) { return (rows * d_hidden 
 // reduction is cut into parts of up to `length` blocks where that ends the launch sooner: the tiles of the last, unfull round;
 // or all of dx's (few rows leave it few tiles with the longest reduction); or all.  By estimate, in blocks (about 0.28 us): a
 // tile costs two besides its own, a part five, for its sums' way to memory, the fold eight and a third for each part.
-// 4096 x 768 x 2048 59 us / 54; 16 rows of it 25 / 15; 600 x 512 x 1376 21 / 16.
+// 4096 x 768 x 2048 59 us / 54 in a graph (63 to 65 called one by one); 16 rows of it 25 / 15; 600 x 512 x 1376 21 / 16.
 constexpr uint32_t kMostPairs = 74, kMostParts = 2 * kMostPairs;
 struct Cut { uint32_t whole, parts, first_part; };
 struct BackwardPlan {
@@ -224,7 +224,9 @@ Status CudaBackend::GatedForward(const see_gated_shape& given, const void* x, co
   k::GatedLaunch l = {};
   k::GatedProblem& p = l.p[0];
   // A pair's accumulator of 128 columns instead of 256 costs nearly as much a block of the reduction (A is read as often), so
-  // it pays only where one round takes the twice as many tiles (600 x 512 x 1376: 7.7 us / 7.1; 4096 x 768 x 2048: 24.4 / 30.6).
+  // it pays only where one round takes the twice as many tiles.  In a graph, us, 256 columns / 128: 600 x 512 x 1376 (66 such
+  // tiles) 9.8 / 9.6, 1024 x 2048 x 1152 (72) 16.9 / 16.4, 600 x 768 x 2048 (96) 13.0 / 14.4, 1024 x 512 x 1376 (88) 11.8 / 12.8;
+  // where 256 columns begin a second round that 128 do not make longer, the rule errs: 1024 x 2048 x 2368 (148) 30.4 / 26.7.
   const uint32_t tn = static_cast<uint64_t>(Up(s.rows, 256)) * Up(s.d_hidden, 64) <= sms_ / 2 ? 128 : 256;
   bool ok = MapOf(&p.a[0], f16, x, s.rows, s.d_in, s.x_stride, 64) && MapOf(&p.b[0], f16, w_gate, s.d_in, s.d_hidden, s.d_hidden, 64) &&
             MapOf(&p.b[1], f16, w_up, s.d_in, s.d_hidden, s.d_hidden, 64) && MapOf(&p.c, f16, hidden, s.rows, s.d_hidden, s.hidden_stride, 32);

@@ -17,7 +17,7 @@
 //
 // Bound by HBM: 14 bytes an element with 16-bit gradients and moments in 8 bits (16 with a 16-bit copy), 28 in f32.  A warp
 // takes blocks of 256 elements, eight a lane, through a ring of two in shared memory that bulk copies fill: the loads of a step
-// straight into registers left half of the bandwidth unused (587 us of 110 million weights, 304 now: 5.8 TB/s).  Of the
+// straight into registers left half of the bandwidth unused (587 us of 110 million weights, 304 to 339 so, by the board: 5.2 to 5.8 TB/s).  Of the
 // instructions, which came next, the roots, quotients and conversions went to the hardware's approximations with a Newton step,
 // and to two elements at once.  The launch carries the table of tensors as a parameter: nothing is uploaded, and a captured
 // launch owns its copy.
@@ -59,7 +59,7 @@ struct AdamRing {
   static constexpr uint32_t kStateBytes = kAdamBlock * kBits / 8;
   static constexpr uint32_t kM = kAdamBlock * 4, kV = kM + kStateBytes, kG = kV + kStateBytes;   // offsets in a slot
   static constexpr uint32_t kSlotBytes = kG + kAdamBlock * 4;
-  // 110 million weights with moments in 8 bits, us: 20 warps 320, 22 310, 23 304, 24 322, 28 337, 32 383.
+  // 110 million weights with moments in 8 bits, us: 20 warps 343, 22 341, 23 330, 24 343, 28 351.
   static constexpr uint32_t kWarps = kBits == 8 ? 23 : 24, kSlots = 2;
   static constexpr uint32_t kBytes = kWarps * kSlots * (kSlotBytes + 8);
 };
@@ -354,7 +354,7 @@ AdamWTensorsKernel(const __grid_constant__ AdamTable<kEntries> table, const Adam
   }
   __syncwarp();
   AwaitPrevious();
-  // A thread block's warps sweep its range of the list side by side (a range to each warp, or one sweep of all, 330 to 350 us); a
+  // A thread block's warps sweep its range of the list side by side (304 us; a range to each warp, or one sweep of all, 330 to 350 on that board); a
   // list that one sweep of all covers is spread over the SMs instead.
   const uint32_t blocks = table.block_end[table.count - 1], all = gridDim.x * R::kWarps;
   const uint32_t each = blocks / gridDim.x, rest = blocks % gridDim.x, begin = blockIdx.x * each + min(blockIdx.x, rest);

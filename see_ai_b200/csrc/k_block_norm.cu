@@ -9,7 +9,8 @@
 // time where widths, strides and addresses allow 16-byte accesses and single columns T apart otherwise; a block has several
 // groups.  Rows reach them through a ring in shared memory, or, single columns and few rows, directly.  A thread has the same
 // columns in every row, so that the backward pass sums dgamma and dbeta over a block's rows in registers; the groups meet in
-// shared memory, the blocks (one to an SM) in NormFoldKernel, both in an order that the sizes alone fix.
+// shared memory, the blocks (one to an SM) in NormFoldKernel, both in a fixed order, which goes by the sizes and by what chooses
+// the kernel and its groups: types, strides, alignment, and whether there is an addend.
 //
 // Sums are f32, but for the mean: the threads' sums are added in double.  A thread's share is summed plainly where it has 16 bits
 // (a few dozen values of 8 or 11 fit); in f32, with what each addition rounds away in NormFwdKernel, where it costs nothing
@@ -934,6 +935,10 @@ cudaError_t Pick(const NormArgs& a, bool backward, uint32_t sms, cudaStream_t s,
   }
   if (vec && a.cols <= 8192) {   // (two slots to a group of the widest)
     const uint32_t n = a.cols / 4, T = n <= 256 ? 32 : (n + 255) / 256 * 32;
+    // Two rows to a group of NormFwdKernel.  About there, us, it / the ring: 768 columns f32 to bf16, 4736 rows 7.2 / 7.2, 5920
+    // 11.2 / 8.9; 2048 f32, 2368 rows 12.8 / 13.0, 2960 16.3 / 13.4; 4096 bf16, 1184 rows 10.3 / 12.8, 1480 13.5 / 13.5.  Rows of few
+    // bytes, and rms ones of 16 bits, would want some more: 64 columns bf16, 14208 rows 4.6 / 5.7; 1024, 9472 rows 10.4 / 12.4; 8192,
+    // 1776 rows 17.7 / 19.9.
     if (a.rows > 2ull * (kNormThreads / T) * sms) {
       if (n <= 64) return RunFwdRing<XT, YT, kRms, 2, true>(a, T, sms, s);
       if (n <= 128) return RunFwdRing<XT, YT, kRms, 4, true>(a, T, sms, s);
@@ -950,7 +955,9 @@ cudaError_t Pick(const NormArgs& a, bool backward, uint32_t sms, cudaStream_t s,
     }
   }
   if (backward) {
-    // Few rows are over before a ring pays (777 x 1029: 8.6 us straight into registers, 14.9), and the widest have no room for one.
+    // Few rows are over before a ring pays, and the widest have no room for one.  About four rows to a group, us, straight into
+    // registers / ring: 9472 x 55 bf16 11.0 / 8.6; 4736 x 333 f32 and bf16 19.5 / 21.1, 7104 26.3 / 24.6; 1776 x 1029 bf16 22.3 / 21.0; 592 x
+    // 4095 bf16 28.4 / 28.7.  Wide f32 rows would want some more: 2664 x 1029 18.9 / 30.0, 1184 x 8001 50.8 / 65.6 (30000 x 1029 155 / 144).
     if (a.cols > 8192 || a.rows <= 4ull * sms * (kNormThreads / f.T)) {
       switch (f.nv) {
         case 8: return RunSingles<XT, YT, kRms, 8>(a, f.T, sms, s, launches);
@@ -963,7 +970,9 @@ cudaError_t Pick(const NormArgs& a, bool backward, uint32_t sms, cudaStream_t s,
     if (each <= 4) return RunOdd<XT, YT, kRms, 4>(a, T, sms, s, launches);
     return each <= 8 ? RunOdd<XT, YT, kRms, 8>(a, T, sms, s, launches) : RunOdd<XT, YT, kRms, 16>(a, T, sms, s, launches);
   }
-  if (a.cols <= 4096 && a.rows > 4ull * sms * (kNormThreads / f.T)) {   // (with two groups at least: 5003 columns 122 us, so 129)
+  // (With two groups at least: 5003 columns 122 us, so 129.  About four rows to a group, us, NormFwdKernel / so: 9472 x 55 bf16 5.0 /
+  // 4.9, 4736 x 333 f32 to bf16 8.9 / 10.4, 7104 12.4 / 12.4, 2220 x 1029 f32 12.8 / 14.0, rms bf16 11.1 / 10.8, 1184 x 4095 18.0 / 18.0.)
+  if (a.cols <= 4096 && a.rows > 4ull * sms * (kNormThreads / f.T)) {
     const uint32_t T = a.cols <= 512 ? 32 : (a.cols + 511) / 512 * 32, each = (a.cols + T - 1) / T;
     if (each <= 2) return RunFwdOdd<XT, YT, kRms, 2>(a, T, sms, s);
     if (each <= 4) return RunFwdOdd<XT, YT, kRms, 4>(a, T, sms, s);
