@@ -275,6 +275,30 @@ typedef struct see_adamw_tensor {
 int see_cuda_adamw_step(see_cuda_backend* h, const see_adamw_tensor* tensors, uint64_t count, int state_bits,
                         const see_step_params* params, const float* grad_scale);
 
+/* ---- Around those: joining a block to the residual stream, losses of preferences and policies, all gradients' norm ----
+ * No counterpart in the reference either: what a step needs on either side of a block, at its end and before AdamW.  The terms
+ * are those of the section above (the caller's device memory, the handle's stream, nothing allocated or waited for, refusals). */
+
+/* norm = |grad_scale| (the sum of g^2 over all elements of `count` tensors)^1/2 (grad_scale: an f32, NULL: 1), and
+ * factor = grad_scale (norm <= max_norm or norm = 0 ? 1 : max_norm / norm), what see_cuda_adamw_step takes as its grad_scale.  Squares are
+ * summed in f32 a few dozen at a time, or in double where f32 would overflow or lose small ones, then in double; norm [1] and
+ * factor [1] are f32.  A norm that is infinite has factor 0, one that is NaN a NaN (a step to be left out: read the norm).
+ * see_cuda_grad_clip writes g times factor to out besides, rounded to the tensor's type; out may be g (NULL: g), where a factor of 1 then writes nothing.
+ * see_cuda_grad_norm ignores out.  `tensors` is HOST memory and is read before the call returns; a tensor of no elements is passed
+ * over, whatever its addresses; up to 2^38 elements each.  max_norm > 0 (infinite: the norm alone).  The same call has the same bits; the sums' order goes by the sizes, alignment and the device's
+ * number of SMs.  workspace: at least see_cuda_grad_workspace() bytes, 16-byte aligned. */
+typedef struct see_grad_tensor {
+  void *g, *out;
+  uint64_t n;
+  int32_t type;
+  uint32_t pad;
+} see_grad_tensor;
+uint64_t see_cuda_grad_workspace(void);
+int see_cuda_grad_norm(see_cuda_backend* h, const see_grad_tensor* tensors, uint64_t count, float max_norm, const float* grad_scale,
+                       float* norm, float* factor, void* workspace, uint64_t workspace_bytes);
+int see_cuda_grad_clip(see_cuda_backend* h, const see_grad_tensor* tensors, uint64_t count, float max_norm, const float* grad_scale,
+                       float* norm, float* factor, void* workspace, uint64_t workspace_bytes);
+
 /* ---- The dispatcher: UpdateEngine over the CUDA backend ----------------------
  * Mirrors the hot-path surface of seeml::update_rt::UpdateEngine (reference:
  * runtime/dispatcher/update_engine.h:211-367).  The engine owns the device slab

@@ -36,6 +36,7 @@ EXPORTED_SYMBOLS = [
     "see_cuda_set_attention_slices", "see_cuda_attention_slices",
     "see_cuda_norm_forward", "see_cuda_norm_backward", "see_cuda_norm_backward_workspace", "see_cuda_adamw_step",
     "see_cuda_gated_forward", "see_cuda_gated_backward", "see_cuda_gated_backward_workspace",
+    "see_cuda_grad_norm", "see_cuda_grad_clip", "see_cuda_grad_workspace",
 ]
 
 # Element types, norms and activations of the operators below.
@@ -80,6 +81,11 @@ class AdamWTensor(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale", "copy")] + [
         ("n", ctypes.c_uint64), ("g_type", ctypes.c_int32), ("copy_type", ctypes.c_int32), ("flags", ctypes.c_uint32),
         ("pad", ctypes.c_uint32)]
+
+
+class GradTensor(ctypes.Structure):
+    _fields_ = [("g", ctypes.c_void_p), ("out", ctypes.c_void_p), ("n", ctypes.c_uint64), ("type", ctypes.c_int32),
+                ("pad", ctypes.c_uint32)]
 
 
 class BackendError(RuntimeError):
@@ -151,6 +157,10 @@ def load_library() -> ctypes.CDLL:
     lib.see_cuda_gated_backward_workspace.argtypes = [u64, u64, u64]
     lib.see_cuda_gated_backward_workspace.restype = u64
     lib.see_cuda_adamw_step.argtypes = [vp, ctypes.POINTER(AdamWTensor), u64, i32, ctypes.POINTER(StepParams), vp]
+    for name in ("see_cuda_grad_norm", "see_cuda_grad_clip"):
+        getattr(lib, name).argtypes = [vp, ctypes.POINTER(GradTensor), u64, ctypes.c_float] + [vp] * 4 + [u64]
+    lib.see_cuda_grad_workspace.argtypes = []
+    lib.see_cuda_grad_workspace.restype = u64
     lib.see_cuda_xent_forward_static.argtypes = [vp, vp, vp, vp, u64, u64, i32, vp]
     lib.see_cuda_static_max_rows.restype = u64
     lib.see_cuda_static_last_error.restype = ctypes.c_char_p
@@ -190,6 +200,20 @@ def adamw_tensors(tensors):
             setattr(entry, key, t.get(key) or None)
         entry.n, entry.g_type, entry.copy_type = t["n"], t.get("g_type", F32), t.get("copy_type", F32)
         entry.flags = ADAMW_NO_DECAY if t.get("no_decay") else 0
+    return table
+
+
+def grad_workspace() -> int:
+    """Bytes that `CudaBackend.grad_norm` and `grad_clip` need beside their operands."""
+    return int(load_library().see_cuda_grad_workspace())
+
+
+def grad_tensors(tensors):
+    """The table `CudaBackend.grad_norm` and `grad_clip` take, of dicts of DEVICE pointers g (and out, where the clipped
+    gradients go; 0 or left out: g itself), the number of elements n and their type."""
+    table = (GradTensor * len(tensors))()
+    for entry, t in zip(table, tensors):
+        entry.g, entry.out, entry.n, entry.type = t.get("g") or None, t.get("out") or None, t["n"], t.get("type", F32)
     return table
 
 
@@ -391,6 +415,17 @@ class CudaBackend:
     def adamw_step(self, tensors, params: StepParams, state_bits: int = 32, grad_scale: int = 0):
         """One AdamW step over a table of adamw_tensors, moments in 8 bits or in 32."""
         self._check(self.lib.see_cuda_adamw_step(self.h, tensors, len(tensors), state_bits, params, grad_scale or None))
+
+    def grad_norm(self, tensors, max_norm: float, norm: int, factor: int, workspace: int, workspace_bytes: int, grad_scale: int = 0):
+        """The norm of all gradients of a table of grad_tensors, and the factor that adamw_step takes as its grad_scale to clip
+        them (grad_scale included).  The workspace has grad_workspace() bytes."""
+        self._check(self.lib.see_cuda_grad_norm(self.h, tensors, len(tensors), max_norm, grad_scale or None, norm or None, factor or None,
+                                                workspace or None, workspace_bytes))
+
+    def grad_clip(self, tensors, max_norm: float, norm: int, factor: int, workspace: int, workspace_bytes: int, grad_scale: int = 0):
+        """The same, and the gradients times the factor to each tensor's out."""
+        self._check(self.lib.see_cuda_grad_clip(self.h, tensors, len(tensors), max_norm, grad_scale or None, norm or None, factor or None,
+                                                workspace or None, workspace_bytes))
 
     def set_profiling(self, on: bool):
         self._check(self.lib.see_cuda_set_profiling(self.h, int(on)))

@@ -9,6 +9,7 @@ namespace see {
 // Bytes for any shape of these sizes, whatever its types and alignment (0: sizes outside the range).
 uint64_t NormBackwardWorkspace(uint64_t rows, uint64_t cols);
 uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden);
+uint64_t GradWorkspace();
 // What a call for these gradients uses of it on a device of `sms`.
 uint64_t GatedBackwardUses(uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool dx, bool dw, uint32_t sms);
 
@@ -24,7 +25,8 @@ Status CheckGatedBackward(see_gated_shape* shape, const void* dhidden, const voi
                           const void* gate, const void* up, const void* dx, const void* dw_gate, const void* dw_up, const void* workspace,
                           uint64_t workspace_bytes);
 Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale);
+Status CheckGrad(const see_grad_tensor* tensors, uint64_t count, bool clip, float max_norm, const float* grad_scale, const float* norm,
+                 const float* factor, const void* workspace, uint64_t workspace_bytes);
 }  // namespace see
-
 
 #endif  // SEE_CUDA_BLOCK_CHECKS_H_

@@ -44,6 +44,12 @@ struct AdamStepScalars {
 cudaError_t AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const AdamStepScalars& a,
                          const float* grad_scale, uint32_t sms, DeviceStatus* status, cudaStream_t s, int* launches);
 
+// ---- all gradients' norm (k_grad_norm.cu) ------------------------------------
+constexpr uint32_t kGradPartials = 1024;      // most thread blocks' sums
+// clip: writes the tensors' out too.  partials [kGradPartials].
+cudaError_t GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, float max_norm, const float* grad_scale, float* norm,
+                     float* factor, double* partials, uint32_t sms, cudaStream_t s, int* launches);
+
 }  // namespace see::k
 
 #endif  // SEE_CUDA_BLOCK_OPS_H_

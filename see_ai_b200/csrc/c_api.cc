@@ -220,6 +220,22 @@ int see_cuda_adamw_step(see_cuda_backend* h, const see_adamw_tensor* tensors, ui
   return Guarded(h, "adamw", params, [&] { return h->backend->AdamWTensors(tensors, count, state_bits, ToParams(params), grad_scale); });
 }
 
+uint64_t see_cuda_grad_workspace(void) { return see::GradWorkspace(); }
+
+int see_cuda_grad_norm(see_cuda_backend* h, const see_grad_tensor* tensors, uint64_t count, float max_norm, const float* grad_scale,
+                       float* norm, float* factor, void* workspace, uint64_t workspace_bytes) {
+  return Guarded(h, "grad norm", h, [&] {
+    return h->backend->GradNorm(tensors, count, false, max_norm, grad_scale, norm, factor, workspace, workspace_bytes);
+  });
+}
+
+int see_cuda_grad_clip(see_cuda_backend* h, const see_grad_tensor* tensors, uint64_t count, float max_norm, const float* grad_scale,
+                       float* norm, float* factor, void* workspace, uint64_t workspace_bytes) {
+  return Guarded(h, "grad clip", h, [&] {
+    return h->backend->GradNorm(tensors, count, true, max_norm, grad_scale, norm, factor, workspace, workspace_bytes);
+  });
+}
+
 int see_cuda_flush(see_cuda_backend* h) {
   auto r = h->backend->Flush();
   return r ? SEE_OK : Fail(h, r.error());

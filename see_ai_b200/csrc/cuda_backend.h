@@ -194,6 +194,9 @@ class CudaBackend {
   Status GatedBackward(const see_gated_shape& shape, const void* dhidden, const void* x, const void* w_gate, const void* w_up,
                        const void* gate, const void* up, void* dx, void* dw_gate, void* dw_up, void* workspace, uint64_t workspace_bytes);
   Status AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale);
+  // Those around them (grad_norm.cc).
+  Status GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, float max_norm, const float* grad_scale, float* norm, float* factor,
+                  void* workspace, uint64_t workspace_bytes);
 
   // Merge deltas launched as a run add their non-finite results to *tally (device memory) from now on; null: they do
   // not.  merge_counted(): how many deltas have been counted that way since the last call of this.
