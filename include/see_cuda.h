@@ -279,6 +279,50 @@ int see_cuda_adamw_step(see_cuda_backend* h, const see_adamw_tensor* tensors, ui
  * No counterpart in the reference either: what a step needs on either side of a block, at its end and before AdamW.  The terms
  * are those of the section above (the caller's device memory, the handle's stream, nothing allocated or waited for, refusals). */
 
+/* Losses over rows of logits, with the gradient of the logits.  logits [rows, classes] (1 .. 2^20 classes, up to 2^31 - 1 rows) of any
+ * type, stride: elements from a row to the next (0: classes); dlogits: of the same type and stride, NULL: not wanted; it may be logits itself (in place).
+ * labels [rows]; a row whose label is not in 0 .. classes - 1 does not count: its logits are not read and its dlogits are zeros.
+ * logp = log softmax(logit_scale logits)[label], sums and logp in f32, sums over rows in double.  loss_grad: an f32 that dlogits is
+ * multiplied by (the scale of the loss), or NULL.  A row that holds a NaN or +inf, or -inf alone, has a NaN loss and NaN
+ * dlogits; finite logits times logit_scale are below 2^127.
+ * The same call has the same bits; the sums' order goes by the sizes, the alignment and the device's number of SMs. */
+enum { SEE_PREFERENCE_SIGMOID = 0, SEE_PREFERENCE_HINGE = 1, SEE_PREFERENCE_SQUARE = 2 };
+/* Sequences 2 i (chosen) and 2 i + 1 (rejected) are a pair; sequence s has the rows starts[s] .. starts[s + 1] - 1 (starts: 2 pairs + 1
+ * ascending row numbers).  Rows before the first and behind the last are neither read nor written.  S_s: the sum of logp over the
+ * sequence's rows that count, or (average != 0) their average; no such row: 0.  ref_logp [2 pairs]: the reference model's S, NULL: 0.
+ *   h_i = beta ((S - ref)[2 i] - (S - ref)[2 i + 1]) - margin,  loss = the average over pairs of
+ *   sigmoid: -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h);  hinge: max(0, 1 - h), no gradient at h = 1;
+ *   square: ((h - 1/2) / beta)^2, whose margin is 0.
+ * beta > 0; smoothing from 0 on and below 1/2, 0 for the others; pairs: 1 to 2^24.  loss [1], margins [pairs] (h) and sequence_logp [2 pairs] (S)
+ * are f32 outputs.  workspace: at least see_cuda_preference_workspace(rows, pairs) bytes, 16-byte aligned. */
+typedef struct see_preference_shape {
+  int32_t type, kind;
+  float beta, smoothing, margin, logit_scale;
+  int32_t average;
+  uint32_t pad;
+  uint64_t rows, classes, stride, pairs;
+} see_preference_shape;
+uint64_t see_cuda_preference_workspace(uint64_t rows, uint64_t pairs);
+int see_cuda_preference_loss(see_cuda_backend* h, const see_preference_shape* shape, const void* logits, const int32_t* labels,
+                             const int32_t* starts, const float* ref_logp, const float* loss_grad, float* loss, float* margins,
+                             float* sequence_logp, void* dlogits, void* workspace, uint64_t workspace_bytes);
+/* With r = exp(logp - old_logp) of a row, A its advantage and x = ref_logp - logp:
+ *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef kl,  kl = exp(x) - x - 1,
+ * and loss [3] = the sums over the rows that count of weight l, weight kl and weight [r A > clip(r) A].  A row clipped so has no
+ * gradient but its KL term's.  old_logp, advantages, weights (NULL: 1), ref_logp (NULL: no KL term, kl_coef 0) and the output
+ * logp (0 where a row does not count) are [rows] in f32; of rows that do not count nothing is read but the label.  clip_low from 0 to 1,
+ * clip_high and kl_coef from 0 on, finite.  workspace: at least see_cuda_policy_workspace(rows) bytes, 16-byte aligned. */
+typedef struct see_policy_shape {
+  int32_t type;
+  float logit_scale, clip_low, clip_high, kl_coef;
+  uint32_t pad;
+  uint64_t rows, classes, stride;
+} see_policy_shape;
+uint64_t see_cuda_policy_workspace(uint64_t rows);
+int see_cuda_policy_loss(see_cuda_backend* h, const see_policy_shape* shape, const void* logits, const int32_t* labels,
+                         const float* old_logp, const float* ref_logp, const float* advantages, const float* weights,
+                         const float* loss_grad, float* loss, float* logp, void* dlogits, void* workspace, uint64_t workspace_bytes);
+
 /* norm = |grad_scale| (the sum of g^2 over all elements of `count` tensors)^1/2 (grad_scale: an f32, NULL: 1), and
  * factor = grad_scale (norm <= max_norm or norm = 0 ? 1 : max_norm / norm), what see_cuda_adamw_step takes as its grad_scale.  Squares are
  * summed in f32 a few dozen at a time, or in double where f32 would overflow or lose small ones, then in double; norm [1] and

@@ -37,6 +37,7 @@ EXPORTED_SYMBOLS = [
     "see_cuda_norm_forward", "see_cuda_norm_backward", "see_cuda_norm_backward_workspace", "see_cuda_adamw_step",
     "see_cuda_gated_forward", "see_cuda_gated_backward", "see_cuda_gated_backward_workspace",
     "see_cuda_grad_norm", "see_cuda_grad_clip", "see_cuda_grad_workspace",
+    "see_cuda_preference_loss", "see_cuda_preference_workspace", "see_cuda_policy_loss", "see_cuda_policy_workspace",
 ]
 
 # Element types, norms and activations of the operators below.
@@ -46,6 +47,8 @@ NORM_LAYER, NORM_RMS = 0, 1
 ACT_RELU, ACT_GELU, ACT_SILU = 1, 2, 3
 ACTS = {"relu": ACT_RELU, "gelu": ACT_GELU, "silu": ACT_SILU}
 ADAMW_BLOCK, ADAMW_NO_DECAY = 256, 1
+PREFERENCE_SIGMOID, PREFERENCE_HINGE, PREFERENCE_SQUARE = 0, 1, 2
+PREFERENCES = {"sigmoid": PREFERENCE_SIGMOID, "hinge": PREFERENCE_HINGE, "square": PREFERENCE_SQUARE}
 
 
 class StepParams(ctypes.Structure):
@@ -86,6 +89,17 @@ class AdamWTensor(ctypes.Structure):
 class GradTensor(ctypes.Structure):
     _fields_ = [("g", ctypes.c_void_p), ("out", ctypes.c_void_p), ("n", ctypes.c_uint64), ("type", ctypes.c_int32),
                 ("pad", ctypes.c_uint32)]
+
+
+class PreferenceShape(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("kind", ctypes.c_int32)] + [
+        (n, ctypes.c_float) for n in ("beta", "smoothing", "margin", "logit_scale")] + [
+        ("average", ctypes.c_int32), ("pad", ctypes.c_uint32)] + [(n, ctypes.c_uint64) for n in ("rows", "classes", "stride", "pairs")]
+
+
+class PolicyShape(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32)] + [(n, ctypes.c_float) for n in ("logit_scale", "clip_low", "clip_high", "kl_coef")] + [
+        ("pad", ctypes.c_uint32)] + [(n, ctypes.c_uint64) for n in ("rows", "classes", "stride")]
 
 
 class BackendError(RuntimeError):
@@ -157,6 +171,12 @@ def load_library() -> ctypes.CDLL:
     lib.see_cuda_gated_backward_workspace.argtypes = [u64, u64, u64]
     lib.see_cuda_gated_backward_workspace.restype = u64
     lib.see_cuda_adamw_step.argtypes = [vp, ctypes.POINTER(AdamWTensor), u64, i32, ctypes.POINTER(StepParams), vp]
+    lib.see_cuda_preference_loss.argtypes = [vp, ctypes.POINTER(PreferenceShape)] + [vp] * 10 + [u64]
+    lib.see_cuda_preference_workspace.argtypes = [u64, u64]
+    lib.see_cuda_preference_workspace.restype = u64
+    lib.see_cuda_policy_loss.argtypes = [vp, ctypes.POINTER(PolicyShape)] + [vp] * 11 + [u64]
+    lib.see_cuda_policy_workspace.argtypes = [u64]
+    lib.see_cuda_policy_workspace.restype = u64
     for name in ("see_cuda_grad_norm", "see_cuda_grad_clip"):
         getattr(lib, name).argtypes = [vp, ctypes.POINTER(GradTensor), u64, ctypes.c_float] + [vp] * 4 + [u64]
     lib.see_cuda_grad_workspace.argtypes = []
@@ -201,6 +221,16 @@ def adamw_tensors(tensors):
         entry.n, entry.g_type, entry.copy_type = t["n"], t.get("g_type", F32), t.get("copy_type", F32)
         entry.flags = ADAMW_NO_DECAY if t.get("no_decay") else 0
     return table
+
+
+def preference_workspace(rows: int, pairs: int) -> int:
+    """Bytes that `CudaBackend.preference_loss` needs beside its operands."""
+    return int(load_library().see_cuda_preference_workspace(rows, pairs))
+
+
+def policy_workspace(rows: int) -> int:
+    """Bytes that `CudaBackend.policy_loss` needs beside its operands."""
+    return int(load_library().see_cuda_policy_workspace(rows))
 
 
 def grad_workspace() -> int:
@@ -415,6 +445,30 @@ class CudaBackend:
     def adamw_step(self, tensors, params: StepParams, state_bits: int = 32, grad_scale: int = 0):
         """One AdamW step over a table of adamw_tensors, moments in 8 bits or in 32."""
         self._check(self.lib.see_cuda_adamw_step(self.h, tensors, len(tensors), state_bits, params, grad_scale or None))
+
+    def preference_loss(self, rows: int, classes: int, pairs: int, logits: int, labels: int, starts: int, loss: int, margins: int,
+                        sequence_logp: int, workspace: int, workspace_bytes: int, ref_logp: int = 0, loss_grad: int = 0, dlogits: int = 0,
+                        type: int = F32, kind: int = PREFERENCE_SIGMOID, beta: float = 0.1, smoothing: float = 0.0, margin: float = 0.0,
+                        logit_scale: float = 1.0, average: bool = False, stride: int = 0):
+        """A preference loss of `pairs` of sequences (2 i chosen, 2 i + 1 rejected; sequence s is the rows starts[s] up to
+        starts[s + 1]) over DEVICE pointers, with the gradient of the logits (dlogits 0: not wanted; logits: in place).  The
+        workspace has preference_workspace(rows, pairs) bytes."""
+        shape = PreferenceShape(type, kind, beta, smoothing, margin, logit_scale, int(average), 0, rows, classes, stride, pairs)
+        self._check(self.lib.see_cuda_preference_loss(self.h, shape, logits or None, labels or None, starts or None, ref_logp or None,
+                                                      loss_grad or None, loss or None, margins or None, sequence_logp or None,
+                                                      dlogits or None, workspace or None, workspace_bytes))
+
+    def policy_loss(self, rows: int, classes: int, logits: int, labels: int, old_logp: int, advantages: int, loss: int, logp: int,
+                    workspace: int, workspace_bytes: int, ref_logp: int = 0, weights: int = 0, loss_grad: int = 0, dlogits: int = 0,
+                    type: int = F32, logit_scale: float = 1.0, clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0,
+                    stride: int = 0):
+        """A clipped policy loss with a KL term over DEVICE pointers, with the gradient of the logits (dlogits 0: not wanted;
+        logits: in place); loss [3]: the loss, the KL term, the clipped rows, each summed by the rows' weights.  The workspace
+        has policy_workspace(rows) bytes."""
+        shape = PolicyShape(type, logit_scale, clip_low, clip_high, kl_coef, 0, rows, classes, stride)
+        self._check(self.lib.see_cuda_policy_loss(self.h, shape, logits or None, labels or None, old_logp or None, ref_logp or None,
+                                                  advantages or None, weights or None, loss_grad or None, loss or None, logp or None,
+                                                  dlogits or None, workspace or None, workspace_bytes))
 
     def grad_norm(self, tensors, max_norm: float, norm: int, factor: int, workspace: int, workspace_bytes: int, grad_scale: int = 0):
         """The norm of all gradients of a table of grad_tensors, and the factor that adamw_step takes as its grad_scale to clip

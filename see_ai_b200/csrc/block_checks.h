@@ -10,6 +10,8 @@ namespace see {
 uint64_t NormBackwardWorkspace(uint64_t rows, uint64_t cols);
 uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden);
 uint64_t GradWorkspace();
+uint64_t PreferenceWorkspace(uint64_t rows, uint64_t pairs);
+uint64_t PolicyWorkspace(uint64_t rows);
 // What a call for these gradients uses of it on a device of `sms`.
 uint64_t GatedBackwardUses(uint64_t rows, uint64_t d_in, uint64_t d_hidden, bool dx, bool dw, uint32_t sms);
 
@@ -25,6 +27,12 @@ Status CheckGatedBackward(see_gated_shape* shape, const void* dhidden, const voi
                           const void* gate, const void* up, const void* dx, const void* dw_gate, const void* dw_up, const void* workspace,
                           uint64_t workspace_bytes);
 Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale);
+Status CheckPreference(see_preference_shape* shape, const void* logits, const int32_t* labels, const int32_t* starts, const float* ref_logp,
+                       const float* loss_grad, const float* loss, const float* margins, const float* sequence_logp, const void* dlogits,
+                       const void* workspace, uint64_t workspace_bytes);
+Status CheckPolicy(see_policy_shape* shape, const void* logits, const int32_t* labels, const float* old_logp, const float* ref_logp,
+                   const float* advantages, const float* weights, const float* loss_grad, const float* loss, const float* logp,
+                   const void* dlogits, const void* workspace, uint64_t workspace_bytes);
 Status CheckGrad(const see_grad_tensor* tensors, uint64_t count, bool clip, float max_norm, const float* grad_scale, const float* norm,
                  const float* factor, const void* workspace, uint64_t workspace_bytes);
 }  // namespace see

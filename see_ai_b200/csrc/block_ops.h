@@ -44,6 +44,33 @@ struct AdamStepScalars {
 cudaError_t AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const AdamStepScalars& a,
                          const float* grad_scale, uint32_t sms, DeviceStatus* status, cudaStream_t s, int* launches);
 
+// ---- losses over rows of logits (k_logit_loss.cu) ------------------------------
+constexpr uint32_t kLogitPartials = 1024;     // most thread blocks' sums
+struct LogitArgs {
+  const void* logits;
+  void* dlogits;                              // or null
+  const int32_t* labels;
+  uint64_t rows, stride;
+  uint32_t classes;
+  float scale, k;                             // k: scale / ln 2
+};
+struct PolicyArgs {
+  const float *old_logp, *ref_logp, *advantages, *weights, *loss_grad;
+  float *loss, *logp;
+  float clip_low, clip_high, kl_coef;
+};
+struct PreferenceArgs {
+  const int32_t* starts;
+  const float *ref_logp, *loss_grad;
+  float *loss, *margins, *sequence_logp, *slopes;
+  uint32_t pairs;
+  int kind, average;
+  float beta, smoothing, margin;
+};
+// partials [kLogitPartials][3]; kept [rows].
+cudaError_t PolicyLoss(const LogitArgs& a, int type, const PolicyArgs& p, double* partials, uint32_t sms, cudaStream_t s, int* launches);
+cudaError_t PreferenceLoss(const LogitArgs& a, int type, const PreferenceArgs& p, float4* kept, uint32_t sms, cudaStream_t s, int* launches);
+
 // ---- all gradients' norm (k_grad_norm.cu) ------------------------------------
 constexpr uint32_t kGradPartials = 1024;      // most thread blocks' sums
 // clip: writes the tensors' out too.  partials [kGradPartials].

@@ -220,6 +220,28 @@ int see_cuda_adamw_step(see_cuda_backend* h, const see_adamw_tensor* tensors, ui
   return Guarded(h, "adamw", params, [&] { return h->backend->AdamWTensors(tensors, count, state_bits, ToParams(params), grad_scale); });
 }
 
+uint64_t see_cuda_preference_workspace(uint64_t rows, uint64_t pairs) { return see::PreferenceWorkspace(rows, pairs); }
+
+int see_cuda_preference_loss(see_cuda_backend* h, const see_preference_shape* shape, const void* logits, const int32_t* labels,
+                             const int32_t* starts, const float* ref_logp, const float* loss_grad, float* loss, float* margins,
+                             float* sequence_logp, void* dlogits, void* workspace, uint64_t workspace_bytes) {
+  return Guarded(h, "preference loss", shape, [&] {
+    return h->backend->PreferenceLoss(*shape, logits, labels, starts, ref_logp, loss_grad, loss, margins, sequence_logp, dlogits, workspace,
+                                      workspace_bytes);
+  });
+}
+
+uint64_t see_cuda_policy_workspace(uint64_t rows) { return see::PolicyWorkspace(rows); }
+
+int see_cuda_policy_loss(see_cuda_backend* h, const see_policy_shape* shape, const void* logits, const int32_t* labels,
+                         const float* old_logp, const float* ref_logp, const float* advantages, const float* weights,
+                         const float* loss_grad, float* loss, float* logp, void* dlogits, void* workspace, uint64_t workspace_bytes) {
+  return Guarded(h, "policy loss", shape, [&] {
+    return h->backend->PolicyLoss(*shape, logits, labels, old_logp, ref_logp, advantages, weights, loss_grad, loss, logp, dlogits, workspace,
+                                  workspace_bytes);
+  });
+}
+
 uint64_t see_cuda_grad_workspace(void) { return see::GradWorkspace(); }
 
 int see_cuda_grad_norm(see_cuda_backend* h, const see_grad_tensor* tensors, uint64_t count, float max_norm, const float* grad_scale,

@@ -194,7 +194,13 @@ class CudaBackend {
   Status GatedBackward(const see_gated_shape& shape, const void* dhidden, const void* x, const void* w_gate, const void* w_up,
                        const void* gate, const void* up, void* dx, void* dw_gate, void* dw_up, void* workspace, uint64_t workspace_bytes);
   Status AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale);
-  // Those around them (grad_norm.cc).
+  // Those around them (logit_loss.cc, grad_norm.cc).
+  Status PreferenceLoss(const see_preference_shape& shape, const void* logits, const int32_t* labels, const int32_t* starts,
+                        const float* ref_logp, const float* loss_grad, float* loss, float* margins, float* sequence_logp, void* dlogits,
+                        void* workspace, uint64_t workspace_bytes);
+  Status PolicyLoss(const see_policy_shape& shape, const void* logits, const int32_t* labels, const float* old_logp, const float* ref_logp,
+                    const float* advantages, const float* weights, const float* loss_grad, float* loss, float* logp, void* dlogits,
+                    void* workspace, uint64_t workspace_bytes);
   Status GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, float max_norm, const float* grad_scale, float* norm, float* factor,
                   void* workspace, uint64_t workspace_bytes);
 
