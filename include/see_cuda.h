@@ -279,6 +279,37 @@ int see_cuda_adamw_step(see_cuda_backend* h, const see_adamw_tensor* tensors, ui
  * No counterpart in the reference either: what a step needs on either side of a block, at its end and before AdamW.  The terms
  * are those of the section above (the caller's device memory, the handle's stream, nothing allocated or waited for, refusals). */
 
+/* x_out = residual_scale x + gate * N1(block) and y = N2(x_out): the norm after a block, its gate, the scaled residual and the norm
+ * before the next block.  N1 and N2 are of one kind, as in see_cuda_norm_forward, over rows of `cols` columns (1 .. 16384), up to
+ * 2^31 - 1 of them; y is made of x_out before that is rounded to its type.  x_type: of x, x_out, dx_out and dx; y_type: of block, y,
+ * dy and dblock; equal, or x_type f32.  Strides: elements from a row to the next (0: cols), of the former and the latter.
+ * residual_scale: finite. */
+typedef struct see_join_shape {
+  int32_t kind, x_type, y_type;
+  float eps, residual_scale;
+  uint32_t pad;
+  uint64_t rows, cols, x_stride, y_stride;
+} see_join_shape;
+/* Weights, or their gradients: [cols] in f32.  post: N1's; pre: N2's.  beta is NULL for rms norms.  post_gamma (with post_beta) NULL:
+ * no norm after the block, N1(block) = block.  gate NULL: 1.  The structs are HOST memory, read before the call returns. */
+typedef struct see_join_weights {
+  float *post_gamma, *post_beta, *gate, *pre_gamma, *pre_beta;
+} see_join_weights;
+/* What the forward pass keeps of each row, [rows] in f32.  The means are NULL for rms norms, post's both without a norm there. */
+typedef struct see_join_stats {
+  float *post_mean, *post_rstd, *pre_mean, *pre_rstd;
+} see_join_stats;
+int see_cuda_join_forward(see_cuda_backend* h, const see_join_shape* shape, const void* x, const void* block,
+                          const see_join_weights* weights, void* x_out, void* y, const see_join_stats* stats);
+/* dx and dblock from dy and dx_out (the gradient that reaches x_out past the norm; NULL: none), and the gradients of the weights
+ * that there are: f32 sums over all rows (zero rows: zeros).  pre_beta is not read.  The same call has the same bits; the sums' order
+ * goes by what see_cuda_norm_backward's goes by.  workspace: at least see_cuda_join_backward_workspace(rows, cols) bytes, 16-byte
+ * aligned. */
+uint64_t see_cuda_join_backward_workspace(uint64_t rows, uint64_t cols);
+int see_cuda_join_backward(see_cuda_backend* h, const see_join_shape* shape, const void* dy, const void* dx_out, const void* x_out,
+                           const void* block, const see_join_weights* weights, const see_join_stats* stats, void* dx, void* dblock,
+                           const see_join_weights* gradients, void* workspace, uint64_t workspace_bytes);
+
 /* Losses over rows of logits, with the gradient of the logits.  logits [rows, classes] (1 .. 2^20 classes, up to 2^31 - 1 rows) of any
  * type, stride: elements from a row to the next (0: classes); dlogits: of the same type and stride, NULL: not wanted; it may be logits itself (in place).
  * labels [rows]; a row whose label is not in 0 .. classes - 1 does not count: its logits are not read and its dlogits are zeros.

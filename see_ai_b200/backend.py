@@ -36,6 +36,7 @@ EXPORTED_SYMBOLS = [
     "see_cuda_set_attention_slices", "see_cuda_attention_slices",
     "see_cuda_norm_forward", "see_cuda_norm_backward", "see_cuda_norm_backward_workspace", "see_cuda_adamw_step",
     "see_cuda_gated_forward", "see_cuda_gated_backward", "see_cuda_gated_backward_workspace",
+    "see_cuda_join_forward", "see_cuda_join_backward", "see_cuda_join_backward_workspace",
     "see_cuda_grad_norm", "see_cuda_grad_clip", "see_cuda_grad_workspace",
     "see_cuda_preference_loss", "see_cuda_preference_workspace", "see_cuda_policy_loss", "see_cuda_policy_workspace",
 ]
@@ -89,6 +90,20 @@ class AdamWTensor(ctypes.Structure):
 class GradTensor(ctypes.Structure):
     _fields_ = [("g", ctypes.c_void_p), ("out", ctypes.c_void_p), ("n", ctypes.c_uint64), ("type", ctypes.c_int32),
                 ("pad", ctypes.c_uint32)]
+
+
+class JoinShape(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int32), ("x_type", ctypes.c_int32), ("y_type", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("residual_scale", ctypes.c_float), ("pad", ctypes.c_uint32)] + [
+        (n, ctypes.c_uint64) for n in ("rows", "cols", "x_stride", "y_stride")]
+
+
+class JoinWeights(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("post_gamma", "post_beta", "gate", "pre_gamma", "pre_beta")]
+
+
+class JoinStats(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("post_mean", "post_rstd", "pre_mean", "pre_rstd")]
 
 
 class PreferenceShape(ctypes.Structure):
@@ -171,6 +186,11 @@ def load_library() -> ctypes.CDLL:
     lib.see_cuda_gated_backward_workspace.argtypes = [u64, u64, u64]
     lib.see_cuda_gated_backward_workspace.restype = u64
     lib.see_cuda_adamw_step.argtypes = [vp, ctypes.POINTER(AdamWTensor), u64, i32, ctypes.POINTER(StepParams), vp]
+    lib.see_cuda_join_forward.argtypes = [vp, ctypes.POINTER(JoinShape), vp, vp, ctypes.POINTER(JoinWeights), vp, vp, ctypes.POINTER(JoinStats)]
+    lib.see_cuda_join_backward.argtypes = [vp, ctypes.POINTER(JoinShape)] + [vp] * 4 + [
+        ctypes.POINTER(JoinWeights), ctypes.POINTER(JoinStats), vp, vp, ctypes.POINTER(JoinWeights), vp, u64]
+    lib.see_cuda_join_backward_workspace.argtypes = [u64, u64]
+    lib.see_cuda_join_backward_workspace.restype = u64
     lib.see_cuda_preference_loss.argtypes = [vp, ctypes.POINTER(PreferenceShape)] + [vp] * 10 + [u64]
     lib.see_cuda_preference_workspace.argtypes = [u64, u64]
     lib.see_cuda_preference_workspace.restype = u64
@@ -221,6 +241,21 @@ def adamw_tensors(tensors):
         entry.n, entry.g_type, entry.copy_type = t["n"], t.get("g_type", F32), t.get("copy_type", F32)
         entry.flags = ADAMW_NO_DECAY if t.get("no_decay") else 0
     return table
+
+
+def join_backward_workspace(rows: int, cols: int) -> int:
+    """Bytes that `CudaBackend.join_backward` needs beside its operands."""
+    return int(load_library().see_cuda_join_backward_workspace(rows, cols))
+
+
+def join_weights(pre_gamma: int, pre_beta: int = 0, gate: int = 0, post_gamma: int = 0, post_beta: int = 0):
+    """The weights `CudaBackend.join_forward` and `join_backward` take, or their gradients: DEVICE pointers, 0 for what is not there."""
+    return JoinWeights(post_gamma or None, post_beta or None, gate or None, pre_gamma or None, pre_beta or None)
+
+
+def join_stats(pre_rstd: int, pre_mean: int = 0, post_rstd: int = 0, post_mean: int = 0):
+    """Where `CudaBackend.join_forward` keeps each row's statistics for `join_backward`: DEVICE pointers, 0 for what is not there."""
+    return JoinStats(post_mean or None, post_rstd or None, pre_mean or None, pre_rstd or None)
 
 
 def preference_workspace(rows: int, pairs: int) -> int:
@@ -445,6 +480,22 @@ class CudaBackend:
     def adamw_step(self, tensors, params: StepParams, state_bits: int = 32, grad_scale: int = 0):
         """One AdamW step over a table of adamw_tensors, moments in 8 bits or in 32."""
         self._check(self.lib.see_cuda_adamw_step(self.h, tensors, len(tensors), state_bits, params, grad_scale or None))
+
+    def join_forward(self, kind: int, rows: int, cols: int, x: int, block: int, weights: JoinWeights, x_out: int, y: int, stats: JoinStats,
+                     x_type: int = F32, y_type: int = F32, eps: float = 1e-5, residual_scale: float = 1.0, x_stride: int = 0, y_stride: int = 0):
+        """x_out = residual_scale x + gate * N1(block), y = N2(x_out) over DEVICE pointers: the norm after a block (join_weights without
+        post_gamma: none), its gate (without gate: 1), the scaled residual and the norm before the next block."""
+        shape = JoinShape(kind, x_type, y_type, eps, residual_scale, 0, rows, cols, x_stride, y_stride)
+        self._check(self.lib.see_cuda_join_forward(self.h, shape, x or None, block or None, weights, x_out or None, y or None, stats))
+
+    def join_backward(self, kind: int, rows: int, cols: int, dy: int, dx_out: int, x_out: int, block: int, weights: JoinWeights,
+                      stats: JoinStats, dx: int, dblock: int, gradients: JoinWeights, workspace: int, workspace_bytes: int,
+                      x_type: int = F32, y_type: int = F32, residual_scale: float = 1.0, x_stride: int = 0, y_stride: int = 0):
+        """Its backward pass with the gradients of the weights; `dx_out` is what reaches x_out past the norm (0: nothing).  The
+        workspace has join_backward_workspace(rows, cols) bytes."""
+        shape = JoinShape(kind, x_type, y_type, 0.0, residual_scale, 0, rows, cols, x_stride, y_stride)
+        self._check(self.lib.see_cuda_join_backward(self.h, shape, dy or None, dx_out or None, x_out or None, block or None, weights, stats,
+                                                    dx or None, dblock or None, gradients, workspace or None, workspace_bytes))
 
     def preference_loss(self, rows: int, classes: int, pairs: int, logits: int, labels: int, starts: int, loss: int, margins: int,
                         sequence_logp: int, workspace: int, workspace_bytes: int, ref_logp: int = 0, loss_grad: int = 0, dlogits: int = 0,

@@ -46,10 +46,11 @@ CU_SOURCES = {
     "k_adamw.cu": ["-fmad=false"],
     "k_gated_umma.cu": [],
     "k_gated_token.cu": [],
+    "k_join.cu": [],
     "k_grad_norm.cu": [],
     "k_logit_loss.cu": [],
 }
-CC_SOURCES = ["extents.cc", "cuda_backend.cc", "c_api.cc", "umma_gemm.cc", "engine.cc", "exchange.cc", "block_ops.cc", "gated.cc", "grad_norm.cc", "logit_loss.cc"]
+CC_SOURCES = ["extents.cc", "cuda_backend.cc", "c_api.cc", "umma_gemm.cc", "engine.cc", "exchange.cc", "block_ops.cc", "gated.cc", "join.cc", "grad_norm.cc", "logit_loss.cc"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O3", "-lineinfo",
               "--expt-extended-lambda", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",

@@ -9,6 +9,7 @@ namespace see {
 // Bytes for any shape of these sizes, whatever its types and alignment (0: sizes outside the range).
 uint64_t NormBackwardWorkspace(uint64_t rows, uint64_t cols);
 uint64_t GatedBackwardWorkspace(uint64_t rows, uint64_t d_in, uint64_t d_hidden);
+uint64_t JoinBackwardWorkspace(uint64_t rows, uint64_t cols);
 uint64_t GradWorkspace();
 uint64_t PreferenceWorkspace(uint64_t rows, uint64_t pairs);
 uint64_t PolicyWorkspace(uint64_t rows);
@@ -27,6 +28,11 @@ Status CheckGatedBackward(see_gated_shape* shape, const void* dhidden, const voi
                           const void* gate, const void* up, const void* dx, const void* dw_gate, const void* dw_up, const void* workspace,
                           uint64_t workspace_bytes);
 Status CheckAdamW(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale);
+Status CheckJoinForward(see_join_shape* shape, const void* x, const void* block, const see_join_weights* weights, const void* x_out,
+                        const void* y, const see_join_stats* stats);
+Status CheckJoinBackward(see_join_shape* shape, const void* dy, const void* dx_out, const void* x_out, const void* block,
+                         const see_join_weights* weights, const see_join_stats* stats, const void* dx, const void* dblock,
+                         const see_join_weights* gradients, const void* workspace, uint64_t workspace_bytes);
 Status CheckPreference(see_preference_shape* shape, const void* logits, const int32_t* labels, const int32_t* starts, const float* ref_logp,
                        const float* loss_grad, const float* loss, const float* margins, const float* sequence_logp, const void* dlogits,
                        const void* workspace, uint64_t workspace_bytes);

@@ -44,6 +44,24 @@ struct AdamStepScalars {
 cudaError_t AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const AdamStepScalars& a,
                          const float* grad_scale, uint32_t sms, DeviceStatus* status, cudaStream_t s, int* launches);
 
+// ---- a block's join to the residual stream (k_join.cu) -------------------------
+struct JoinArgs {
+  const void *x = nullptr, *block = nullptr;   // x: of the backward pass, what the forward pass made of it
+  void *x_out = nullptr, *y = nullptr;
+  const void *dy = nullptr, *dx_out = nullptr;
+  void *dx = nullptr, *dblock = nullptr;
+  see_join_weights w = {}, grads = {};
+  see_join_stats stats = {};
+  float* partials = nullptr;                   // [4][blocks][cols]
+  uint64_t rows = 0, x_stride = 0, y_stride = 0;
+  uint32_t cols = 0;
+  int x_type = SEE_F32, y_type = SEE_F32;
+  bool rms = false;
+  float eps = 0.0f, scale = 1.0f;
+  DeviceStatus* status = nullptr;
+};
+cudaError_t Join(const JoinArgs& a, bool backward, uint32_t sms, cudaStream_t s, int* launches);
+
 // ---- losses over rows of logits (k_logit_loss.cu) ------------------------------
 constexpr uint32_t kLogitPartials = 1024;     // most thread blocks' sums
 struct LogitArgs {

@@ -220,6 +220,21 @@ int see_cuda_adamw_step(see_cuda_backend* h, const see_adamw_tensor* tensors, ui
   return Guarded(h, "adamw", params, [&] { return h->backend->AdamWTensors(tensors, count, state_bits, ToParams(params), grad_scale); });
 }
 
+int see_cuda_join_forward(see_cuda_backend* h, const see_join_shape* shape, const void* x, const void* block,
+                          const see_join_weights* weights, void* x_out, void* y, const see_join_stats* stats) {
+  return Guarded(h, "join forward", shape, [&] { return h->backend->JoinForward(*shape, x, block, weights, x_out, y, stats); });
+}
+
+uint64_t see_cuda_join_backward_workspace(uint64_t rows, uint64_t cols) { return see::JoinBackwardWorkspace(rows, cols); }
+
+int see_cuda_join_backward(see_cuda_backend* h, const see_join_shape* shape, const void* dy, const void* dx_out, const void* x_out,
+                           const void* block, const see_join_weights* weights, const see_join_stats* stats, void* dx, void* dblock,
+                           const see_join_weights* gradients, void* workspace, uint64_t workspace_bytes) {
+  return Guarded(h, "join backward", shape, [&] {
+    return h->backend->JoinBackward(*shape, dy, dx_out, x_out, block, weights, stats, dx, dblock, gradients, workspace, workspace_bytes);
+  });
+}
+
 uint64_t see_cuda_preference_workspace(uint64_t rows, uint64_t pairs) { return see::PreferenceWorkspace(rows, pairs); }
 
 int see_cuda_preference_loss(see_cuda_backend* h, const see_preference_shape* shape, const void* logits, const int32_t* labels,

@@ -194,7 +194,12 @@ class CudaBackend {
   Status GatedBackward(const see_gated_shape& shape, const void* dhidden, const void* x, const void* w_gate, const void* w_up,
                        const void* gate, const void* up, void* dx, void* dw_gate, void* dw_up, void* workspace, uint64_t workspace_bytes);
   Status AdamWTensors(const see_adamw_tensor* tensors, uint64_t count, int state_bits, const StepParams& params, const float* grad_scale);
-  // Those around them (logit_loss.cc, grad_norm.cc).
+  // Those around them (join.cc, logit_loss.cc, grad_norm.cc).
+  Status JoinForward(const see_join_shape& shape, const void* x, const void* block, const see_join_weights* weights, void* x_out, void* y,
+                     const see_join_stats* stats);
+  Status JoinBackward(const see_join_shape& shape, const void* dy, const void* dx_out, const void* x_out, const void* block,
+                      const see_join_weights* weights, const see_join_stats* stats, void* dx, void* dblock, const see_join_weights* gradients,
+                      void* workspace, uint64_t workspace_bytes);
   Status PreferenceLoss(const see_preference_shape& shape, const void* logits, const int32_t* labels, const int32_t* starts,
                         const float* ref_logp, const float* loss_grad, float* loss, float* margins, float* sequence_logp, void* dlogits,
                         void* workspace, uint64_t workspace_bytes);

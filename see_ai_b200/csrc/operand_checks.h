@@ -85,7 +85,7 @@ class Operands {
   }
 
  private:
-  Operand ops_[12];
+  Operand ops_[24];
   size_t count_ = 0;
 };
 
