@@ -47,6 +47,8 @@ CU_SOURCES = {
     "k_gated_umma.cu": [],
     "k_gated_token.cu": [],
     "k_join.cu": [],
+    "k_join_fwd.cu": [],
+    "k_join_bwd.cu": [],
     "k_grad_norm.cu": [],
     "k_logit_loss.cu": [],
 }

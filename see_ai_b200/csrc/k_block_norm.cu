@@ -18,11 +18,10 @@
 // to 31.5 at 32768 x 768).  The variance is the average square of the deviations, a second pass over the registers, less the
 // square of what that mean is off (its rounding; in the ring kernels the average deviation): beside a small eps that would show in
 // rows far from zero, whose squares a sum of x^2 would lose altogether.
-#include <atomic>
-
 #include "act_expr.cuh"
 #include "block_ops.h"
 #include "launch.cuh"
+#include "row_groups.cuh"
 #include "umma_device.cuh"
 #include "vec_types.cuh"
 
@@ -31,73 +30,12 @@ namespace see::k {
 namespace {
 
 constexpr uint32_t kNormThreads = 512;
-constexpr uint32_t kWideThreads = 768;
-constexpr size_t kRingBytes = 200 * 1024, kMostShared = 224 * 1024;   // of a block
-
-template <bool kBoth>
-__device__ __forceinline__ float2 WarpSum(float2 v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, o);
-    if (kBoth) v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, o);
-  }
-  return v;
-}
-
-// The sums of a group's T threads, in all of them.  `slots`: two sets of 16 per block, used in turn, so that one barrier
-// a sum is enough: who writes a set again has passed the barrier that the readers of its last use arrived at after it.
-template <bool kBoth>   // or v.x alone
-__device__ __forceinline__ float2 GroupSum(float2 v, uint32_t T, uint32_t group, float2 (*slots)[kWideThreads / 32], uint32_t& turn) {
-  v = WarpSum<kBoth>(v);
-  if (T == 32) return v;
-  float2* set = slots[turn] + group * (T / 32);
-  turn ^= 1;
-  if ((threadIdx.x & 31) == 0) set[(threadIdx.x - group * T) >> 5] = v;
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(T) : "memory");
-  float2 sum = set[0];
-  for (uint32_t w = 1; w < T / 32; ++w) {
-    sum.x += set[w].x;
-    if (kBoth) sum.y += set[w].y;
-  }
-  return sum;
-}
-
-// The same of one double.
-__device__ __forceinline__ double GroupSum(double v, uint32_t T, uint32_t group, float2 (*slots)[kWideThreads / 32], uint32_t& turn) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  if (T == 32) return v;
-  double* set = reinterpret_cast<double*>(slots[turn]) + group * (T / 32);
-  turn ^= 1;
-  if ((threadIdx.x & 31) == 0) set[(threadIdx.x - group * T) >> 5] = v;
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(T) : "memory");
-  double sum = set[0];
-  for (uint32_t w = 1; w < T / 32; ++w) sum += set[w];
-  return sum;
-}
 
 // sum + x into sum, what that rounds away into rest (Knuth's TwoSum: no order of magnitudes asked for).
 __device__ __forceinline__ void AddExactly(float& sum, float& rest, float x) {
   const float s = sum + x, z = s - sum;
   rest += (sum - (s - z)) + (x - z);
   sum = s;
-}
-
-// The variance, from the average square of deviations from a mean that is off by `off`, their own average.  (What is not finite stays.)
-__device__ __forceinline__ float Variance(float square, float off) {
-  const float less = square - off * off;
-  return !isfinite(off * off) ? square : less < 0.0f ? 0.0f : less;
-}
-
-template <typename T, int VEC>
-__device__ __forceinline__ void LoadCols(const T* p, float* v) {
-  if constexpr (VEC == 8) Load8<T>(p, v);
-  else v[0] = ToF32(*p);
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void StoreCols(T* p, const float* v) {
-  if constexpr (VEC == 8) Store8<T>(p, v);
-  else *p = FromF32<T>(v[0]);
 }
 
 template <typename XT, typename YT, bool kRms, int VEC, int NV>
@@ -208,18 +146,6 @@ template <typename T> __device__ __forceinline__ void StoreFour(T* p, const f32x
 // Each group has `slots` of its own, filled by one thread's bulk copies (a whole row each, counted on the slot's mbarrier)
 // and emptied into registers; a slot is asked to be filled again as soon as the group has read it, so that between 60 and
 // 200 KB are on their way to an SM at any time.
-__device__ __forceinline__ void GroupBarrier(uint32_t T, uint32_t group) {
-  if (T == 32) __syncwarp();
-  else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(T) : "memory");
-}
-// A bulk copy of this device's memory always lands; that nothing can wait for good even so, the wait is bounded, and a thread
-// that ran out raises the flag and goes on (the others of its group count on it at their barriers).
-__device__ __forceinline__ void AwaitRow(uint64_t* bar, uint32_t parity, DeviceStatus* status) {
-  if (umma_dev::MbarWait(bar, parity)) return;
-  status->wait_timeout = 1;
-  umma_dev::DrainDelay();
-}
-
 // The forward pass of more than two rows to a group.  NV: times four columns to a thread.  Up to 768 columns a row is a warp's
 // and gamma and beta stay in registers (kHold); of wider ones they lie in shared memory, which leaves registers for half as many
 // threads again.  Read from global memory for every row, as NormFwdKernel does, they are twice an f32 row's bytes.  NormFwdKernel
@@ -478,27 +404,6 @@ NormBwdRingKernel(const __grid_constant__ NormArgs a, uint32_t T, uint32_t slots
 // and is used from where it begins.  The others are copied element by element.  Threads then take single columns, T apart.
 // Straight into registers / so, us: 30000 x 1029 f32 155 / 144, bf16 295 / 127; 8000 x 5003 f32 and bf16 566 / 215;
 // 40373 x 55 f32 and f16 with an addend 34 / 23.
-template <typename T>
-struct OddRow {
-  const uint8_t* from;   // 16-byte aligned, at most 15 bytes before the row
-  uint32_t skip, bytes;  // ... in front of it; to copy, a multiple of 16
-  __device__ __forceinline__ OddRow(const void* base, uint64_t row, uint64_t stride, uint32_t cols) {
-    const uint64_t at = reinterpret_cast<uint64_t>(static_cast<const T*>(base) + row * stride);
-    skip = static_cast<uint32_t>(at & 15);
-    from = reinterpret_cast<const uint8_t*>(at - skip);
-    bytes = (skip + cols * static_cast<uint32_t>(sizeof(T)) + 15) & ~15u;
-  }
-};
-template <typename T> __host__ __device__ constexpr uint32_t OddSlot(uint32_t cols) { return (cols * sizeof(T) + 45) / 16 * 16; }
-
-// Element-wise, by the whole group; the caller synchronises.
-template <typename T>
-__device__ __forceinline__ void CopyRow(uint8_t* slot, const void* base, uint64_t row, uint64_t stride, uint32_t cols, uint32_t t, uint32_t threads) {
-  const T* from = static_cast<const T*>(base) + row * stride;
-  T* to = reinterpret_cast<T*>(slot + (reinterpret_cast<uint64_t>(from) & 15));
-  for (uint32_t c = t; c < cols; c += threads) to[c] = from[c];
-}
-
 // NV single columns a thread.
 template <typename XT, typename YT, bool kRms, int NV>
 __global__ void __launch_bounds__(kNormThreads, 1)
@@ -822,21 +727,6 @@ cudaError_t Fold(const NormArgs& a, uint64_t grid, cudaStream_t s, int* launches
   if (grid == 1) return cudaSuccess;
   ++*launches;
   return Next(NormFoldKernel, dim3((a.cols + 31) / 32, kRms ? 1 : 2), 1024, 0, s)(a.partials, a.dgamma, a.dbeta, static_cast<uint32_t>(grid), a.cols);
-}
-// A kernel's limit of shared memory is a device's: what has been granted is remembered for each (the call takes the driver a
-// microsecond or two).
-template <auto kKernel>
-cudaError_t AllowShared(size_t bytes) {
-  if (bytes <= 32 * 1024) return cudaSuccess;   // (the static part counts too)
-  static std::atomic<size_t> granted[64] = {};
-  int dev = 0;
-  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
-  if (dev >= 0 && dev < 64 && granted[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
-  // (grants only grow: the most that any call asks for)
-  if (cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostShared)); e != cudaSuccess)
-    return e;
-  if (dev >= 0 && dev < 64) granted[dev].store(kMostShared, std::memory_order_release);
-  return cudaSuccess;
 }
 uint64_t Blocks(uint64_t rows, uint32_t groups, uint32_t sms) {
   const uint64_t blocks = (rows + groups - 1) / groups, most = sms < kNormPartials ? sms : kNormPartials;

@@ -8,9 +8,7 @@
 //
 // A mean is that of the threads' f32 sums, added in double, corrected by the average deviation from it; the variance is the average
 // square of the deviations less the square of that correction.  y comes of x' before it is rounded to the stream's type.
-#include "block_ops.h"
-#include "launch.cuh"
-#include "vec_types.cuh"
+#include "join.cuh"
 
 namespace see::k {
 
@@ -53,12 +51,6 @@ __device__ __forceinline__ float BlockMean(float sum, float (*slots)[kThreads / 
   wide = set[0];
   for (uint32_t w = 1; w < kThreads / 32; ++w) wide += set[w];
   return static_cast<float>(wide / static_cast<double>(cols));
-}
-
-// The variance, from the average square of deviations whose own average is `off`.  (What is not finite stays.)
-__device__ __forceinline__ float Variance(float square, float off) {
-  const float less = square - off * off;
-  return !isfinite(off * off) ? square : less < 0.0f ? 0.0f : less;
 }
 
 struct Stats {
@@ -231,40 +223,41 @@ JoinFoldKernel(const __grid_constant__ JoinArgs a, uint32_t blocks, int rms) {
   if (a.w.gate) a.grads.gate[col] = !post ? sums[2] : a.w.post_gamma[col] * sums[2] + (rms ? 0.0f : a.w.post_beta[col] * sums[3]);
 }
 
-template <typename F>
-cudaError_t AllowShared(F* kernel, size_t bytes) {
-  return bytes <= 40 * 1024 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-}
-
+// Rows of more columns than the ring kernels take.
 template <typename XT, typename YT, bool kRms>
-cudaError_t Pick(const JoinArgs& a, bool backward, cudaStream_t s, int* launches) {
+cudaError_t Pick(const JoinArgs& a, bool backward, cudaStream_t s, uint32_t* grid) {
   const size_t smem = a.cols * sizeof(float);
-  ++*launches;
   if (!backward) {
-    auto* kernel = JoinFwdKernel<XT, YT, kRms>;
-    if (cudaError_t e = AllowShared(kernel, smem); e != cudaSuccess) return e;
+    constexpr auto* kernel = JoinFwdKernel<XT, YT, kRms>;
+    if (cudaError_t e = AllowShared<kernel>(smem); e != cudaSuccess) return e;
     return Next(kernel, static_cast<unsigned>(a.rows), kThreads, smem, s)(a);
   }
-  auto* kernel = JoinBwdKernel<XT, YT, kRms>;
-  if (cudaError_t e = AllowShared(kernel, smem); e != cudaSuccess) return e;
-  const uint32_t grid = static_cast<uint32_t>(NormPartialRows(a.rows));
-  if (cudaError_t e = Next(kernel, grid, kThreads, smem, s)(a); e != cudaSuccess) return e;
-  ++*launches;
-  return Next(JoinFoldKernel, (a.cols + 31) / 32, 1024, 0, s)(a, grid, kRms ? 1 : 0);
+  constexpr auto* kernel = JoinBwdKernel<XT, YT, kRms>;
+  if (cudaError_t e = AllowShared<kernel>(smem); e != cudaSuccess) return e;
+  *grid = static_cast<uint32_t>(NormPartialRows(a.rows));
+  return Next(kernel, *grid, kThreads, smem, s)(a);
 }
 template <typename XT, typename YT>
-cudaError_t Pick(const JoinArgs& a, bool backward, cudaStream_t s, int* launches) {
-  return a.rms ? Pick<XT, YT, true>(a, backward, s, launches) : Pick<XT, YT, false>(a, backward, s, launches);
+cudaError_t Pick(const JoinArgs& a, bool backward, cudaStream_t s, uint32_t* grid) {
+  return a.rms ? Pick<XT, YT, true>(a, backward, s, grid) : Pick<XT, YT, false>(a, backward, s, grid);
+}
+cudaError_t Pick(const JoinArgs& a, bool backward, uint32_t sms, cudaStream_t s, uint32_t* grid) {
+  if (a.cols <= kJoinRingCols) return backward ? JoinBackwardRing(a, sms, s, grid) : JoinForwardRing(a, sms, s);
+  if (a.x_type == SEE_BF16) return Pick<Bf16, Bf16>(a, backward, s, grid);
+  if (a.x_type == SEE_F16) return Pick<F16, F16>(a, backward, s, grid);
+  if (a.y_type == SEE_BF16) return Pick<float, Bf16>(a, backward, s, grid);
+  return a.y_type == SEE_F16 ? Pick<float, F16>(a, backward, s, grid) : Pick<float, float>(a, backward, s, grid);
 }
 
 }  // namespace
 
 cudaError_t Join(const JoinArgs& a, bool backward, uint32_t sms, cudaStream_t s, int* launches) {
-  if (a.x_type == SEE_BF16) return Pick<Bf16, Bf16>(a, backward, s, launches);
-  if (a.x_type == SEE_F16) return Pick<F16, F16>(a, backward, s, launches);
-  if (a.y_type == SEE_BF16) return Pick<float, Bf16>(a, backward, s, launches);
-  if (a.y_type == SEE_F16) return Pick<float, F16>(a, backward, s, launches);
-  return Pick<float, float>(a, backward, s, launches);
+  uint32_t grid = 0;
+  if (cudaError_t e = Pick(a, backward, sms, s, &grid); e != cudaSuccess) return e;
+  ++*launches;
+  if (!backward) return cudaSuccess;
+  ++*launches;
+  return Next(JoinFoldKernel, (a.cols + 31) / 32, 1024, 0, s)(a, grid, a.rms ? 1 : 0);
 }
 
 }  // namespace see::k
