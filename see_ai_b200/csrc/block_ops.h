@@ -63,7 +63,7 @@ struct JoinArgs {
 cudaError_t Join(const JoinArgs& a, bool backward, uint32_t sms, cudaStream_t s, int* launches);
 
 // ---- losses over rows of logits (k_logit_loss.cu) ------------------------------
-constexpr uint32_t kLogitPartials = 1024;     // most thread blocks' sums
+constexpr uint32_t kLogitPartials = 4096;     // most groups' sums
 struct LogitArgs {
   const void* logits;
   void* dlogits;                              // or null
@@ -71,6 +71,8 @@ struct LogitArgs {
   uint64_t rows, stride;
   uint32_t classes;
   float scale, k;                             // k: scale / ln 2
+  double inv_k;
+  DeviceStatus* status;
 };
 struct PolicyArgs {
   const float *old_logp, *ref_logp, *advantages, *weights, *loss_grad;
@@ -80,7 +82,8 @@ struct PolicyArgs {
 struct PreferenceArgs {
   const int32_t* starts;
   const float *ref_logp, *loss_grad;
-  float *loss, *margins, *sequence_logp, *slopes;
+  float *loss, *margins, *sequence_logp;
+  double* losses;                             // [pairs]
   uint32_t pairs;
   int kind, average;
   float beta, smoothing, margin;

@@ -28,14 +28,15 @@ Operand Logits(const char* name, const Shape& s, const void* p, bool written) {
 }
 
 template <typename Shape>
-k::LogitArgs ArgsOf(const Shape& s, const void* logits, const int32_t* labels, void* dlogits) {
-  return {logits, s.rows ? dlogits : nullptr, labels, s.rows, s.stride, static_cast<uint32_t>(s.classes), s.logit_scale,
-          static_cast<float>(kLog2E * static_cast<double>(s.logit_scale))};
+k::LogitArgs ArgsOf(const Shape& s, const void* logits, const int32_t* labels, void* dlogits, k::DeviceStatus* status) {
+  const float k = static_cast<float>(kLog2E * static_cast<double>(s.logit_scale));
+  return {logits, s.rows ? dlogits : nullptr, labels, s.rows, s.stride, static_cast<uint32_t>(s.classes), s.logit_scale, k, 1.0 / static_cast<double>(k),
+          status};
 }
 
 }  // namespace
 
-uint64_t PreferenceWorkspace(uint64_t rows, uint64_t pairs) {   // what is kept of a row, and a slope to each sequence
+uint64_t PreferenceWorkspace(uint64_t rows, uint64_t pairs) {   // what is kept of a row, and each pair's loss
   return rows > 0x7FFFFFFFull || pairs == 0 || pairs > (1u << 24) ? 0 : rows * 16 + (pairs * 8 + 15) / 16 * 16;
 }
 uint64_t PolicyWorkspace(uint64_t rows) { return rows > 0x7FFFFFFFull ? 0 : k::kLogitPartials * 3 * sizeof(double); }
@@ -77,12 +78,12 @@ Status CudaBackend::PreferenceLoss(const see_preference_shape& given, const void
       !r)
     return r;
   float4* kept = static_cast<float4*>(workspace);
-  const k::PreferenceArgs p = {starts,       ref_logp, loss_grad,     loss,        margins, sequence_logp, reinterpret_cast<float*>(kept + s.rows),
+  const k::PreferenceArgs p = {starts, ref_logp, loss_grad, loss, margins, sequence_logp, reinterpret_cast<double*>(kept + s.rows),
                                static_cast<uint32_t>(s.pairs), s.kind, s.average, s.beta, s.smoothing, s.margin};
   OnDevice on(device_);
   if (!on.ok()) return Check(cudaGetLastError(), "preference loss: device");
   int launches = 0;
-  const cudaError_t e = k::PreferenceLoss(ArgsOf(s, logits, labels, dlogits), s.type, p, kept, sms_, stream_, &launches);
+  const cudaError_t e = k::PreferenceLoss(ArgsOf(s, logits, labels, dlogits, d_status_), s.type, p, kept, sms_, stream_, &launches);
   counters_.kernel_launches += static_cast<uint64_t>(launches);
   return Check(e, "preference loss");
 }
@@ -127,7 +128,7 @@ Status CudaBackend::PolicyLoss(const see_policy_shape& given, const void* logits
   if (!on.ok()) return Check(cudaGetLastError(), "policy loss: device");
   int launches = 0;
   const cudaError_t e =
-      k::PolicyLoss(ArgsOf(s, logits, labels, dlogits), s.type, p, static_cast<double*>(workspace), sms_, stream_, &launches);
+      k::PolicyLoss(ArgsOf(s, logits, labels, dlogits, d_status_), s.type, p, static_cast<double*>(workspace), sms_, stream_, &launches);
   counters_.kernel_launches += static_cast<uint64_t>(launches);
   return Check(e, "policy loss");
 }
