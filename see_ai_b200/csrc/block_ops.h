@@ -63,7 +63,7 @@ struct JoinArgs {
 cudaError_t Join(const JoinArgs& a, bool backward, uint32_t sms, cudaStream_t s, int* launches);
 
 // ---- losses over rows of logits (k_logit_loss.cu) ------------------------------
-constexpr uint32_t kLogitPartials = 4096;     // most groups' sums
+constexpr uint32_t kPolicyPartials = 592;     // most thread blocks' sums
 struct LogitArgs {
   const void* logits;
   void* dlogits;                              // or null
@@ -88,8 +88,8 @@ struct PreferenceArgs {
   int kind, average;
   float beta, smoothing, margin;
 };
-// partials [kLogitPartials][3]; kept [rows].
-cudaError_t PolicyLoss(const LogitArgs& a, int type, const PolicyArgs& p, double* partials, uint32_t sms, cudaStream_t s, int* launches);
+// kept [rows], and behind it, of the policy loss, [kPolicyPartials][3] doubles and 16 bytes.
+cudaError_t PolicyLoss(const LogitArgs& a, int type, const PolicyArgs& p, float4* kept, uint32_t sms, cudaStream_t s, int* launches);
 cudaError_t PreferenceLoss(const LogitArgs& a, int type, const PreferenceArgs& p, float4* kept, uint32_t sms, cudaStream_t s, int* launches);
 
 // ---- all gradients' norm (k_grad_norm.cu) ------------------------------------

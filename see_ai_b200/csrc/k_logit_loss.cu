@@ -40,6 +40,14 @@ __device__ __forceinline__ void Elements(uint4 r, float* v) {
   }
 }
 
+// -inf, and 16 bytes of it.
+template <typename T> __device__ __forceinline__ constexpr uint32_t NoElement() { return sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, Bf16> ? 0xFF80u : 0xFC00u; }
+template <typename T>
+__device__ __forceinline__ uint4 Nothing() {
+  const uint32_t w = sizeof(T) == 4 ? NoElement<T>() : NoElement<T>() * 0x10001u;
+  return make_uint4(w, w, w, w);
+}
+
 // A row of logits and of dlogits.
 template <typename T>
 struct Row {
@@ -63,11 +71,10 @@ struct Row {
     if (Whole(at)) return *reinterpret_cast<const uint4*>(z + at);
     using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
     const Bits* bits = reinterpret_cast<const Bits*>(z);
-    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, Bf16> ? 0xFF80u : 0xFC00u;
     uint32_t r[4] = {};
 #pragma unroll
     for (int j = 0; j < kPerUnit<T>; ++j)
-      r[j * sizeof(T) / 4] |= (at + j >= 0 && at + j < static_cast<int32_t>(classes) ? static_cast<uint32_t>(bits[at + j]) : kNone) << (j * sizeof(T) % 4 * 8);
+      r[j * sizeof(T) / 4] |= (at + j >= 0 && at + j < static_cast<int32_t>(classes) ? static_cast<uint32_t>(bits[at + j]) : NoElement<T>()) << (j * sizeof(T) % 4 * 8);
     return make_uint4(r[0], r[1], r[2], r[3]);
   }
   __device__ __forceinline__ void Load(uint32_t unit, float* v) const { Elements<T>(Raw(unit), v); }
@@ -209,21 +216,41 @@ __device__ __forceinline__ PolicyRow PolicyRowOf(const PolicyArgs& p, uint64_t r
   return {p.old_logp[row], p.ref_logp ? p.ref_logp[row] : 0.0f, p.advantages[row], p.weights ? p.weights[row] : 1.0f};
 }
 struct PolicyTerms {
-  float slope, loss, kl, clipped;   // slope: of the weighted loss by logp
+  float slope, loss, kl;   // slope: of the loss by logp; none of them weighted
+  bool clipped;
 };
-__device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, const PolicyRow& row, double logp) {
-  const float a = row.advantage, w = row.weight;
-  const float r = expf(static_cast<float>(logp - static_cast<double>(row.old)));
-  const float cut = r < 1.0f - p.clip_low ? 1.0f - p.clip_low : r > 1.0f + p.clip_high ? 1.0f + p.clip_high : r;
-  const bool clipped = r * a > cut * a;
-  float loss = clipped ? -(cut * a) : -(r * a), slope = clipped ? 0.0f : -(r * a), kl = 0.0f;
+// off, above: logp less old_logp, ref_logp less logp.
+__device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, float advantage, float off, float above) {
+  const float a = advantage, r = expf(off), cut = r < 1.0f - p.clip_low ? 1.0f - p.clip_low : r > 1.0f + p.clip_high ? 1.0f + p.clip_high : r;
+  PolicyTerms t;
+  t.clipped = r * a > cut * a;
+  t.loss = t.clipped ? -(cut * a) : -(r * a);
+  t.slope = t.clipped ? 0.0f : -(r * a);
+  t.kl = 0.0f;
   if (p.ref_logp) {
-    const float x = static_cast<float>(static_cast<double>(row.ref) - logp), grown = expm1f(x);
-    kl = grown - x;
-    loss += p.kl_coef * kl;
-    slope -= p.kl_coef * grown;
+    const float grown = expm1f(above);
+    t.kl = grown - above;
+    t.loss += p.kl_coef * t.kl;
+    t.slope -= p.kl_coef * grown;
   }
-  return {w * slope, w * loss, w * kl, clipped ? w : 0.0f};
+  return t;
+}
+__device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, const PolicyRow& row, double logp) {
+  return PolicyOf(p, row.advantage, static_cast<float>(logp - static_cast<double>(row.old)), static_cast<float>(static_cast<double>(row.ref) - logp));
+}
+// The loss's weighted derivative by a row's logp.  Of 16-bit logits it goes into dlogits of 8 or 11 bits: logp in f32, a millionth off, is
+// enough, and takes each warp 20 instructions instead of 100; of f32 logits the double one.
+template <typename T>
+__device__ __forceinline__ float SlopeOf(const LogitArgs& a, const PolicyArgs& p, const PolicyRow& row, const RowSums& q) {
+  if constexpr (sizeof(T) == 4) {
+    return row.weight * PolicyOf(p, row, LogpOf(a, q)).slope;
+  } else {
+    constexpr float kLn2 = 0.6931471805599453f;
+    float log2s;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(log2s) : "f"(q.s));
+    const float logp = kLn2 * (fmaf(q.z_label, a.k, -q.mk) - log2s);
+    return row.weight * PolicyOf(p, row.advantage, logp - row.old, row.ref - logp).slope;
+  }
 }
 
 __device__ __forceinline__ double WarpSum(double v) {
@@ -231,16 +258,73 @@ __device__ __forceinline__ double WarpSum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
+__device__ __forceinline__ float WarpMax(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(r) : "f"(v));
+  return r;
+}
 
-// A warp to each of the three sums.
-__global__ void __launch_bounds__(96)
-PolicyFoldKernel(const double* __restrict__ partials, uint32_t count, float* __restrict__ loss) {
+constexpr uint32_t kFinishThreads = 256;
+
+// From what is kept of the rows: logp and the loss's three sums, a block's rows in its partials; the block that comes last (*arrived, which the rows'
+// kernel has set to 0) adds them up, in the blocks' order.
+__global__ void __launch_bounds__(kFinishThreads)
+PolicyFinishKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const float4* __restrict__ kept,
+                   double* __restrict__ partials, uint32_t* __restrict__ arrived) {
   AwaitPrevious();
-  const uint32_t which = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  double sum = 0.0;
-  for (uint32_t i = lane; i < count; i += 32) sum += partials[i * 3 + which];
-  sum = WarpSum(sum);
-  if (lane == 0) loss[which] = static_cast<float>(sum);
+  __shared__ double meet[kFinishThreads / 32][3];
+  __shared__ bool last;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double sums[3] = {};
+  for (uint64_t r = static_cast<uint64_t>(blockIdx.x) * kFinishThreads + threadIdx.x; r < a.rows; r += static_cast<uint64_t>(gridDim.x) * kFinishThreads) {
+    double logp = 0.0;
+    const float4 q = kept[r];   // (all at once; of a row that does not count, whatever is there)
+    const PolicyRow row = PolicyRowOf(p, r);
+    if (Counts(a.labels[r], a.classes)) {
+      logp = LogpOf(a, {q.x, q.y, q.z, q.w});
+      const PolicyTerms t = PolicyOf(p, row, logp);
+      sums[0] += static_cast<double>(row.weight * t.loss);
+      sums[1] += static_cast<double>(row.weight * t.kl);
+      sums[2] += t.clipped ? static_cast<double>(row.weight) : 0.0;
+    }
+    p.logp[r] = static_cast<float>(logp);
+  }
+  auto block_sum = [&] {   // in warp 0's lanes, the three sums
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      sums[i] = WarpSum(sums[i]);
+      if (lane == 0) meet[warp][i] = sums[i];
+    }
+    __syncthreads();
+    if (warp == 0)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) sums[i] = WarpSum(lane < kFinishThreads / 32 ? meet[lane][i] : 0.0);
+  };
+  block_sum();
+  if (gridDim.x == 1) {
+    if (threadIdx.x == 0)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) p.loss[i] = static_cast<float>(sums[i]);
+    return;
+  }
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) partials[blockIdx.x * 3 + i] = sums[i];
+    __threadfence();
+    last = atomicAdd(arrived, 1u) == gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    sums[i] = 0.0;
+    for (uint32_t b = threadIdx.x; b < gridDim.x; b += kFinishThreads) sums[i] += __ldcg(&partials[b * 3 + i]);
+  }
+  block_sum();
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) p.loss[i] = static_cast<float>(sums[i]);
 }
 
 // Rows of a preference loss that are a sequence's.
@@ -260,12 +344,6 @@ __device__ __forceinline__ void Pairs(const uint4& r, f32x2 (&v)[kPairs<T>]) {
   Elements<T>(r, f);
 #pragma unroll
   for (int j = 0; j < kPairs<T>; ++j) v[j] = PackF2(f[2 * j], f[2 * j + 1]);
-}
-// -inf in every element.
-template <typename T>
-__device__ __forceinline__ uint4 Nothing() {
-  const uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, Bf16> ? 0xFF80FF80u : 0xFC00FC00u;
-  return make_uint4(w, w, w, w);
 }
 __device__ __forceinline__ uint32_t Max2(uint32_t a, uint32_t b, Bf16) {
   uint32_t r;
@@ -296,14 +374,36 @@ __device__ __forceinline__ float Largest(const uint4 (&raw)[NU]) {
   }
 }
 
-// kC > 1: the blocks of a cluster share each row.
+// What a block shows the others of its cluster, and a barrier that counts them; two of each, used in turn.
+struct Exchange {
+  float2 parts[2][8];   // k M and the sum, of a block
+  uint64_t bars[2];
+};
+__device__ __forceinline__ bool AwaitCluster(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = umma_dev::SmemAddr(bar);
+  for (uint32_t it = 0; it < umma_dev::kWaitLimit; ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
+// A group's row: `blocks` blocks of a cluster share it, `part` units each.
 template <typename T, int NU, bool kPolicy, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 1)
 LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const Sequences seq, float4* __restrict__ kept,
-                double* __restrict__ partials, uint32_t threads, uint32_t slots, uint32_t blocks, uint32_t part) {
+                uint32_t* __restrict__ arrived, uint32_t threads, uint32_t slots, uint32_t blocks, uint32_t part) {
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
   extern __shared__ __align__(128) uint8_t dyn[];
-  __shared__ float2 sums[2][kThreads / 32];        // k M and the sum, of a warp
-  __shared__ float2 parts[2][8];                   // of a block
+  __shared__ float2 sums[2][kThreads / 32];                // k M and the sum, of a warp
+  __shared__ Exchange exchange[2];                         // of a group
   const uint32_t groups = blockDim.x / threads, group = threadIdx.x / threads, t = threadIdx.x - group * threads, lane = threadIdx.x & 31;
   const uint32_t rank = kCluster ? blockIdx.x % blocks : 0, cluster = kCluster ? blockIdx.x / blocks : blockIdx.x;
   const uint32_t clusters = kCluster ? gridDim.x / blocks : gridDim.x;
@@ -313,6 +413,8 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
   const uint64_t first = static_cast<uint64_t>(cluster) * groups + group, step = static_cast<uint64_t>(clusters) * groups;
   if (t == 0) {
     for (uint32_t i = 0; i < slots; ++i) umma_dev::MbarInit(&bars[i], 1);
+    if constexpr (kCluster)
+      for (uint32_t i = 0; i < 2; ++i) umma_dev::MbarInit(&exchange[group].bars[i], blocks);
     umma_dev::MbarInitFence();
   }
   AwaitPrevious();
@@ -343,6 +445,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     if (!counts(r, label)) return;
     const Share w = share_of(Row<T>(a, r));
     if (!w.bulk) return;
+    umma_dev::FenceProxyAsync();   // (elements were written there)
     umma_dev::MbarExpectTx(&bars[slot], w.count * 16);
     umma_dev::BulkLoad(ring + static_cast<size_t>(slot) * slot_bytes, reinterpret_cast<const void*>(w.from), w.count * 16, &bars[slot]);
   };
@@ -351,21 +454,38 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     int32_t labels[9];
 #pragma unroll
     for (uint32_t i = 0; i < 9; ++i) labels[i] = i <= slots && first + i * step < a.rows ? a.labels[first + i * step] : -1;
+#pragma unroll 1
+    for (uint32_t i = 0; i < slots && first + i * step < a.rows; ++i) {
+      fill(first + i * step, labels[0], i);
 #pragma unroll
-    for (uint32_t i = 0; i < 9; ++i) {
-      if (i < slots && first + i * step < a.rows) fill(first + i * step, labels[i], i);
-      if (i == slots) fill_label = labels[i];
+      for (uint32_t j = 0; j < 8; ++j) labels[j] = labels[j + 1];
     }
+    fill_label = labels[0];
   }
   const float grad = (kPolicy && p.loss_grad ? *p.loss_grad : 1.0f) * a.scale;
+  __syncwarp();
   if constexpr (kCluster) umma_dev::ClusterSync();   // (every block of it has begun: its shared memory may be written)
-  else GroupBarrier(threads, group);                  // the barriers are there
-  double total[3] = {};
-  uint32_t turn = 0, slot = 0, parities = 0;   // a bit for each slot, of the copies that went through it
-  int32_t next_label = first < a.rows ? a.labels[first] : -1;
+  else GroupBarrier(threads, group);                 // the barriers are there
+  if (kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
+  uint32_t turn = 0, slot = 0, parities = 0, exchanged = 0;   // a bit for each slot, of the copies that went through it; rows exchanged
+  // What a row brings besides its logits is asked for while the one before it is at work.
+  int32_t label = -1, next_label = -1;
+  T next_z_label = {};   // (as it is read: a conversion would wait for it)
+  PolicyRow next_brings = {};
+  auto ask = [&](uint64_t r) {   // (next_label is there)
+    if (r >= a.rows || !counts(r, next_label)) return;
+    next_z_label = static_cast<const T*>(a.logits)[r * a.stride + next_label];
+    if (kPolicy) next_brings = PolicyRowOf(p, r);
+  };
+  if (first < a.rows) next_label = a.labels[first];
+  ask(first);
+  int32_t label_behind = first + step < a.rows ? a.labels[first + step] : -1;
   for (uint64_t r = first; r < a.rows; r += step) {
-    const int32_t label = next_label;
-    if (r + step < a.rows) next_label = a.labels[r + step];
+    label = next_label;
+    next_label = label_behind;
+    label_behind = r + 2 * step < a.rows ? a.labels[r + 2 * step] : -1;
+    const T raw_label = next_z_label;
+    [[maybe_unused]] const PolicyRow brings = next_brings;
     const Row<T> row(a, r);
     const Share w = share_of(row);
     const uint32_t now = slot;
@@ -380,184 +500,177 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
       const float none[kPerUnit<T>] = {};
       for (uint32_t u = t; u < w.count; u += threads) row.Store(w.first + u, none);
     };
+    ask(r + step);
     if (!counts(r, label)) {
-      if (kPolicy) {
-        if (t == 0 && rank == 0) p.logp[r] = 0.0f;
-        if (a.dlogits) zeros();
-      }
+      if (kPolicy && a.dlogits) zeros();
       refill();
       continue;
     }
-    const float z_label = ToF32(row.z[label]);
-    PolicyRow brings = {};
-    if (kPolicy) brings = PolicyRowOf(p, r);
-    uint4 raw[NU];
+    // Its part in the slot, each thread's own units; -inf in place of the label and of what sticks out of the row.
+    uint4* mine = reinterpret_cast<uint4*>(ring + static_cast<size_t>(now) * slot_bytes);
+    const uint32_t label_unit = (static_cast<uint32_t>(label) + row.skip) / kPerUnit<T> - w.first;   // (of another block: beyond count)
     if (w.bulk) {
       AwaitRow(&bars[now], parities >> now & 1u, a.status);
       parities ^= 1u << now;
-      const uint4* from = reinterpret_cast<const uint4*>(ring + static_cast<size_t>(now) * slot_bytes);
-#pragma unroll
-      for (int i = 0; i < NU; ++i) raw[i] = t + i * threads < w.count ? from[t + i * threads] : Nothing<T>();
+      Bits* bits = reinterpret_cast<Bits*>(mine);
+      if (t == 0 && w.first == 0)
+        for (uint32_t j = 0; j < row.skip; ++j) bits[j] = NoElement<T>();
+      if (w.first + w.count == row.units && t == (w.count - 1) % threads)
+        for (uint32_t j = row.skip + a.classes - w.first * kPerUnit<T>; j < w.count * kPerUnit<T>; ++j) bits[j] = NoElement<T>();
+    } else {
+      for (uint32_t u = t; u < w.count; u += threads) mine[u] = row.Raw(w.first + u);
     }
-    // What sticks out of the row, and the rows at the matrix's ends.
+    if (label_unit < w.count && t == label_unit % threads)
+      reinterpret_cast<Bits*>(mine)[static_cast<uint32_t>(label) + row.skip - w.first * kPerUnit<T>] = NoElement<T>();
+    asm volatile("" ::: "memory");   // (as elements, then as units)
+    uint4 raw[NU];
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const uint32_t u = w.first + t + i * threads;
-      if (!w.bulk || u == 0 || u == row.units - 1) raw[i] = t + i * threads < w.count ? row.Raw(u) : Nothing<T>();
-    }
+    for (int i = 0; i < NU; ++i) raw[i] = t + i * threads < w.count ? mine[t + i * threads] : Nothing<T>();
     float mk = __fmul_rn(Largest<T, NU>(raw), a.k);   // -inf: nothing here
     const f32x2 k2 = Splat2(a.k), away = Splat2(mk == MinusInf() ? 0.0f : -mk);
-    const uint32_t label_unit = (static_cast<uint32_t>(label) + row.skip) / kPerUnit<T>, label_at = (static_cast<uint32_t>(label) + row.skip) % kPerUnit<T>;
-    f32x2 e[NU][kPairs<T>], sum2 = 0;
+    f32x2 e[NU][kPairs<T>], sum2[kPairs<T>] = {};
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      f32x2 v[kPairs<T>];
-      Pairs<T>(raw[i], v);
+      Pairs<T>(raw[i], e[i]);
 #pragma unroll
       for (int j = 0; j < kPairs<T>; ++j) {
         float lo, hi;
-        UnpackF2(Fma2(v[j], k2, away), &lo, &hi);
+        UnpackF2(Fma2(e[i][j], k2, away), &lo, &hi);
         e[i][j] = PackF2(Ex2Approx(lo), Ex2Approx(hi));
+        sum2[j] = AddF2(sum2[j], e[i][j]);
       }
-      if (w.first + t + i * threads == label_unit) {   // the label is not among the others
-#pragma unroll
-        for (int j = 0; j < kPairs<T>; ++j) {
-          float lo, hi;
-          UnpackF2(e[i][j], &lo, &hi);
-          e[i][j] = PackF2(label_at == 2 * j ? 0.0f : lo, label_at == 2 * j + 1 ? 0.0f : hi);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kPairs<T>; ++j) sum2 = AddF2(sum2, e[i][j]);
     }
+#pragma unroll
+    for (int j = 1; j < kPairs<T>; ++j) sum2[0] = AddF2(sum2[0], sum2[j]);
     float lo, sum;
-    UnpackF2(sum2, &lo, &sum);
+    UnpackF2(sum2[0], &lo, &sum);
     sum += lo;
     // Warps, groups, blocks: the largest k M, and sums relative to it.  (A part without numbers has factor 0; NaN stays NaN.)
     auto factor = [](float own, float all) { return own == MinusInf() ? 0.0f : Ex2Approx(own - all); };
     const float own = mk;
     auto join = [&](uint32_t most) {
-      float top = mk;
-      for (uint32_t o = most; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      const float top = WarpMax(mk);   // (beyond `most` the lanes repeat themselves)
       sum *= factor(mk, top);
       mk = top;
-      for (uint32_t o = most; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+#pragma unroll
+      for (uint32_t o = 16; o > 0; o >>= 1)
+        if (o <= most) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     };
     join(16);
     if (threads > 32) {
       float2* set = sums[turn] + group * (threads / 32);
       if (lane == 0) set[t >> 5] = make_float2(mk, sum);
       GroupBarrier(threads, group);
-      const float2 mine = lane < threads / 32 ? set[lane] : make_float2(MinusInf(), 0.0f);
-      mk = mine.x;
-      sum = mine.y;
-      join(16);
+      const float2 warp_part = (lane & 15) < threads / 32 ? set[lane & 15] : make_float2(MinusInf(), 0.0f);
+      mk = warp_part.x;
+      sum = warp_part.y;
+      join(8);
     } else {
       __syncwarp();
     }
-    refill();   // (the slot is read)
     if constexpr (kCluster) {
+      Exchange& x = exchange[group];
       if (t < blocks) {
-        const uint32_t to = umma_dev::MapToCta(umma_dev::SmemAddr(&parts[turn][rank]), t);
+        const uint32_t to = umma_dev::MapToCta(umma_dev::SmemAddr(&x.parts[turn][rank]), t);
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(mk), "f"(sum) : "memory");
+        umma_dev::MbarArriveCluster(umma_dev::MapToCta(umma_dev::SmemAddr(&x.bars[turn]), t));
       }
+      refill();   // (the slot is read)
       __syncwarp();
-      umma_dev::ClusterSync();
-      const float2 mine = lane < blocks ? parts[turn][lane] : make_float2(MinusInf(), 0.0f);
-      mk = mine.x;
-      sum = mine.y;
+      if (!AwaitCluster(&x.bars[turn], exchanged >> 1 & 1u)) {
+        a.status->wait_timeout = 1;
+        umma_dev::DrainDelay();
+      }
+      ++exchanged;
+      const float2 block_part = (lane & 7) < blocks ? x.parts[turn][lane & 7] : make_float2(MinusInf(), 0.0f);
+      mk = block_part.x;
+      sum = block_part.y;
       join(4);
-      mk = __shfl_sync(0xFFFFFFFFu, mk, 0);
-      sum = __shfl_sync(0xFFFFFFFFu, sum, 0);
+    } else {
+      refill();
     }
     turn ^= 1;
-    RowSums q = {z_label, mk == MinusInf() ? 0.0f : mk, sum, 0.0f};
+    // The label joins the maximum, so that its term is 1 at most.
+    const float z_label = ToF32(raw_label);
+    const float mk_label = __fmul_rn(z_label, a.k), all = fmaxf(mk, mk_label);
+    RowSums q = {z_label, all == MinusInf() ? 0.0f : all, sum * factor(mk, all), 0.0f};
     q.s = q.others + LabelTerm(a, z_label, q.mk);
-    if constexpr (!kPolicy) {
-      if (t == 0 && rank == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
-    } else {
-      const double logp = LogpOf(a, q);
-      const PolicyTerms terms = PolicyOf(p, brings, logp);
-      if (t == 0 && rank == 0) {
-        p.logp[r] = static_cast<float>(logp);
-        total[0] += terms.loss;
-        total[1] += terms.kl;
-        total[2] += terms.clipped;
-      }
+    if (t == 0 && rank == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
+    if constexpr (kPolicy) {
       if (!a.dlogits) continue;
-      const float slope = terms.slope * grad;
+      const float slope = SlopeOf<T>(a, p, brings, q) * grad;
       if (slope == 0.0f) {
         zeros();
         continue;
       }
-      const f32x2 by = Splat2(factor(own, q.mk) * (-slope / q.s));
+      const float each = -slope / q.s;
+      const f32x2 by = Splat2(factor(own, q.mk) * each);
+      // Units that lie wholly in the row; then, their owners, the two that may not.
+      const uint32_t whole_first = w.first == 0 && row.skip != 0 ? 1 : 0;
+      const uint32_t whole_end = min(w.count, (row.skip + a.classes) / kPerUnit<T> - w.first);   // (without units: 0)
+      const uint32_t whole = row.alike && whole_end > whole_first ? whole_end - whole_first : 0;
+      T* to = row.d - row.skip + static_cast<size_t>(w.first) * kPerUnit<T>;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         const uint32_t u = t + i * threads;
-        if (u >= w.count) continue;
-        float v[kPerUnit<T>];
+        if (u - whole_first < whole) {
+          float v[kPerUnit<T>];
 #pragma unroll
-        for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(e[i][j], by), &v[2 * j], &v[2 * j + 1]);
-        row.Store(w.first + u, v);
-        if (w.first + u == label_unit) row.d[label] = FromF32<T>(slope * (q.others / q.s));
+          for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(e[i][j], by), &v[2 * j], &v[2 * j + 1]);
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to + static_cast<size_t>(u) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+          else Store8<T>(to + static_cast<size_t>(u) * 8, v);
+        }
       }
+      if (whole_first || whole + whole_first != w.count) {   // (from memory: of a matrix in place, these elements are still logits)
+        for (uint32_t u = t; u < w.count; u += threads) {
+          if (u - whole_first < whole) continue;
+          float v[kPerUnit<T>];
+          row.Load(w.first + u, v);
+#pragma unroll
+          for (int j = 0; j < kPerUnit<T>; ++j) v[j] = each * Ex2Approx(fmaf(v[j], a.k, -q.mk));
+          row.Store(w.first + u, v);
+        }
+      }
+      if (label_unit < w.count && t == label_unit % threads) row.d[label] = FromF32<T>(slope * (q.others / q.s));
     }
   }
-  if (kPolicy && t == 0 && rank == 0)
-#pragma unroll
-    for (int i = 0; i < 3; ++i) partials[(static_cast<size_t>(cluster) * groups + group) * 3 + i] = total[i];
 }
 
 // Rows that no cluster holds in its registers, read twice: a block to a row.
 template <typename T, bool kPolicy>
 __global__ void __launch_bounds__(kThreads)
 LogitWideKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const Sequences seq, float4* __restrict__ kept,
-                double* __restrict__ partials) {
+                uint32_t* __restrict__ arrived) {
   AwaitPrevious();
   __shared__ Part slots[2][kThreads / 32];
+  if (kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
   const float grad = (kPolicy && p.loss_grad ? *p.loss_grad : 1.0f) * a.scale;
-  double sums[3] = {};
   uint32_t turn = 0;
   for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const Row<T> row(a, r);
     const int32_t label = a.labels[r];
     if (!kPolicy && (static_cast<int64_t>(r) < seq.starts[0] || static_cast<int64_t>(r) >= seq.starts[seq.count])) continue;
     if (!Counts(label, a.classes)) {
-      if (!kPolicy) continue;
-      if (threadIdx.x == 0) p.logp[r] = 0.0f;
-      if (a.dlogits) Zeros(row);
+      if (kPolicy && a.dlogits) Zeros(row);
       continue;
     }
     const RowSums q = SumsOf(row, label, a.k, slots[turn]);
     turn ^= 1;
-    if (!kPolicy) {
-      if (threadIdx.x == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
-      continue;
-    }
-    const double logp = LogpOf(a, q);
-    const PolicyTerms t = PolicyOf(p, PolicyRowOf(p, r), logp);
-    if (threadIdx.x == 0) {
-      p.logp[r] = static_cast<float>(logp);
-      sums[0] += t.loss;
-      sums[1] += t.kl;
-      sums[2] += t.clipped;
-    }
-    if (!a.dlogits) continue;
-    const float slope = t.slope * grad;
+    if (threadIdx.x == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
+    if (!kPolicy || !a.dlogits) continue;
+    const float slope = SlopeOf<T>(a, p, PolicyRowOf(p, r), q) * grad;
     if (slope == 0.0f) Zeros(row);
     else Gradient(row, label, a.k, q.mk, q.others, q.s, slope);
   }
-  if (kPolicy && threadIdx.x == 0)
-    for (int i = 0; i < 3; ++i) partials[blockIdx.x * 3 + i] = sums[i];
 }
 
 // ---- the preference loss ----------------------------------------------------------------------------------
-// log(1 + e^x), exact in its tails.
-__device__ __forceinline__ double Softplus(double x) { return x > 0.0 ? x + log1p(exp(-x)) : log1p(exp(x)); }
+// log(1 + e^x), in its tails too.
+__device__ __forceinline__ double Softplus(double x) { return (x > 0.0 ? x : 0.0) + log1p(exp(-fabs(x))); }
 
-constexpr uint32_t kPairThreads = 256;
+constexpr uint32_t kPairThreads = 512;
 
-// A pair to a block: the first four warps sum the chosen rows, the others the rejected ones.  Then each row's kept.x becomes the
+// A pair to a block: the first eight warps sum the chosen rows, the others the rejected ones.  Then each row's kept.x becomes the
 // loss's derivative by its logp, logit_scale and loss_grad included, 0 where it does not count.  losses [pairs]: added up by PreferenceFoldKernel.
 __global__ void __launch_bounds__(kPairThreads)
 PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PreferenceArgs p, float4* __restrict__ kept) {
@@ -588,35 +701,33 @@ PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant
     double ratio[2], per_row[2];
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
-      const uint32_t w = i * (kPairThreads / 64);
-      sum = (sums[w][0] + sums[w + 1][0]) + (sums[w + 2][0] + sums[w + 3][0]);
-      counted = (sums[w][1] + sums[w + 1][1]) + (sums[w + 2][1] + sums[w + 3][1]);
+      sum = counted = 0.0;
+#pragma unroll
+      for (uint32_t w = i * (kPairThreads / 64); w < (i + 1) * (kPairThreads / 64); ++w) {
+        sum += sums[w][0];
+        counted += sums[w][1];
+      }
       per_row[i] = p.average && counted > 0.0 ? 1.0 / counted : 1.0;
       sum *= per_row[i];
       if (threadIdx.x == 0) p.sequence_logp[2 * pair + i] = static_cast<float>(sum);
       ratio[i] = sum - (p.ref_logp ? static_cast<double>(p.ref_logp[2 * pair + i]) : 0.0);
     }
     const double beta = p.beta, h = beta * (ratio[0] - ratio[1]) - static_cast<double>(p.margin), smoothing = p.smoothing;
-    double slope, loss;
-    if (p.kind == SEE_PREFERENCE_SIGMOID) {
-      loss = (1.0 - smoothing) * Softplus(-h) + smoothing * Softplus(h);
-      slope = smoothing - 1.0 / (1.0 + exp(h));
-    } else if (p.kind == SEE_PREFERENCE_HINGE) {
-      loss = h >= 1.0 ? 0.0 : 1.0 - h;
-      slope = h >= 1.0 ? 0.0 : h < 1.0 ? -1.0 : h;   // (NaN stays)
-    } else {
-      const double off = (h - 0.5) / beta;
-      loss = off * off;
-      slope = 2.0 * off / beta;
+    double slope;
+    if (p.kind == SEE_PREFERENCE_SIGMOID) slope = smoothing - static_cast<double>(1.0f / (1.0f + expf(static_cast<float>(h))));
+    else if (p.kind == SEE_PREFERENCE_HINGE) slope = h >= 1.0 ? 0.0 : h < 1.0 ? -1.0 : h;   // (NaN stays)
+    else slope = 2.0 * (h - 0.5) / (beta * beta);
+    if (a.dlogits) {
+      const double each = slope * beta / static_cast<double>(p.pairs);
+      const float of_row = static_cast<float>((side ? -each * per_row[1] : each * per_row[0]) * static_cast<double>(grad));
+      for (int64_t r = begin + t; r < end; r += kPairThreads / 2) kept[r].x = Counts(a.labels[r], a.classes) ? of_row : 0.0f;
     }
-    if (threadIdx.x == 0) {
-      p.margins[pair] = static_cast<float>(h);
-      p.losses[pair] = loss;
-    }
-    if (!a.dlogits) continue;
-    const double each = slope * beta / static_cast<double>(p.pairs);
-    const float of_row = static_cast<float>((side ? -each * per_row[1] : each * per_row[0]) * static_cast<double>(grad));
-    for (int64_t r = begin + t; r < end; r += kPairThreads / 2) kept[r].x = Counts(a.labels[r], a.classes) ? of_row : 0.0f;
+    if (threadIdx.x != 0) continue;   // (its functions take a microsecond: after the rows)
+    const double off = (h - 0.5) / beta;
+    p.margins[pair] = static_cast<float>(h);
+    p.losses[pair] = p.kind == SEE_PREFERENCE_SIGMOID ? (1.0 - smoothing) * Softplus(-h) + smoothing * Softplus(h)
+                     : p.kind == SEE_PREFERENCE_HINGE ? (h >= 1.0 ? 0.0 : 1.0 - h)
+                                                      : off * off;
   }
 }
 
@@ -689,40 +800,39 @@ PreferenceGradientKernel(const __grid_constant__ LogitArgs a, const __grid_const
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------
-// How rows are shared: T threads and `blocks` blocks of a cluster to a row, `part` units to a block, `units` of them to a thread.
+// How rows are shared: `threads` threads and `blocks` blocks of a cluster to a row, `part` units to a block, `units` of them to a thread.
 struct Sharing {
-  uint32_t T, units, blocks, part, groups, slots, clusters;
+  uint32_t threads, units, blocks, part, groups, slots, clusters;
   size_t bytes;
 };
+constexpr uint32_t kMostUnits = 8;   // to a thread: 32 or 64 elements
 template <typename T>
 bool ShareRows(const LogitArgs& a, uint32_t sms, Sharing* out) {
-  constexpr uint32_t kMostUnits = 64 / kPerUnit<T>;   // to a thread: 64 elements
   const uint32_t all = (a.classes + 2 * (kPerUnit<T> - 1)) / kPerUnit<T>;   // units, wherever a row begins
+  auto of = [all](uint32_t blocks) { return (all + blocks - 1) / blocks; };
   uint32_t blocks = 1;
-  while (blocks < 8 && ((all + blocks - 1) / blocks > kThreads * kMostUnits || (all + blocks - 1) / blocks * 32 > kMostShared - 2048)) blocks *= 2;
-  // Few rows are shared by more blocks, down to a kilobyte each.
-  while (blocks < 8 && a.rows * blocks * 2 <= sms && all / blocks > 128) blocks *= 2;
-  const uint32_t part = (all + blocks - 1) / blocks;
-  if (part > kThreads * kMostUnits) return false;
-  uint32_t units = kMostUnits;
-  if (a.rows * blocks <= sms) {   // a row to an SM: spread it over its threads
-    units = 1;
-    while (part > kThreads * units) units *= 2;
-  }
-  while (units > 1 && part <= 32 * (units / 2)) units /= 2;   // (a warp's row)
+  while (blocks < 8 && of(blocks) > kThreads * kMostUnits) blocks *= 2;
+  // Few rows are shared by more blocks, down to two kilobytes each.
+  while (blocks < 8 && a.rows * blocks * 2 <= sms && all / blocks > 256) blocks *= 2;
   Sharing s;
-  s.T = (((part + units - 1) / units) + 31) / 32 * 32;
-  s.units = units;
   s.blocks = blocks;
-  s.part = part;
-  s.groups = blocks > 1 ? 1 : kThreads / s.T;
-  const uint64_t each = (a.rows + sms - 1) / sms;
+  s.part = of(blocks);
+  if (s.part > kThreads * kMostUnits) return false;
+  s.units = kMostUnits;
+  if (a.rows * blocks <= sms) {   // a row to an SM: spread it over its threads
+    s.units = 1;
+    while (s.part > kThreads * s.units) s.units *= 2;
+  }
+  while (s.units > 1 && s.part <= 32 * (s.units / 2)) s.units /= 2;   // (a warp's row)
+  s.threads = (((s.part + s.units - 1) / s.units) + 31) / 32 * 32;
+  s.groups = kThreads / s.threads;
+  if (blocks > 1 && s.groups > 2) s.groups = 2;
+  const uint64_t most = sms / blocks, each = (a.rows + most - 1) / most;
   if (s.groups > each) s.groups = static_cast<uint32_t>(each);
-  const size_t slot = static_cast<size_t>(part) * 16, budget = kMostShared - 2048;
-  while (s.groups > 1 && 2 * s.groups * slot > budget) --s.groups;
-  s.slots = static_cast<uint32_t>(budget / (s.groups * (slot + 8)));
-  s.slots = s.slots < 1 ? 1 : s.slots > 8 ? 8 : s.slots;
-  const uint64_t wanted = (a.rows + s.groups - 1) / s.groups, most = sms / blocks;
+  const size_t slot = static_cast<size_t>(s.part) * 16, budget = kMostShared - 2048;
+  s.slots = static_cast<uint32_t>(budget / (s.groups * (slot + 8)));   // (a group's part is 64 KB at most, two groups' 32 KB each)
+  s.slots = s.slots > 8 ? 8 : s.slots;
+  const uint64_t wanted = (a.rows + s.groups - 1) / s.groups;
   s.clusters = static_cast<uint32_t>(wanted < most ? wanted : most);
   const uint64_t turns = (wanted + s.clusters - 1) / s.clusters;
   if (s.slots > turns) s.slots = static_cast<uint32_t>(turns);
@@ -731,53 +841,78 @@ bool ShareRows(const LogitArgs& a, uint32_t sms, Sharing* out) {
   return true;
 }
 
+// How many clusters of `blocks` blocks of a kernel the device holds at a time: fewer than its SMs would make, for a cluster lies within
+// one of their groups.  A grid beyond that would leave whole rows to a second round.  Asked for once for each device and size.
+template <auto kKernel>
+cudaError_t MostClusters(uint32_t blocks, uint32_t threads, size_t bytes, uint32_t* most) {
+  static std::atomic<int> known[64][4] = {};   // by device, and blocks 2, 4, 8
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  const uint32_t which = blocks == 2 ? 0 : blocks == 4 ? 1 : 2;
+  int n = dev >= 0 && dev < 64 ? known[dev][which].load(std::memory_order_acquire) : 0;
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = blocks;
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = bytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg); e != cudaSuccess) return e;
+    if (n < 1) n = 1;
+    if (dev >= 0 && dev < 64) known[dev][which].store(n, std::memory_order_release);
+  }
+  *most = static_cast<uint32_t>(n);
+  return cudaSuccess;
+}
+
 template <typename T, int NU, bool kPolicy, bool kCluster>
-cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, double* partials, const Sharing& w, cudaStream_t s) {
+cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, uint32_t* arrived, Sharing& w, cudaStream_t s) {
   constexpr auto* kernel = LogitRowsKernel<T, NU, kPolicy, kCluster>;
-  if (cudaError_t e = AllowShared<kernel>(w.bytes); e != cudaSuccess) return e;
-  return Next(kernel, w.clusters * w.blocks, w.groups * w.T, w.bytes, s, w.blocks)(a, p, seq, kept, partials, w.T, w.slots, w.blocks, w.part);
+  if (cudaError_t e = AllowShared<kernel>(kCluster ? kMostShared - 2048 : w.bytes); e != cudaSuccess) return e;
+  if constexpr (kCluster) {
+    uint32_t most;
+    if (cudaError_t e = MostClusters<kernel>(w.blocks, w.groups * w.threads, kMostShared - 2048, &most); e != cudaSuccess) return e;
+    if (w.clusters > most) w.clusters = most;
+  }
+  return Next(kernel, w.clusters * w.blocks, w.groups * w.threads, w.bytes, s, w.blocks)(a, p, seq, kept, arrived, w.threads, w.slots, w.blocks, w.part);
 }
 template <typename T, bool kPolicy, bool kCluster>
-cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, double* partials, const Sharing& w, cudaStream_t s) {
+cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, uint32_t* arrived, Sharing& w, cudaStream_t s) {
   switch (w.units) {
-    case 1: return RunRows<T, 1, kPolicy, kCluster>(a, p, seq, kept, partials, w, s);
-    case 2: return RunRows<T, 2, kPolicy, kCluster>(a, p, seq, kept, partials, w, s);
-    case 4: return RunRows<T, 4, kPolicy, kCluster>(a, p, seq, kept, partials, w, s);
-    case 8: return RunRows<T, 8, kPolicy, kCluster>(a, p, seq, kept, partials, w, s);
-    default:
-      if constexpr (sizeof(T) == 4) return RunRows<T, 16, kPolicy, kCluster>(a, p, seq, kept, partials, w, s);
-      return cudaErrorInvalidValue;
+    case 1: return RunRows<T, 1, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
+    case 2: return RunRows<T, 2, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
+    case 4: return RunRows<T, 4, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
+    default: return RunRows<T, kMostUnits, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
   }
 }
-// The rows' pass; *count: partial sums of the policy loss.
 template <typename T, bool kPolicy>
-cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, double* partials, uint32_t sms, cudaStream_t s,
-                    uint32_t* count) {
+cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, uint32_t* arrived, uint32_t sms, cudaStream_t s) {
   Sharing w;
-  if (ShareRows<T>(a, sms, &w)) {
-    *count = w.clusters * w.groups;
-    return w.blocks > 1 ? RunRows<T, kPolicy, true>(a, p, seq, kept, partials, w, s) : RunRows<T, kPolicy, false>(a, p, seq, kept, partials, w, s);
-  }
-  *count = static_cast<uint32_t>(a.rows < 4 * sms ? a.rows : 4 * sms);
-  return Next(LogitWideKernel<T, kPolicy>, *count, kThreads, 0, s)(a, p, seq, kept, partials);
+  if (!ShareRows<T>(a, sms, &w))
+    return Next(LogitWideKernel<T, kPolicy>, static_cast<unsigned>(a.rows < 4 * sms ? a.rows : 4 * sms), kThreads, 0, s)(a, p, seq, kept, arrived);
+  return w.blocks > 1 ? RunRows<T, kPolicy, true>(a, p, seq, kept, arrived, w, s) : RunRows<T, kPolicy, false>(a, p, seq, kept, arrived, w, s);
 }
 
 template <typename T>
-cudaError_t Policy(const LogitArgs& a, const PolicyArgs& p, double* partials, uint32_t sms, cudaStream_t s, int* launches) {
-  uint32_t count = 0;
-  if (a.rows) {
-    if (cudaError_t e = RunRows<T, true>(a, p, {}, nullptr, partials, sms, s, &count); e != cudaSuccess) return e;
-    ++*launches;
-  }
-  ++*launches;
-  return Next(PolicyFoldKernel, 1, 96, 0, s)(static_cast<const double*>(partials), count, p.loss);
+cudaError_t Policy(const LogitArgs& a, const PolicyArgs& p, float4* kept, uint32_t sms, cudaStream_t s, int* launches) {
+  if (a.rows == 0) return cudaMemsetAsync(p.loss, 0, 3 * sizeof(float), s);
+  double* partials = reinterpret_cast<double*>(kept + a.rows);
+  uint32_t* arrived = reinterpret_cast<uint32_t*>(partials + 3 * kPolicyPartials);
+  if (cudaError_t e = RunRows<T, true>(a, p, {}, kept, arrived, sms, s); e != cudaSuccess) return e;
+  *launches += 2;
+  const uint64_t blocks = (a.rows + kFinishThreads - 1) / kFinishThreads;
+  return Next(PolicyFinishKernel, static_cast<unsigned>(blocks < kPolicyPartials ? blocks : kPolicyPartials), kFinishThreads, 0, s)(
+      a, p, static_cast<const float4*>(kept), partials, arrived);
 }
 
 template <typename T>
 cudaError_t Preference(const LogitArgs& a, const PreferenceArgs& p, float4* kept, uint32_t sms, cudaStream_t s, int* launches) {
   if (a.rows) {
-    uint32_t count;
-    if (cudaError_t e = RunRows<T, false>(a, {}, {p.starts, 2 * p.pairs}, kept, nullptr, sms, s, &count); e != cudaSuccess) return e;
+    if (cudaError_t e = RunRows<T, false>(a, {}, {p.starts, 2 * p.pairs}, kept, nullptr, sms, s); e != cudaSuccess) return e;
     ++*launches;
   }
   if (cudaError_t e = Next(PreferencePairsKernel, p.pairs < 4 * sms ? p.pairs : 4 * sms, kPairThreads, 0, s)(a, p, kept); e != cudaSuccess) return e;
@@ -792,9 +927,9 @@ cudaError_t Preference(const LogitArgs& a, const PreferenceArgs& p, float4* kept
 
 }  // namespace
 
-cudaError_t PolicyLoss(const LogitArgs& a, int type, const PolicyArgs& p, double* partials, uint32_t sms, cudaStream_t s, int* launches) {
-  if (type == SEE_F32) return Policy<float>(a, p, partials, sms, s, launches);
-  return type == SEE_BF16 ? Policy<Bf16>(a, p, partials, sms, s, launches) : Policy<F16>(a, p, partials, sms, s, launches);
+cudaError_t PolicyLoss(const LogitArgs& a, int type, const PolicyArgs& p, float4* kept, uint32_t sms, cudaStream_t s, int* launches) {
+  if (type == SEE_F32) return Policy<float>(a, p, kept, sms, s, launches);
+  return type == SEE_BF16 ? Policy<Bf16>(a, p, kept, sms, s, launches) : Policy<F16>(a, p, kept, sms, s, launches);
 }
 cudaError_t PreferenceLoss(const LogitArgs& a, int type, const PreferenceArgs& p, float4* kept, uint32_t sms, cudaStream_t s, int* launches) {
   if (type == SEE_F32) return Preference<float>(a, p, kept, sms, s, launches);

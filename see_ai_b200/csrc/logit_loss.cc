@@ -39,7 +39,7 @@ k::LogitArgs ArgsOf(const Shape& s, const void* logits, const int32_t* labels, v
 uint64_t PreferenceWorkspace(uint64_t rows, uint64_t pairs) {   // what is kept of a row, and each pair's loss
   return rows > 0x7FFFFFFFull || pairs == 0 || pairs > (1u << 24) ? 0 : rows * 16 + (pairs * 8 + 15) / 16 * 16;
 }
-uint64_t PolicyWorkspace(uint64_t rows) { return rows > 0x7FFFFFFFull ? 0 : k::kLogitPartials * 3 * sizeof(double); }
+uint64_t PolicyWorkspace(uint64_t rows) { return rows > 0x7FFFFFFFull ? 0 : rows * 16 + k::kPolicyPartials * 3 * sizeof(double) + 16; }
 
 Status CheckPreference(see_preference_shape* shape, const void* logits, const int32_t* labels, const int32_t* starts, const float* ref_logp,
                        const float* loss_grad, const float* loss, const float* margins, const float* sequence_logp, const void* dlogits,
@@ -128,7 +128,7 @@ Status CudaBackend::PolicyLoss(const see_policy_shape& given, const void* logits
   if (!on.ok()) return Check(cudaGetLastError(), "policy loss: device");
   int launches = 0;
   const cudaError_t e =
-      k::PolicyLoss(ArgsOf(s, logits, labels, dlogits, d_status_), s.type, p, static_cast<double*>(workspace), sms_, stream_, &launches);
+      k::PolicyLoss(ArgsOf(s, logits, labels, dlogits, d_status_), s.type, p, static_cast<float4*>(workspace), sms_, stream_, &launches);
   counters_.kernel_launches += static_cast<uint64_t>(launches);
   return Check(e, "policy loss");
 }
