@@ -11,6 +11,7 @@
 // is wider still is read from memory twice (LogitWideKernel).
 //
 // logp is made in double: a sequence's sum of hundreds of them is held against a reference's.
+#include <cstdlib>
 #include <type_traits>
 
 #include "act_expr.cuh"
@@ -355,6 +356,12 @@ __device__ __forceinline__ uint32_t Max2(uint32_t a, uint32_t b, F16) {
   asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// 2^x of both.
+__device__ __forceinline__ f32x2 Powers(f32x2 x) {
+  float lo, hi;
+  UnpackF2(x, &lo, &hi);
+  return PackF2(Ex2Approx(lo), Ex2Approx(hi));
+}
 // The largest of a thread's elements that is a number.
 template <typename T, int NU>
 __device__ __forceinline__ float Largest(const uint4 (&raw)[NU]) {
@@ -395,67 +402,73 @@ __device__ __forceinline__ bool AwaitCluster(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
-// A group's row: `blocks` blocks of a cluster share it, `part` units each.
+// How a launch shares its rows: `threads` threads and `blocks` blocks of a cluster to a row, `part` units to a block.  Rows from `edge` on to
+// `edge` before the last are copied in bulk: what sticks out of theirs is the matrix's too.
+struct RowsPlan {
+  uint32_t threads, over_threads, slots, blocks, part, edge;   // over_threads: 2^32 / threads, rounded up
+};
+
 template <typename T, int NU, bool kPolicy, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 1)
 LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const Sequences seq, float4* __restrict__ kept,
-                uint32_t* __restrict__ arrived, uint32_t threads, uint32_t slots, uint32_t blocks, uint32_t part) {
+                uint32_t* __restrict__ arrived, const RowsPlan plan) {
   using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+  constexpr uint32_t E = kPerUnit<T>;
   extern __shared__ __align__(128) uint8_t dyn[];
-  __shared__ float2 sums[2][kThreads / 32];                // k M and the sum, of a warp
-  __shared__ Exchange exchange[2];                         // of a group
-  const uint32_t groups = blockDim.x / threads, group = threadIdx.x / threads, t = threadIdx.x - group * threads, lane = threadIdx.x & 31;
-  const uint32_t rank = kCluster ? blockIdx.x % blocks : 0, cluster = kCluster ? blockIdx.x / blocks : blockIdx.x;
-  const uint32_t clusters = kCluster ? gridDim.x / blocks : gridDim.x;
-  const uint32_t slot_bytes = part * 16;
-  uint8_t* ring = dyn + static_cast<size_t>(group) * slots * slot_bytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + static_cast<size_t>(groups) * slots * slot_bytes) + group * slots;
-  const uint64_t first = static_cast<uint64_t>(cluster) * groups + group, step = static_cast<uint64_t>(clusters) * groups;
+  __shared__ float2 sums[2][kThreads / 32];            // k M and the sum, of a warp
+  __shared__ uint32_t brought[2][kThreads / 32][8];    // of a group: the label's logit, and a PolicyRow
+  __shared__ Exchange exchange[2];                     // of a group
+  const uint32_t threads = plan.threads, group = threadIdx.x / threads, t = threadIdx.x - group * threads, lane = threadIdx.x & 31;
+  const uint32_t groups = blockDim.x / threads, rank = kCluster ? blockIdx.x % plan.blocks : 0;
+  const uint32_t slot_bytes = plan.part * 16, begin = rank * plan.part;   // begin: of this block's units of a row
+  uint8_t* ring = dyn + static_cast<size_t>(group) * plan.slots * slot_bytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + static_cast<size_t>(groups) * plan.slots * slot_bytes) + group * plan.slots;
+  const uint32_t rows = static_cast<uint32_t>(a.rows), step = (kCluster ? gridDim.x / plan.blocks : gridDim.x) * groups;
+  const uint32_t first = (kCluster ? blockIdx.x / plan.blocks : blockIdx.x) * groups + group;
   if (t == 0) {
-    for (uint32_t i = 0; i < slots; ++i) umma_dev::MbarInit(&bars[i], 1);
+    for (uint32_t i = 0; i < plan.slots; ++i) umma_dev::MbarInit(&bars[i], 1);
     if constexpr (kCluster)
-      for (uint32_t i = 0; i < 2; ++i) umma_dev::MbarInit(&exchange[group].bars[i], blocks);
+      for (uint32_t i = 0; i < 2; ++i) umma_dev::MbarInit(&exchange[group].bars[i], plan.blocks);
     umma_dev::MbarInitFence();
   }
   AwaitPrevious();
-  const uint64_t begin = reinterpret_cast<uint64_t>(a.logits), end = begin + ((a.rows - 1) * a.stride + a.classes) * sizeof(T);
-  // The units of this block's part of a row, and whether they can be copied whole.
-  struct Share {
-    uint64_t from;
-    uint32_t first, count;
-    bool bulk;
+  auto logit_row = [&](uint32_t r) { return static_cast<const T*>(a.logits) + static_cast<uint64_t>(r) * a.stride; };
+  auto skip_of = [](const T* z) { return static_cast<uint32_t>(reinterpret_cast<uint64_t>(z) & 15) / static_cast<uint32_t>(sizeof(T)); };
+  auto units_of = [&](uint32_t skip) {   // of this block
+    const uint32_t all = (skip + a.classes + E - 1) / E;
+    return kCluster ? (all > begin ? min(plan.part, all - begin) : 0u) : all;
   };
-  auto share_of = [&](const Row<T>& row) {
-    Share w;
-    w.first = rank * part;
-    w.count = row.units > w.first ? min(part, row.units - w.first) : 0;
-    w.from = reinterpret_cast<uint64_t>(row.z) - row.skip * sizeof(T) + static_cast<uint64_t>(w.first) * 16;
-    w.bulk = w.count != 0 && w.from >= begin && w.from + static_cast<uint64_t>(w.count) * 16 <= end;
-    return w;
+  auto counts = [&](uint32_t r, int32_t label) {
+    if (!Counts(label, a.classes)) return false;
+    return kPolicy || (static_cast<int64_t>(r) >= seq.starts[0] && static_cast<int64_t>(r) < seq.starts[seq.count]);
   };
-  int64_t seq_first = 0, seq_end = 0;
-  if (!kPolicy) {
-    seq_first = seq.starts[0];
-    seq_end = seq.starts[seq.count];
-  }
-  auto counts = [&](uint64_t r, int32_t label) {
-    return Counts(label, a.classes) && (kPolicy || (static_cast<int64_t>(r) >= seq_first && static_cast<int64_t>(r) < seq_end));
-  };
-  auto fill = [&](uint64_t r, int32_t label, uint32_t slot) {   // the group's thread 0
-    if (!counts(r, label)) return;
-    const Share w = share_of(Row<T>(a, r));
-    if (!w.bulk) return;
+  auto bulk = [&](uint32_t r) { return r >= plan.edge && r < rows - plan.edge; };   // (edge is rows at most)
+  auto fill = [&](uint32_t r, int32_t label, uint32_t slot) {   // the group's thread 0
+    if (!counts(r, label) || !bulk(r)) return;
+    const T* z = logit_row(r);
+    const uint32_t skip = skip_of(z), bytes = units_of(skip) * 16;
+    if (bytes == 0) return;
     umma_dev::FenceProxyAsync();   // (elements were written there)
-    umma_dev::MbarExpectTx(&bars[slot], w.count * 16);
-    umma_dev::BulkLoad(ring + static_cast<size_t>(slot) * slot_bytes, reinterpret_cast<const void*>(w.from), w.count * 16, &bars[slot]);
+    umma_dev::MbarExpectTx(&bars[slot], bytes);
+    umma_dev::BulkLoad(ring + static_cast<size_t>(slot) * slot_bytes, reinterpret_cast<const uint4*>(z - skip) + begin, bytes, &bars[slot]);
+  };
+  // What a row brings besides its logits is asked for while the one before it is at work: each item by one of the group's first threads, as it is read.
+  uint32_t ahead = 0;
+  auto ask = [&](uint32_t r, int32_t label) {
+    if (r >= rows || t > (kPolicy ? 4u : 0u) || !counts(r, label)) return;
+    if (t == 0) ahead = reinterpret_cast<const Bits*>(logit_row(r))[label];
+    else if (t == 1) ahead = __float_as_uint(p.old_logp[r]);
+    else if (t == 2) ahead = p.ref_logp ? __float_as_uint(p.ref_logp[r]) : 0u;
+    else if (t == 3) ahead = __float_as_uint(p.advantages[r]);
+    else ahead = p.weights ? __float_as_uint(p.weights[r]) : 0x3F800000u;
   };
   int32_t fill_label = -1;   // of the row that goes into the slot that the next one leaves
   if (t == 0) {
     int32_t labels[9];
 #pragma unroll
-    for (uint32_t i = 0; i < 9; ++i) labels[i] = i <= slots && first + i * step < a.rows ? a.labels[first + i * step] : -1;
+    for (uint32_t i = 0; i < 9; ++i) labels[i] = i <= plan.slots && first + i * step < rows ? a.labels[first + i * step] : -1;
 #pragma unroll 1
-    for (uint32_t i = 0; i < slots && first + i * step < a.rows; ++i) {
+    for (uint32_t i = 0; i < plan.slots && first + i * step < rows; ++i) {
       fill(first + i * step, labels[0], i);
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) labels[j] = labels[j + 1];
@@ -463,91 +476,85 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     fill_label = labels[0];
   }
   const float grad = (kPolicy && p.loss_grad ? *p.loss_grad : 1.0f) * a.scale;
+  if (kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
+  int32_t next_label = first < rows ? a.labels[first] : -1, label_behind = first + step < rows ? a.labels[first + step] : -1;
+  ask(first, next_label);
   __syncwarp();
   if constexpr (kCluster) umma_dev::ClusterSync();   // (every block of it has begun: its shared memory may be written)
   else GroupBarrier(threads, group);                 // the barriers are there
-  if (kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
   uint32_t turn = 0, slot = 0, parities = 0, exchanged = 0;   // a bit for each slot, of the copies that went through it; rows exchanged
-  // What a row brings besides its logits is asked for while the one before it is at work.
-  int32_t label = -1, next_label = -1;
-  T next_z_label = {};   // (as it is read: a conversion would wait for it)
-  PolicyRow next_brings = {};
-  auto ask = [&](uint64_t r) {   // (next_label is there)
-    if (r >= a.rows || !counts(r, next_label)) return;
-    next_z_label = static_cast<const T*>(a.logits)[r * a.stride + next_label];
-    if (kPolicy) next_brings = PolicyRowOf(p, r);
-  };
-  if (first < a.rows) next_label = a.labels[first];
-  ask(first);
-  int32_t label_behind = first + step < a.rows ? a.labels[first + step] : -1;
-  for (uint64_t r = first; r < a.rows; r += step) {
-    label = next_label;
+  for (uint32_t r = first; r < rows; r += step) {
+    const int32_t label = next_label;
     next_label = label_behind;
-    label_behind = r + 2 * step < a.rows ? a.labels[r + 2 * step] : -1;
-    const T raw_label = next_z_label;
-    [[maybe_unused]] const PolicyRow brings = next_brings;
-    const Row<T> row(a, r);
-    const Share w = share_of(row);
-    const uint32_t now = slot;
-    if (++slot == slots) slot = 0;
+    label_behind = r + 2 * step < rows ? a.labels[r + 2 * step] : -1;
+    const uint32_t item = ahead, now = slot;
+    ask(r + step, next_label);
+    if (++slot == plan.slots) slot = 0;
     auto refill = [&] {
       if (t != 0) return;
-      const uint64_t next = r + slots * step;
-      if (next < a.rows) fill(next, fill_label, now);
-      if (next + step < a.rows) fill_label = a.labels[next + step];
+      const uint32_t next = r + plan.slots * step;
+      if (next < rows) fill(next, fill_label, now);
+      if (next + step < rows) fill_label = a.labels[next + step];
     };
     auto zeros = [&] {
-      const float none[kPerUnit<T>] = {};
-      for (uint32_t u = t; u < w.count; u += threads) row.Store(w.first + u, none);
+      const Row<T> row(a, r);
+      const float none[E] = {};
+      const uint32_t end = units_of(row.skip);
+      for (uint32_t u = t; u < end; u += threads) row.Store(begin + u, none);
     };
-    ask(r + step);
     if (!counts(r, label)) {
       if (kPolicy && a.dlogits) zeros();
       refill();
       continue;
     }
-    // Its part in the slot, each thread's own units; -inf in place of the label and of what sticks out of the row.
-    uint4* mine = reinterpret_cast<uint4*>(ring + static_cast<size_t>(now) * slot_bytes);
-    const uint32_t label_unit = (static_cast<uint32_t>(label) + row.skip) / kPerUnit<T> - w.first;   // (of another block: beyond count)
-    if (w.bulk) {
-      AwaitRow(&bars[now], parities >> now & 1u, a.status);
-      parities ^= 1u << now;
-      Bits* bits = reinterpret_cast<Bits*>(mine);
-      if (t == 0 && w.first == 0)
-        for (uint32_t j = 0; j < row.skip; ++j) bits[j] = NoElement<T>();
-      if (w.first + w.count == row.units && t == (w.count - 1) % threads)
-        for (uint32_t j = row.skip + a.classes - w.first * kPerUnit<T>; j < w.count * kPerUnit<T>; ++j) bits[j] = NoElement<T>();
-    } else {
-      for (uint32_t u = t; u < w.count; u += threads) mine[u] = row.Raw(w.first + u);
-    }
-    if (label_unit < w.count && t == label_unit % threads)
-      reinterpret_cast<Bits*>(mine)[static_cast<uint32_t>(label) + row.skip - w.first * kPerUnit<T>] = NoElement<T>();
-    asm volatile("" ::: "memory");   // (as elements, then as units)
     uint4 raw[NU];
-#pragma unroll
-    for (int i = 0; i < NU; ++i) raw[i] = t + i * threads < w.count ? mine[t + i * threads] : Nothing<T>();
-    float mk = __fmul_rn(Largest<T, NU>(raw), a.k);   // -inf: nothing here
-    const f32x2 k2 = Splat2(a.k), away = Splat2(mk == MinusInf() ? 0.0f : -mk);
-    f32x2 e[NU][kPairs<T>], sum2[kPairs<T>] = {};
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      Pairs<T>(raw[i], e[i]);
-#pragma unroll
-      for (int j = 0; j < kPairs<T>; ++j) {
-        float lo, hi;
-        UnpackF2(Fma2(e[i][j], k2, away), &lo, &hi);
-        e[i][j] = PackF2(Ex2Approx(lo), Ex2Approx(hi));
-        sum2[j] = AddF2(sum2[j], e[i][j]);
+    bool owner;   // of the label
+    {
+      // This block's part in the slot, each thread's own units; -inf in place of the label and of what sticks out of the row.
+      const uint32_t skip = skip_of(logit_row(r)), count = units_of(skip);
+      uint4* mine = reinterpret_cast<uint4*>(ring + static_cast<size_t>(now) * slot_bytes);
+      Bits* elements = reinterpret_cast<Bits*>(mine);
+      auto owns = [&](uint32_t u) { return u < count && u - __umulhi(u, plan.over_threads) * threads == t; };
+      if (bulk(r)) {
+        if (count != 0) {
+          AwaitRow(&bars[now], parities >> now & 1u, a.status);
+          parities ^= 1u << now;
+        }
+        if (t == 0 && begin == 0)
+          for (uint32_t j = 0; j < skip; ++j) elements[j] = NoElement<T>();
+        const uint32_t end = skip + a.classes - begin * E;   // of the row, in elements
+        if (end < count * E && owns(count - 1))
+          for (uint32_t j = end; j < count * E; ++j) elements[j] = NoElement<T>();
+      } else {
+        const Row<T> row(a, r);
+        for (uint32_t u = t; u < count; u += threads) mine[u] = row.Raw(begin + u);
       }
-    }
+      const uint32_t at = static_cast<uint32_t>(label) + skip - begin * E;   // (of another block: beyond count)
+      owner = owns(at / E);
+      if (owner) elements[at] = NoElement<T>();
+      asm volatile("" ::: "memory");   // (as elements, then as units)
 #pragma unroll
-    for (int j = 1; j < kPairs<T>; ++j) sum2[0] = AddF2(sum2[0], sum2[j]);
-    float lo, sum;
-    UnpackF2(sum2[0], &lo, &sum);
-    sum += lo;
+      for (int i = 0; i < NU; ++i) raw[i] = t + i * threads < count ? mine[t + i * threads] : Nothing<T>();
+    }
+    float mk = __fmul_rn(Largest<T, NU>(raw), a.k), sum;   // -inf: nothing here
+    {
+      const f32x2 k2 = Splat2(a.k), away = Splat2(mk == MinusInf() ? 0.0f : -mk);
+      f32x2 sum2[kPairs<T>] = {};
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        f32x2 v[kPairs<T>];
+        Pairs<T>(raw[i], v);
+#pragma unroll
+        for (int j = 0; j < kPairs<T>; ++j) sum2[j] = AddF2(sum2[j], Powers(Fma2(v[j], k2, away)));
+      }
+#pragma unroll
+      for (int j = 1; j < kPairs<T>; ++j) sum2[0] = AddF2(sum2[0], sum2[j]);
+      float lo;
+      UnpackF2(sum2[0], &lo, &sum);
+      sum += lo;
+    }
     // Warps, groups, blocks: the largest k M, and sums relative to it.  (A part without numbers has factor 0; NaN stays NaN.)
     auto factor = [](float own, float all) { return own == MinusInf() ? 0.0f : Ex2Approx(own - all); };
-    const float own = mk;
     auto join = [&](uint32_t most) {
       const float top = WarpMax(mk);   // (beyond `most` the lanes repeat themselves)
       sum *= factor(mk, top);
@@ -557,6 +564,8 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
         if (o <= most) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     };
     join(16);
+    uint32_t* items = brought[turn][group];
+    if (t < 5) items[t] = item;
     if (threads > 32) {
       float2* set = sums[turn] + group * (threads / 32);
       if (lane == 0) set[t >> 5] = make_float2(mk, sum);
@@ -570,7 +579,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     }
     if constexpr (kCluster) {
       Exchange& x = exchange[group];
-      if (t < blocks) {
+      if (t < plan.blocks) {
         const uint32_t to = umma_dev::MapToCta(umma_dev::SmemAddr(&x.parts[turn][rank]), t);
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(mk), "f"(sum) : "memory");
         umma_dev::MbarArriveCluster(umma_dev::MapToCta(umma_dev::SmemAddr(&x.bars[turn]), t));
@@ -582,7 +591,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
         umma_dev::DrainDelay();
       }
       ++exchanged;
-      const float2 block_part = (lane & 7) < blocks ? x.parts[turn][lane & 7] : make_float2(MinusInf(), 0.0f);
+      const float2 block_part = (lane & 7) < plan.blocks ? x.parts[turn][lane & 7] : make_float2(MinusInf(), 0.0f);
       mk = block_part.x;
       sum = block_part.y;
       join(4);
@@ -591,47 +600,59 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     }
     turn ^= 1;
     // The label joins the maximum, so that its term is 1 at most.
-    const float z_label = ToF32(raw_label);
-    const float mk_label = __fmul_rn(z_label, a.k), all = fmaxf(mk, mk_label);
+    T raw_label;
+    if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(items[0]);
+    else raw_label.bits = static_cast<uint16_t>(items[0]);
+    const float z_label = ToF32(raw_label), mk_label = __fmul_rn(z_label, a.k), all = fmaxf(mk, mk_label);
     RowSums q = {z_label, all == MinusInf() ? 0.0f : all, sum * factor(mk, all), 0.0f};
     q.s = q.others + LabelTerm(a, z_label, q.mk);
     if (t == 0 && rank == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
     if constexpr (kPolicy) {
       if (!a.dlogits) continue;
+      const PolicyRow brings = {__uint_as_float(items[1]), __uint_as_float(items[2]), __uint_as_float(items[3]), __uint_as_float(items[4])};
       const float slope = SlopeOf<T>(a, p, brings, q) * grad;
       if (slope == 0.0f) {
         zeros();
         continue;
       }
       const float each = -slope / q.s;
-      const f32x2 by = Splat2(factor(own, q.mk) * each);
+      uint32_t again = r;
+      asm volatile("" : "+r"(again));   // (the row's addresses anew: kept across the sums they cost registers that the units need)
+      const Row<T> row(a, again);
+      const uint32_t count = units_of(row.skip);
       // Units that lie wholly in the row; then, their owners, the two that may not.
-      const uint32_t whole_first = w.first == 0 && row.skip != 0 ? 1 : 0;
-      const uint32_t whole_end = min(w.count, (row.skip + a.classes) / kPerUnit<T> - w.first);   // (without units: 0)
+      const uint32_t whole_first = begin == 0 && row.skip != 0 ? 1 : 0, whole_end = min(count, (row.skip + a.classes) / E - begin);   // (without units: 0)
       const uint32_t whole = row.alike && whole_end > whole_first ? whole_end - whole_first : 0;
-      T* to = row.d - row.skip + static_cast<size_t>(w.first) * kPerUnit<T>;
+      {
+        const f32x2 k2 = Splat2(a.k), away = Splat2(-q.mk), by = Splat2(each);
+        uint4* to = reinterpret_cast<uint4*>(row.d - row.skip) + begin + t;
 #pragma unroll
-      for (int i = 0; i < NU; ++i) {
-        const uint32_t u = t + i * threads;
-        if (u - whole_first < whole) {
-          float v[kPerUnit<T>];
+        for (int i = 0; i < NU; ++i) {
+          if (t + i * threads - whole_first < whole) {
+            // (unpacked anew: values of the first time, kept, would be spilled)
+            asm volatile("" : "+r"(raw[i].x), "+r"(raw[i].y), "+r"(raw[i].z), "+r"(raw[i].w));
+            f32x2 pair[kPairs<T>];
+            float v[E];
+            Pairs<T>(raw[i], pair);
 #pragma unroll
-          for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(e[i][j], by), &v[2 * j], &v[2 * j + 1]);
-          if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to + static_cast<size_t>(u) * 4) = make_float4(v[0], v[1], v[2], v[3]);
-          else Store8<T>(to + static_cast<size_t>(u) * 8, v);
+            for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(Powers(Fma2(pair[j], k2, away)), by), &v[2 * j], &v[2 * j + 1]);
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+            else Store8<T>(reinterpret_cast<T*>(to), v);
+          }
+          to += threads;
         }
       }
-      if (whole_first || whole + whole_first != w.count) {   // (from memory: of a matrix in place, these elements are still logits)
-        for (uint32_t u = t; u < w.count; u += threads) {
+      if (whole_first || whole + whole_first != count) {   // (from memory: of a matrix in place, these elements are still logits)
+        for (uint32_t u = t; u < count; u += threads) {
           if (u - whole_first < whole) continue;
-          float v[kPerUnit<T>];
-          row.Load(w.first + u, v);
+          float v[E];
+          row.Load(begin + u, v);
 #pragma unroll
-          for (int j = 0; j < kPerUnit<T>; ++j) v[j] = each * Ex2Approx(fmaf(v[j], a.k, -q.mk));
-          row.Store(w.first + u, v);
+          for (uint32_t j = 0; j < E; ++j) v[j] = each * Ex2Approx(fmaf(v[j], a.k, -q.mk));
+          row.Store(begin + u, v);
         }
       }
-      if (label_unit < w.count && t == label_unit % threads) row.d[label] = FromF32<T>(slope * (q.others / q.s));
+      if (owner) row.d[label] = FromF32<T>(slope * (q.others / q.s));
     }
   }
 }
@@ -802,16 +823,17 @@ PreferenceGradientKernel(const __grid_constant__ LogitArgs a, const __grid_const
 // ---- launches ------------------------------------------------------------------------------------------------
 // How rows are shared: `threads` threads and `blocks` blocks of a cluster to a row, `part` units to a block, `units` of them to a thread.
 struct Sharing {
-  uint32_t threads, units, blocks, part, groups, slots, clusters;
+  uint32_t threads, units, blocks, part, groups, slots, clusters, edge;
   size_t bytes;
 };
-constexpr uint32_t kMostUnits = 8;   // to a thread: 32 or 64 elements
+constexpr uint32_t kMostUnits = 16;   // to a thread, 64 registers
 template <typename T>
 bool ShareRows(const LogitArgs& a, uint32_t sms, Sharing* out) {
   const uint32_t all = (a.classes + 2 * (kPerUnit<T> - 1)) / kPerUnit<T>;   // units, wherever a row begins
   auto of = [all](uint32_t blocks) { return (all + blocks - 1) / blocks; };
   uint32_t blocks = 1;
-  while (blocks < 8 && of(blocks) > kThreads * kMostUnits) blocks *= 2;
+  const uint32_t lim = getenv("SEE_LIM") ? atoi(getenv("SEE_LIM")) : kThreads / 2;
+  while (blocks < 8 && of(blocks) > lim * kMostUnits) blocks *= 2;   // two rows to a block: one computes while the other's sums meet
   // Few rows are shared by more blocks, down to two kilobytes each.
   while (blocks < 8 && a.rows * blocks * 2 <= sms && all / blocks > 256) blocks *= 2;
   Sharing s;
@@ -830,13 +852,18 @@ bool ShareRows(const LogitArgs& a, uint32_t sms, Sharing* out) {
   const uint64_t most = sms / blocks, each = (a.rows + most - 1) / most;
   if (s.groups > each) s.groups = static_cast<uint32_t>(each);
   const size_t slot = static_cast<size_t>(s.part) * 16, budget = kMostShared - 2048;
-  s.slots = static_cast<uint32_t>(budget / (s.groups * (slot + 8)));   // (a group's part is 64 KB at most, two groups' 32 KB each)
+  while (s.groups * (slot + 8) > budget) --s.groups;   // (a group's part is 128 KB at most)
+  s.slots = static_cast<uint32_t>(budget / (s.groups * (slot + 8)));
   s.slots = s.slots > 8 ? 8 : s.slots;
   const uint64_t wanted = (a.rows + s.groups - 1) / s.groups;
   s.clusters = static_cast<uint32_t>(wanted < most ? wanted : most);
   const uint64_t turns = (wanted + s.clusters - 1) / s.clusters;
   if (s.slots > turns) s.slots = static_cast<uint32_t>(turns);
   s.bytes = s.groups * s.slots * (slot + 8);
+  const uint64_t pitch = a.stride * sizeof(T);
+  const bool exact = ((reinterpret_cast<uintptr_t>(a.logits) | pitch | a.classes * sizeof(T)) & 15) == 0;
+  s.edge = exact ? 0 : static_cast<uint32_t>((15 + pitch) / pitch);
+  if (2ull * s.edge > a.rows) s.edge = static_cast<uint32_t>(a.rows);   // (none in bulk)
   *out = s;
   return true;
 }
@@ -878,7 +905,8 @@ cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& se
     if (cudaError_t e = MostClusters<kernel>(w.blocks, w.groups * w.threads, kMostShared - 2048, &most); e != cudaSuccess) return e;
     if (w.clusters > most) w.clusters = most;
   }
-  return Next(kernel, w.clusters * w.blocks, w.groups * w.threads, w.bytes, s, w.blocks)(a, p, seq, kept, arrived, w.threads, w.slots, w.blocks, w.part);
+  return Next(kernel, w.clusters * w.blocks, w.groups * w.threads, w.bytes, s, w.blocks)(
+      a, p, seq, kept, arrived, RowsPlan{w.threads, static_cast<uint32_t>(0xFFFFFFFFu / w.threads) + 1, w.slots, w.blocks, w.part, w.edge});
 }
 template <typename T, bool kPolicy, bool kCluster>
 cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, uint32_t* arrived, Sharing& w, cudaStream_t s) {
@@ -886,6 +914,7 @@ cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& se
     case 1: return RunRows<T, 1, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
     case 2: return RunRows<T, 2, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
     case 4: return RunRows<T, 4, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
+    case 8: return RunRows<T, 8, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
     default: return RunRows<T, kMostUnits, kPolicy, kCluster>(a, p, seq, kept, arrived, w, s);
   }
 }
