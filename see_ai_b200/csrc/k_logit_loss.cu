@@ -11,7 +11,6 @@
 // is wider still is read from memory twice (LogitWideKernel).
 //
 // logp is made in double: a sequence's sum of hundreds of them is held against a reference's.
-#include <cstdlib>
 #include <type_traits>
 
 #include "act_expr.cuh"
@@ -47,6 +46,23 @@ template <typename T>
 __device__ __forceinline__ uint4 Nothing() {
   const uint32_t w = sizeof(T) == 4 ? NoElement<T>() : NoElement<T>() * 0x10001u;
   return make_uint4(w, w, w, w);
+}
+
+// The elements from `from` on and before `to` (and not `but`), -inf in place of the others.
+template <typename T>
+__device__ __forceinline__ uint4 Only(const uint4& r, int32_t from, int32_t to, int32_t but) {
+  uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = i >= from && i < to && i != but ? w[i] : NoElement<T>();
+    } else {
+      const uint32_t lo = 2 * i >= from && 2 * i < to && 2 * i != but ? w[i] & 0xFFFFu : NoElement<T>();
+      const uint32_t hi = 2 * i + 1 >= from && 2 * i + 1 < to && 2 * i + 1 != but ? w[i] >> 16 : NoElement<T>();
+      w[i] = lo | hi << 16;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // A row of logits and of dlogits.
@@ -408,11 +424,13 @@ struct RowsPlan {
   uint32_t threads, over_threads, slots, blocks, part, edge;   // over_threads: 2^32 / threads, rounded up
 };
 
+// Blocks to an SM: of short rows, whose time is a row's chain, two.
+constexpr uint32_t BlocksOf(uint32_t units) { return units <= 2 ? 2 : 1; }
+
 template <typename T, int NU, bool kPolicy, bool kCluster>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, BlocksOf(NU))
 LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const Sequences seq, float4* __restrict__ kept,
                 uint32_t* __restrict__ arrived, const RowsPlan plan) {
-  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
   constexpr uint32_t E = kPerUnit<T>;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ float2 sums[2][kThreads / 32];            // k M and the sum, of a warp
@@ -456,7 +474,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
   uint32_t ahead = 0;
   auto ask = [&](uint32_t r, int32_t label) {
     if (r >= rows || t > (kPolicy ? 4u : 0u) || !counts(r, label)) return;
-    if (t == 0) ahead = reinterpret_cast<const Bits*>(logit_row(r))[label];
+    if (t == 0) ahead = reinterpret_cast<const std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>*>(logit_row(r))[label];
     else if (t == 1) ahead = __float_as_uint(p.old_logp[r]);
     else if (t == 2) ahead = p.ref_logp ? __float_as_uint(p.ref_logp[r]) : 0u;
     else if (t == 3) ahead = __float_as_uint(p.advantages[r]);
@@ -513,30 +531,36 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
       // This block's part in the slot, each thread's own units; -inf in place of the label and of what sticks out of the row.
       const uint32_t skip = skip_of(logit_row(r)), count = units_of(skip);
       uint4* mine = reinterpret_cast<uint4*>(ring + static_cast<size_t>(now) * slot_bytes);
-      Bits* elements = reinterpret_cast<Bits*>(mine);
       auto owns = [&](uint32_t u) { return u < count && u - __umulhi(u, plan.over_threads) * threads == t; };
+      const int32_t at = label + static_cast<int32_t>(skip - begin * E), end = static_cast<int32_t>(skip + a.classes - begin * E);
+      auto patch = [&](uint32_t u) {   // (the label of another unit: beyond the unit's elements)
+        const int32_t from = static_cast<int32_t>(u * E);
+        mine[u] = Only<T>(mine[u], static_cast<int32_t>(skip - begin * E) - from, end - from, at - from);
+      };
+      owner = at >= 0 && owns(static_cast<uint32_t>(at) / E);
       if (bulk(r)) {
         if (count != 0) {
           AwaitRow(&bars[now], parities >> now & 1u, a.status);
           parities ^= 1u << now;
         }
-        if (t == 0 && begin == 0)
-          for (uint32_t j = 0; j < skip; ++j) elements[j] = NoElement<T>();
-        const uint32_t end = skip + a.classes - begin * E;   // of the row, in elements
-        if (end < count * E && owns(count - 1))
-          for (uint32_t j = end; j < count * E; ++j) elements[j] = NoElement<T>();
+        if (t == 0 && begin == 0 && skip != 0) patch(0);
+        if (end < static_cast<int32_t>(count * E) && owns(count - 1)) patch(count - 1);
       } else {
         const Row<T> row(a, r);
         for (uint32_t u = t; u < count; u += threads) mine[u] = row.Raw(begin + u);
       }
-      const uint32_t at = static_cast<uint32_t>(label) + skip - begin * E;   // (of another block: beyond count)
-      owner = owns(at / E);
-      if (owner) elements[at] = NoElement<T>();
-      asm volatile("" ::: "memory");   // (as elements, then as units)
+      if (owner) patch(static_cast<uint32_t>(at) / E);
 #pragma unroll
       for (int i = 0; i < NU; ++i) raw[i] = t + i * threads < count ? mine[t + i * threads] : Nothing<T>();
     }
     float mk = __fmul_rn(Largest<T, NU>(raw), a.k), sum;   // -inf: nothing here
+    // A lone slot is filled while the exponentials are made, unless dlogits will be stored meanwhile: loads and stores in turn are faster then
+    // (8192 rows of 32000 in bf16: 172 us, early 184; a preference loss's rows 84, early 76).
+    const bool early = plan.slots == 1 && !(kPolicy && a.dlogits);
+    if (early) {
+      GroupBarrier(threads, group);
+      refill();
+    }
     {
       const f32x2 k2 = Splat2(a.k), away = Splat2(mk == MinusInf() ? 0.0f : -mk);
       f32x2 sum2[kPairs<T>] = {};
@@ -584,7 +608,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(mk), "f"(sum) : "memory");
         umma_dev::MbarArriveCluster(umma_dev::MapToCta(umma_dev::SmemAddr(&x.bars[turn]), t));
       }
-      refill();   // (the slot is read)
+      if (!early) refill();   // (the slot is read)
       __syncwarp();
       if (!AwaitCluster(&x.bars[turn], exchanged >> 1 & 1u)) {
         a.status->wait_timeout = 1;
@@ -595,7 +619,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
       mk = block_part.x;
       sum = block_part.y;
       join(4);
-    } else {
+    } else if (!early) {
       refill();
     }
     turn ^= 1;
@@ -620,31 +644,52 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
       asm volatile("" : "+r"(again));   // (the row's addresses anew: kept across the sums they cost registers that the units need)
       const Row<T> row(a, again);
       const uint32_t count = units_of(row.skip);
-      // Units that lie wholly in the row; then, their owners, the two that may not.
+      // Units that lie wholly in the row, then, by their owners, the two that may not.
       const uint32_t whole_first = begin == 0 && row.skip != 0 ? 1 : 0, whole_end = min(count, (row.skip + a.classes) / E - begin);   // (without units: 0)
-      const uint32_t whole = row.alike && whole_end > whole_first ? whole_end - whole_first : 0;
-      {
-        const f32x2 k2 = Splat2(a.k), away = Splat2(-q.mk), by = Splat2(each);
+      const uint32_t whole = whole_end > whole_first ? whole_end - whole_first : 0;
+      const f32x2 k2 = Splat2(a.k), away = Splat2(-q.mk), by = Splat2(each);
+      auto unit = [&](const uint4& r, float (&v)[E]) {
+        f32x2 pair[kPairs<T>];
+        Pairs<T>(r, pair);
+#pragma unroll
+        for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(Powers(Fma2(pair[j], k2, away)), by), &v[2 * j], &v[2 * j + 1]);
+      };
+      auto store_whole = [&] {
         uint4* to = reinterpret_cast<uint4*>(row.d - row.skip) + begin + t;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
           if (t + i * threads - whole_first < whole) {
             // (unpacked anew: values of the first time, kept, would be spilled)
             asm volatile("" : "+r"(raw[i].x), "+r"(raw[i].y), "+r"(raw[i].z), "+r"(raw[i].w));
-            f32x2 pair[kPairs<T>];
             float v[E];
-            Pairs<T>(raw[i], pair);
-#pragma unroll
-            for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(Powers(Fma2(pair[j], k2, away)), by), &v[2 * j], &v[2 * j + 1]);
+            unit(raw[i], v);
             if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
             else Store8<T>(reinterpret_cast<T*>(to), v);
           }
           to += threads;
         }
-      }
-      if (whole_first || whole + whole_first != count) {   // (from memory: of a matrix in place, these elements are still logits)
+      };
+      if (row.alike && whole == count) {
+        store_whole();
+      } else if (row.alike) {
+        float v[E];
+        if (whole_first && t == 0) {
+          unit(raw[0], v);
+          row.Store(begin, v);
+        }
+        if (whole + whole_first != count) {   // the last one sticks out too
+          uint4 last = raw[0];
+#pragma unroll
+          for (int i = 1; i < NU; ++i)
+            if (t + i * threads == count - 1) last = raw[i];
+          if (count - 1 - __umulhi(count - 1, plan.over_threads) * threads == t) {
+            unit(last, v);
+            row.Store(begin + count - 1, v);
+          }
+        }
+        store_whole();
+      } else {   // (from memory, element by element)
         for (uint32_t u = t; u < count; u += threads) {
-          if (u - whole_first < whole) continue;
           float v[E];
           row.Load(begin + u, v);
 #pragma unroll
@@ -832,8 +877,7 @@ bool ShareRows(const LogitArgs& a, uint32_t sms, Sharing* out) {
   const uint32_t all = (a.classes + 2 * (kPerUnit<T> - 1)) / kPerUnit<T>;   // units, wherever a row begins
   auto of = [all](uint32_t blocks) { return (all + blocks - 1) / blocks; };
   uint32_t blocks = 1;
-  const uint32_t lim = getenv("SEE_LIM") ? atoi(getenv("SEE_LIM")) : kThreads / 2;
-  while (blocks < 8 && of(blocks) > lim * kMostUnits) blocks *= 2;   // two rows to a block: one computes while the other's sums meet
+  while (blocks < 8 && of(blocks) > kThreads * kMostUnits) blocks *= 2;
   // Few rows are shared by more blocks, down to two kilobytes each.
   while (blocks < 8 && a.rows * blocks * 2 <= sms && all / blocks > 256) blocks *= 2;
   Sharing s;
@@ -849,9 +893,10 @@ bool ShareRows(const LogitArgs& a, uint32_t sms, Sharing* out) {
   s.threads = (((s.part + s.units - 1) / s.units) + 31) / 32 * 32;
   s.groups = kThreads / s.threads;
   if (blocks > 1 && s.groups > 2) s.groups = 2;
-  const uint64_t most = sms / blocks, each = (a.rows + most - 1) / most;
+  const uint32_t resident = BlocksOf(s.units);
+  const uint64_t most = resident * sms / blocks, each = (a.rows + most - 1) / most;
   if (s.groups > each) s.groups = static_cast<uint32_t>(each);
-  const size_t slot = static_cast<size_t>(s.part) * 16, budget = kMostShared - 2048;
+  const size_t slot = static_cast<size_t>(s.part) * 16, budget = (kMostShared - 4096) / resident;
   while (s.groups * (slot + 8) > budget) --s.groups;   // (a group's part is 128 KB at most)
   s.slots = static_cast<uint32_t>(budget / (s.groups * (slot + 8)));
   s.slots = s.slots > 8 ? 8 : s.slots;
@@ -869,7 +914,8 @@ bool ShareRows(const LogitArgs& a, uint32_t sms, Sharing* out) {
 }
 
 // How many clusters of `blocks` blocks of a kernel the device holds at a time: fewer than its SMs would make, for a cluster lies within
-// one of their groups.  A grid beyond that would leave whole rows to a second round.  Asked for once for each device and size.
+// one of their groups.  A grid beyond that would leave whole rows to a second round (132 SMs of 148 in clusters of four, 120 of eight).
+// Asked for once for each device and size, of blocks at their largest.
 template <auto kKernel>
 cudaError_t MostClusters(uint32_t blocks, uint32_t threads, size_t bytes, uint32_t* most) {
   static std::atomic<int> known[64][4] = {};   // by device, and blocks 2, 4, 8
@@ -899,10 +945,10 @@ cudaError_t MostClusters(uint32_t blocks, uint32_t threads, size_t bytes, uint32
 template <typename T, int NU, bool kPolicy, bool kCluster>
 cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, uint32_t* arrived, Sharing& w, cudaStream_t s) {
   constexpr auto* kernel = LogitRowsKernel<T, NU, kPolicy, kCluster>;
-  if (cudaError_t e = AllowShared<kernel>(kCluster ? kMostShared - 2048 : w.bytes); e != cudaSuccess) return e;
+  if (cudaError_t e = AllowShared<kernel>(kCluster ? kMostShared - 4096 : w.bytes); e != cudaSuccess) return e;
   if constexpr (kCluster) {
     uint32_t most;
-    if (cudaError_t e = MostClusters<kernel>(w.blocks, w.groups * w.threads, kMostShared - 2048, &most); e != cudaSuccess) return e;
+    if (cudaError_t e = MostClusters<kernel>(w.blocks, kThreads, (kMostShared - 4096) / BlocksOf(NU), &most); e != cudaSuccess) return e;
     if (w.clusters > most) w.clusters = most;
   }
   return Next(kernel, w.clusters * w.blocks, w.groups * w.threads, w.bytes, s, w.blocks)(
