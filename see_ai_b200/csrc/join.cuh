@@ -4,11 +4,55 @@
 
 #include <initializer_list>
 
+#include <type_traits>
+
+#include "act_expr.cuh"
 #include "block_ops.h"
 #include "launch.cuh"
 #include "row_groups.cuh"
 
 namespace see::k {
+
+// A thread's columns of one access: four as two pairs for the packed f32 instructions, or one as it is.
+template <int VEC> using Lane = std::conditional_t<VEC == 1, float, f32x2>;
+template <int VEC> constexpr int kLanes = VEC == 1 ? 1 : VEC / 2;
+template <typename P> __device__ __forceinline__ P SplatOf(float v);
+template <> __device__ __forceinline__ float SplatOf<float>(float v) { return v; }
+template <> __device__ __forceinline__ f32x2 SplatOf<f32x2>(float v) { return Splat2(v); }
+__device__ __forceinline__ float Add(float a, float b) { return a + b; }
+__device__ __forceinline__ f32x2 Add(f32x2 a, f32x2 b) { return AddF2(a, b); }
+__device__ __forceinline__ float Mul(float a, float b) { return a * b; }
+__device__ __forceinline__ f32x2 Mul(f32x2 a, f32x2 b) { return Mul2(a, b); }
+__device__ __forceinline__ float Fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ f32x2 Fma(f32x2 a, f32x2 b, f32x2 c) { return Fma2(a, b, c); }
+__device__ __forceinline__ float Total(float a) { return a; }
+__device__ __forceinline__ float Total(f32x2 a) {
+  float lo, hi;
+  UnpackF2(a, &lo, &hi);
+  return lo + hi;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void LoadLanes(const T* p, Lane<VEC> (&v)[kLanes<VEC>]) {
+  float f[VEC];
+  LoadCols<T, VEC>(p, f);
+  if constexpr (VEC == 1) {
+    v[0] = f[0];
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) v[j] = PackF2(f[2 * j], f[2 * j + 1]);
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void StoreLanes(T* p, const Lane<VEC> (&v)[kLanes<VEC>]) {
+  float f[VEC];
+  if constexpr (VEC == 1) {
+    f[0] = v[0];
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) UnpackF2(v[j], &f[2 * j], &f[2 * j + 1]);
+  }
+  StoreCols<T, VEC>(p, f);
+}
 
 // How many rows at either end of the matrices are not copied in bulk: rows whose 16-byte surroundings may lie outside.
 inline uint32_t JoinEdge(const JoinArgs& a, std::initializer_list<const void*> x_like, std::initializer_list<const void*> y_like) {

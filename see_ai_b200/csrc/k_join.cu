@@ -187,40 +187,39 @@ JoinBwdKernel(const __grid_constant__ JoinArgs a) {
   }
 }
 
-// The blocks' partial sums of 32 columns: warp w adds rows w, w + 32, ...; then the warps' sums in order; then the weights' gradients.
+// The blocks' partial sums of 32 columns, blockIdx.y 0: P1 and P2, 1: S1 and S2.  Half of the warps add a sum's rows w, w + 16, ... (rms: all of them, w + 32); then
+// the warps' sums in order; then the weights' gradients.
 __global__ void __launch_bounds__(1024)
 JoinFoldKernel(const __grid_constant__ JoinArgs a, uint32_t blocks, int rms) {
   AwaitPrevious();
   __shared__ float meet[32][33];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, col = blockIdx.x * 32 + warp;
-  float sums[4];
+  const uint32_t second = rms ? 0 : warp >> 4, way = rms ? warp : warp & 15, ways = rms ? 32 : 16;
+  const float* p = a.partials + static_cast<size_t>(2 * blockIdx.y + second) * blocks * a.cols;
+  float s = 0.0f;
+  if (c < a.cols)
+#pragma unroll 8
+    for (uint32_t r = way; r < blocks; r += ways) s += p[static_cast<size_t>(r) * a.cols + c];
+  meet[warp][lane] = s;
+  __syncthreads();
+  // Column `warp` of the block's 32, one warp's sum a lane: the first sum's in the lower lanes, the second's in the upper ones.
+  s = meet[lane][warp];
 #pragma unroll
-  for (int which = 0; which < 4; ++which) {
-    sums[which] = 0.0f;
-    if (rms && (which & 1)) continue;
-    const float* p = a.partials + static_cast<size_t>(which) * blocks * a.cols;
-    float s = 0.0f;
-    if (c < a.cols)
-#pragma unroll 4
-      for (uint32_t r = warp; r < blocks; r += 32) s += p[static_cast<size_t>(r) * a.cols + c];
-    __syncthreads();
-    meet[warp][lane] = s;
-    __syncthreads();
-    s = meet[lane][warp];   // column `warp` of the block's 32, one warp's sum a lane
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    sums[which] = s;
-  }
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  const float upper = __shfl_sync(0xFFFFFFFFu, s, 16), first = rms ? s + upper : s;
   if (lane != 0 || col >= a.cols) return;
+  if (blockIdx.y == 0) {
+    a.grads.pre_gamma[col] = first;
+    if (!rms) a.grads.pre_beta[col] = upper;
+    return;
+  }
   const bool post = a.w.post_gamma != nullptr;
   const float gate = a.w.gate ? a.w.gate[col] : 1.0f;
-  a.grads.pre_gamma[col] = sums[0];
-  if (!rms) a.grads.pre_beta[col] = sums[1];
   if (post) {
-    a.grads.post_gamma[col] = gate * sums[2];
-    if (!rms) a.grads.post_beta[col] = gate * sums[3];
+    a.grads.post_gamma[col] = gate * first;
+    if (!rms) a.grads.post_beta[col] = gate * upper;
   }
-  if (a.w.gate) a.grads.gate[col] = !post ? sums[2] : a.w.post_gamma[col] * sums[2] + (rms ? 0.0f : a.w.post_beta[col] * sums[3]);
+  if (a.w.gate) a.grads.gate[col] = !post ? first : a.w.post_gamma[col] * first + (rms ? 0.0f : a.w.post_beta[col] * upper);
 }
 
 // Rows of more columns than the ring kernels take.
@@ -257,7 +256,7 @@ cudaError_t Join(const JoinArgs& a, bool backward, uint32_t sms, cudaStream_t s,
   ++*launches;
   if (!backward) return cudaSuccess;
   ++*launches;
-  return Next(JoinFoldKernel, (a.cols + 31) / 32, 1024, 0, s)(a, grid, a.rms ? 1 : 0);
+  return Next(JoinFoldKernel, dim3((a.cols + 31) / 32, a.w.post_gamma || a.w.gate ? 2 : 1), 1024, 0, s)(a, grid, a.rms ? 1 : 0);
 }
 
 }  // namespace see::k

@@ -12,6 +12,8 @@ namespace {
 template <typename XT, typename YT, bool kRms, int VEC, int NV, uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads, 1)
 JoinBwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots, uint32_t edge) {
+  using P = Lane<VEC>;
+  constexpr int L = kLanes<VEC>;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ __align__(8) float2 sums[2][kWideThreads / 32];
   const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
@@ -50,13 +52,13 @@ JoinBwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
   __syncthreads();
   const float per_col = 1.0f / static_cast<float>(a.cols);
   // (sums: P1, S1 and, layer, P2, S2)
-  float p1[NV][VEC], s1[NV][VEC], p2[kRms ? 1 : NV][VEC], s2[kRms ? 1 : NV][VEC];
+  P p1[NV][L], s1[NV][L], p2[kRms ? 1 : NV][L], s2[kRms ? 1 : NV][L];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      p1[i][j] = s1[i][j] = 0.0f;
-      if (!kRms) p2[i][j] = s2[i][j] = 0.0f;
+    for (int j = 0; j < L; ++j) {
+      p1[i][j] = s1[i][j] = SplatOf<P>(0.0f);
+      if (!kRms) p2[i][j] = s2[i][j] = SplatOf<P>(0.0f);
     }
   uint32_t turn = 0, slot = 0, parities = 0;   // a bit for each slot, of the copies that went through it
   float2 next2 = make_float2(0.0f, 0.0f), next1 = make_float2(0.0f, 1.0f);   // statistics, asked for a row ahead
@@ -86,64 +88,64 @@ JoinBwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
     const YT* b = reinterpret_cast<const YT*>(at + y_slot + OddRow<YT>(a.block, row, a.y_stride, a.cols).skip);
     const XT* x = reinterpret_cast<const XT*>(at + 2 * y_slot + OddRow<XT>(a.x, row, a.x_stride, a.cols).skip);
     const XT* more = reinterpret_cast<const XT*>(at + 2 * y_slot + x_slot + OddRow<XT>(a.dx_out, row, a.x_stride, a.cols).skip);
-    float d[NV][VEC], u[NV][VEC];
-    float2 sum = make_float2(0.0f, 0.0f);
+    P d[NV][L], u[NV][L], with_u = SplatOf<P>(0.0f), plain = with_u;
+    const P rstd2 = SplatOf<P>(two.y), away2 = SplatOf<P>(-two.x), rstd1 = SplatOf<P>(one.y), away1 = SplatOf<P>(-one.x), scale = SplatOf<P>(a.scale);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * T) * VEC;
       if (c < a.cols) {
-        float g[VEC];
-        LoadCols<float, VEC>(weights + c, g);
-        LoadCols<YT, VEC>(dy + c, d[i]);
-        LoadCols<XT, VEC>(x + c, u[i]);
+        P g[L];
+        LoadLanes<float, VEC>(weights + c, g);
+        LoadLanes<YT, VEC>(dy + c, d[i]);
+        LoadLanes<XT, VEC>(x + c, u[i]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          u[i][j] = (kRms ? u[i][j] : u[i][j] - two.x) * two.y;
-          p1[i][j] = fmaf(d[i][j], u[i][j], p1[i][j]);
-          if (!kRms) p2[i][j] += d[i][j];
-          d[i][j] *= g[j];
-          sum.x = fmaf(d[i][j], u[i][j], sum.x);
-          if (!kRms) sum.y += d[i][j];
+        for (int j = 0; j < L; ++j) {
+          u[i][j] = Mul(kRms ? u[i][j] : Add(u[i][j], away2), rstd2);
+          p1[i][j] = Fma(d[i][j], u[i][j], p1[i][j]);
+          if (!kRms) p2[i][j] = Add(p2[i][j], d[i][j]);
+          d[i][j] = Mul(d[i][j], g[j]);
+          with_u = Fma(d[i][j], u[i][j], with_u);
+          if (!kRms) plain = Add(plain, d[i][j]);
         }
       }
     }
-    sum = GroupSum<!kRms>(sum, T, group, sums, turn);
-    float pull = sum.x * per_col, shift = sum.y * per_col;
-    sum = make_float2(0.0f, 0.0f);
+    float2 sum = GroupSum<!kRms>(make_float2(Total(with_u), kRms ? 0.0f : Total(plain)), T, group, sums, turn);
+    P pull = SplatOf<P>(-sum.x * per_col), shift = SplatOf<P>(-sum.y * per_col);
+    with_u = plain = SplatOf<P>(0.0f);
     XT* dx = static_cast<XT*>(a.dx) + row * a.x_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * T) * VEC;
       if (c < a.cols) {
-        float w[VEC], r[VEC];
+        P w[L], r[L];
         if (a.dx_out) {
-          LoadCols<XT, VEC>(more + c, r);
+          LoadLanes<XT, VEC>(more + c, r);
         } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) r[j] = 0.0f;
+          for (int j = 0; j < L; ++j) r[j] = SplatOf<P>(0.0f);
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) d[i][j] = fmaf(kRms ? fmaf(-u[i][j], pull, d[i][j]) : fmaf(-u[i][j], pull, d[i][j] - shift), two.y, r[j]);
-        LoadCols<YT, VEC>(b + c, u[i]);
-        LoadCols<float, VEC>(weights + pitch + c, w);
+        for (int j = 0; j < L; ++j) d[i][j] = Fma(Fma(u[i][j], pull, kRms ? d[i][j] : Add(d[i][j], shift)), rstd2, r[j]);
+        LoadLanes<YT, VEC>(b + c, u[i]);
+        LoadLanes<float, VEC>(weights + pitch + c, w);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          r[j] = a.scale * d[i][j];
-          u[i][j] = (kRms ? u[i][j] : u[i][j] - one.x) * one.y;
-          s1[i][j] = fmaf(d[i][j], u[i][j], s1[i][j]);
-          if (!kRms) s2[i][j] += d[i][j];
-          d[i][j] *= w[j];
-          sum.x = fmaf(d[i][j], u[i][j], sum.x);
-          if (!kRms) sum.y += d[i][j];
+        for (int j = 0; j < L; ++j) {
+          r[j] = Mul(scale, d[i][j]);
+          u[i][j] = Mul(kRms ? u[i][j] : Add(u[i][j], away1), rstd1);
+          s1[i][j] = Fma(d[i][j], u[i][j], s1[i][j]);
+          if (!kRms) s2[i][j] = Add(s2[i][j], d[i][j]);
+          d[i][j] = Mul(d[i][j], w[j]);
+          with_u = Fma(d[i][j], u[i][j], with_u);
+          if (!kRms) plain = Add(plain, d[i][j]);
         }
-        StoreCols<XT, VEC>(dx + c, r);
+        StoreLanes<XT, VEC>(dx + c, r);
       }
     }
-    pull = shift = 0.0f;
+    pull = shift = SplatOf<P>(0.0f);
     if (post) {
-      sum = GroupSum<!kRms>(sum, T, group, sums, turn);
-      pull = sum.x * per_col;
-      shift = sum.y * per_col;
+      sum = GroupSum<!kRms>(make_float2(Total(with_u), kRms ? 0.0f : Total(plain)), T, group, sums, turn);
+      pull = SplatOf<P>(-sum.x * per_col);
+      shift = SplatOf<P>(-sum.y * per_col);
     }
     if (!post || T == 32) GroupBarrier(T, group);   // the slot is read (a wider group has met at the sum's barrier)
     if (t == 0 && row + slots * step < a.rows) fill(row + slots * step, slot);
@@ -154,8 +156,8 @@ JoinBwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
       const uint32_t c = (t + i * T) * VEC;
       if (c < a.cols) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) d[i][j] = (kRms ? fmaf(-u[i][j], pull, d[i][j]) : fmaf(-u[i][j], pull, d[i][j] - shift)) * one.y;
-        StoreCols<YT, VEC>(db + c, d[i]);
+        for (int j = 0; j < L; ++j) d[i][j] = Mul(Fma(u[i][j], pull, kRms ? d[i][j] : Add(d[i][j], shift)), rstd1);
+        StoreLanes<YT, VEC>(db + c, d[i]);
       }
     }
   }
@@ -168,7 +170,7 @@ JoinBwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * T) * VEC;
       if (c < a.cols)
-        StoreCols<float, VEC>(meet + group * pitch + c, which == 0 ? p1[i] : which == 1 ? p2[kRms ? 0 : i] : which == 2 ? s1[i] : s2[kRms ? 0 : i]);
+        StoreLanes<float, VEC>(meet + group * pitch + c, which == 0 ? p1[i] : which == 1 ? p2[kRms ? 0 : i] : which == 2 ? s1[i] : s2[kRms ? 0 : i]);
     }
     __syncthreads();
     float* out = a.partials + (static_cast<size_t>(which) * gridDim.x + blockIdx.x) * a.cols;
@@ -196,7 +198,24 @@ cudaError_t Pick(const JoinArgs& a, uint32_t sms, cudaStream_t s, uint32_t* grid
   // Sixteen columns to a thread at most: the four sums of layer norms take 64 registers, and a row's values 32.
   constexpr uint32_t kThreads = kRms ? 512 : 384;
   if (JoinFours(a, {a.x, a.dx_out, a.dx}, {a.dy, a.block, a.dblock})) {
-    const uint32_t n = a.cols / 4, T = Warps((n + 3) / 4), each = (n + T - 1) / T;
+    const uint32_t n = a.cols / 4;
+    // Layer norms of wide rows: eight or twelve columns a thread (16384 x 4096 bf16 253 us, with sixteen, which spill, 304).
+    if (!kRms && n > 768) {
+      if (n <= 1024) return Run<XT, YT, kRms, 4, 2, 512>(a, Warps((n + 1) / 2), sms, s, grid);
+      if (n <= 1536) return Run<XT, YT, kRms, 4, 3, 512>(a, Warps((n + 2) / 3), sms, s, grid);
+    }
+    if (a.rows <= sms) {   // a row to an SM: over as many threads as it has work for
+      const uint32_t T = n < kThreads ? Warps(n) : kThreads;
+      if (n <= T) return Run<XT, YT, kRms, 4, 1, kThreads>(a, T, sms, s, grid);
+      if (n <= 2 * T) return Run<XT, YT, kRms, 4, 2, kThreads>(a, T, sms, s, grid);
+    }
+    // Rms norms: a warp's row, which needs no barriers, of up to 768 columns of 16 bits (32768 rows 58 us, on 64 threads 72; an f32 stream's rows leave the
+    // ring too few of them: 88, 83); two groups of rows of up to 5120 columns.
+    if constexpr (kRms && sizeof(XT) == 2)
+      if (n > 128 && n <= 192) return Run<XT, YT, kRms, 4, 6, 384>(a, 32, sms, s, grid);
+    if constexpr (kRms)
+      if (n > 1024 && n <= 1280) return Run<XT, YT, kRms, 4, 5, 512>(a, 256, sms, s, grid);
+    const uint32_t T = Warps((n + 3) / 4), each = (n + T - 1) / T;
     if (each <= 1) return Run<XT, YT, kRms, 4, 1, kThreads>(a, T, sms, s, grid);
     if (each <= 2) return Run<XT, YT, kRms, 4, 2, kThreads>(a, T, sms, s, grid);
     if (each <= 3) return Run<XT, YT, kRms, 4, 3, kThreads>(a, T, sms, s, grid);
@@ -205,6 +224,7 @@ cudaError_t Pick(const JoinArgs& a, uint32_t sms, cudaStream_t s, uint32_t* grid
   const uint32_t T = Warps((a.cols + 15) / 16), each = (a.cols + T - 1) / T;
   if (each <= 4) return Run<XT, YT, kRms, 1, 4, kThreads>(a, T, sms, s, grid);
   if (each <= 8) return Run<XT, YT, kRms, 1, 8, kThreads>(a, T, sms, s, grid);
+  if (each <= 12 && T <= 384) return Run<XT, YT, kRms, 1, 12, kThreads>(a, T, sms, s, grid);
   return T <= 192 ? Run<XT, YT, kRms, 1, 16, kThreads>(a, T, sms, s, grid) : Run<XT, YT, kRms, 1, 16, 512>(a, T, sms, s, grid);
 }
 template <typename XT, typename YT>

@@ -9,42 +9,44 @@ namespace see::k {
 
 namespace {
 
-constexpr uint32_t kThreads = 512;
 
-// The statistics of a group's row in v, of which `there` says which columns a thread has.
+// The statistics of a group's row in v, of which a thread has the columns (t + i T) VEC below cols, and zeros beyond.
 template <bool kRms, int VEC, int NV>
-__device__ __forceinline__ float2 StatsOf(const float (&v)[NV][VEC], uint32_t t, uint32_t T, uint32_t group, uint32_t cols, float eps, float per_col,
-                                          float2 (*sums)[kWideThreads / 32], uint32_t& turn) {
-  float total = 0.0f;
+__device__ __forceinline__ float2 StatsOf(const Lane<VEC> (&v)[NV][kLanes<VEC>], uint32_t t, uint32_t T, uint32_t group, uint32_t cols, float eps,
+                                          float per_col, float2 (*sums)[kWideThreads / 32], uint32_t& turn) {
+  using P = Lane<VEC>;
+  P total = SplatOf<P>(0.0f);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) total = kRms ? fmaf(v[i][j], v[i][j], total) : total + v[i][j];   // (zeros beyond the row)
+    for (int j = 0; j < kLanes<VEC>; ++j) total = kRms ? Fma(v[i][j], v[i][j], total) : Add(total, v[i][j]);
+  const float sum = GroupSum<false>(make_float2(Total(total), 0.0f), T, group, sums, turn).x * per_col;
   if constexpr (kRms) {
-    return make_float2(0.0f, 1.0f / sqrtf(GroupSum<false>(make_float2(total, 0.0f), T, group, sums, turn).x * per_col + eps));
+    return make_float2(0.0f, 1.0f / sqrtf(sum + eps));
   } else {
-    float mean = static_cast<float>(GroupSum(static_cast<double>(total), T, group, sums, turn) / static_cast<double>(cols));
-    float2 s = make_float2(0.0f, 0.0f);
+    const P away = SplatOf<P>(-sum);
+    P first = SplatOf<P>(0.0f), second = first;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((t + i * T) * VEC < cols) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float d = v[i][j] - mean;
-          s.x += d;
-          s.y = fmaf(d, d, s.y);
+        for (int j = 0; j < kLanes<VEC>; ++j) {
+          const P d = Add(v[i][j], away);
+          first = Add(first, d);
+          second = Fma(d, d, second);
         }
       }
-    s = GroupSum<true>(s, T, group, sums, turn);
+    const float2 s = GroupSum<true>(make_float2(Total(first), Total(second)), T, group, sums, turn);
     const float off = s.x * per_col, var = Variance(s.y * per_col, off);
-    if (isfinite(off)) mean += off;
-    return make_float2(mean, 1.0f / sqrtf(var + eps));
+    return make_float2(isfinite(off) ? sum + off : sum, 1.0f / sqrtf(var + eps));
   }
 }
 
-template <typename XT, typename YT, bool kRms, int VEC, int NV>
+template <typename XT, typename YT, bool kRms, int VEC, int NV, uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads, 1)
 JoinFwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots, uint32_t edge) {
+  using P = Lane<VEC>;
+  constexpr int L = kLanes<VEC>;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ __align__(8) float2 sums[2][kWideThreads / 32];
   const uint32_t groups = blockDim.x / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
@@ -96,54 +98,56 @@ JoinFwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
     }
     const XT* x = reinterpret_cast<const XT*>(at + OddRow<XT>(a.x, row, a.x_stride, a.cols).skip);
     const YT* b = reinterpret_cast<const YT*>(at + x_slot + OddRow<YT>(a.block, row, a.y_stride, a.cols).skip);
-    float v[NV][VEC];
+    P v[NV][L];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * T) * VEC;
       if (c < a.cols) {
-        LoadCols<YT, VEC>(b + c, v[i]);
+        LoadLanes<YT, VEC>(b + c, v[i]);
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
+        for (int j = 0; j < L; ++j) v[i][j] = SplatOf<P>(0.0f);
       }
     }
     float2 one = make_float2(0.0f, 1.0f);
     if (post) one = StatsOf<kRms, VEC, NV>(v, t, T, group, a.cols, a.eps, per_col, sums, turn);
     XT* x_out = static_cast<XT*>(a.x_out) + row * a.x_stride;
+    const P scale = SplatOf<P>(a.scale), rstd1 = SplatOf<P>(one.y), away1 = SplatOf<P>(-one.x);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * T) * VEC;
       if (c < a.cols) {
-        float w[VEC], beta[VEC], r[VEC];
-        LoadCols<float, VEC>(weights + c, w);
-        if (!kRms) LoadCols<float, VEC>(weights + 2 * pitch + c, beta);
-        LoadCols<XT, VEC>(x + c, r);
+        P w[L], beta[L], r[L];
+        LoadLanes<float, VEC>(weights + c, w);
+        if (!kRms) LoadLanes<float, VEC>(weights + 2 * pitch + c, beta);
+        LoadLanes<XT, VEC>(x + c, r);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float unit = kRms ? v[i][j] * one.y : (v[i][j] - one.x) * one.y;
-          v[i][j] = fmaf(a.scale, r[j], kRms ? unit * w[j] : fmaf(unit, w[j], beta[j]));
+        for (int j = 0; j < L; ++j) {
+          const P unit = Mul(kRms ? v[i][j] : Add(v[i][j], away1), rstd1);
+          v[i][j] = Fma(scale, r[j], kRms ? Mul(unit, w[j]) : Fma(unit, w[j], beta[j]));
         }
-        StoreCols<XT, VEC>(x_out + c, v[i]);
+        StoreLanes<XT, VEC>(x_out + c, v[i]);
       }
     }
     GroupBarrier(T, group);   // the slot is read
     if (t == 0 && row + slots * step < a.rows) fill(row + slots * step, slot);
     if (++slot == slots) slot = 0;
     const float2 two = StatsOf<kRms, VEC, NV>(v, t, T, group, a.cols, a.eps, per_col, sums, turn);
+    const P rstd2 = SplatOf<P>(two.y), away2 = SplatOf<P>(-two.x);
     YT* y = static_cast<YT*>(a.y) + row * a.y_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * T) * VEC;
       if (c < a.cols) {
-        float w[VEC], beta[VEC];
-        LoadCols<float, VEC>(weights + pitch + c, w);
-        if (!kRms) LoadCols<float, VEC>(weights + 3 * pitch + c, beta);
+        P w[L], beta[L];
+        LoadLanes<float, VEC>(weights + pitch + c, w);
+        if (!kRms) LoadLanes<float, VEC>(weights + 3 * pitch + c, beta);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float unit = kRms ? v[i][j] * two.y : (v[i][j] - two.x) * two.y;
-          w[j] = kRms ? unit * w[j] : fmaf(unit, w[j], beta[j]);
+        for (int j = 0; j < L; ++j) {
+          const P unit = Mul(kRms ? v[i][j] : Add(v[i][j], away2), rstd2);
+          w[j] = kRms ? Mul(unit, w[j]) : Fma(unit, w[j], beta[j]);
         }
-        StoreCols<YT, VEC>(y + c, w);
+        StoreLanes<YT, VEC>(y + c, w);
       }
     }
     if (t == 0) {
@@ -157,11 +161,11 @@ JoinFwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
   }
 }
 
-template <typename XT, typename YT, bool kRms, int VEC, int NV>
+template <typename XT, typename YT, bool kRms, int VEC, int NV, uint32_t kThreads>
 cudaError_t Run(const JoinArgs& a, uint32_t T, uint32_t sms, cudaStream_t s) {
   const size_t weights = static_cast<size_t>((a.cols + 3) & ~3u) * 4 * (kRms ? 2 : 4);
   const JoinRing r = RingOf(a.rows, kThreads, T, OddSlot<XT>(a.cols) + OddSlot<YT>(a.cols), weights, sms);
-  constexpr auto* kernel = JoinFwdRingKernel<XT, YT, kRms, VEC, NV>;
+  constexpr auto* kernel = JoinFwdRingKernel<XT, YT, kRms, VEC, NV, kThreads>;
   if (cudaError_t e = AllowShared<kernel>(r.bytes); e != cudaSuccess) return e;
   return Next(kernel, r.grid, r.groups * T, r.bytes, s)(a, T, r.slots, JoinEdge(a, {a.x}, {a.block}));
 }
@@ -169,14 +173,21 @@ cudaError_t Run(const JoinArgs& a, uint32_t T, uint32_t sms, cudaStream_t s) {
 template <typename XT, typename YT, bool kRms>
 cudaError_t Pick(const JoinArgs& a, uint32_t sms, cudaStream_t s) {
   if (JoinFours(a, {a.x, a.x_out}, {a.block, a.y})) {
-    const uint32_t n = a.cols / 4, T = Warps((n + 7) / 8), each = (n + T - 1) / T;
-    if (each <= 2) return Run<XT, YT, kRms, 4, 2>(a, T, sms, s);
-    if (each <= 4) return Run<XT, YT, kRms, 4, 4>(a, T, sms, s);
-    return each <= 6 ? Run<XT, YT, kRms, 4, 6>(a, T, sms, s) : Run<XT, YT, kRms, 4, 8>(a, T, sms, s);
+    const uint32_t n = a.cols / 4;
+    if (a.rows <= sms) {   // a row to an SM: over as many threads as it has work for
+      const uint32_t T = n < 512 ? Warps(n) : 512;
+      if (n <= T) return Run<XT, YT, kRms, 4, 1, 512>(a, T, sms, s);
+      return n <= 2 * T ? Run<XT, YT, kRms, 4, 2, 512>(a, T, sms, s) : Run<XT, YT, kRms, 4, 4, 512>(a, T, sms, s);
+    }
+    const uint32_t T = Warps((n + 7) / 8), each = (n + T - 1) / T;
+    if (each <= 2) return Run<XT, YT, kRms, 4, 2, 512>(a, T, sms, s);
+    if (each <= 4) return Run<XT, YT, kRms, 4, 4, 512>(a, T, sms, s);
+    return each <= 6 ? Run<XT, YT, kRms, 4, 6, 512>(a, T, sms, s) : Run<XT, YT, kRms, 4, 8, 512>(a, T, sms, s);
   }
   const uint32_t T = Warps((a.cols + 15) / 16), each = (a.cols + T - 1) / T;
-  if (each <= 4) return Run<XT, YT, kRms, 1, 4>(a, T, sms, s);
-  return each <= 8 ? Run<XT, YT, kRms, 1, 8>(a, T, sms, s) : Run<XT, YT, kRms, 1, 16>(a, T, sms, s);
+  if (each <= 4) return Run<XT, YT, kRms, 1, 4, 512>(a, T, sms, s);
+  if (each <= 8) return Run<XT, YT, kRms, 1, 8, 512>(a, T, sms, s);
+  return each <= 12 ? Run<XT, YT, kRms, 1, 12, 768>(a, T, sms, s) : Run<XT, YT, kRms, 1, 16, 768>(a, T, sms, s);
 }
 template <typename XT, typename YT>
 cudaError_t Pick(const JoinArgs& a, uint32_t sms, cudaStream_t s) {
