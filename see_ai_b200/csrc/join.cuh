@@ -54,27 +54,47 @@ __device__ __forceinline__ void StoreLanes(T* p, const Lane<VEC> (&v)[kLanes<VEC
   StoreCols<T, VEC>(p, f);
 }
 
-// How many rows at either end of the matrices are not copied in bulk: rows whose 16-byte surroundings may lie outside.
-inline uint32_t JoinEdge(const JoinArgs& a, std::initializer_list<const void*> x_like, std::initializer_list<const void*> y_like) {
-  const uint64_t xs = a.x_type == SEE_F32 ? 4 : 2, ys = a.y_type == SEE_F32 ? 4 : 2;
+// A row at an end of the matrix for the ring, without anything beside it: its 16-byte units are copied in bulk, the elements before and behind them (fewer than 16 bytes each) by the
+// group's threads.  The row begins `skip` bytes into its slot.
+template <typename T>
+struct EndRow {
+  const uint8_t* from;         // the units
+  uint32_t skip, to, bytes;    // bytes into the slot; ... of the units
+  uint32_t head, tail;         // elements before the units; the first one behind them
+  __device__ __forceinline__ EndRow(const void* base, uint64_t row, uint64_t stride, uint32_t cols) {
+    const uint64_t at = reinterpret_cast<uint64_t>(static_cast<const T*>(base) + row * stride), end = at + cols * sizeof(T);
+    const uint64_t first = (at + 15) & ~15ull, last = end & ~15ull;
+    skip = static_cast<uint32_t>(at & 15);
+    from = reinterpret_cast<const uint8_t*>(first);
+    to = skip == 0 ? 0 : 16;
+    bytes = last > first ? static_cast<uint32_t>(last - first) : 0;
+    head = bytes ? static_cast<uint32_t>(first - at) / sizeof(T) : cols;
+    tail = bytes ? static_cast<uint32_t>(last - at) / sizeof(T) : cols;
+  }
+};
+// The elements beside the units; the caller synchronises.
+template <typename T>
+__device__ __forceinline__ void CopyEnds(uint8_t* slot, const void* base, uint64_t row, uint64_t stride, uint32_t cols, uint32_t t, uint32_t threads) {
+  const EndRow<T> r(base, row, stride, cols);
+  const T* from = static_cast<const T*>(base) + row * stride;
+  T* to = reinterpret_cast<T*>(slot + r.skip);
+  for (uint32_t c = t; c < r.head; c += threads) to[c] = from[c];
+  for (uint32_t c = r.tail + t; c < cols; c += threads) to[c] = from[c];
+}
+
+// Rows that begin and end on 16 bytes in every matrix: four columns at a time, and nothing beside them.
+inline bool JoinFours(const JoinArgs& a, std::initializer_list<const void*> x_like, std::initializer_list<const void*> y_like) {
   auto exact = [&](std::initializer_list<const void*> list, uint64_t size, uint64_t stride) {
     for (const void* p : list)
-      if (p && (reinterpret_cast<uintptr_t>(p) & 15)) return false;
+      if (reinterpret_cast<uintptr_t>(p) & 15) return false;
     return (a.cols * size & 15) == 0 && (stride * size & 15) == 0;
   };
-  if (exact(x_like, xs, a.x_stride) && exact(y_like, ys, a.y_stride)) return 0;
-  const uint64_t narrow = a.x_stride * xs < a.y_stride * ys ? a.x_stride * xs : a.y_stride * ys;
-  return static_cast<uint32_t>((15 + narrow) / narrow);
+  return exact(x_like, a.x_type == SEE_F32 ? 4 : 2, a.x_stride) && exact(y_like, a.y_type == SEE_F32 ? 4 : 2, a.y_stride);
 }
-// Four columns at a time: addresses and strides allow it everywhere.
-inline bool JoinFours(const JoinArgs& a, std::initializer_list<const void*> x_like, std::initializer_list<const void*> y_like) {
-  auto aligned = [](std::initializer_list<const void*> list, uintptr_t by) {
-    for (const void* p : list)
-      if (reinterpret_cast<uintptr_t>(p) & (by - 1)) return false;
-    return true;
-  };
-  return a.cols % 4 == 0 && a.x_stride % 4 == 0 && a.y_stride % 4 == 0 && aligned(x_like, a.x_type == SEE_F32 ? 16 : 8) &&
-         aligned(y_like, a.y_type == SEE_F32 ? 16 : 8);
+// Of others: how many rows at either end of the matrices are not copied with what lies beside them, for that may lie outside.
+inline uint32_t JoinEdge(const JoinArgs& a) {
+  const uint64_t x = a.x_stride * (a.x_type == SEE_F32 ? 4 : 2), y = a.y_stride * (a.y_type == SEE_F32 ? 4 : 2), narrow = x < y ? x : y;
+  return static_cast<uint32_t>((15 + narrow) / narrow);
 }
 inline uint32_t Warps(uint32_t n) { return (n + 31) / 32 * 32; }
 

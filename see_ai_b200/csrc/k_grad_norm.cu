@@ -27,14 +27,14 @@ struct GradEntry {
 };
 struct GradTable {
   GradEntry entry[kEntries];
-  uint32_t count;
+  uint64_t each;          // units to a block,
+  uint32_t rest, count;   // and one more to the first `rest`; tensors
 };
 
 // Calls step(entry, first unit, units) for all of a block's range, or, of kBack, from its end on.
 template <bool kBack, typename F>
 __device__ __forceinline__ void Walk(const GradTable& t, F step) {
-  const uint64_t all = t.entry[t.count - 1].unit_end, each = all / gridDim.x, rest = all % gridDim.x;
-  const uint64_t b = kBack ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const uint64_t each = t.each, rest = t.rest, b = kBack ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
   const uint64_t begin = b * each + min(b, rest), end = begin + each + (b < rest);
   if (begin == end) return;
   uint32_t lo = 0, hi = t.count - 1;   // the tensor of the first unit, or the last
@@ -251,10 +251,13 @@ bool Fill(GradTable* table, const see_grad_tensor* tensors, uint64_t count, uint
   }
   return table->count != 0;
 }
-// Blocks: a unit to a thread at least.
-unsigned Grid(const GradTable& table, uint32_t sms) {
-  const uint64_t blocks = (table.entry[table.count - 1].unit_end + kThreads - 1) / kThreads, most = sms * kGradBlocks < kGradPartials ? sms * kGradBlocks : kGradPartials;
-  return static_cast<unsigned>(blocks < most ? blocks : most);
+// Blocks: four units to a thread at least.  Cuts the table's units into their ranges.
+unsigned Cut(GradTable& table, uint32_t sms) {
+  const uint64_t units = table.entry[table.count - 1].unit_end, blocks = (units + 4 * kThreads - 1) / (4 * kThreads);
+  const uint64_t most = sms * kGradBlocks < kGradPartials ? sms * kGradBlocks : kGradPartials, grid = blocks < most ? blocks : most;
+  table.each = units / grid;
+  table.rest = static_cast<uint32_t>(units % grid);
+  return static_cast<unsigned>(grid);
 }
 
 }  // namespace
@@ -265,7 +268,7 @@ cudaError_t GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, 
   uint64_t next = 0;
   unsigned used = 0;   // partial sums
   while (Fill(&table, tensors, count, &next)) {
-    const unsigned grid = Grid(table, sms);
+    const unsigned grid = Cut(table, sms);
     // (blocks that an earlier launch had are added to; those that it had not are new)
     if (used != 0 && grid > used) {
       if (cudaError_t e = cudaMemsetAsync(partials + used, 0, (grid - used) * sizeof(double), s); e != cudaSuccess) return e;
@@ -280,7 +283,8 @@ cudaError_t GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, 
   }
   next = 0;
   while (Fill(&table, tensors, count, &next)) {
-    if (cudaError_t e = Next(GradScaleKernel, Grid(table, sms), kThreads, 0, s)(table, static_cast<const double*>(partials), used, max_norm, grad_scale,
+    const unsigned grid = Cut(table, sms);
+    if (cudaError_t e = Next(GradScaleKernel, grid, kThreads, 0, s)(table, static_cast<const double*>(partials), used, max_norm, grad_scale,
                                                                                  norm, factor);
         e != cudaSuccess)
       return e;

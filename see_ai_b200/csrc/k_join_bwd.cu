@@ -27,18 +27,24 @@ JoinBwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
     for (uint32_t i = 0; i < slots; ++i) umma_dev::MbarInit(&bars[i], 1);
     umma_dev::MbarInitFence();
   }
-  auto inner = [&](uint64_t row) { return row >= edge && row + edge < a.rows; };
+  auto inner = [&](uint64_t row) { return VEC == 4 || (row >= edge && row + edge < a.rows); };
+  auto copy = [&](auto x, auto more, auto dy, auto b, uint8_t* dst, uint64_t* bar, uint32_t x_to, uint32_t more_to, uint32_t dy_to, uint32_t b_to) {
+    umma_dev::MbarExpectTx(bar, x.bytes + dy.bytes + b.bytes + (a.dx_out ? more.bytes : 0));
+    if (dy.bytes) umma_dev::BulkLoad(dst + dy_to, dy.from, dy.bytes, bar);
+    if (x.bytes) umma_dev::BulkLoad(dst + 2 * y_slot + x_to, x.from, x.bytes, bar);
+    if (b.bytes) umma_dev::BulkLoad(dst + y_slot + b_to, b.from, b.bytes, bar);
+    if (a.dx_out && more.bytes) umma_dev::BulkLoad(dst + 2 * y_slot + x_slot + more_to, more.from, more.bytes, bar);
+  };
   auto fill = [&](uint64_t row, uint32_t slot) {   // the group's thread 0
-    if (!inner(row)) return;
-    umma_dev::FenceProxyAsync();   // (an edge row's elements may have been written there)
     uint8_t* dst = ring + static_cast<size_t>(slot) * slot_bytes;
-    const OddRow<XT> x(a.x, row, a.x_stride, a.cols), more(a.dx_out, row, a.x_stride, a.cols);
-    const OddRow<YT> dy(a.dy, row, a.y_stride, a.cols), b(a.block, row, a.y_stride, a.cols);
-    umma_dev::MbarExpectTx(&bars[slot], x.bytes + dy.bytes + b.bytes + (a.dx_out ? more.bytes : 0));
-    umma_dev::BulkLoad(dst, dy.from, dy.bytes, &bars[slot]);
-    umma_dev::BulkLoad(dst + 2 * y_slot, x.from, x.bytes, &bars[slot]);
-    umma_dev::BulkLoad(dst + y_slot, b.from, b.bytes, &bars[slot]);
-    if (a.dx_out) umma_dev::BulkLoad(dst + 2 * y_slot + x_slot, more.from, more.bytes, &bars[slot]);
+    if (inner(row)) {
+      copy(OddRow<XT>(a.x, row, a.x_stride, a.cols), OddRow<XT>(a.dx_out, row, a.x_stride, a.cols), OddRow<YT>(a.dy, row, a.y_stride, a.cols),
+           OddRow<YT>(a.block, row, a.y_stride, a.cols), dst, &bars[slot], 0, 0, 0, 0);
+    } else {
+      const EndRow<XT> x(a.x, row, a.x_stride, a.cols), more(a.dx_out, row, a.x_stride, a.cols);
+      const EndRow<YT> dy(a.dy, row, a.y_stride, a.cols), b(a.block, row, a.y_stride, a.cols);
+      copy(x, more, dy, b, dst, &bars[slot], x.to, more.to, dy.to, b.to);
+    }
   };
   AwaitPrevious();
   if (t == 0)
@@ -74,20 +80,22 @@ JoinBwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
     const float2 two = next2, one = next1;
     if (row + step < a.rows) ask(row + step);
     uint8_t* at = ring + static_cast<size_t>(slot) * slot_bytes;
-    if (inner(row)) {
-      AwaitRow(&bars[slot], parities >> slot & 1u, a.status);
-      parities ^= 1u << slot;
-    } else {
-      CopyRow<YT>(at, a.dy, row, a.y_stride, a.cols, t, T);
-      CopyRow<YT>(at + y_slot, a.block, row, a.y_stride, a.cols, t, T);
-      CopyRow<XT>(at + 2 * y_slot, a.x, row, a.x_stride, a.cols, t, T);
-      if (a.dx_out) CopyRow<XT>(at + 2 * y_slot + x_slot, a.dx_out, row, a.x_stride, a.cols, t, T);
+    if (!inner(row)) {
+      CopyEnds<YT>(at, a.dy, row, a.y_stride, a.cols, t, T);
+      CopyEnds<YT>(at + y_slot, a.block, row, a.y_stride, a.cols, t, T);
+      CopyEnds<XT>(at + 2 * y_slot, a.x, row, a.x_stride, a.cols, t, T);
+      if (a.dx_out) CopyEnds<XT>(at + 2 * y_slot + x_slot, a.dx_out, row, a.x_stride, a.cols, t, T);
+      umma_dev::FenceProxyAsync();   // (the slot is filled in bulk again)
       GroupBarrier(T, group);
     }
-    const YT* dy = reinterpret_cast<const YT*>(at + OddRow<YT>(a.dy, row, a.y_stride, a.cols).skip);
-    const YT* b = reinterpret_cast<const YT*>(at + y_slot + OddRow<YT>(a.block, row, a.y_stride, a.cols).skip);
-    const XT* x = reinterpret_cast<const XT*>(at + 2 * y_slot + OddRow<XT>(a.x, row, a.x_stride, a.cols).skip);
-    const XT* more = reinterpret_cast<const XT*>(at + 2 * y_slot + x_slot + OddRow<XT>(a.dx_out, row, a.x_stride, a.cols).skip);
+    AwaitRow(&bars[slot], parities >> slot & 1u, a.status);
+    parities ^= 1u << slot;
+    auto x_skip = [&](const void* p) { return VEC == 4 ? 0 : reinterpret_cast<uint64_t>(static_cast<const XT*>(p) + row * a.x_stride) & 15; };
+    auto y_skip = [&](const void* p) { return VEC == 4 ? 0 : reinterpret_cast<uint64_t>(static_cast<const YT*>(p) + row * a.y_stride) & 15; };
+    const YT* dy = reinterpret_cast<const YT*>(at + y_skip(a.dy));
+    const YT* b = reinterpret_cast<const YT*>(at + y_slot + y_skip(a.block));
+    const XT* x = reinterpret_cast<const XT*>(at + 2 * y_slot + x_skip(a.x));
+    const XT* more = reinterpret_cast<const XT*>(at + 2 * y_slot + x_slot + x_skip(a.dx_out));
     P d[NV][L], u[NV][L], with_u = SplatOf<P>(0.0f), plain = with_u;
     const P rstd2 = SplatOf<P>(two.y), away2 = SplatOf<P>(-two.x), rstd1 = SplatOf<P>(one.y), away1 = SplatOf<P>(-one.x), scale = SplatOf<P>(a.scale);
 #pragma unroll
@@ -190,7 +198,7 @@ cudaError_t Run(const JoinArgs& a, uint32_t T, uint32_t sms, cudaStream_t s, uin
   constexpr auto* kernel = JoinBwdRingKernel<XT, YT, kRms, VEC, NV, kThreads>;
   if (cudaError_t e = AllowShared<kernel>(r.bytes); e != cudaSuccess) return e;
   *grid = r.grid;
-  return Next(kernel, r.grid, r.groups * T, r.bytes, s)(a, T, r.slots, JoinEdge(a, {a.x, a.dx_out}, {a.dy, a.block}));
+  return Next(kernel, r.grid, r.groups * T, r.bytes, s)(a, T, r.slots, JoinEdge(a));
 }
 
 template <typename XT, typename YT, bool kRms>
@@ -210,11 +218,9 @@ cudaError_t Pick(const JoinArgs& a, uint32_t sms, cudaStream_t s, uint32_t* grid
       if (n <= 2 * T) return Run<XT, YT, kRms, 4, 2, kThreads>(a, T, sms, s, grid);
     }
     // Rms norms: a warp's row, which needs no barriers, of up to 768 columns of 16 bits (32768 rows 58 us, on 64 threads 72; an f32 stream's rows leave the
-    // ring too few of them: 88, 83); two groups of rows of up to 5120 columns.
+    // ring too few of them: 88, 83).
     if constexpr (kRms && sizeof(XT) == 2)
       if (n > 128 && n <= 192) return Run<XT, YT, kRms, 4, 6, 384>(a, 32, sms, s, grid);
-    if constexpr (kRms)
-      if (n > 1024 && n <= 1280) return Run<XT, YT, kRms, 4, 5, 512>(a, 256, sms, s, grid);
     const uint32_t T = Warps((n + 3) / 4), each = (n + T - 1) / T;
     if (each <= 1) return Run<XT, YT, kRms, 4, 1, kThreads>(a, T, sms, s, grid);
     if (each <= 2) return Run<XT, YT, kRms, 4, 2, kThreads>(a, T, sms, s, grid);

@@ -59,16 +59,22 @@ JoinFwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
     for (uint32_t i = 0; i < slots; ++i) umma_dev::MbarInit(&bars[i], 1);
     umma_dev::MbarInitFence();
   }
-  auto inner = [&](uint64_t row) { return row >= edge && row + edge < a.rows; };
+  auto inner = [&](uint64_t row) { return VEC == 4 || (row >= edge && row + edge < a.rows); };
   auto fill = [&](uint64_t row, uint32_t slot) {   // the group's thread 0
-    if (!inner(row)) return;
-    umma_dev::FenceProxyAsync();   // (an edge row's elements may have been written there)
     uint8_t* dst = ring + static_cast<size_t>(slot) * slot_bytes;
-    const OddRow<XT> x(a.x, row, a.x_stride, a.cols);
-    const OddRow<YT> b(a.block, row, a.y_stride, a.cols);
-    umma_dev::MbarExpectTx(&bars[slot], x.bytes + b.bytes);
-    umma_dev::BulkLoad(dst + x_slot, b.from, b.bytes, &bars[slot]);
-    umma_dev::BulkLoad(dst, x.from, x.bytes, &bars[slot]);
+    if (inner(row)) {
+      const OddRow<XT> x(a.x, row, a.x_stride, a.cols);
+      const OddRow<YT> b(a.block, row, a.y_stride, a.cols);
+      umma_dev::MbarExpectTx(&bars[slot], x.bytes + b.bytes);
+      umma_dev::BulkLoad(dst + x_slot, b.from, b.bytes, &bars[slot]);
+      umma_dev::BulkLoad(dst, x.from, x.bytes, &bars[slot]);
+    } else {
+      const EndRow<XT> x(a.x, row, a.x_stride, a.cols);
+      const EndRow<YT> b(a.block, row, a.y_stride, a.cols);
+      umma_dev::MbarExpectTx(&bars[slot], x.bytes + b.bytes);
+      if (b.bytes) umma_dev::BulkLoad(dst + x_slot + b.to, b.from, b.bytes, &bars[slot]);
+      if (x.bytes) umma_dev::BulkLoad(dst + x.to, x.from, x.bytes, &bars[slot]);
+    }
   };
   AwaitPrevious();
   if (t == 0)
@@ -88,16 +94,16 @@ JoinFwdRingKernel(const __grid_constant__ JoinArgs a, uint32_t T, uint32_t slots
   uint32_t turn = 0, slot = 0, parities = 0;   // a bit for each slot, of the copies that went through it
   for (uint64_t row = first; row < a.rows; row += step) {
     uint8_t* at = ring + static_cast<size_t>(slot) * slot_bytes;
-    if (inner(row)) {
-      AwaitRow(&bars[slot], parities >> slot & 1u, a.status);
-      parities ^= 1u << slot;
-    } else {
-      CopyRow<XT>(at, a.x, row, a.x_stride, a.cols, t, T);
-      CopyRow<YT>(at + x_slot, a.block, row, a.y_stride, a.cols, t, T);
+    if (!inner(row)) {
+      CopyEnds<XT>(at, a.x, row, a.x_stride, a.cols, t, T);
+      CopyEnds<YT>(at + x_slot, a.block, row, a.y_stride, a.cols, t, T);
+      umma_dev::FenceProxyAsync();   // (the slot is filled in bulk again)
       GroupBarrier(T, group);
     }
-    const XT* x = reinterpret_cast<const XT*>(at + OddRow<XT>(a.x, row, a.x_stride, a.cols).skip);
-    const YT* b = reinterpret_cast<const YT*>(at + x_slot + OddRow<YT>(a.block, row, a.y_stride, a.cols).skip);
+    AwaitRow(&bars[slot], parities >> slot & 1u, a.status);
+    parities ^= 1u << slot;
+    const XT* x = reinterpret_cast<const XT*>(at + (VEC == 4 ? 0 : reinterpret_cast<uint64_t>(static_cast<const XT*>(a.x) + row * a.x_stride) & 15));
+    const YT* b = reinterpret_cast<const YT*>(at + x_slot + (VEC == 4 ? 0 : reinterpret_cast<uint64_t>(static_cast<const YT*>(a.block) + row * a.y_stride) & 15));
     P v[NV][L];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -167,7 +173,7 @@ cudaError_t Run(const JoinArgs& a, uint32_t T, uint32_t sms, cudaStream_t s) {
   const JoinRing r = RingOf(a.rows, kThreads, T, OddSlot<XT>(a.cols) + OddSlot<YT>(a.cols), weights, sms);
   constexpr auto* kernel = JoinFwdRingKernel<XT, YT, kRms, VEC, NV, kThreads>;
   if (cudaError_t e = AllowShared<kernel>(r.bytes); e != cudaSuccess) return e;
-  return Next(kernel, r.grid, r.groups * T, r.bytes, s)(a, T, r.slots, JoinEdge(a, {a.x}, {a.block}));
+  return Next(kernel, r.grid, r.groups * T, r.bytes, s)(a, T, r.slots, JoinEdge(a));
 }
 
 template <typename XT, typename YT, bool kRms>
