@@ -466,7 +466,6 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     const T* z = logit_row(r);
     const uint32_t skip = skip_of(z), bytes = units_of(skip) * 16;
     if (bytes == 0) return;
-    umma_dev::FenceProxyAsync();   // (elements were written there)
     umma_dev::MbarExpectTx(&bars[slot], bytes);
     umma_dev::BulkLoad(ring + static_cast<size_t>(slot) * slot_bytes, reinterpret_cast<const uint4*>(z - skip) + begin, bytes, &bars[slot]);
   };
@@ -536,6 +535,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
       auto patch = [&](uint32_t u) {   // (the label of another unit: beyond the unit's elements)
         const int32_t from = static_cast<int32_t>(u * E);
         mine[u] = Only<T>(mine[u], static_cast<int32_t>(skip - begin * E) - from, end - from, at - from);
+        umma_dev::FenceProxyAsync();   // (the next row's copy comes there)
       };
       owner = at >= 0 && owns(static_cast<uint32_t>(at) / E);
       if (bulk(r)) {
@@ -548,6 +548,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
       } else {
         const Row<T> row(a, r);
         for (uint32_t u = t; u < count; u += threads) mine[u] = row.Raw(begin + u);
+        umma_dev::FenceProxyAsync();   // (other rows' copies come there)
       }
       if (owner) patch(static_cast<uint32_t>(at) / E);
 #pragma unroll
