@@ -8,7 +8,7 @@
 //
 // A row is walked in units of 16 bytes by address, of which the first and the last may stick out of it, whatever its alignment.  Rows reach
 // registers through a ring in shared memory (LogitRowsKernel); wide rows, and few ones, are shared by the blocks of a cluster.  What
-// is wider still is read from memory twice (LogitWideKernel).
+// is wider still is walked twice (LogitStreamKernel).
 //
 // logp is made in double: a sequence's sum of hundreds of them is held against a reference's.
 #include <type_traits>
@@ -108,26 +108,6 @@ struct Row {
   }
 };
 
-// A maximum m, its product mk = k m (0 where m is -inf), and sum = the sum of e relative to it.
-struct Part {
-  float m, mk, sum;
-};
-__device__ __forceinline__ Part NoPart() { return {MinusInf(), 0.0f, 0.0f}; }
-// (sums of nothing are 0, or NaN if what they are of is: neither is scaled)
-__device__ __forceinline__ float Rescaled(const Part& p, float mk) { return p.m == MinusInf() ? p.sum : p.sum * Ex2Approx(p.mk - mk); }
-__device__ __forceinline__ Part Joined(const Part& a, const Part& b) {
-  const Part& top = a.m >= b.m ? a : b;
-  return {top.m, top.mk, Rescaled(a, top.mk) + Rescaled(b, top.mk)};
-}
-__device__ __forceinline__ Part WarpJoin(Part p) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Part other = {__shfl_xor_sync(0xFFFFFFFFu, p.m, o), __shfl_xor_sync(0xFFFFFFFFu, p.mk, o), __shfl_xor_sync(0xFFFFFFFFu, p.sum, o)};
-    p = threadIdx.x & o ? Joined(other, p) : Joined(p, other);   // (one order in both)
-  }
-  return p;
-}
-
 // log((1 + t) / (1 - t)) for |t| up to 0.18, from the series of atanh; what is left out is below 3e-12 of it.
 __device__ __forceinline__ double LogRatio(double t) {
   const double q = t * t;
@@ -167,59 +147,6 @@ __device__ __forceinline__ double LogpOf(const LogitArgs& a, const RowSums& q) {
     return -LogRatio(Quotient(ratio, 2.0 + ratio));
   }
   return static_cast<double>(a.scale) * (static_cast<double>(q.z_label) - static_cast<double>(q.mk) * a.inv_k) - LogOf(q.s);
-}
-
-// By a block's threads; `slots` is free after the caller's next barrier.
-template <typename T>
-__device__ __forceinline__ RowSums SumsOf(const Row<T>& row, uint32_t label, float k, Part (&slots)[kThreads / 32]) {
-  const uint32_t label_unit = (label + row.skip) / kPerUnit<T>, label_slot = (label + row.skip) % kPerUnit<T>;
-  const float z_label = ToF32(row.z[label]);
-  Part p = NoPart();
-  for (uint32_t u = threadIdx.x; u < row.units; u += kThreads) {
-    float v[kPerUnit<T>], top = MinusInf();
-    row.Load(u, v);
-#pragma unroll
-    for (int j = 0; j < kPerUnit<T>; ++j) top = fmaxf(top, v[j]);
-    if (top > p.m) {
-      const float mk = __fmul_rn(top, k);
-      p = {top, mk, Rescaled(p, mk)};
-    }
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kPerUnit<T>; ++j) {
-      const float e = Ex2Approx(fmaf(v[j], k, -p.mk));
-      sum += u == label_unit && static_cast<uint32_t>(j) == label_slot ? 0.0f : e;
-    }
-    p.sum += sum;
-  }
-  p = WarpJoin(p);
-  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = p;
-  __syncthreads();
-  p = (threadIdx.x & 31) < kThreads / 32 ? slots[threadIdx.x & 31] : NoPart();
-  p = WarpJoin(p);
-  return {z_label, p.mk, p.sum, p.sum + Ex2Approx(fmaf(z_label, k, -p.mk))};
-}
-
-// dlogits of a row; slope includes logit_scale.
-template <typename T>
-__device__ __forceinline__ void Gradient(const Row<T>& row, uint32_t label, float k, float mk, float others, float s, float slope) {
-  const uint32_t label_unit = (label + row.skip) / kPerUnit<T>, label_slot = (label + row.skip) % kPerUnit<T>;
-  const float by = -slope / s, of_label = slope * (others / s);
-  for (uint32_t u = threadIdx.x; u < row.units; u += kThreads) {
-    float v[kPerUnit<T>];
-    row.Load(u, v);
-#pragma unroll
-    for (int j = 0; j < kPerUnit<T>; ++j) {
-      v[j] = by * Ex2Approx(fmaf(v[j], k, -mk));
-      if (u == label_unit && static_cast<uint32_t>(j) == label_slot) v[j] = of_label;
-    }
-    row.Store(u, v);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void Zeros(const Row<T>& row) {
-  const float v[kPerUnit<T>] = {};
-  for (uint32_t u = threadIdx.x; u < row.units; u += kThreads) row.Store(u, v);
 }
 
 __device__ __forceinline__ bool Counts(int32_t label, uint32_t classes) { return label >= 0 && static_cast<uint32_t>(label) < classes; }
@@ -703,31 +630,232 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
   }
 }
 
-// Rows that no cluster holds in its registers, read twice: a block to a row.
+// ---- rows as streams ----------------------------------------------------------------------------------------
+// Rows wider than a cluster's registers (and others: RunRows): a group of 256 threads walks a row 16 KB at a time (four units a thread) through its ring: first
+// for the sums, then, a policy loss's, from L2 for dlogits.  The ring runs ahead over both walks and into the next row, so that loads never pause while
+// sums meet; the other groups of the SM compute meanwhile.
+constexpr uint32_t kWalkers = 256, kWalkUnits = 4, kChunk = kWalkers * kWalkUnits;   // threads of a group; units to a thread, and in a chunk
+constexpr uint32_t kStreams = 3, kStreamSlots = (kMostShared - 8192) / (kStreams * kChunk * 16);   // groups to an SM, and chunks on their way to each
+
 template <typename T, bool kPolicy>
-__global__ void __launch_bounds__(kThreads)
-LogitWideKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const Sequences seq, float4* __restrict__ kept,
-                uint32_t* __restrict__ arrived) {
+__global__ void __launch_bounds__(kStreams * kWalkers, 1)
+LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const Sequences seq, float4* __restrict__ kept,
+                  uint32_t* __restrict__ arrived) {
+  constexpr uint32_t E = kPerUnit<T>;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ float2 sums[2][kStreams * kWalkers / 32];   // k M and the sum, of a warp
+  __shared__ uint32_t brought[2][kStreams][8];           // of a group: the label's logit, and a PolicyRow
+  __shared__ uint64_t all_bars[kStreams][kStreamSlots];
+  const uint32_t group = threadIdx.x / kWalkers, t = threadIdx.x % kWalkers, lane = threadIdx.x & 31;
+  uint4* ring = reinterpret_cast<uint4*>(dyn) + group * kStreamSlots * kChunk;
+  uint64_t* bars = all_bars[group];
+  const uint32_t rows = static_cast<uint32_t>(a.rows), step = gridDim.x * kStreams, first = group * gridDim.x + blockIdx.x;   // (every SM gets rows before one gets two)
+  const bool twice = kPolicy && a.dlogits;
+  if (t == 0) {
+    for (uint32_t i = 0; i < kStreamSlots; ++i) umma_dev::MbarInit(&bars[i], 1);
+    umma_dev::MbarInitFence();
+  }
   AwaitPrevious();
-  __shared__ Part slots[2][kThreads / 32];
-  if (kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
+  auto logit_row = [&](uint32_t r) { return static_cast<const T*>(a.logits) + static_cast<uint64_t>(r) * a.stride; };
+  auto counts = [&](uint32_t r, int32_t label) {
+    if (!Counts(label, a.classes)) return false;
+    return kPolicy || (static_cast<int64_t>(r) >= seq.starts[0] && static_cast<int64_t>(r) < seq.starts[seq.count]);
+  };
+  // A row's units and chunks, and whether a chunk can be copied whole: the matrix's first and last may begin before it or end behind it.
+  struct Walk {
+    const uint4* from;
+    uint32_t skip, units, chunks;
+  };
+  auto walk_of = [&](uint32_t r) {
+    Walk w;
+    const T* z = logit_row(r);
+    w.skip = static_cast<uint32_t>(reinterpret_cast<uint64_t>(z) & 15) / static_cast<uint32_t>(sizeof(T));
+    w.from = reinterpret_cast<const uint4*>(z - w.skip);
+    w.units = (w.skip + a.classes + E - 1) / E;
+    w.chunks = (w.units + kChunk - 1) / kChunk;
+    return w;
+  };
+  auto bulk = [&](const Walk& w, uint32_t chunk) {
+    const T* begin = static_cast<const T*>(a.logits);
+    const uint4* last = w.from + min((chunk + 1) * kChunk, w.units);
+    return reinterpret_cast<const T*>(w.from + chunk * kChunk) >= begin &&
+           reinterpret_cast<const T*>(last) <= begin + static_cast<uint64_t>(rows - 1) * a.stride + a.classes;
+  };
+  // The chunk that is asked for next (by the group's thread 0), ahead of the one at work.
+  uint32_t f_row = first, f_chunk = 0, f_slot = 0;
+  int32_t f_label = -1, f_next = -1;
+  if (t == 0) {
+    if (first < rows) f_label = a.labels[first];
+    if (first + step < rows) f_next = a.labels[first + step];
+  }
+  auto fill = [&] {
+    if (t != 0) return;
+    auto next_row = [&] {
+      f_row += step;
+      f_label = f_next;
+      f_next = f_row + step < rows ? a.labels[f_row + step] : -1;
+      f_chunk = 0;
+    };
+    while (f_row < rows && f_chunk == 0 && !counts(f_row, f_label)) next_row();
+    if (f_row >= rows) return;
+    const Walk w = walk_of(f_row);
+    const uint32_t chunk = f_chunk < w.chunks ? f_chunk : f_chunk - w.chunks, units = min(kChunk, w.units - chunk * kChunk);
+    if (bulk(w, chunk)) {
+      umma_dev::MbarExpectTx(&bars[f_slot], units * 16);
+      umma_dev::BulkLoad(ring + f_slot * kChunk, w.from + chunk * kChunk, units * 16, &bars[f_slot]);
+    }
+    if (++f_slot == kStreamSlots) f_slot = 0;
+    if (++f_chunk == w.chunks * (twice ? 2 : 1)) next_row();
+  };
+  // What a row brings besides its logits is asked for while the one before it is at work: each item by one of the group's first threads, as it is read.
+  uint32_t ahead = 0;
+  auto ask = [&](uint32_t r, int32_t label) {
+    if (r >= rows || t > (kPolicy ? 4u : 0u) || !counts(r, label)) return;
+    if (t == 0) ahead = reinterpret_cast<const std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>*>(logit_row(r))[label];
+    else if (t == 1) ahead = __float_as_uint(p.old_logp[r]);
+    else if (t == 2) ahead = p.ref_logp ? __float_as_uint(p.ref_logp[r]) : 0u;
+    else if (t == 3) ahead = __float_as_uint(p.advantages[r]);
+    else ahead = p.weights ? __float_as_uint(p.weights[r]) : 0x3F800000u;
+  };
+#pragma unroll 1
+  for (uint32_t i = 0; i < kStreamSlots; ++i) fill();
   const float grad = (kPolicy && p.loss_grad ? *p.loss_grad : 1.0f) * a.scale;
-  uint32_t turn = 0;
-  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  if (kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
+  int32_t next_label = first < rows ? a.labels[first] : -1, label_behind = first + step < rows ? a.labels[first + step] : -1;
+  ask(first, next_label);
+  __syncwarp();
+  GroupBarrier(kWalkers, group);   // the barriers are there
+  uint32_t turn = 0, slot = 0, parities = 0;   // a bit for each slot, of the copies that went through it
+  for (uint32_t r = first; r < rows; r += step) {
+    const int32_t label = next_label;
+    next_label = label_behind;
+    label_behind = r + 2 * step < rows ? a.labels[r + 2 * step] : -1;
+    const uint32_t item = ahead;
+    ask(r + step, next_label);
     const Row<T> row(a, r);
-    const int32_t label = a.labels[r];
-    if (!kPolicy && (static_cast<int64_t>(r) < seq.starts[0] || static_cast<int64_t>(r) >= seq.starts[seq.count])) continue;
-    if (!Counts(label, a.classes)) {
-      if (kPolicy && a.dlogits) Zeros(row);
+    if (!counts(r, label)) {
+      if (twice) {
+        const float none[E] = {};
+        for (uint32_t u = t; u < row.units; u += kWalkers) row.Store(u, none);
+      }
       continue;
     }
-    const RowSums q = SumsOf(row, label, a.k, slots[turn]);
+    const Walk w = walk_of(r);
+    const uint32_t label_unit = (static_cast<uint32_t>(label) + w.skip) / E, ends_at = w.skip + a.classes;
+    // A chunk's units of this thread, asked for by their number in the row; beyond it: nothing.
+    uint4 raw[kWalkUnits];
+    auto read = [&](uint32_t chunk) {
+      const uint32_t u0 = chunk * kChunk + t;
+      if (bulk(w, chunk)) {
+        AwaitRow(&bars[slot], parities >> slot & 1u, a.status);
+        parities ^= 1u << slot;
+        const uint4* from = ring + slot * kChunk + t;
+#pragma unroll
+        for (uint32_t i = 0; i < kWalkUnits; ++i) raw[i] = u0 + i * kWalkers < w.units ? from[i * kWalkers] : Nothing<T>();
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kWalkUnits; ++i) raw[i] = u0 + i * kWalkers < w.units ? row.Raw(u0 + i * kWalkers) : Nothing<T>();
+      }
+      if (++slot == kStreamSlots) slot = 0;
+    };
+    const f32x2 k2 = Splat2(a.k);
+    float mk = MinusInf(), sum = 0.0f;   // k M and the sum relative to it, of the others
+    auto factor = [](float own, float all) { return own == MinusInf() ? 0.0f : Ex2Approx(own - all); };
+    for (uint32_t chunk = 0; chunk < w.chunks; ++chunk) {
+      read(chunk);
+      const uint32_t u0 = chunk * kChunk, u1 = u0 + kChunk;
+      if ((chunk == 0 && w.skip != 0) || u1 * E > ends_at || (label_unit >= u0 && label_unit < u1)) {   // -inf in place of the label and of what sticks out
+#pragma unroll
+        for (uint32_t i = 0; i < kWalkUnits; ++i) {
+          const uint32_t u = u0 + t + i * kWalkers;
+          const int32_t e0 = static_cast<int32_t>(u * E);
+          if ((u == 0 && w.skip != 0) || u == w.units - 1 || u == label_unit)
+            raw[i] = Only<T>(raw[i], static_cast<int32_t>(w.skip) - e0, static_cast<int32_t>(ends_at) - e0, label + static_cast<int32_t>(w.skip) - e0);
+        }
+      }
+      const float top = fmaxf(mk, __fmul_rn(Largest<T, kWalkUnits>(raw), a.k));
+      GroupBarrier(kWalkers, group);   // the slot is read
+      fill();
+      const f32x2 away = Splat2(top == MinusInf() ? 0.0f : -top);
+      f32x2 sum2[kPairs<T>] = {};
+#pragma unroll
+      for (uint32_t i = 0; i < kWalkUnits; ++i) {
+        f32x2 v[kPairs<T>];
+        Pairs<T>(raw[i], v);
+#pragma unroll
+        for (int j = 0; j < kPairs<T>; ++j) sum2[j] = AddF2(sum2[j], Powers(Fma2(v[j], k2, away)));
+      }
+#pragma unroll
+      for (int j = 1; j < kPairs<T>; ++j) sum2[0] = AddF2(sum2[0], sum2[j]);
+      float lo, hi;
+      UnpackF2(sum2[0], &lo, &hi);
+      sum = fmaf(sum, factor(mk, top), lo + hi);
+      mk = top;
+    }
+    // Warps and the group: the largest k M, and sums relative to it.
+    auto join = [&](uint32_t most) {
+      const float top = WarpMax(mk);
+      sum *= factor(mk, top);
+      mk = top;
+#pragma unroll
+      for (uint32_t o = 16; o > 0; o >>= 1)
+        if (o <= most) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    };
+    join(16);
+    uint32_t* items = brought[turn][group];
+    float2* set = sums[turn] + group * (kWalkers / 32);
+    if (t < 5) items[t] = item;
+    if (lane == 0) set[t >> 5] = make_float2(mk, sum);
+    GroupBarrier(kWalkers, group);
+    const float2 warp_part = set[lane & 7];
+    mk = warp_part.x;
+    sum = warp_part.y;
+    join(4);
     turn ^= 1;
-    if (threadIdx.x == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
-    if (!kPolicy || !a.dlogits) continue;
-    const float slope = SlopeOf<T>(a, p, PolicyRowOf(p, r), q) * grad;
-    if (slope == 0.0f) Zeros(row);
-    else Gradient(row, label, a.k, q.mk, q.others, q.s, slope);
+    T raw_label;
+    if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(items[0]);
+    else raw_label.bits = static_cast<uint16_t>(items[0]);
+    const float z_label = ToF32(raw_label), mk_label = __fmul_rn(z_label, a.k), all = fmaxf(mk, mk_label);
+    RowSums q = {z_label, all == MinusInf() ? 0.0f : all, sum * factor(mk, all), 0.0f};
+    q.s = q.others + LabelTerm(a, z_label, q.mk);
+    if (t == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
+    if constexpr (kPolicy) {
+      if (!twice) continue;
+      const PolicyRow brings = {__uint_as_float(items[1]), __uint_as_float(items[2]), __uint_as_float(items[3]), __uint_as_float(items[4])};
+      const float slope = SlopeOf<T>(a, p, brings, q) * grad;   // (0: zeros come out)
+      const f32x2 by = Splat2(-slope / q.s), away = Splat2(-q.mk);
+      for (uint32_t chunk = 0; chunk < w.chunks; ++chunk) {
+        read(chunk);
+        uint4 out[kWalkUnits];
+#pragma unroll
+        for (uint32_t i = 0; i < kWalkUnits; ++i) {
+          f32x2 pair[kPairs<T>];
+          float v[E];
+          Pairs<T>(raw[i], pair);
+#pragma unroll
+          for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(Powers(Fma2(pair[j], k2, away)), by), &v[2 * j], &v[2 * j + 1]);
+          if constexpr (sizeof(T) == 4) out[i] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+          else out[i] = make_uint4(Pack2<T>(v[0], v[1]), Pack2<T>(v[2], v[3]), Pack2<T>(v[4], v[5]), Pack2<T>(v[6], v[7]));
+        }
+        GroupBarrier(kWalkers, group);   // the slot is read
+        fill();
+        const uint32_t u0 = chunk * kChunk + t;
+        if (row.alike && (chunk != 0 || w.skip == 0) && (chunk + 1) * kChunk * E <= ends_at) {
+          uint4* to = reinterpret_cast<uint4*>(row.d - w.skip) + u0;
+#pragma unroll
+          for (uint32_t i = 0; i < kWalkUnits; ++i) to[i * kWalkers] = out[i];
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < kWalkUnits; ++i) {
+            if (u0 + i * kWalkers >= w.units) continue;
+            float v[E];
+            Elements<T>(out[i], v);
+            row.Store(u0 + i * kWalkers, v);
+          }
+        }
+        if (label_unit / kChunk == chunk && label_unit % kWalkers == t) row.d[label] = FromF32<T>(slope * (q.others / q.s));
+      }
+    }
   }
 }
 
@@ -968,8 +1096,15 @@ cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& se
 template <typename T, bool kPolicy>
 cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, uint32_t* arrived, uint32_t sms, cudaStream_t s) {
   Sharing w;
-  if (!ShareRows<T>(a, sms, &w))
-    return Next(LogitWideKernel<T, kPolicy>, static_cast<unsigned>(a.rows < 4 * sms ? a.rows : 4 * sms), kThreads, 0, s)(a, p, seq, kept, arrived);
+  // Of a preference loss's rows, which have no second walk, those of more than half of an SM's threads too: 768 rows of 128256 in bf16 107 us with pairs and
+  // gradient, in clusters 119; 1500 of 50001 in f16 98, one row to an SM 101.  A policy loss's second walk costs more than that: 8192 rows of 32000 in bf16
+  // 227 us, in registers 172; 2048 of 128256 254, in clusters 204.
+  if (!ShareRows<T>(a, sms, &w) || (!kPolicy && a.rows > 2 * sms && w.threads > kThreads / 2)) {
+    constexpr auto* kernel = LogitStreamKernel<T, kPolicy>;
+    constexpr size_t bytes = kStreams * kStreamSlots * kChunk * 16;
+    if (cudaError_t e = AllowShared<kernel>(bytes); e != cudaSuccess) return e;
+    return Next(kernel, static_cast<unsigned>(a.rows < sms ? a.rows : sms), kStreams * kWalkers, bytes, s)(a, p, seq, kept, arrived);
+  }
   return w.blocks > 1 ? RunRows<T, kPolicy, true>(a, p, seq, kept, arrived, w, s) : RunRows<T, kPolicy, false>(a, p, seq, kept, arrived, w, s);
 }
 
