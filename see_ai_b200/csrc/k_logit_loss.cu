@@ -94,12 +94,17 @@ struct Row {
       r[j * sizeof(T) / 4] |= (at + j >= 0 && at + j < static_cast<int32_t>(classes) ? static_cast<uint32_t>(bits[at + j]) : NoElement<T>()) << (j * sizeof(T) % 4 * 8);
     return make_uint4(r[0], r[1], r[2], r[3]);
   }
+  // The same of what nobody reads again, so that it does not stay in L2.
+  __device__ __forceinline__ uint4 RawOnce(uint32_t unit) const {
+    const int32_t at = At(unit);
+    return Whole(at) ? __ldcs(reinterpret_cast<const uint4*>(z + at)) : Raw(unit);
+  }
   __device__ __forceinline__ void Load(uint32_t unit, float* v) const { Elements<T>(Raw(unit), v); }
   __device__ __forceinline__ void Store(uint32_t unit, const float* v) const {
     const int32_t at = At(unit);
     if (alike && Whole(at)) {
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(d + at) = make_float4(v[0], v[1], v[2], v[3]);
-      else Store8<T>(d + at, v);
+      if constexpr (sizeof(T) == 4) __stcs(reinterpret_cast<float4*>(d + at), make_float4(v[0], v[1], v[2], v[3]));
+      else __stcs(reinterpret_cast<uint4*>(d + at), make_uint4(Pack2<T>(v[0], v[1]), Pack2<T>(v[2], v[3]), Pack2<T>(v[4], v[5]), Pack2<T>(v[6], v[7])));
       return;
     }
 #pragma unroll
@@ -972,7 +977,7 @@ PreferenceGradientKernel(const __grid_constant__ LogitArgs a, const __grid_const
       if (slope != 0.0f) {
 #pragma unroll
         for (int i = 0; i < kGradUnits; ++i)
-          if (u0 + i * 32 < row.units) raw[i] = row.Raw(u0 + i * 32);
+          if (u0 + i * 32 < row.units) raw[i] = row.RawOnce(u0 + i * 32);
       }
 #pragma unroll
       for (int i = 0; i < kGradUnits; ++i) {
@@ -1129,8 +1134,11 @@ cudaError_t Preference(const LogitArgs& a, const PreferenceArgs& p, float4* kept
   if (cudaError_t e = Next(PreferencePairsKernel, p.pairs < 4 * sms ? p.pairs : 4 * sms, kPairThreads, 0, s)(a, p, kept); e != cudaSuccess) return e;
   *launches += 2;
   if (!a.dlogits) return Next(PreferenceFoldKernel, 1, 256, 0, s)(p);
+  // Warps to a row: as many as its pieces of 128 units keep busy, or, of few rows, as many as there are pieces for.
   const uint32_t pieces = (a.classes / kPerUnit<T> + 32 * kGradUnits) / (32 * kGradUnits);
-  const uint32_t warps = pieces >= 8 ? 8 : pieces >= 4 ? 4 : pieces >= 2 ? 2 : 1, rows_a_block = kGradThreads / 32 / warps;
+  uint32_t warps = kGradThreads / 32;
+  while (warps > 1 && (a.rows < 8 * sms ? warps > pieces : (pieces + warps - 1) / warps * warps * 15 > pieces * 16)) warps /= 2;
+  const uint32_t rows_a_block = kGradThreads / 32 / warps;
   const uint64_t blocks = (a.rows + rows_a_block - 1) / rows_a_block, most = 6ull * sms;
   return Next(PreferenceGradientKernel<T>, static_cast<unsigned>(blocks < most ? blocks : most), kGradThreads, 0, s)(
       a, p, static_cast<const float4*>(kept), warps);
