@@ -635,6 +635,119 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
   }
 }
 
+// ---- short rows ------------------------------------------------------------------------------------------------
+// Rows of up to 128 units, more than a few: a warp to a row, straight into registers, the next row asked for while this one is at work.  Their time is
+// instructions: 16384 rows of 250 in bf16 with the ring's bookkeeping 29 us, so 18.5; 65536 in f32 64, so 52.
+constexpr uint32_t kShortThreads = 256;
+template <typename T, int NU, bool kPolicy>
+__global__ void __launch_bounds__(kShortThreads)
+LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const Sequences seq, float4* __restrict__ kept,
+                 uint32_t* __restrict__ arrived) {
+  AwaitPrevious();
+  constexpr uint32_t E = kPerUnit<T>;
+  const uint32_t lane = threadIdx.x & 31, rows = static_cast<uint32_t>(a.rows), step = gridDim.x * (kShortThreads / 32);
+  const uint32_t first = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;   // (every block gets rows before one gets two)
+  if (kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
+  const uint64_t begin = reinterpret_cast<uint64_t>(a.logits), end = begin + (static_cast<uint64_t>(rows - 1) * a.stride + a.classes) * sizeof(T);
+  const float grad = (kPolicy && p.loss_grad ? *p.loss_grad : 1.0f) * a.scale;
+  auto counts = [&](uint32_t r, int32_t label) {
+    if (!Counts(label, a.classes)) return false;
+    return kPolicy || (static_cast<int64_t>(r) >= seq.starts[0] && static_cast<int64_t>(r) < seq.starts[seq.count]);
+  };
+  // Units as they lie, what is beside the row with them where it is the matrix's too; and, a lane each, what the row brings besides.
+  uint4 next_raw[NU];
+  uint32_t next_item = 0;
+  auto ask = [&](uint32_t r, int32_t label) {
+    if (r >= rows || !counts(r, label)) return;
+    const Row<T> row(a, r);
+    const uint64_t from = reinterpret_cast<uint64_t>(row.z) - row.skip * sizeof(T);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const uint32_t u = lane + i * 32;
+      const uint64_t at = from + static_cast<uint64_t>(u) * 16;
+      if (u >= row.units) next_raw[i] = Nothing<T>();
+      else if (at >= begin && at + 16 <= end) next_raw[i] = *reinterpret_cast<const uint4*>(at);
+      else next_raw[i] = row.Raw(u);
+    }
+    if (lane == 0) next_item = reinterpret_cast<const std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>*>(row.z)[label];
+    if (!kPolicy) return;
+    const float* from_item = lane == 1 ? p.old_logp : lane == 2 ? p.ref_logp : lane == 3 ? p.advantages : lane == 4 ? p.weights : nullptr;
+    if (from_item) next_item = __float_as_uint(from_item[r]);
+    else if (lane == 4) next_item = 0x3F800000u;
+  };
+  int32_t next_label = first < rows ? a.labels[first] : -1, label_behind = first + step < rows ? a.labels[first + step] : -1;
+  ask(first, next_label);
+  const f32x2 k2 = Splat2(a.k);
+  for (uint32_t r = first; r < rows; r += step) {
+    const int32_t label = next_label;
+    next_label = label_behind;
+    label_behind = r + 2 * step < rows ? a.labels[r + 2 * step] : -1;
+    uint4 raw[NU];
+#pragma unroll
+    for (int i = 0; i < NU; ++i) raw[i] = next_raw[i];
+    const uint32_t item = next_item;
+    ask(r + step, next_label);
+    const Row<T> row(a, r);
+    if (!counts(r, label)) {
+      if (kPolicy && a.dlogits) {
+        const float none[E] = {};
+        for (uint32_t u = lane; u < row.units; u += 32) row.Store(u, none);
+      }
+      continue;
+    }
+    const uint32_t label_unit = (static_cast<uint32_t>(label) + row.skip) / E, whole_end = (row.skip + a.classes) / E;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {   // -inf in place of the label and of what sticks out
+      const uint32_t u = lane + i * 32;
+      const int32_t e0 = static_cast<int32_t>(u * E) - static_cast<int32_t>(row.skip);
+      if ((e0 < 0 || u >= whole_end || u == label_unit) && u < row.units) raw[i] = Only<T>(raw[i], -e0, static_cast<int32_t>(a.classes) - e0, label - e0);
+    }
+    float mk = __fmul_rn(Largest<T, NU>(raw), a.k);
+    mk = WarpMax(mk);
+    const f32x2 away = Splat2(mk == MinusInf() ? 0.0f : -mk);
+    f32x2 sum2 = 0;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      f32x2 v[kPairs<T>];
+      Pairs<T>(raw[i], v);
+#pragma unroll
+      for (int j = 0; j < kPairs<T>; ++j) sum2 = AddF2(sum2, Powers(Fma2(v[j], k2, away)));
+    }
+    float lo, sum;
+    UnpackF2(sum2, &lo, &sum);
+    sum += lo;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    const uint32_t label_bits = __shfl_sync(0xFFFFFFFFu, item, 0);
+    T raw_label;
+    if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(label_bits);
+    else raw_label.bits = static_cast<uint16_t>(label_bits);
+    const float z_label = ToF32(raw_label), mk_label = __fmul_rn(z_label, a.k), all = fmaxf(mk, mk_label);
+    RowSums q = {z_label, all == MinusInf() ? 0.0f : all, mk == MinusInf() ? 0.0f * sum : sum * Ex2Approx(mk - all), 0.0f};
+    q.s = q.others + LabelTerm(a, z_label, q.mk);
+    if (lane == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
+    if constexpr (kPolicy) {
+      if (!a.dlogits) continue;
+      const PolicyRow brings = {__uint_as_float(__shfl_sync(0xFFFFFFFFu, item, 1)), __uint_as_float(__shfl_sync(0xFFFFFFFFu, item, 2)),
+                                __uint_as_float(__shfl_sync(0xFFFFFFFFu, item, 3)), __uint_as_float(__shfl_sync(0xFFFFFFFFu, item, 4))};
+      const float slope = SlopeOf<T>(a, p, brings, q) * grad;   // (0: zeros come out)
+      const f32x2 by = Splat2(-slope / q.s), away_all = Splat2(-q.mk);
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        const uint32_t u = lane + i * 32;
+        if (u >= row.units) continue;
+        f32x2 pair[kPairs<T>];
+        float v[E];
+        Pairs<T>(raw[i], pair);
+#pragma unroll
+        for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(Powers(Fma2(pair[j], k2, away_all)), by), &v[2 * j], &v[2 * j + 1]);
+        row.Store(u, v);
+        if (u == label_unit) row.d[label] = FromF32<T>(slope * (q.others / q.s));
+      }
+    }
+  }
+}
+
 // ---- rows as streams ----------------------------------------------------------------------------------------
 // Rows wider than a cluster's registers (and others: RunRows): a group of 256 threads walks a row 16 KB at a time (four units a thread) through its ring: first
 // for the sums, then, a policy loss's, from L2 for dlogits.  The ring runs ahead over both walks and into the next row, so that loads never pause while
@@ -1100,6 +1213,15 @@ cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& se
 }
 template <typename T, bool kPolicy>
 cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& seq, float4* kept, uint32_t* arrived, uint32_t sms, cudaStream_t s) {
+  // Short rows, from a few to a warp on.
+  const uint32_t all = (a.classes + 2 * (kPerUnit<T> - 1)) / kPerUnit<T>;
+  if (all <= 128 && a.rows > 8 * sms) {
+    const uint64_t blocks = (a.rows + kShortThreads / 32 - 1) / (kShortThreads / 32), most = 4ull * sms;
+    const unsigned grid = static_cast<unsigned>(blocks < most ? blocks : most);
+    if (all <= 32) return Next(LogitShortKernel<T, 1, kPolicy>, grid, kShortThreads, 0, s)(a, p, seq, kept, arrived);
+    if (all <= 64) return Next(LogitShortKernel<T, 2, kPolicy>, grid, kShortThreads, 0, s)(a, p, seq, kept, arrived);
+    return Next(LogitShortKernel<T, 4, kPolicy>, grid, kShortThreads, 0, s)(a, p, seq, kept, arrived);
+  }
   Sharing w;
   // Of a preference loss's rows, which have no second walk, those of more than half of an SM's threads too: 768 rows of 128256 in bf16 107 us with pairs and
   // gradient, in clusters 119; 1500 of 50001 in f16 98, one row to an SM 101.  A policy loss's second walk costs more than that: 8192 rows of 32000 in bf16

@@ -79,7 +79,8 @@ class Policy:
 
 
 SIZES = [(1, 1), (5, 2), (3, 7), (40, 8), (33, 33), (1, 250), (300, 250), (17, 1000), (9, 4096), (200, 5003), (1, 32000), (160, 32000), (3, 50001),
-         (2, 128003), (155, 100000), (2, 300001), (1, 1 << 20)]
+         (2, 128003), (155, 100000), (2, 300001), (1, 1 << 20),
+         (1300, 1), (1500, 55), (2400, 250), (1190, 511), (1185, 1003)]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
@@ -102,7 +103,8 @@ def test_formula(be, rows, classes, dtype):
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("rows,classes,stride,begin,d_begin", [(7, 33, 40, 8, 8), (7, 33, 37, 3, 3), (50, 250, 251, 1, 2), (6, 5003, 5011, 5, 0),
                                                               (3, 32000, 32008, 8, 1), (5, 32000, 33001, 7, 7), (2, 128003, 128003, 1, 5),
-                                                              (2, 300001, 300001, 3, 4), (4, 1, 1, 0, 0), (9, 3, 5, 2, 1)])
+                                                              (2, 300001, 300001, 3, 4), (4, 1, 1, 0, 0), (9, 3, 5, 2, 1), (1300, 250, 251, 3, 3),
+                                                              (1300, 1003, 1016, 8, 1)])
 def test_strides_and_alignments(be, rows, classes, stride, begin, d_begin, dtype):
     c = Policy(rows, classes, dtype, stride=stride, begin=begin, d_begin=d_begin)
     c(be)

@@ -105,7 +105,8 @@ def test_formula(be, name, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
-@pytest.mark.parametrize("lengths,classes", [([3, 2], 128003), ([90, 70], 50001), ([1, 2], 300001), ([700, 900], 2000)])
+@pytest.mark.parametrize("lengths,classes", [([3, 2], 128003), ([90, 70], 50001), ([1, 2], 300001), ([700, 900], 2000), ([160, 150], 70001),
+                                             ([700, 600, 9, 0], 251), ([800, 500], 40)])
 def test_wide_and_long(be, lengths, classes, dtype):
     c = Preference(lengths, classes, dtype, average=True)
     c(be)
