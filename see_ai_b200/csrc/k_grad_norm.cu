@@ -266,9 +266,10 @@ cudaError_t GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, 
                      float* factor, double* partials, uint32_t sms, cudaStream_t s, int* launches) {
   GradTable table;
   uint64_t next = 0;
-  unsigned used = 0;   // partial sums
+  unsigned used = 0, grid = 0, tables = 0;   // used: partial sums
   while (Fill(&table, tensors, count, &next)) {
-    const unsigned grid = Cut(table, sms);
+    ++tables;
+    grid = Cut(table, sms);
     // (blocks that an earlier launch had are added to; those that it had not are new)
     if (used != 0 && grid > used) {
       if (cudaError_t e = cudaMemsetAsync(partials + used, 0, (grid - used) * sizeof(double), s); e != cudaSuccess) return e;
@@ -276,19 +277,21 @@ cudaError_t GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, 
     if (cudaError_t e = Next(GradSquaresKernel, grid, kThreads, 0, s)(table, partials, used == 0 ? 1 : 0); e != cudaSuccess) return e;
     ++*launches;
     used = used > grid ? used : grid;
+    if (next >= count) break;
   }
   if (!clip || used == 0) {
     ++*launches;
     return Next(GradFactorKernel, 1, kThreads, 0, s)(static_cast<const double*>(partials), used, max_norm, grad_scale, norm, factor);
   }
+  auto scale = [&] {
+    ++*launches;
+    return Next(GradScaleKernel, grid, kThreads, 0, s)(table, static_cast<const double*>(partials), used, max_norm, grad_scale, norm, factor);
+  };
+  if (tables == 1) return scale();   // (the table is there)
   next = 0;
   while (Fill(&table, tensors, count, &next)) {
-    const unsigned grid = Cut(table, sms);
-    if (cudaError_t e = Next(GradScaleKernel, grid, kThreads, 0, s)(table, static_cast<const double*>(partials), used, max_norm, grad_scale,
-                                                                                 norm, factor);
-        e != cudaSuccess)
-      return e;
-    ++*launches;
+    grid = Cut(table, sms);
+    if (cudaError_t e = scale(); e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }

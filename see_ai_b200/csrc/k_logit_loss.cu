@@ -997,12 +997,13 @@ PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant
     const int64_t begin = min(max(static_cast<int64_t>(p.starts[s]), static_cast<int64_t>(0)), most);
     const int64_t end = min(static_cast<int64_t>(p.starts[s + 1]), most);
     double sum = 0.0, counted = 0.0;
-    for (int64_t r = begin + t; r < end; r += kPairThreads / 2)
+    for (int64_t r = begin + t; r < end; r += kPairThreads / 2) {
+      const float4 q = kept[r];   // (asked for beside the label; of a row that does not count, whatever is there)
       if (Counts(a.labels[r], a.classes)) {
-        const float4 q = kept[r];
         sum += LogpOf(a, {q.x, q.y, q.z, q.w});
         counted += 1.0;
       }
+    }
     sum = WarpSum(sum);
     counted = WarpSum(counted);
     __syncthreads();   // (the last pair's are read)

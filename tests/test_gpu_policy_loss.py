@@ -213,8 +213,9 @@ def test_gradient_against_differences(be):
         assert abs(slope - want) <= 1e-4 * (1 + abs(want))
 
 
-def test_same_bits_replayed_and_two_at_once(be):
-    c = Policy(200, 5003, "bf16", seed=7)
+@pytest.mark.parametrize("rows,classes", [(200, 5003), (3, 128003), (1300, 250), (400, 50001), (2, 300001)])
+def test_same_bits_replayed_and_two_at_once(be, rows, classes):
+    c = Policy(rows, classes, "bf16", seed=7)
     c(be)
     want = c.d.clone(), c.loss.clone(), c.logp.clone()
     side = torch.cuda.Stream()
@@ -231,7 +232,7 @@ def test_same_bits_replayed_and_two_at_once(be):
         graph.replay()
         assert torch.equal(c.d, want[0]) and torch.equal(c.loss, want[1]) and torch.equal(c.logp, want[2])
     torch.cuda.synchronize()
-    others = [(B.CudaBackend(0), Policy(200, 5003, "bf16", seed=7)) for _ in range(2)]
+    others = [(B.CudaBackend(0), Policy(rows, classes, "bf16", seed=7)) for _ in range(2)]
     torch.cuda.synchronize()
     for _ in range(5):
         for b, o in others:

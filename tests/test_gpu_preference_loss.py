@@ -199,8 +199,9 @@ def test_gradient_against_differences(be, kind):
         assert abs(slope - want) <= 1e-4 * (1 + abs(want))
 
 
-def test_same_bits_replayed_and_two_at_once(be):
-    c = Preference([100, 90, 3, 50], 5003, "bf16", seed=7)
+@pytest.mark.parametrize("lengths,classes", [([100, 90, 3, 50], 5003), ([4, 3], 128003), ([700, 650], 250), ([160, 150], 50001)])
+def test_same_bits_replayed_and_two_at_once(be, lengths, classes):
+    c = Preference(lengths, classes, "bf16", seed=7)
     c(be)
     inside = ~c.outside
     want = c.d.clone(), c.loss.clone(), c.sums.clone()
@@ -218,7 +219,7 @@ def test_same_bits_replayed_and_two_at_once(be):
         graph.replay()
         assert torch.equal(c.d, want[0]) and torch.equal(c.loss, want[1]) and torch.equal(c.sums, want[2])
     torch.cuda.synchronize()
-    others = [(B.CudaBackend(0), Preference([100, 90, 3, 50], 5003, "bf16", seed=7)) for _ in range(2)]
+    others = [(B.CudaBackend(0), Preference(lengths, classes, "bf16", seed=7)) for _ in range(2)]
     torch.cuda.synchronize()
     for _ in range(5):
         for b, o in others:
