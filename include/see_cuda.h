@@ -311,11 +311,12 @@ int see_cuda_join_backward(see_cuda_backend* h, const see_join_shape* shape, con
                            const see_join_weights* gradients, void* workspace, uint64_t workspace_bytes);
 
 /* Losses over rows of logits, with the gradient of the logits.  logits [rows, classes] (1 .. 2^20 classes, up to 2^31 - 1 rows) of any
- * type, stride: elements from a row to the next (0: classes); dlogits: of the same type and stride, NULL: not wanted; it may be logits itself (in place).
- * labels [rows]; a row whose label is not in 0 .. classes - 1 does not count: its logits are not read and its dlogits are zeros.
- * logp = log softmax(logit_scale logits)[label], sums and logp in f32, sums over rows in double.  loss_grad: an f32 that dlogits is
- * multiplied by (the scale of the loss), or NULL.  A row that holds a NaN or +inf, or -inf alone, has a NaN loss and NaN
- * dlogits; finite logits times logit_scale are below 2^127.
+ * type, stride: elements from a row to the next (0: classes); dlogits: of the same type and stride, NULL: not wanted; it may be logits
+ * itself (in place).
+ * labels [rows]; a row whose label is not in 0 .. classes - 1 does not count: what its logits are does not matter, and its dlogits are
+ * zeros.  logp = log softmax(logit_scale logits)[label]: sums over classes in f32, logp and sums over rows in double.  loss_grad: an f32
+ * that dlogits is multiplied by (the scale of the loss), or NULL.  A row that holds a NaN or +inf, or -inf alone, has a NaN loss and NaN
+ * dlogits; finite logits are below 2^126 / logit_scale.
  * The same call has the same bits; the sums' order goes by the sizes, the alignment and the device's number of SMs. */
 enum { SEE_PREFERENCE_SIGMOID = 0, SEE_PREFERENCE_HINGE = 1, SEE_PREFERENCE_SQUARE = 2 };
 /* Sequences 2 i (chosen) and 2 i + 1 (rejected) are a pair; sequence s has the rows starts[s] .. starts[s + 1] - 1 (starts: 2 pairs + 1
@@ -324,8 +325,8 @@ enum { SEE_PREFERENCE_SIGMOID = 0, SEE_PREFERENCE_HINGE = 1, SEE_PREFERENCE_SQUA
  *   h_i = beta ((S - ref)[2 i] - (S - ref)[2 i + 1]) - margin,  loss = the average over pairs of
  *   sigmoid: -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h);  hinge: max(0, 1 - h), no gradient at h = 1;
  *   square: ((h - 1/2) / beta)^2, whose margin is 0.
- * beta > 0; smoothing from 0 on and below 1/2, 0 for the others; pairs: 1 to 2^24.  loss [1], margins [pairs] (h) and sequence_logp [2 pairs] (S)
- * are f32 outputs.  workspace: at least see_cuda_preference_workspace(rows, pairs) bytes, 16-byte aligned. */
+ * beta > 0; smoothing from 0 on and below 1/2, 0 for the others; pairs: 1 to 2^24.  loss [1], margins [pairs] (h) and
+ * sequence_logp [2 pairs] (S) are f32 outputs.  workspace: at least see_cuda_preference_workspace(rows, pairs) bytes, 16-byte aligned. */
 typedef struct see_preference_shape {
   int32_t type, kind;
   float beta, smoothing, margin, logit_scale;
@@ -341,7 +342,7 @@ int see_cuda_preference_loss(see_cuda_backend* h, const see_preference_shape* sh
  *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef kl,  kl = exp(x) - x - 1,
  * and loss [3] = the sums over the rows that count of weight l, weight kl and weight [r A > clip(r) A].  A row clipped so has no
  * gradient but its KL term's.  old_logp, advantages, weights (NULL: 1), ref_logp (NULL: no KL term, kl_coef 0) and the output
- * logp (0 where a row does not count) are [rows] in f32; of rows that do not count nothing is read but the label.  clip_low from 0 to 1,
+ * logp (0 where a row does not count) are [rows] in f32; what they are in rows that do not count does not matter.  clip_low from 0 to 1,
  * clip_high and kl_coef from 0 on, finite.  workspace: at least see_cuda_policy_workspace(rows) bytes, 16-byte aligned. */
 typedef struct see_policy_shape {
   int32_t type;
@@ -357,11 +358,12 @@ int see_cuda_policy_loss(see_cuda_backend* h, const see_policy_shape* shape, con
 /* norm = |grad_scale| (the sum of g^2 over all elements of `count` tensors)^1/2 (grad_scale: an f32, NULL: 1), and
  * factor = grad_scale (norm <= max_norm or norm = 0 ? 1 : max_norm / norm), what see_cuda_adamw_step takes as its grad_scale.  Squares are
  * summed in f32 a few dozen at a time, or in double where f32 would overflow or lose small ones, then in double; norm [1] and
- * factor [1] are f32.  A norm that is infinite has factor 0, one that is NaN a NaN (a step to be left out: read the norm).
- * see_cuda_grad_clip writes g times factor to out besides, rounded to the tensor's type; out may be g (NULL: g), where a factor of 1 then writes nothing.
- * see_cuda_grad_norm ignores out.  `tensors` is HOST memory and is read before the call returns; a tensor of no elements is passed
- * over, whatever its addresses; up to 2^38 elements each.  max_norm > 0 (infinite: the norm alone).  The same call has the same bits; the sums' order goes by the sizes, alignment and the device's
- * number of SMs.  workspace: at least see_cuda_grad_workspace() bytes, 16-byte aligned. */
+ * factor [1] are f32.  Beyond a finite max_norm an infinite norm has factor 0, and a NaN one a NaN: steps to be left out (read the
+ * norm).  see_cuda_grad_clip writes g times factor to out besides, rounded to the tensor's type; out may be g (NULL: g), where a factor
+ * of 1 then writes nothing.  see_cuda_grad_norm ignores out.  `tensors` is HOST memory and is read before the call returns; a tensor of
+ * no elements is passed over, whatever its addresses; up to 2^38 elements each.  max_norm > 0 (infinite: the norm alone).  The same call
+ * has the same bits; the sums' order goes by the sizes, alignment and the device's number of SMs.  workspace: at least
+ * see_cuda_grad_workspace() bytes, 16-byte aligned. */
 typedef struct see_grad_tensor {
   void *g, *out;
   uint64_t n;

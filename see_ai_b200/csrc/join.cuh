@@ -54,8 +54,8 @@ __device__ __forceinline__ void StoreLanes(T* p, const Lane<VEC> (&v)[kLanes<VEC
   StoreCols<T, VEC>(p, f);
 }
 
-// A row at an end of the matrix for the ring, without anything beside it: its 16-byte units are copied in bulk, the elements before and behind them (fewer than 16 bytes each) by the
-// group's threads.  The row begins `skip` bytes into its slot.
+// A row at an end of the matrix for the ring, without anything beside it: its 16-byte units are copied in bulk, the elements before and
+// behind them (fewer than 16 bytes each) by the group's threads.  The row begins `skip` bytes into its slot.
 template <typename T>
 struct EndRow {
   const uint8_t* from;         // the units

@@ -2,11 +2,11 @@
 //   norm = |grad_scale| (sum g^2)^1/2,   factor = grad_scale min(1, max_norm / norm),   out = g factor
 // Bound by HBM: each gradient is read once, and once more (from L2, as far as it holds them) and written where it is clipped.
 //
-// All tensors' units of 16 bytes, one tensor behind the other, are cut into equal ranges, one to a thread block, which walks its own eight accesses
-// to a thread at a time.  (Chunks of 32 KB taken in turn: 43 us for 87 million elements of bf16, for a last round of few chunks.)  Units that are
-// no whole 16 bytes of their tensor are taken element by element.  A thread's squares of one step are summed in f32, 32 to 64 of them; where that
-// sum is not finite or so small that squares may have been lost, they are summed again in double.  What is beyond is double: the
-// blocks' sums meet in the workspace and are added in a fixed order.
+// All tensors' units of 16 bytes, one tensor behind the other, are cut into equal ranges, one to a thread block, which walks its own
+// eight accesses to a thread at a time.  (Chunks of 32 KB taken in turn: 43 us for 87 million elements of bf16, for a last round of few
+// chunks.)  Units that are no whole 16 bytes of their tensor are taken element by element.  A thread's squares of one step are summed in
+// f32, 32 to 64 of them; where that sum is not finite or so small that squares may have been lost, they are summed again in double.
+// What is beyond is double: the blocks' sums meet in the workspace and are added in a fixed order.
 #include "block_ops.h"
 #include "launch.cuh"
 #include "vec_types.cuh"

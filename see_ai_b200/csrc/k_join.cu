@@ -187,8 +187,8 @@ JoinBwdKernel(const __grid_constant__ JoinArgs a) {
   }
 }
 
-// The blocks' partial sums of 32 columns, blockIdx.y 0: P1 and P2, 1: S1 and S2.  Half of the warps add a sum's rows w, w + 16, ... (rms: all of them, w + 32); then
-// the warps' sums in order; then the weights' gradients.
+// The blocks' partial sums of 32 columns, blockIdx.y 0: P1 and P2, 1: S1 and S2.  Half of the warps add a sum's rows w, w + 16, ...
+// (rms: all of them, w + 32); then the warps' sums in order; then the weights' gradients.
 __global__ void __launch_bounds__(1024)
 JoinFoldKernel(const __grid_constant__ JoinArgs a, uint32_t blocks, int rms) {
   AwaitPrevious();

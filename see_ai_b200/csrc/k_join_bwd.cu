@@ -1,8 +1,8 @@
 // The backward pass of a block's join to the residual stream for rows of up to 8192 columns (k_join.cu has the formulas).
 //
-// As in the forward pass a row belongs to a group of T threads and reaches it through a ring, here all four of its matrices at once.  A thread
-// has the same columns in every row, so that the four sums over rows stay in its registers; a block's groups meet in shared memory,
-// the blocks in JoinFoldKernel, in a fixed order.
+// As in the forward pass a row belongs to a group of T threads and reaches it through a ring, here all four of its matrices at once.  A
+// thread has the same columns in every row, so that the four sums over rows stay in its registers; a block's groups meet in shared
+// memory, the blocks in JoinFoldKernel, in a fixed order.
 #include "join.cuh"
 
 namespace see::k {
@@ -217,8 +217,8 @@ cudaError_t Pick(const JoinArgs& a, uint32_t sms, cudaStream_t s, uint32_t* grid
       if (n <= T) return Run<XT, YT, kRms, 4, 1, kThreads>(a, T, sms, s, grid);
       if (n <= 2 * T) return Run<XT, YT, kRms, 4, 2, kThreads>(a, T, sms, s, grid);
     }
-    // Rms norms: a warp's row, which needs no barriers, of up to 768 columns of 16 bits (32768 rows 58 us, on 64 threads 72; an f32 stream's rows leave the
-    // ring too few of them: 88, 83).
+    // Rms norms: a warp's row, which needs no barriers, of up to 768 columns of 16 bits (32768 rows 58 us, on 64 threads 72; an f32
+    // stream's rows leave the ring too few of them: 88, 83).
     if constexpr (kRms && sizeof(XT) == 2)
       if (n > 128 && n <= 192) return Run<XT, YT, kRms, 4, 6, 384>(a, 32, sms, s, grid);
     const uint32_t T = Warps((n + 3) / 4), each = (n + T - 1) / T;

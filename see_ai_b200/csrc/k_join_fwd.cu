@@ -1,8 +1,8 @@
 // The forward pass of a block's join to the residual stream for rows of up to 8192 columns (k_join.cu has the formulas).
 //
 // A row belongs to a group of T threads, which hold it in registers, four consecutive columns at a time or, where addresses or widths do
-// not allow that, single ones T apart.  x and block reach the groups through rings in shared memory, filled by bulk copies; the weights, the gate
-// already times the first norm's, lie there beside them.
+// not allow that, single ones T apart.  x and block reach the groups through rings in shared memory, filled by bulk copies; the weights,
+// the gate already times the first norm's, lie there beside them.
 #include "join.cuh"
 
 namespace see::k {

@@ -6,9 +6,9 @@
 // slope being the loss's derivative by logp.  The product k M is rounded once and the same in every exponent of a row, so that its
 // rounding cancels between e_c and s.  Bound by HBM: logits are read once, dlogits written once.
 //
-// A row is walked in units of 16 bytes by address, of which the first and the last may stick out of it, whatever its alignment.  Rows reach
-// registers through a ring in shared memory (LogitRowsKernel); wide rows, and few ones, are shared by the blocks of a cluster.  What
-// is wider still is walked twice (LogitStreamKernel).
+// A row is walked in units of 16 bytes by address, of which the first and the last may stick out of it, whatever its alignment.  Rows
+// reach registers through a ring in shared memory (LogitRowsKernel); wide rows, and few ones, are shared by the blocks of a cluster.
+// What is wider still is walked twice (LogitStreamKernel).
 //
 // logp is made in double: a sequence's sum of hundreds of them is held against a reference's.
 #include <type_traits>
@@ -41,7 +41,10 @@ __device__ __forceinline__ void Elements(uint4 r, float* v) {
 }
 
 // -inf, and 16 bytes of it.
-template <typename T> __device__ __forceinline__ constexpr uint32_t NoElement() { return sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, Bf16> ? 0xFF80u : 0xFC00u; }
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t NoElement() {
+  return sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, Bf16> ? 0xFF80u : 0xFC00u;
+}
 template <typename T>
 __device__ __forceinline__ uint4 Nothing() {
   const uint32_t w = sizeof(T) == 4 ? NoElement<T>() : NoElement<T>() * 0x10001u;
@@ -187,8 +190,8 @@ __device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, float advan
 __device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, const PolicyRow& row, double logp) {
   return PolicyOf(p, row.advantage, static_cast<float>(logp - static_cast<double>(row.old)), static_cast<float>(static_cast<double>(row.ref) - logp));
 }
-// The loss's weighted derivative by a row's logp.  Of 16-bit logits it goes into dlogits of 8 or 11 bits: logp in f32, a millionth off, is
-// enough, and takes each warp 20 instructions instead of 100; of f32 logits the double one.
+// The loss's weighted derivative by a row's logp.  Of 16-bit logits it goes into dlogits of 8 or 11 bits: logp in f32, a millionth off,
+// is enough, and takes each warp 20 instructions instead of 100; of f32 logits the double one.
 template <typename T>
 __device__ __forceinline__ float SlopeOf(const LogitArgs& a, const PolicyArgs& p, const PolicyRow& row, const RowSums& q) {
   if constexpr (sizeof(T) == 4) {
@@ -215,8 +218,8 @@ __device__ __forceinline__ float WarpMax(float v) {
 
 constexpr uint32_t kFinishThreads = 256;
 
-// From what is kept of the rows: logp and the loss's three sums, a block's rows in its partials; the block that comes last (*arrived, which the rows'
-// kernel has set to 0) adds them up, in the blocks' order.
+// From what is kept of the rows: logp and the loss's three sums, a block's rows in its partials; the block that comes last (*arrived,
+// which the rows' kernel has set to 0) adds them up, in the blocks' order.
 __global__ void __launch_bounds__(kFinishThreads)
 PolicyFinishKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const float4* __restrict__ kept,
                    double* __restrict__ partials, uint32_t* __restrict__ arrived) {
@@ -283,9 +286,11 @@ struct Sequences {
 };
 
 // ---- rows in registers --------------------------------------------------------------------------------------
-// A group of T threads holds a row, or where C blocks of a cluster share it, its part of `part` units: NU units to a thread, first as they lie in memory, then
-// as e relative to the thread's own maximum.  One exponential an element and no second reading: 8192 rows of 32000 in bf16 would take 4000 cycles of an
-// SM's exponential units a row with two, of the 5500 that HBM takes.  The rows that a group comes to next are on their way into its slots meanwhile.
+// A group of threads holds a row in registers as it lies in memory, NU units to a thread, or, where the blocks of a cluster share it, its
+// part.  Exponentials are made twice, for the sums and for dlogits: 64 elements of 16 bits take 32 registers so, and two rows are at work
+// on an SM at a time, one while the other's sums meet (8192 rows of 32000 in bf16 172 us; with the first exponentials kept, one row to an
+// SM, 198).  Two exponentials an element take 4000 cycles of an SM's units a row, of the 5500 that HBM takes.  The rows that a group comes
+// to next are on their way into its slots meanwhile.
 template <typename T> constexpr int kPairs = kPerUnit<T> / 2;
 template <typename T>
 __device__ __forceinline__ void Pairs(const uint4& r, f32x2 (&v)[kPairs<T>]) {
@@ -350,8 +355,8 @@ __device__ __forceinline__ bool AwaitCluster(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
-// How a launch shares its rows: `threads` threads and `blocks` blocks of a cluster to a row, `part` units to a block.  Rows from `edge` on to
-// `edge` before the last are copied in bulk: what sticks out of theirs is the matrix's too.
+// How a launch shares its rows: `threads` threads and `blocks` blocks of a cluster to a row, `part` units to a block.  Rows from `edge`
+// on to `edge` before the last are copied in bulk: what sticks out of theirs is the matrix's too.
 struct RowsPlan {
   uint32_t threads, over_threads, slots, blocks, part, edge;   // over_threads: 2^32 / threads, rounded up
 };
@@ -401,7 +406,8 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     umma_dev::MbarExpectTx(&bars[slot], bytes);
     umma_dev::BulkLoad(ring + static_cast<size_t>(slot) * slot_bytes, reinterpret_cast<const uint4*>(z - skip) + begin, bytes, &bars[slot]);
   };
-  // What a row brings besides its logits is asked for while the one before it is at work: each item by one of the group's first threads, as it is read.
+  // What a row brings besides its logits is asked for while the one before it is at work: each item by one of the group's first threads,
+  // as it is read.
   uint32_t ahead = 0;
   auto ask = [&](uint32_t r, int32_t label) {
     if (r >= rows || t > (kPolicy ? 4u : 0u) || !counts(r, label)) return;
@@ -487,8 +493,8 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
       for (int i = 0; i < NU; ++i) raw[i] = t + i * threads < count ? mine[t + i * threads] : Nothing<T>();
     }
     float mk = __fmul_rn(Largest<T, NU>(raw), a.k), sum;   // -inf: nothing here
-    // A lone slot is filled while the exponentials are made, unless dlogits will be stored meanwhile: loads and stores in turn are faster then
-    // (8192 rows of 32000 in bf16: 172 us, early 184; a preference loss's rows 84, early 76).
+    // A lone slot is filled while the exponentials are made, unless dlogits will be stored meanwhile: loads and stores in turn are
+    // faster then (8192 rows of 32000 in bf16: 172 us, early 184; a preference loss's rows 84, early 76).
     const bool early = plan.slots == 1 && !(kPolicy && a.dlogits);
     if (early) {
       GroupBarrier(threads, group);
@@ -636,8 +642,8 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
 }
 
 // ---- short rows ------------------------------------------------------------------------------------------------
-// Rows of up to 128 units, more than a few: a warp to a row, straight into registers, the next row asked for while this one is at work.  Their time is
-// instructions: 16384 rows of 250 in bf16 with the ring's bookkeeping 29 us, so 18.5; 65536 in f32 64, so 52.
+// Rows of up to 128 units, more than a few: a warp to a row, straight into registers, the next row asked for while this one is at work.
+// Their time is instructions: 16384 rows of 250 in bf16 with the ring's bookkeeping 29 us, so 18.5; 65536 in f32 64, so 52.
 constexpr uint32_t kShortThreads = 256;
 template <typename T, int NU, bool kPolicy>
 __global__ void __launch_bounds__(kShortThreads)
@@ -749,9 +755,9 @@ LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Po
 }
 
 // ---- rows as streams ----------------------------------------------------------------------------------------
-// Rows wider than a cluster's registers (and others: RunRows): a group of 256 threads walks a row 16 KB at a time (four units a thread) through its ring: first
-// for the sums, then, a policy loss's, from L2 for dlogits.  The ring runs ahead over both walks and into the next row, so that loads never pause while
-// sums meet; the other groups of the SM compute meanwhile.
+// Rows wider than a cluster's registers (and others: RunRows): a group of 256 threads walks a row 16 KB at a time (four units a thread)
+// through its ring: first for the sums, then, a policy loss's, from L2 for dlogits.  The ring runs ahead over both walks and into the
+// next row, so that loads never pause while sums meet; the other groups of the SM compute meanwhile.
 constexpr uint32_t kWalkers = 256, kWalkUnits = 4, kChunk = kWalkers * kWalkUnits;   // threads of a group; units to a thread, and in a chunk
 constexpr uint32_t kStreams = 3, kStreamSlots = (kMostShared - 8192) / (kStreams * kChunk * 16);   // groups to an SM, and chunks on their way to each
 
@@ -825,7 +831,8 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
     if (++f_slot == kStreamSlots) f_slot = 0;
     if (++f_chunk == w.chunks * (twice ? 2 : 1)) next_row();
   };
-  // What a row brings besides its logits is asked for while the one before it is at work: each item by one of the group's first threads, as it is read.
+  // What a row brings besides its logits is asked for while the one before it is at work: each item by one of the group's first threads,
+  // as it is read.
   uint32_t ahead = 0;
   auto ask = [&](uint32_t r, int32_t label) {
     if (r >= rows || t > (kPolicy ? 4u : 0u) || !counts(r, label)) return;
@@ -983,8 +990,9 @@ __device__ __forceinline__ double Softplus(double x) { return (x > 0.0 ? x : 0.0
 
 constexpr uint32_t kPairThreads = 512;
 
-// A pair to a block: the first eight warps sum the chosen rows, the others the rejected ones.  Then each row's kept.x becomes the
-// loss's derivative by its logp, logit_scale and loss_grad included, 0 where it does not count.  losses [pairs]: added up by PreferenceFoldKernel.
+// A pair to a block: the first eight warps sum the chosen rows, the others the rejected ones.  Then each row's kept.x becomes the loss's
+// derivative by its logp, logit_scale and loss_grad included, 0 where it does not count.  losses [pairs]: added up by
+// PreferenceFoldKernel.
 __global__ void __launch_bounds__(kPairThreads)
 PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PreferenceArgs p, float4* __restrict__ kept) {
   AwaitPrevious();
@@ -1224,9 +1232,9 @@ cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& se
     return Next(LogitShortKernel<T, 4, kPolicy>, grid, kShortThreads, 0, s)(a, p, seq, kept, arrived);
   }
   Sharing w;
-  // Of a preference loss's rows, which have no second walk, those of more than half of an SM's threads too: 768 rows of 128256 in bf16 107 us with pairs and
-  // gradient, in clusters 119; 1500 of 50001 in f16 98, one row to an SM 101.  A policy loss's second walk costs more than that: 8192 rows of 32000 in bf16
-  // 227 us, in registers 172; 2048 of 128256 254, in clusters 204.
+  // Of a preference loss's rows, which have no second walk, those of more than half of an SM's threads too: 768 rows of 128256 in bf16
+  // 107 us with pairs and gradient, in clusters 119; 1500 of 50001 in f16 98, one row to an SM 101.  A policy loss's second walk costs
+  // more than that: 8192 rows of 32000 in bf16 227 us, in registers 172; 2048 of 128256 254, in clusters 204.
   if (!ShareRows<T>(a, sms, &w) || (!kPolicy && a.rows > 2 * sms && w.threads > kThreads / 2)) {
     constexpr auto* kernel = LogitStreamKernel<T, kPolicy>;
     constexpr size_t bytes = kStreams * kStreamSlots * kChunk * 16;
