@@ -8,7 +8,8 @@
 //
 // A row is walked in units of 16 bytes by address, of which the first and the last may stick out of it, whatever its alignment.  Rows
 // reach registers through a ring in shared memory (LogitRowsKernel); wide rows, and few ones, are shared by the blocks of a cluster.
-// What is wider still is walked twice (LogitStreamKernel).
+// A policy loss's rows that are wider still are walked twice (LogitStreamKernel), a preference loss's that are many and wide go through
+// rings of single warps (LogitSumsKernel).
 //
 // logp is made in double: a sequence's sum of hundreds of them is held against a reference's.
 #include <type_traits>
@@ -494,7 +495,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     }
     float mk = __fmul_rn(Largest<T, NU>(raw), a.k), sum;   // -inf: nothing here
     // A lone slot is filled while the exponentials are made, unless dlogits will be stored meanwhile: loads and stores in turn are
-    // faster then (8192 rows of 32000 in bf16: 172 us, early 184; a preference loss's rows 84, early 76).
+    // faster then (8192 rows of 32000 in bf16: 172 us, early 184; a preference loss of 16 x 512 x 16001 in f32 357, early 344).
     const bool early = plan.slots == 1 && !(kPolicy && a.dlogits);
     if (early) {
       GroupBarrier(threads, group);
@@ -754,16 +755,203 @@ LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Po
   }
 }
 
+// ---- rows for their sums alone ----------------------------------------------------------------------------------
+// A preference loss's rows, whose pairs decide on dlogits first, many of them and wide: `warps` warps of a block to a row, each with a ring
+// of its own that runs ahead over its chunks of the block's rows.  (A group's ring costs a barrier a chunk.)  A policy loss that wants no
+// dlogits would gain from it too (8192 rows of 32000 in bf16 109 us, so 93), but would not have the bits of the one that does.
+//
+// Only rows that count cost anything, and where they lie is known to the device alone.  So every block counts over the labels of a window
+// of rows and lists each gridDim.x-th that counts for itself.  Each gridDim.x-th of all rows left an SM with 13 % more than its share of
+// 8 pairs' answers: their sums took 88 us, so 78.
+constexpr uint32_t kSumThreads = 768, kSumWarps = 8;   // kSumWarps: to a row, at most
+constexpr uint32_t kSumUnits = 8, kSumChunk = kSumUnits * 32, kSumSlots = 2;   // units to a lane, and to a warp, at a time; chunks on their way to a warp
+constexpr uint32_t kListed = 512, kCounted = 32768;   // rows of a block, and of a window, at most
+template <typename T>
+__global__ void __launch_bounds__(kSumThreads, 1)
+LogitSumsKernel(const __grid_constant__ LogitArgs a, const Sequences seq, float4* __restrict__ kept, uint32_t warps, uint32_t window) {
+  constexpr uint32_t E = kPerUnit<T>;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ float2 sums[2][kSumThreads / 32];   // k M and the sum, of a warp
+  __shared__ uint32_t before[kSumThreads / 32];
+  __shared__ uint64_t all_bars[kSumThreads / 32][kSumSlots];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / warps, part = warp - group * warps, groups = kSumThreads / 32 / warps;
+  uint4* ring = reinterpret_cast<uint4*>(dyn) + warp * kSumSlots * kSumChunk;
+  int2* list = reinterpret_cast<int2*>(dyn + kSumThreads / 32 * kSumSlots * kSumChunk * 16);   // [kListed] row and label
+  uint32_t* masks = reinterpret_cast<uint32_t*>(list + kListed);                               // [kCounted / 32]
+  uint64_t* bars = all_bars[warp];
+  if (lane == 0) {
+    for (uint32_t i = 0; i < kSumSlots; ++i) umma_dev::MbarInit(&bars[i], 1);
+    umma_dev::MbarInitFence();
+  }
+  AwaitPrevious();
+  const uint32_t rows_begin = static_cast<uint32_t>(max(seq.starts[0], 0));
+  const uint32_t rows_end = min(static_cast<uint32_t>(a.rows), static_cast<uint32_t>(max(seq.starts[seq.count], 0)));
+  const uint64_t begin = reinterpret_cast<uint64_t>(a.logits), end = begin + ((a.rows - 1) * a.stride + a.classes) * sizeof(T);
+  // Whether these units of a row can be copied whole: the matrix's first and last may begin before it or end behind it.
+  auto bulk = [&](const uint4* from, uint32_t units) {
+    return reinterpret_cast<uint64_t>(from) >= begin && reinterpret_cast<uint64_t>(from + units) <= end;
+  };
+  const uint32_t stride_units = warps * kSumChunk;   // of a warp's chunks in a row
+  uint32_t slot = 0, parities = 0;                   // a bit for each slot, of the copies that went through it
+  const f32x2 k2 = Splat2(a.k);
+  auto factor = [](float own, float all) { return own == MinusInf() ? 0.0f : Ex2Approx(own - all); };
+  uint32_t turn = 0;
+  for (uint32_t base = rows_begin; base < rows_end; base += window) {
+    const uint32_t count = min(window, rows_end - base), words = (count + 31) / 32;   // a bit for each row, set if it counts
+#pragma unroll 8
+    for (uint32_t w = warp; w < words; w += kSumThreads / 32) {
+      const uint32_t i = w * 32 + lane;
+      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, i < count && Counts(a.labels[base + min(i, count - 1)], a.classes));
+      if (lane == 0) masks[w] = mask;
+    }
+    __syncthreads();
+    const uint32_t m0 = 2 * threadIdx.x < words ? masks[2 * threadIdx.x] : 0, m1 = 2 * threadIdx.x + 1 < words ? masks[2 * threadIdx.x + 1] : 0;
+    const uint32_t own = __popc(m0) + __popc(m1);
+    uint32_t at = own;
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o *= 2) {
+      const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, at, o);
+      if (lane >= o) at += v;
+    }
+    if (lane == 31) before[warp] = at;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kSumThreads / 32; ++w) {
+      if (w < warp) at += before[w];
+      all += before[w];
+    }
+    at -= own;   // rows that count, before this thread's
+    const uint32_t apart = gridDim.x, which = blockIdx.x;
+    for (uint32_t n = at + (which + apart - at % apart) % apart; n < at + own; n += apart) {   // this block's among this thread's
+      uint32_t i = n - at, m = m0, word = 2 * threadIdx.x;
+      if (i >= __popc(m0)) {
+        i -= __popc(m0);
+        m = m1;
+        ++word;
+      }
+      for (; i != 0; --i) m &= m - 1;
+      const uint32_t r = base + word * 32 + __ffs(static_cast<int>(m)) - 1;
+      list[n / apart] = make_int2(static_cast<int>(r), a.labels[r]);
+    }
+    const uint32_t listed = all > which ? (all - which - 1) / apart + 1 : 0;
+    __syncthreads();
+    // The chunk that is asked for next (by lane 0), ahead of the one at work.
+    uint32_t f_row = group, f_unit = 0, f_units = 0, f_slot = slot;
+    const uint4* f_from = nullptr;
+    auto fill = [&] {
+      if (lane != 0) return;
+      while (f_unit >= f_units) {   // the next row (one may be too narrow for this warp)
+        if (f_row >= listed) return;
+        const Row<T> row(a, static_cast<uint32_t>(list[f_row].x));
+        f_row += groups;
+        f_from = reinterpret_cast<const uint4*>(row.z - row.skip);
+        f_units = row.units;
+        f_unit = part * kSumChunk;
+      }
+      const uint32_t units = min(kSumChunk, f_units - f_unit);
+      if (bulk(f_from + f_unit, units)) {
+        umma_dev::MbarExpectTx(&bars[f_slot], units * 16);
+        umma_dev::BulkLoad(ring + f_slot * kSumChunk, f_from + f_unit, units * 16, &bars[f_slot]);
+      }
+      if (++f_slot == kSumSlots) f_slot = 0;
+      f_unit += stride_units;
+    };
+#pragma unroll 1
+    for (uint32_t i = 0; i < kSumSlots; ++i) fill();
+    for (uint32_t i = group; i < listed; i += groups) {
+      const uint32_t r = static_cast<uint32_t>(list[i].x);
+      const int32_t label = list[i].y;
+      const Row<T> row(a, r);
+      uint32_t label_bits = 0;
+      if (part == 0 && lane == 0) label_bits = reinterpret_cast<const std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>*>(row.z)[label];
+      const uint32_t label_unit = (static_cast<uint32_t>(label) + row.skip) / E, ends_at = row.skip + a.classes;
+      const uint4* from = reinterpret_cast<const uint4*>(row.z - row.skip);
+      float mk = MinusInf(), sum = 0.0f;   // k M and the sum relative to it, of the others
+      for (uint32_t u0 = part * kSumChunk; u0 < row.units; u0 += stride_units) {
+        uint4 raw[kSumUnits];
+        const uint32_t u1 = u0 + kSumChunk, units = min(kSumChunk, row.units - u0);
+        if (bulk(from + u0, units)) {
+          AwaitRow(&bars[slot], parities >> slot & 1u, a.status);
+          parities ^= 1u << slot;
+          const uint4* in = ring + slot * kSumChunk + lane;
+#pragma unroll
+          for (uint32_t j = 0; j < kSumUnits; ++j) raw[j] = lane + j * 32 < units ? in[j * 32] : Nothing<T>();
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < kSumUnits; ++j) raw[j] = lane + j * 32 < units ? row.Raw(u0 + lane + j * 32) : Nothing<T>();
+        }
+        if (++slot == kSumSlots) slot = 0;
+        if ((u0 == 0 && row.skip != 0) || u1 * E > ends_at || (label_unit >= u0 && label_unit < u1)) {   // -inf in place of the label and of what sticks out
+#pragma unroll
+          for (uint32_t j = 0; j < kSumUnits; ++j) {
+            const uint32_t u = u0 + lane + j * 32;
+            const int32_t e0 = static_cast<int32_t>(u * E);
+            if ((u == 0 && row.skip != 0) || u == row.units - 1 || u == label_unit)
+              raw[j] = Only<T>(raw[j], static_cast<int32_t>(row.skip) - e0, static_cast<int32_t>(ends_at) - e0, label + static_cast<int32_t>(row.skip) - e0);
+          }
+        }
+        const float top = fmaxf(mk, __fmul_rn(Largest<T, kSumUnits>(raw), a.k));
+        __syncwarp();   // the slot is read
+        fill();
+        const f32x2 away = Splat2(top == MinusInf() ? 0.0f : -top);
+        f32x2 sum2[2] = {};
+#pragma unroll
+        for (uint32_t j = 0; j < kSumUnits; ++j) {
+          f32x2 v[kPairs<T>];
+          Pairs<T>(raw[j], v);
+#pragma unroll
+          for (int l = 0; l < kPairs<T>; ++l) sum2[l & 1] = AddF2(sum2[l & 1], Powers(Fma2(v[l], k2, away)));
+        }
+        float lo, hi;
+        UnpackF2(AddF2(sum2[0], sum2[1]), &lo, &hi);
+        sum = fmaf(sum, factor(mk, top), lo + hi);
+        mk = top;
+      }
+      // Lanes, warps: the largest k M, and sums relative to it.
+      auto join = [&](uint32_t most) {
+        const float top = WarpMax(mk);   // (beyond `most` the lanes repeat themselves)
+        sum *= factor(mk, top);
+        mk = top;
+#pragma unroll
+        for (uint32_t o = 16; o > 0; o >>= 1)
+          if (o <= most) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      };
+      join(16);
+      if (warps > 1) {
+        float2* set = sums[turn] + group * warps;
+        if (lane == 0) set[part] = make_float2(mk, sum);
+        GroupBarrier(warps * 32, group);
+        turn ^= 1;
+        if (part != 0) continue;
+        const float2 warp_part = (lane & (kSumWarps - 1)) < warps ? set[lane & (kSumWarps - 1)] : make_float2(MinusInf(), 0.0f);
+        mk = warp_part.x;
+        sum = warp_part.y;
+        join(kSumWarps / 2);
+      }
+      if (lane != 0) continue;
+      T raw_label;
+      if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(label_bits);
+      else raw_label.bits = static_cast<uint16_t>(label_bits);
+      const float z_label = ToF32(raw_label), mk_label = __fmul_rn(z_label, a.k), top = fmaxf(mk, mk_label);
+      RowSums q = {z_label, top == MinusInf() ? 0.0f : top, sum * factor(mk, top), 0.0f};
+      q.s = q.others + LabelTerm(a, z_label, q.mk);
+      kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
+    }
+    __syncthreads();   // the list is read
+  }
+}
+
 // ---- rows as streams ----------------------------------------------------------------------------------------
-// Rows wider than a cluster's registers (and others: RunRows): a group of 256 threads walks a row 16 KB at a time (four units a thread)
-// through its ring: first for the sums, then, a policy loss's, from L2 for dlogits.  The ring runs ahead over both walks and into the
-// next row, so that loads never pause while sums meet; the other groups of the SM compute meanwhile.
+// A policy loss's rows wider than a cluster's registers: a group of 256 threads walks a row 16 KB at a time (four units a thread) through
+// its ring, first for the sums, then, from L2, for dlogits.  The ring runs ahead over both walks and into the next row, so that loads
+// never pause while sums meet; the other groups of the SM compute meanwhile.
 constexpr uint32_t kWalkers = 256, kWalkUnits = 4, kChunk = kWalkers * kWalkUnits;   // threads of a group; units to a thread, and in a chunk
 constexpr uint32_t kStreams = 3, kStreamSlots = (kMostShared - 8192) / (kStreams * kChunk * 16);   // groups to an SM, and chunks on their way to each
 
-template <typename T, bool kPolicy>
+template <typename T>
 __global__ void __launch_bounds__(kStreams * kWalkers, 1)
-LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const Sequences seq, float4* __restrict__ kept,
+LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, float4* __restrict__ kept,
                   uint32_t* __restrict__ arrived) {
   constexpr uint32_t E = kPerUnit<T>;
   extern __shared__ __align__(128) uint8_t dyn[];
@@ -774,17 +962,13 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
   uint4* ring = reinterpret_cast<uint4*>(dyn) + group * kStreamSlots * kChunk;
   uint64_t* bars = all_bars[group];
   const uint32_t rows = static_cast<uint32_t>(a.rows), step = gridDim.x * kStreams, first = group * gridDim.x + blockIdx.x;   // (every SM gets rows before one gets two)
-  const bool twice = kPolicy && a.dlogits;
+  const bool twice = a.dlogits != nullptr;
   if (t == 0) {
     for (uint32_t i = 0; i < kStreamSlots; ++i) umma_dev::MbarInit(&bars[i], 1);
     umma_dev::MbarInitFence();
   }
   AwaitPrevious();
   auto logit_row = [&](uint32_t r) { return static_cast<const T*>(a.logits) + static_cast<uint64_t>(r) * a.stride; };
-  auto counts = [&](uint32_t r, int32_t label) {
-    if (!Counts(label, a.classes)) return false;
-    return kPolicy || (static_cast<int64_t>(r) >= seq.starts[0] && static_cast<int64_t>(r) < seq.starts[seq.count]);
-  };
   // A row's units and chunks, and whether a chunk can be copied whole: the matrix's first and last may begin before it or end behind it.
   struct Walk {
     const uint4* from;
@@ -820,7 +1004,7 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
       f_next = f_row + step < rows ? a.labels[f_row + step] : -1;
       f_chunk = 0;
     };
-    while (f_row < rows && f_chunk == 0 && !counts(f_row, f_label)) next_row();
+    while (f_row < rows && f_chunk == 0 && !Counts(f_label, a.classes)) next_row();
     if (f_row >= rows) return;
     const Walk w = walk_of(f_row);
     const uint32_t chunk = f_chunk < w.chunks ? f_chunk : f_chunk - w.chunks, units = min(kChunk, w.units - chunk * kChunk);
@@ -835,7 +1019,7 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
   // as it is read.
   uint32_t ahead = 0;
   auto ask = [&](uint32_t r, int32_t label) {
-    if (r >= rows || t > (kPolicy ? 4u : 0u) || !counts(r, label)) return;
+    if (r >= rows || t > 4 || !Counts(label, a.classes)) return;
     if (t == 0) ahead = reinterpret_cast<const std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>*>(logit_row(r))[label];
     else if (t == 1) ahead = __float_as_uint(p.old_logp[r]);
     else if (t == 2) ahead = p.ref_logp ? __float_as_uint(p.ref_logp[r]) : 0u;
@@ -844,8 +1028,8 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
   };
 #pragma unroll 1
   for (uint32_t i = 0; i < kStreamSlots; ++i) fill();
-  const float grad = (kPolicy && p.loss_grad ? *p.loss_grad : 1.0f) * a.scale;
-  if (kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
+  const float grad = (p.loss_grad ? *p.loss_grad : 1.0f) * a.scale;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
   int32_t next_label = first < rows ? a.labels[first] : -1, label_behind = first + step < rows ? a.labels[first + step] : -1;
   ask(first, next_label);
   __syncwarp();
@@ -858,11 +1042,9 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
     const uint32_t item = ahead;
     ask(r + step, next_label);
     const Row<T> row(a, r);
-    if (!counts(r, label)) {
-      if (twice) {
-        const float none[E] = {};
-        for (uint32_t u = t; u < row.units; u += kWalkers) row.Store(u, none);
-      }
+    if (!Counts(label, a.classes)) {
+      const float none[E] = {};
+      for (uint32_t u = t; twice && u < row.units; u += kWalkers) row.Store(u, none);
       continue;
     }
     const Walk w = walk_of(r);
@@ -944,42 +1126,40 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
     RowSums q = {z_label, all == MinusInf() ? 0.0f : all, sum * factor(mk, all), 0.0f};
     q.s = q.others + LabelTerm(a, z_label, q.mk);
     if (t == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
-    if constexpr (kPolicy) {
-      if (!twice) continue;
-      const PolicyRow brings = {__uint_as_float(items[1]), __uint_as_float(items[2]), __uint_as_float(items[3]), __uint_as_float(items[4])};
-      const float slope = SlopeOf<T>(a, p, brings, q) * grad;   // (0: zeros come out)
-      const f32x2 by = Splat2(-slope / q.s), away = Splat2(-q.mk);
-      for (uint32_t chunk = 0; chunk < w.chunks; ++chunk) {
-        read(chunk);
-        uint4 out[kWalkUnits];
+    if (!twice) continue;
+    const PolicyRow brings = {__uint_as_float(items[1]), __uint_as_float(items[2]), __uint_as_float(items[3]), __uint_as_float(items[4])};
+    const float slope = SlopeOf<T>(a, p, brings, q) * grad;   // (0: zeros come out)
+    const f32x2 by = Splat2(-slope / q.s), away = Splat2(-q.mk);
+    for (uint32_t chunk = 0; chunk < w.chunks; ++chunk) {
+      read(chunk);
+      uint4 out[kWalkUnits];
+#pragma unroll
+      for (uint32_t i = 0; i < kWalkUnits; ++i) {
+        f32x2 pair[kPairs<T>];
+        float v[E];
+        Pairs<T>(raw[i], pair);
+#pragma unroll
+        for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(Powers(Fma2(pair[j], k2, away)), by), &v[2 * j], &v[2 * j + 1]);
+        if constexpr (sizeof(T) == 4) out[i] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        else out[i] = make_uint4(Pack2<T>(v[0], v[1]), Pack2<T>(v[2], v[3]), Pack2<T>(v[4], v[5]), Pack2<T>(v[6], v[7]));
+      }
+      GroupBarrier(kWalkers, group);   // the slot is read
+      fill();
+      const uint32_t u0 = chunk * kChunk + t;
+      if (row.alike && (chunk != 0 || w.skip == 0) && (chunk + 1) * kChunk * E <= ends_at) {
+        uint4* to = reinterpret_cast<uint4*>(row.d - w.skip) + u0;
+#pragma unroll
+        for (uint32_t i = 0; i < kWalkUnits; ++i) to[i * kWalkers] = out[i];
+      } else {
 #pragma unroll
         for (uint32_t i = 0; i < kWalkUnits; ++i) {
-          f32x2 pair[kPairs<T>];
+          if (u0 + i * kWalkers >= w.units) continue;
           float v[E];
-          Pairs<T>(raw[i], pair);
-#pragma unroll
-          for (int j = 0; j < kPairs<T>; ++j) UnpackF2(Mul2(Powers(Fma2(pair[j], k2, away)), by), &v[2 * j], &v[2 * j + 1]);
-          if constexpr (sizeof(T) == 4) out[i] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-          else out[i] = make_uint4(Pack2<T>(v[0], v[1]), Pack2<T>(v[2], v[3]), Pack2<T>(v[4], v[5]), Pack2<T>(v[6], v[7]));
+          Elements<T>(out[i], v);
+          row.Store(u0 + i * kWalkers, v);
         }
-        GroupBarrier(kWalkers, group);   // the slot is read
-        fill();
-        const uint32_t u0 = chunk * kChunk + t;
-        if (row.alike && (chunk != 0 || w.skip == 0) && (chunk + 1) * kChunk * E <= ends_at) {
-          uint4* to = reinterpret_cast<uint4*>(row.d - w.skip) + u0;
-#pragma unroll
-          for (uint32_t i = 0; i < kWalkUnits; ++i) to[i * kWalkers] = out[i];
-        } else {
-#pragma unroll
-          for (uint32_t i = 0; i < kWalkUnits; ++i) {
-            if (u0 + i * kWalkers >= w.units) continue;
-            float v[E];
-            Elements<T>(out[i], v);
-            row.Store(u0 + i * kWalkers, v);
-          }
-        }
-        if (label_unit / kChunk == chunk && label_unit % kWalkers == t) row.d[label] = FromF32<T>(slope * (q.others / q.s));
       }
+      if (label_unit / kChunk == chunk && label_unit % kWalkers == t) row.d[label] = FromF32<T>(slope * (q.others / q.s));
     }
   }
 }
@@ -1232,14 +1412,25 @@ cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& se
     return Next(LogitShortKernel<T, 4, kPolicy>, grid, kShortThreads, 0, s)(a, p, seq, kept, arrived);
   }
   Sharing w;
-  // Of a preference loss's rows, which have no second walk, those of more than half of an SM's threads too: 768 rows of 128256 in bf16
-  // 107 us with pairs and gradient, in clusters 119; 1500 of 50001 in f16 98, one row to an SM 101.  A policy loss's second walk costs
-  // more than that: 8192 rows of 32000 in bf16 227 us, in registers 172; 2048 of 128256 254, in clusters 204.
-  if (!ShareRows<T>(a, sms, &w) || (!kPolicy && a.rows > 2 * sms && w.threads > kThreads / 2)) {
-    constexpr auto* kernel = LogitStreamKernel<T, kPolicy>;
-    constexpr size_t bytes = kStreams * kStreamSlots * kChunk * 16;
+  const bool shared = ShareRows<T>(a, sms, &w);
+  if constexpr (kPolicy) {
+    if (!shared) {   // (for 8192 rows of 32000 in bf16 227 us, in registers 172; for 2048 of 128256 254, in clusters 204)
+      constexpr auto* kernel = LogitStreamKernel<T>;
+      constexpr size_t bytes = kStreams * kStreamSlots * kChunk * 16;
+      if (cudaError_t e = AllowShared<kernel>(bytes); e != cudaSuccess) return e;
+      return Next(kernel, static_cast<unsigned>(a.rows < sms ? a.rows : sms), kStreams * kWalkers, bytes, s)(a, p, kept, arrived);
+    }
+  } else if (!shared || (a.rows > 2 * sms && (w.threads > kThreads / 2 || a.classes >= 20000))) {
+    // Many rows wider than two groups of an SM hold, or of 20000 classes on: with pairs and gradient, 8 x 512 x 32000 in bf16 take 189 us,
+    // in groups' registers 195; 16 x 100 x 50001 117 and 128; 16 x 512 x 20001 in f16 244 and 251.  But 16 x 512 x 16000 191 and 182, in
+    // f32 356 and 344.
+    const uint32_t chunks = (all + kSumChunk - 1) / kSumChunk, window = sms * kListed;
+    uint32_t warps = kSumWarps;   // to a row: as many as its chunks keep busy
+    while (warps > 1 && (chunks + warps - 1) / warps * warps * 15 > chunks * 16) warps /= 2;
+    constexpr auto* kernel = LogitSumsKernel<T>;
+    constexpr size_t bytes = kSumThreads / 32 * kSumSlots * kSumChunk * 16 + kListed * sizeof(int2) + kCounted / 8;
     if (cudaError_t e = AllowShared<kernel>(bytes); e != cudaSuccess) return e;
-    return Next(kernel, static_cast<unsigned>(a.rows < sms ? a.rows : sms), kStreams * kWalkers, bytes, s)(a, p, seq, kept, arrived);
+    return Next(kernel, sms, kSumThreads, bytes, s)(a, seq, kept, warps, window < kCounted ? window : kCounted);
   }
   return w.blocks > 1 ? RunRows<T, kPolicy, true>(a, p, seq, kept, arrived, w, s) : RunRows<T, kPolicy, false>(a, p, seq, kept, arrived, w, s);
 }

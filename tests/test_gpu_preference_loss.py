@@ -113,6 +113,55 @@ def test_wide_and_long(be, lengths, classes, dtype):
     c.check(c.d)
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("lengths,classes,stride,begin,d_begin", [([150, 170], 20000, 20000, 0, 0), ([40, 60] * 4, 20011, 20013, 3, 3),
+                                                                 ([301, 0, 1, 20], 33001, 33001, 5, 2), ([0, 310], 20481, 20488, 7, 7),
+                                                                 ([200, 220], 45056, 45056, 1, 1)])
+def test_many_wide_rows(be, lengths, classes, stride, begin, d_begin, dtype):
+    """Rows that single warps' rings walk, where a block lists those that count: chunks of 256 units that end beside a row's end, too."""
+    c = Preference(lengths, classes, dtype, before=5, stride=stride, begin=begin, d_begin=d_begin)
+    c(be)
+    c.check(c.d)
+    outputs = [t.clone() for t in (c.loss, c.margins, c.sums)]
+    c(be, None)
+    assert all(torch.equal(a, b) for a, b in zip(outputs, (c.loss, c.margins, c.sums)))
+    c.d[:] = 9.0
+    assert (c.d_buf == 9).all()
+
+
+def test_many_wide_rows_of_which_none_counts(be):
+    c = Preference([200, 200], 20000, "bf16", reference=False)
+    c.labels.fill_(-1)
+    c.logits.fill_(math.nan)
+    c(be)
+    assert (c.sums == 0).all() and (c.margins == 0).all() and abs(float(c.loss) - math.log(2)) < 1e-6
+    assert (c.d[:400] == 0).all()
+
+
+def test_rows_that_count_far_apart(be):
+    """More rows than are counted at a time, most of which do not count and hold NaN: the same as those that count alone.  A row's
+    log-probability is the same there; their sums in double are in another order, and each output is rounded once to f32."""
+    few = Preference([230, 170], 20000, "bf16", behind=0)
+    few(be)
+    few.check(few.d)
+    rows, split = 33100, 16500
+    logits = torch.full((rows, 20000), math.nan, device="cuda", dtype=torch.bfloat16)
+    labels = torch.full((rows,), -1, device="cuda", dtype=torch.int32)
+    generator = torch.Generator().manual_seed(1)
+    at = torch.cat([torch.randperm(split, generator=generator)[:230].sort().values,
+                    split + torch.randperm(rows - split, generator=generator)[:170].sort().values])
+    at[-1], at[0] = rows - 1, 0
+    at = at.cuda()
+    logits[at], labels[at] = few.logits, few.labels
+    starts = torch.tensor([0, split, rows], device="cuda", dtype=torch.int32)
+    loss, margins, sums = (torch.full((n,), 7.0, device="cuda") for n in (1, 1, 2))
+    work = torch.full((B.preference_workspace(rows, 1),), 0xFF, device="cuda", dtype=torch.uint8)
+    be.preference_loss(rows, 20000, 1, logits.data_ptr(), labels.data_ptr(), starts.data_ptr(), loss.data_ptr(), margins.data_ptr(), sums.data_ptr(),
+                       work.data_ptr(), work.numel(), ref_logp=few.ref.data_ptr(), type=B.TYPES["bf16"], kind=B.PREFERENCES["sigmoid"], **few.options)
+    for got, want in ((loss, few.loss), (margins, few.margins), (sums, few.sums)):
+        assert ((got - want).abs() <= 2.0 ** -23 * want.abs() + 1e-12).all()
+
+
 OPTIONS = [dict(kind="sigmoid", smoothing=0.1), dict(kind="sigmoid", margin=0.5, average=True), dict(kind="hinge"), dict(kind="hinge", margin=-0.4, average=True),
            dict(kind="square"), dict(kind="square", beta=2.0, average=True), dict(reference=False, beta=0.01), dict(reference=False, average=True, beta=2.0),
            dict(scale=0.7), dict(scale=1.6)]
