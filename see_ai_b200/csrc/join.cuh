@@ -3,7 +3,6 @@
 #define SEE_CUDA_JOIN_CUH_
 
 #include <initializer_list>
-
 #include <type_traits>
 
 #include "act_expr.cuh"

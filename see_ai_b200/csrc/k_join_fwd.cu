@@ -9,7 +9,6 @@ namespace see::k {
 
 namespace {
 
-
 // The statistics of a group's row in v, of which a thread has the columns (t + i T) VEC below cols, and zeros beyond.
 template <bool kRms, int VEC, int NV>
 __device__ __forceinline__ float2 StatsOf(const Lane<VEC> (&v)[NV][kLanes<VEC>], uint32_t t, uint32_t T, uint32_t group, uint32_t cols, float eps,
