@@ -70,7 +70,7 @@ struct LogitArgs {
   const int32_t* labels;
   uint64_t rows, stride;
   uint32_t classes;
-  float scale, k;                             // k: scale / ln 2
+  float scale, k, k_rest;                     // k: scale / ln 2; k_rest: what its rounding leaves, above 0 (of the policy loss: next to nothing)
   double inv_k;
   DeviceStatus* status;
 };

@@ -11,7 +11,11 @@
 // A policy loss's rows that are wider still are walked twice (LogitStreamKernel), a preference loss's that are many and wide go through
 // rings of single warps (LogitSumsKernel).
 //
-// logp is made in double: a sequence's sum of hundreds of them is held against a reference's.
+// logp is made in double.  A preference loss holds sums of hundreds of them against a reference's, where what is off the same way in each
+// row adds up, so it does more: k M is rounded up to an integer, so that sums are carried over to a larger maximum without rounding; its
+// exponents have what k's rounding leaves too (k rounded downwards, the rest above 0: -inf stays); and log s has kLow on top, by which
+// ex2.approx falls short on average (measured over 2^24 arguments from each of several ranges from -60 on).  Margins of 8 pairs of 512
+// rows are 2e-7 off so, 1e-6 without.  The policy loss, whose rows are rounded to f32 each, does without.
 #include <type_traits>
 
 #include "act_expr.cuh"
@@ -144,18 +148,26 @@ __device__ __forceinline__ double LogOf(float s) {
   return fma(static_cast<double>(e), 0.6931471805599453, LogRatio(Quotient(m - 1.0, m + 1.0)));
 }
 
+constexpr double kLow = 5.1e-8;
+// k M as it is used.
+template <bool kPolicy>
+__device__ __forceinline__ float Shift(float km) { return kPolicy ? km : ceilf(km); }
+
 // Of a row: the label's logit, k M, the sum over the others, the sum over all.
 struct RowSums {
   float z_label, mk, others, s;
 };
-__device__ __forceinline__ float LabelTerm(const LogitArgs& a, float z_label, float mk) { return Ex2Approx(fmaf(z_label, a.k, -mk)); }
+__device__ __forceinline__ float LabelTerm(const LogitArgs& a, float z_label, float mk) {
+  return Ex2Approx(fmaf(z_label, a.k_rest, fmaf(z_label, a.k, -mk)));
+}
+template <bool kPolicy>
 __device__ __forceinline__ double LogpOf(const LogitArgs& a, const RowSums& q) {
   const float e = LabelTerm(a, q.z_label, q.mk);
   if (3.0f * q.others < e) {   // -log1p(others / e)
     const double ratio = Quotient(static_cast<double>(q.others), static_cast<double>(e));
     return -LogRatio(Quotient(ratio, 2.0 + ratio));
   }
-  return static_cast<double>(a.scale) * (static_cast<double>(q.z_label) - static_cast<double>(q.mk) * a.inv_k) - LogOf(q.s);
+  return static_cast<double>(a.scale) * (static_cast<double>(q.z_label) - static_cast<double>(q.mk) * a.inv_k) - LogOf(q.s) - (kPolicy ? 0.0 : kLow);
 }
 
 __device__ __forceinline__ bool Counts(int32_t label, uint32_t classes) { return label >= 0 && static_cast<uint32_t>(label) < classes; }
@@ -196,7 +208,7 @@ __device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, const Polic
 template <typename T>
 __device__ __forceinline__ float SlopeOf(const LogitArgs& a, const PolicyArgs& p, const PolicyRow& row, const RowSums& q) {
   if constexpr (sizeof(T) == 4) {
-    return row.weight * PolicyOf(p, row, LogpOf(a, q)).slope;
+    return row.weight * PolicyOf(p, row, LogpOf<true>(a, q)).slope;
   } else {
     constexpr float kLn2 = 0.6931471805599453f;
     float log2s;
@@ -234,7 +246,7 @@ PolicyFinishKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ 
     const float4 q = kept[r];   // (all at once; of a row that does not count, whatever is there)
     const PolicyRow row = PolicyRowOf(p, r);
     if (Counts(a.labels[r], a.classes)) {
-      logp = LogpOf(a, {q.x, q.y, q.z, q.w});
+      logp = LogpOf<true>(a, {q.x, q.y, q.z, q.w});
       const PolicyTerms t = PolicyOf(p, row, logp);
       sums[0] += static_cast<double>(row.weight * t.loss);
       sums[1] += static_cast<double>(row.weight * t.kl);
@@ -493,7 +505,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
 #pragma unroll
       for (int i = 0; i < NU; ++i) raw[i] = t + i * threads < count ? mine[t + i * threads] : Nothing<T>();
     }
-    float mk = __fmul_rn(Largest<T, NU>(raw), a.k), sum;   // -inf: nothing here
+    float mk = Shift<kPolicy>(__fmul_rn(Largest<T, NU>(raw), a.k)), sum;   // -inf: nothing here
     // A lone slot is filled while the exponentials are made, unless dlogits will be stored meanwhile: loads and stores in turn are
     // faster then (8192 rows of 32000 in bf16: 172 us, early 184; a preference loss of 16 x 512 x 16001 in f32 357, early 344).
     const bool early = plan.slots == 1 && !(kPolicy && a.dlogits);
@@ -502,14 +514,14 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
       refill();
     }
     {
-      const f32x2 k2 = Splat2(a.k), away = Splat2(mk == MinusInf() ? 0.0f : -mk);
+      const f32x2 k2 = Splat2(a.k), rest2 = Splat2(a.k_rest), away = Splat2(mk == MinusInf() ? 0.0f : -mk);
       f32x2 sum2[kPairs<T>] = {};
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         f32x2 v[kPairs<T>];
         Pairs<T>(raw[i], v);
 #pragma unroll
-        for (int j = 0; j < kPairs<T>; ++j) sum2[j] = AddF2(sum2[j], Powers(Fma2(v[j], k2, away)));
+        for (int j = 0; j < kPairs<T>; ++j) sum2[j] = AddF2(sum2[j], Powers(kPolicy ? Fma2(v[j], k2, away) : Fma2(v[j], rest2, Fma2(v[j], k2, away))));
       }
 #pragma unroll
       for (int j = 1; j < kPairs<T>; ++j) sum2[0] = AddF2(sum2[0], sum2[j]);
@@ -567,7 +579,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     T raw_label;
     if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(items[0]);
     else raw_label.bits = static_cast<uint16_t>(items[0]);
-    const float z_label = ToF32(raw_label), mk_label = __fmul_rn(z_label, a.k), all = fmaxf(mk, mk_label);
+    const float z_label = ToF32(raw_label), mk_label = Shift<kPolicy>(__fmul_rn(z_label, a.k)), all = fmaxf(mk, mk_label);
     RowSums q = {z_label, all == MinusInf() ? 0.0f : all, sum * factor(mk, all), 0.0f};
     q.s = q.others + LabelTerm(a, z_label, q.mk);
     if (t == 0 && rank == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
@@ -684,7 +696,7 @@ LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Po
   };
   int32_t next_label = first < rows ? a.labels[first] : -1, label_behind = first + step < rows ? a.labels[first + step] : -1;
   ask(first, next_label);
-  const f32x2 k2 = Splat2(a.k);
+  const f32x2 k2 = Splat2(a.k), rest2 = Splat2(a.k_rest);
   for (uint32_t r = first; r < rows; r += step) {
     const int32_t label = next_label;
     next_label = label_behind;
@@ -709,8 +721,7 @@ LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Po
       const int32_t e0 = static_cast<int32_t>(u * E) - static_cast<int32_t>(row.skip);
       if ((e0 < 0 || u >= whole_end || u == label_unit) && u < row.units) raw[i] = Only<T>(raw[i], -e0, static_cast<int32_t>(a.classes) - e0, label - e0);
     }
-    float mk = __fmul_rn(Largest<T, NU>(raw), a.k);
-    mk = WarpMax(mk);
+    float mk = WarpMax(Shift<kPolicy>(__fmul_rn(Largest<T, NU>(raw), a.k)));
     const f32x2 away = Splat2(mk == MinusInf() ? 0.0f : -mk);
     f32x2 sum2 = 0;
 #pragma unroll
@@ -718,7 +729,7 @@ LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Po
       f32x2 v[kPairs<T>];
       Pairs<T>(raw[i], v);
 #pragma unroll
-      for (int j = 0; j < kPairs<T>; ++j) sum2 = AddF2(sum2, Powers(Fma2(v[j], k2, away)));
+      for (int j = 0; j < kPairs<T>; ++j) sum2 = AddF2(sum2, Powers(kPolicy ? Fma2(v[j], k2, away) : Fma2(v[j], rest2, Fma2(v[j], k2, away))));
     }
     float lo, sum;
     UnpackF2(sum2, &lo, &sum);
@@ -729,7 +740,7 @@ LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Po
     T raw_label;
     if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(label_bits);
     else raw_label.bits = static_cast<uint16_t>(label_bits);
-    const float z_label = ToF32(raw_label), mk_label = __fmul_rn(z_label, a.k), all = fmaxf(mk, mk_label);
+    const float z_label = ToF32(raw_label), mk_label = Shift<kPolicy>(__fmul_rn(z_label, a.k)), all = fmaxf(mk, mk_label);
     RowSums q = {z_label, all == MinusInf() ? 0.0f : all, mk == MinusInf() ? 0.0f * sum : sum * Ex2Approx(mk - all), 0.0f};
     q.s = q.others + LabelTerm(a, z_label, q.mk);
     if (lane == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
@@ -793,7 +804,7 @@ LogitSumsKernel(const __grid_constant__ LogitArgs a, const Sequences seq, float4
   };
   const uint32_t stride_units = warps * kSumChunk;   // of a warp's chunks in a row
   uint32_t slot = 0, parities = 0;                   // a bit for each slot, of the copies that went through it
-  const f32x2 k2 = Splat2(a.k);
+  const f32x2 k2 = Splat2(a.k), rest2 = Splat2(a.k_rest);
   auto factor = [](float own, float all) { return own == MinusInf() ? 0.0f : Ex2Approx(own - all); };
   uint32_t turn = 0;
   for (uint32_t base = rows_begin; base < rows_end; base += window) {
@@ -891,7 +902,7 @@ LogitSumsKernel(const __grid_constant__ LogitArgs a, const Sequences seq, float4
               raw[j] = Only<T>(raw[j], static_cast<int32_t>(row.skip) - e0, static_cast<int32_t>(ends_at) - e0, label + static_cast<int32_t>(row.skip) - e0);
           }
         }
-        const float top = fmaxf(mk, __fmul_rn(Largest<T, kSumUnits>(raw), a.k));
+        const float top = fmaxf(mk, Shift<false>(__fmul_rn(Largest<T, kSumUnits>(raw), a.k)));
         __syncwarp();   // the slot is read
         fill();
         const f32x2 away = Splat2(top == MinusInf() ? 0.0f : -top);
@@ -901,7 +912,7 @@ LogitSumsKernel(const __grid_constant__ LogitArgs a, const Sequences seq, float4
           f32x2 v[kPairs<T>];
           Pairs<T>(raw[j], v);
 #pragma unroll
-          for (int l = 0; l < kPairs<T>; ++l) sum2[l & 1] = AddF2(sum2[l & 1], Powers(Fma2(v[l], k2, away)));
+          for (int l = 0; l < kPairs<T>; ++l) sum2[l & 1] = AddF2(sum2[l & 1], Powers(Fma2(v[l], rest2, Fma2(v[l], k2, away))));
         }
         float lo, hi;
         UnpackF2(AddF2(sum2[0], sum2[1]), &lo, &hi);
@@ -933,7 +944,7 @@ LogitSumsKernel(const __grid_constant__ LogitArgs a, const Sequences seq, float4
       T raw_label;
       if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(label_bits);
       else raw_label.bits = static_cast<uint16_t>(label_bits);
-      const float z_label = ToF32(raw_label), mk_label = __fmul_rn(z_label, a.k), top = fmaxf(mk, mk_label);
+      const float z_label = ToF32(raw_label), mk_label = Shift<false>(__fmul_rn(z_label, a.k)), top = fmaxf(mk, mk_label);
       RowSums q = {z_label, top == MinusInf() ? 0.0f : top, sum * factor(mk, top), 0.0f};
       q.s = q.others + LabelTerm(a, z_label, q.mk);
       kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
@@ -1188,7 +1199,7 @@ PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant
     for (int64_t r = begin + t; r < end; r += kPairThreads / 2) {
       const float4 q = kept[r];   // (asked for beside the label; of a row that does not count, whatever is there)
       if (Counts(a.labels[r], a.classes)) {
-        sum += LogpOf(a, {q.x, q.y, q.z, q.w});
+        sum += LogpOf<false>(a, {q.x, q.y, q.z, q.w});
         counted += 1.0;
       }
     }
@@ -1265,7 +1276,7 @@ PreferenceGradientKernel(const __grid_constant__ LogitArgs a, const __grid_const
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side_by_side = kGradThreads / 32 / warps;
   const int64_t begin = max(static_cast<int64_t>(p.starts[0]), static_cast<int64_t>(0));
   const int64_t end = min(static_cast<int64_t>(p.starts[2 * p.pairs]), static_cast<int64_t>(a.rows));
-  const float k = a.k;
+  const float k = a.k, rest = a.k_rest;
   for (int64_t r = end - 1 - (static_cast<int64_t>(blockIdx.x) * side_by_side + warp / warps); r >= begin;
        r -= static_cast<int64_t>(gridDim.x) * side_by_side) {
     const float4 q = kept[r];
@@ -1292,7 +1303,7 @@ PreferenceGradientKernel(const __grid_constant__ LogitArgs a, const __grid_const
         } else {
           Elements<T>(raw[i], v);
 #pragma unroll
-          for (int j = 0; j < kPerUnit<T>; ++j) v[j] = by * Ex2Approx(fmaf(v[j], k, -mk));
+          for (int j = 0; j < kPerUnit<T>; ++j) v[j] = by * Ex2Approx(fmaf(v[j], rest, fmaf(v[j], k, -mk)));
         }
         row.Store(u, v);
         if (u == label_unit) row.d[label] = FromF32<T>(slope == 0.0f ? 0.0f : slope * (q.z / q.w));
@@ -1421,7 +1432,7 @@ cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& se
       return Next(kernel, static_cast<unsigned>(a.rows < sms ? a.rows : sms), kStreams * kWalkers, bytes, s)(a, p, kept, arrived);
     }
   } else if (!shared || (a.rows > 2 * sms && (w.threads > kThreads / 2 || a.classes >= 20000))) {
-    // Many rows wider than two groups of an SM hold, or of 20000 classes on: with pairs and gradient, 8 x 512 x 32000 in bf16 take 189 us,
+    // Many rows wider than two groups of an SM hold, or of 20000 classes on: with pairs and gradient, 8 x 512 x 32000 in bf16 take 190 us,
     // in groups' registers 195; 16 x 100 x 50001 117 and 128; 16 x 512 x 20001 in f16 244 and 251.  But 16 x 512 x 16000 191 and 182, in
     // f32 356 and 344.
     const uint32_t chunks = (all + kSumChunk - 1) / kSumChunk, window = sms * kListed;

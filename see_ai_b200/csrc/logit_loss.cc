@@ -1,5 +1,7 @@
 // The checks of the losses over rows of logits, and their dispatch.
+#include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "block_checks.h"
 #include "block_ops.h"
@@ -27,11 +29,15 @@ Operand Logits(const char* name, const Shape& s, const void* p, bool written) {
   return {name, p, s.rows, s.classes * size, s.stride * size, size, written};
 }
 
+// whole: with what k's rounding leaves (a preference loss's).
 template <typename Shape>
-k::LogitArgs ArgsOf(const Shape& s, const void* logits, const int32_t* labels, void* dlogits, k::DeviceStatus* status) {
-  const float k = static_cast<float>(kLog2E * static_cast<double>(s.logit_scale));
-  return {logits, s.rows ? dlogits : nullptr, labels, s.rows, s.stride, static_cast<uint32_t>(s.classes), s.logit_scale, k, 1.0 / static_cast<double>(k),
-          status};
+k::LogitArgs ArgsOf(const Shape& s, const void* logits, const int32_t* labels, void* dlogits, bool whole, k::DeviceStatus* status) {
+  const double exact = kLog2E * static_cast<double>(s.logit_scale);
+  float k = static_cast<float>(exact);
+  if (whole && static_cast<double>(k) > exact) k = std::nextafter(k, 0.0f);
+  const float rest = whole ? static_cast<float>(exact - static_cast<double>(k)) : 0.0f;
+  return {logits, s.rows ? dlogits : nullptr, labels, s.rows, s.stride, static_cast<uint32_t>(s.classes), s.logit_scale, k,
+          std::max(rest, std::numeric_limits<float>::min()), 1.0 / (whole ? exact : static_cast<double>(k)), status};
 }
 
 }  // namespace
@@ -83,7 +89,7 @@ Status CudaBackend::PreferenceLoss(const see_preference_shape& given, const void
   OnDevice on(device_);
   if (!on.ok()) return Check(cudaGetLastError(), "preference loss: device");
   int launches = 0;
-  const cudaError_t e = k::PreferenceLoss(ArgsOf(s, logits, labels, dlogits, d_status_), s.type, p, kept, sms_, stream_, &launches);
+  const cudaError_t e = k::PreferenceLoss(ArgsOf(s, logits, labels, dlogits, true, d_status_), s.type, p, kept, sms_, stream_, &launches);
   counters_.kernel_launches += static_cast<uint64_t>(launches);
   return Check(e, "preference loss");
 }
@@ -128,7 +134,7 @@ Status CudaBackend::PolicyLoss(const see_policy_shape& given, const void* logits
   if (!on.ok()) return Check(cudaGetLastError(), "policy loss: device");
   int launches = 0;
   const cudaError_t e =
-      k::PolicyLoss(ArgsOf(s, logits, labels, dlogits, d_status_), s.type, p, static_cast<float4*>(workspace), sms_, stream_, &launches);
+      k::PolicyLoss(ArgsOf(s, logits, labels, dlogits, false, d_status_), s.type, p, static_cast<float4*>(workspace), sms_, stream_, &launches);
   counters_.kernel_launches += static_cast<uint64_t>(launches);
   return Check(e, "policy loss");
 }
