@@ -162,6 +162,17 @@ def test_rows_that_count_far_apart(be):
         assert ((got - want).abs() <= 2.0 ** -23 * want.abs() + 1e-12).all()
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("lengths,classes", [([700, 10], 2000), ([9, 600], 20000), ([1500, 3], 250)])
+def test_what_is_off_alike_does_not_add_up(be, lengths, classes, dtype):
+    """A margin of many rows against few.  A row's log-probability is off by a rounding or two of its sum, 2^-24 each, in either direction:
+    6e-9 on the average of 500 rows and more.  ex2.approx's average is known to 1e-9.  3e-8 leaves room for neither's 2^-24 in one direction."""
+    c = Preference(lengths, classes, dtype, beta=0.1)
+    c(be)
+    want = float(c.want()["margins"])
+    assert abs(float(c.margins) - want) <= 0.1 * sum(lengths) * 3e-8 + 2.0 ** -24 * abs(want)
+
+
 OPTIONS = [dict(kind="sigmoid", smoothing=0.1), dict(kind="sigmoid", margin=0.5, average=True), dict(kind="hinge"), dict(kind="hinge", margin=-0.4, average=True),
            dict(kind="square"), dict(kind="square", beta=2.0, average=True), dict(reference=False, beta=0.01), dict(reference=False, average=True, beta=2.0),
            dict(scale=0.7), dict(scale=1.6)]
