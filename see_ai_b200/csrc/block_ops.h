@@ -93,8 +93,7 @@ cudaError_t PolicyLoss(const LogitArgs& a, int type, const PolicyArgs& p, float4
 cudaError_t PreferenceLoss(const LogitArgs& a, int type, const PreferenceArgs& p, float4* kept, uint32_t sms, cudaStream_t s, int* launches);
 
 // ---- all gradients' norm (k_grad_norm.cu) ------------------------------------
-constexpr uint32_t kGradPartials = 1024;      // most thread blocks' sums
-// clip: writes the tensors' out too.  partials [kGradPartials].
+// clip: writes the tensors' out too.  partials [kGradPartials] (grad_table.h).
 cudaError_t GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, float max_norm, const float* grad_scale, float* norm,
                      float* factor, double* partials, uint32_t sms, cudaStream_t s, int* launches);
 

@@ -5,6 +5,7 @@
 #include "block_checks.h"
 #include "block_ops.h"
 #include "cuda_backend.h"
+#include "grad_table.h"
 
 namespace see {
 

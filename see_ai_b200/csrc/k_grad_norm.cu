@@ -8,6 +8,7 @@
 // f32, 32 to 64 of them; where that sum is not finite or so small that squares may have been lost, they are summed again in double.
 // What is beyond is double: the blocks' sums meet in the workspace and are added in a fixed order.
 #include "block_ops.h"
+#include "grad_table.h"
 #include "launch.cuh"
 #include "vec_types.cuh"
 
@@ -15,21 +16,7 @@ namespace see::k {
 
 namespace {
 
-constexpr uint32_t kThreads = 256, kUnits = 8, kStep = kThreads * kUnits;   // units to a thread, and to a block, at a time
-constexpr uint32_t kEntries = 160;                                          // tensors a launch
-constexpr uint32_t kGradBlocks = 4;                                         // to an SM
-
-struct GradEntry {
-  const uint8_t* g;
-  uint8_t* out;
-  uint64_t n, unit_end;   // elements; units, counted over the launch's tensors
-  uint8_t type, wide;     // wide: out is aligned to 16 bytes as g is
-};
-struct GradTable {
-  GradEntry entry[kEntries];
-  uint64_t each;          // units to a block,
-  uint32_t rest, count;   // and one more to the first `rest`; tensors
-};
+constexpr uint32_t kThreads = kGradThreads, kUnits = 8, kStep = kThreads * kUnits;   // units to a thread, and to a block, at a time
 
 // Calls step(entry, first unit, units) for all of a block's range, or, of kBack, from its end on.
 template <bool kBack, typename F>
@@ -236,64 +223,33 @@ GradScaleKernel(const __grid_constant__ GradTable table, const double* __restric
   });
 }
 
-// The table of the next tensors from `next` on; false: none are left.
-bool Fill(GradTable* table, const see_grad_tensor* tensors, uint64_t count, uint64_t* next) {
-  table->count = 0;
-  uint64_t units = 0;
-  for (; *next < count && table->count < kEntries; ++*next) {
-    const see_grad_tensor& t = tensors[*next];
-    if (t.n == 0) continue;
-    const uint64_t at = reinterpret_cast<uint64_t>(t.g) & 15;
-    units += (at + t.n * (t.type == SEE_F32 ? 4 : 2) + 15) / 16;
-    void* out = t.out ? t.out : t.g;
-    table->entry[table->count++] = {static_cast<const uint8_t*>(t.g), static_cast<uint8_t*>(out), t.n, units, static_cast<uint8_t>(t.type),
-                                    static_cast<uint8_t>(at == (reinterpret_cast<uint64_t>(out) & 15))};
-  }
-  return table->count != 0;
-}
-// Blocks: four units to a thread at least.  Cuts the table's units into their ranges.
-unsigned Cut(GradTable& table, uint32_t sms) {
-  const uint64_t units = table.entry[table.count - 1].unit_end, blocks = (units + 4 * kThreads - 1) / (4 * kThreads);
-  const uint64_t most = sms * kGradBlocks < kGradPartials ? sms * kGradBlocks : kGradPartials, grid = blocks < most ? blocks : most;
-  table.each = units / grid;
-  table.rest = static_cast<uint32_t>(units % grid);
-  return static_cast<unsigned>(grid);
-}
-
 }  // namespace
 
 cudaError_t GradNorm(const see_grad_tensor* tensors, uint64_t count, bool clip, float max_norm, const float* grad_scale, float* norm,
                      float* factor, double* partials, uint32_t sms, cudaStream_t s, int* launches) {
   GradTable table;
-  uint64_t next = 0;
-  unsigned used = 0, grid = 0, tables = 0;   // used: partial sums
-  while (Fill(&table, tensors, count, &next)) {
-    ++tables;
-    grid = Cut(table, sms);
+  unsigned used = 0, blocks = 0, tables = 0;   // used: partial sums
+  cudaError_t e = EachGradTable(&table, tensors, count, sms, cudaSuccess, &tables, &blocks, [&](const GradTable& t, unsigned grid) {
     // (blocks that an earlier launch had are added to; those that it had not are new)
     if (used != 0 && grid > used) {
       if (cudaError_t e = cudaMemsetAsync(partials + used, 0, (grid - used) * sizeof(double), s); e != cudaSuccess) return e;
     }
-    if (cudaError_t e = Next(GradSquaresKernel, grid, kThreads, 0, s)(table, partials, used == 0 ? 1 : 0); e != cudaSuccess) return e;
     ++*launches;
+    const int first = used == 0 ? 1 : 0;
     used = used > grid ? used : grid;
-    if (next >= count) break;
-  }
+    return Next(GradSquaresKernel, grid, kThreads, 0, s)(t, partials, first);
+  });
+  if (e != cudaSuccess) return e;
   if (!clip || used == 0) {
     ++*launches;
     return Next(GradFactorKernel, 1, kThreads, 0, s)(static_cast<const double*>(partials), used, max_norm, grad_scale, norm, factor);
   }
-  auto scale = [&] {
+  auto scale = [&](const GradTable& t, unsigned grid) {
     ++*launches;
-    return Next(GradScaleKernel, grid, kThreads, 0, s)(table, static_cast<const double*>(partials), used, max_norm, grad_scale, norm, factor);
+    return Next(GradScaleKernel, grid, kThreads, 0, s)(t, static_cast<const double*>(partials), used, max_norm, grad_scale, norm, factor);
   };
-  if (tables == 1) return scale();   // (the table is there)
-  next = 0;
-  while (Fill(&table, tensors, count, &next)) {
-    grid = Cut(table, sms);
-    if (cudaError_t e = scale(); e != cudaSuccess) return e;
-  }
-  return cudaSuccess;
+  if (tables == 1) return scale(table, blocks);   // (the table is there)
+  return EachGradTable(&table, tensors, count, sms, cudaSuccess, &tables, &blocks, scale);
 }
 
 }  // namespace see::k
