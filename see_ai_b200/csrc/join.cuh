@@ -7,6 +7,7 @@
 
 #include "act_expr.cuh"
 #include "block_ops.h"
+#include "join_ring.h"
 #include "launch.cuh"
 #include "row_groups.cuh"
 
@@ -97,27 +98,7 @@ inline uint32_t JoinEdge(const JoinArgs& a) {
 }
 inline uint32_t Warps(uint32_t n) { return (n + 31) / 32 * 32; }
 
-// Groups of T threads with `slots` slots each, of what `budget` bytes hold; every SM gets rows before one gets two.
-struct JoinRing {
-  uint32_t groups, slots, grid;
-  size_t bytes;
-};
-inline JoinRing RingOf(uint64_t rows, uint32_t threads, uint32_t T, size_t slot_bytes, size_t weights, uint32_t sms) {
-  const size_t budget = kMostShared - 1024 - weights;
-  const uint64_t most = sms < kNormPartials ? sms : kNormPartials, each = (rows + most - 1) / most;
-  uint32_t groups = threads / T;
-  if (groups > each) groups = static_cast<uint32_t>(each);
-  while (groups > 1 && 2 * groups * slot_bytes > budget) --groups;   // two slots to a group, unless it is alone
-  uint32_t slots = static_cast<uint32_t>(budget / (groups * slot_bytes));
-  const uint64_t turns = (rows + most * groups - 1) / (most * groups);
-  slots = slots < 1 ? 1 : slots > 8 ? 8 : slots;
-  if (slots > turns) slots = static_cast<uint32_t>(turns);
-  const uint64_t grid = (rows + groups - 1) / groups;
-  return {groups, slots, static_cast<uint32_t>(grid < most ? grid : most), groups * slots * (slot_bytes + 8) + weights};
-}
-
 // Up to kJoinRingCols columns, one launch; grid: the rows of partial sums that the backward pass leaves.
-constexpr uint32_t kJoinRingCols = 8192;
 cudaError_t JoinForwardRing(const JoinArgs& a, uint32_t sms, cudaStream_t s);
 cudaError_t JoinBackwardRing(const JoinArgs& a, uint32_t sms, cudaStream_t s, uint32_t* grid);
 

@@ -6,6 +6,7 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "block_ops.h"
 #include "kernels.h"
 #include "umma_device.cuh"
 #include "vec_types.cuh"
@@ -13,7 +14,7 @@
 namespace see::k {
 
 constexpr uint32_t kWideThreads = 768;                                // most threads of a block
-constexpr size_t kRingBytes = 200 * 1024, kMostShared = 224 * 1024;   // of a block
+constexpr size_t kRingBytes = 200 * 1024;                              // of a block
 
 template <bool kBoth>
 __device__ __forceinline__ float2 WarpSum(float2 v) {
@@ -125,6 +126,7 @@ __device__ __forceinline__ void CopyRow(uint8_t* slot, const void* base, uint64_
 // microsecond or two).
 template <auto kKernel>
 cudaError_t AllowShared(size_t bytes) {
+  if (bytes > kMostShared) return cudaErrorInvalidValue;
   if (bytes <= 32 * 1024) return cudaSuccess;   // (the static part counts too)
   static std::atomic<size_t> granted[64] = {};
   int dev = 0;

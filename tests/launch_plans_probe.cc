@@ -2,9 +2,11 @@
 // name, a tab, "ok" or what is wrong first.  Built and read by test_launch_plans.py.
 #include <cstdio>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../see_ai_b200/csrc/grad_table.h"
+#include "../see_ai_b200/csrc/join_ring.h"
 
 namespace {
 
@@ -60,9 +62,36 @@ void GradTables() {
   Say("grad tables", "");
 }
 
+// Rings of both passes of the join, of every width, of each pair of types and kind of norm, for groups of all sizes that hold such a row.
+void JoinRings() {
+  using namespace see::k;
+  auto slot = [](size_t cols, size_t size) { return (cols * size + 45) / 16 * 16; };
+  for (size_t cols = 1; cols <= kJoinRingCols; ++cols)
+    for (auto [x, y] : {std::pair<size_t, size_t>{4, 4}, {4, 2}, {2, 2}})
+      for (int pass = 0; pass < 4; ++pass) {   // forward, rms and layer; backward, without and with dx_out
+        const size_t slot_bytes = pass < 2 ? slot(cols, x) + slot(cols, y) : (pass - 1) * slot(cols, x) + 2 * slot(cols, y);
+        const size_t weights = (cols + 3) / 4 * 16 * (pass == 1 ? 4 : 2);
+        for (uint32_t threads : {384, 512, 768})
+          for (uint32_t T = 32; T <= threads; T += 32) {
+            if (T * 32 < cols) continue;
+            for (uint64_t rows : {1ull, 149ull, 1000ull, 5000ull, 22000ull, 0x7FFFFFFFull}) {
+              const JoinRing r = RingOf(rows, threads, T, slot_bytes, weights, 148);
+              if (r.bytes <= kMostShared && r.slots > 0 && r.slots <= kJoinMostSlots && r.groups > 0 && r.groups * T <= threads && r.grid > 0 &&
+                  r.bytes == r.groups * r.slots * (slot_bytes + kJoinBarrier) + weights)
+                continue;
+              return Say("join rings", std::to_string(rows) + " x " + std::to_string(cols) + ", pass " + std::to_string(pass) + ", " +
+                                           std::to_string(threads) + " threads, " + std::to_string(T) + " to a row: " + std::to_string(r.groups) + " groups of " +
+                                           std::to_string(r.slots) + " slots, " + std::to_string(r.bytes) + " bytes");
+            }
+          }
+      }
+  Say("join rings", "");
+}
+
 }  // namespace
 
 int main() {
   GradTables();
+  JoinRings();
   return 0;
 }

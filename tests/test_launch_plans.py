@@ -8,7 +8,7 @@ import pytest
 from see_ai_b200 import build
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-FAMILIES = ["grad tables"]
+FAMILIES = ["grad tables", "join rings"]
 
 
 @pytest.fixture(scope="module")
