@@ -1,0 +1,84 @@
+"""The policy loss where little decides much: ratios at a corner of the clip, policies next to their reference.
+
+Tolerances are logit_reference's, and the slope of 16-bit logits may be off by 2^-15 of itself, a sixteenth of f16's half step."""
+
+import math
+
+import pytest
+import torch
+
+import logit_reference as R
+from see_ai_b200 import backend as B
+from test_gpu_policy_loss import Policy
+
+pytestmark = pytest.mark.gpu
+
+# A warp's rows, a group's, a cluster's, streams (f32's and 16 bits').
+SIZES = [(1300, 250), (1190, 1003), (200, 5003), (160, 32000), (5, 128003), (2, 300001), (2, 1 << 20)]
+
+
+@pytest.fixture(scope="module")
+def be():
+    b = B.CudaBackend(0)
+    b.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield b
+    torch.cuda.synchronize()
+    b.close()
+
+
+def formula(c):
+    """R.policy's, at any ratio that is not within what logp may be off of a corner; and with what 16-bit slopes may be off."""
+    want = R.policy(c.reference, c.old, c.ref, c.a, c.w, *c.clip, c.kl)
+    if c.dtype != "f32":
+        want["slope_off"] = want["slope_off"] + 2.0 ** -15 * want["slope"].abs()
+    return want
+
+
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("rows,classes", SIZES)
+@pytest.mark.parametrize("clip", [(0.0, 0.0), (0.2, 0.28)])
+def test_rows_without_a_gradient_are_those_counted_as_clipped(be, rows, classes, dtype, clip):
+    """old_logp of the operator itself, moved to the corners: which side of them a ratio lies on is a rounding's choice, but one."""
+    c = Policy(rows, classes, dtype, clip=clip, kl=0.0, weighted=False)
+    c(be, None)
+    corner = torch.tensor([math.log(1 - clip[0]), math.log(1 + clip[1])], device="cuda")
+    c.old = c.logp - corner[torch.arange(rows, device="cuda") % 2] * (1 + 1e-6 * torch.randn(rows, device="cuda"))
+    c.a = torch.where(torch.rand(rows, device="cuda") < 0.5, -1.0, 1.0)
+    c(be)
+    still = (c.d == 0).all(1) & c.reference.counts
+    assert float(c.loss[2]) == int(still.sum())
+
+
+def certain(rows, classes, dtype, lead, seed, **options):
+    """Labels that lead by `lead`: their log-probability, next to 0, has digits far below f32's of 1."""
+    c = Policy(rows, classes, dtype, seed=seed, spread=0.5, **options)
+    z = 0.5 * torch.randn(rows, classes, device="cuda")
+    c.labels = torch.randint(classes, (rows,), device="cuda", dtype=torch.int32)
+    z.scatter_(1, c.labels.long()[:, None], lead)
+    c.logits.copy_(z)
+    c.reference = R.Rows(c.logits, c.labels, c.scale)
+    c.old = (c.reference.logp + 0.1 * torch.sign(torch.randn(rows, device="cuda"))).float()
+    c.a, c.w = torch.randn(rows, device="cuda"), torch.rand(rows, device="cuda") if c.w is not None else None
+    return c
+
+
+def near_reference(c, least, most):
+    rows = c.rows
+    x = torch.exp(torch.rand(rows, device="cuda") * (math.log(most) - math.log(least)) + math.log(least)) * torch.sign(torch.randn(rows, device="cuda"))
+    c.ref = (c.reference.logp + x).float()
+
+
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("advantage", ["none", "cancels", "some"])
+@pytest.mark.parametrize("rows,classes", [(1300, 250), (33, 250), (200, 5003), (5, 128003)])
+def test_gradient_next_to_the_reference(be, rows, classes, dtype, advantage):
+    c = certain(rows, classes, dtype, 16.0, 11, kl=0.5)
+    near_reference(c, 1e-6, 1e-2)
+    if advantage == "none":
+        c.a.zero_()
+    elif advantage == "cancels":   # what the KL term leaves of the policy's
+        x = c.ref.double() - c.reference.logp
+        c.a = (-0.5 * torch.expm1(x) / torch.exp(c.reference.logp - c.old.double()) * 1.01).float()
+    c(be)
+    want = formula(c)
+    c.reference.check_dlogits(c.d, want["slope"], want["slope_off"])
