@@ -184,7 +184,7 @@ __device__ __forceinline__ PolicyRow PolicyRowOf(const PolicyArgs& p, uint64_t r
   return {p.old_logp[row], p.ref_logp ? p.ref_logp[row] : 0.0f, p.advantages[row], p.weights ? p.weights[row] : 1.0f};
 }
 struct PolicyTerms {
-  float slope, loss, kl;   // slope: of the loss by logp; none of them weighted
+  float slope, loss;   // slope: of the loss by logp, with its KL term; loss: without; none of them weighted
   bool clipped;
 };
 __device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, const PolicyRow& row, double logp) {
@@ -194,14 +194,12 @@ __device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, const Polic
   t.clipped = r * a > cut * a;
   t.loss = t.clipped ? -(cut * a) : -(r * a);
   t.slope = t.clipped ? 0.0f : -(r * a);
-  t.kl = 0.0f;
-  if (p.ref_logp) {
-    const float grown = expm1f(above);
-    t.kl = grown - above;
-    t.loss += p.kl_coef * t.kl;
-    t.slope -= p.kl_coef * grown;
-  }
+  if (p.ref_logp) t.slope -= p.kl_coef * expm1f(above);
   return t;
+}
+// exp(x) - x - 1, some x^2 / 2: in double, and next to 0 by its series, since the difference would leave none of an f32's digits.
+__device__ __forceinline__ double KlOf(double x) {
+  return fabs(x) < 0x1p-10 ? x * x * fma(x, fma(x, 1.0 / 24.0, 1.0 / 6.0), 0.5) : expm1(x) - x;
 }
 // The loss's weighted derivative by a row's logp, as it goes into dlogits.  Of 16-bit logits, 8 or 11 bits: mostly a logp in f32 is enough,
 // and takes each warp some 40 instructions instead of 100.  It is not next to a corner, where the row is on the side that
@@ -260,8 +258,9 @@ PolicyFinishKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ 
     if (Counts(a.labels[r], a.classes)) {
       logp = LogpOf<true>(a, {q.x, q.y, q.z, q.w});
       const PolicyTerms t = PolicyOf(p, row, logp);
-      sums[0] += static_cast<double>(row.weight * t.loss);
-      sums[1] += static_cast<double>(row.weight * t.kl);
+      const double kl = p.ref_logp ? KlOf(static_cast<double>(row.ref) - logp) : 0.0;
+      sums[0] += static_cast<double>(row.weight) * fma(static_cast<double>(p.kl_coef), kl, static_cast<double>(t.loss));
+      sums[1] += static_cast<double>(row.weight) * kl;
       sums[2] += t.clipped ? static_cast<double>(row.weight) : 0.0;
     }
     p.logp[r] = static_cast<float>(logp);

@@ -1,6 +1,9 @@
 """The policy loss where little decides much: ratios at a corner of the clip, policies next to their reference.
 
-Tolerances are logit_reference's, and the slope of 16-bit logits may be off by 2^-15 of itself, a sixteenth of f16's half step."""
+Tolerances are logit_reference's, but for two that are narrower or wider there:
+- kl = exp(x) - x - 1 of an x that is off by `off`: |exp(x) - 1| off, and 4 roundings of f32 of kl itself (its own, the weight's product,
+  the sum's, the result's).  No term in |x|: that would be the digits lost by a subtraction in f32.
+- the slope of 16-bit logits may be off by 2^-15 of itself, a sixteenth of f16's half step."""
 
 import math
 
@@ -29,6 +32,12 @@ def be():
 def formula(c):
     """R.policy's, at any ratio that is not within what logp may be off of a corner; and with what 16-bit slopes may be off."""
     want = R.policy(c.reference, c.old, c.ref, c.a, c.w, *c.clip, c.kl)
+    if c.ref is not None:
+        x = torch.where(c.reference.counts, c.ref.double() - c.reference.logp, 0.0)
+        off = c.reference.logp_off + 2.0 ** -50 * (c.reference.logp.abs() + x.abs())   # (a double difference)
+        kl = torch.where(x.abs() < 1e-3, x * x * (0.5 + x / 6 + x * x / 24 + x ** 3 / 120), torch.expm1(x) - x)
+        w = torch.where(c.reference.counts, c.w.double() if c.w is not None else 1.0, 0.0)
+        want["kl"], want["kl_off"] = kl * w, (torch.expm1(x).abs() * off + 0.51 * off * off + 4 * R.ULP * kl) * w
     if c.dtype != "f32":
         want["slope_off"] = want["slope_off"] + 2.0 ** -15 * want["slope"].abs()
     return want
@@ -82,3 +91,15 @@ def test_gradient_next_to_the_reference(be, rows, classes, dtype, advantage):
     c(be)
     want = formula(c)
     c.reference.check_dlogits(c.d, want["slope"], want["slope_off"])
+
+
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("rows", [1, 40, 3000])
+@pytest.mark.parametrize("least,most", [(1e-9, 1e-6), (1e-5, 1e-2), (0.1, 3.0)])
+def test_kl_keeps_its_digits(be, rows, dtype, least, most):
+    c = certain(rows, 250, dtype, 24.0, 12, kl=0.5)
+    near_reference(c, least, most)
+    c(be, None)
+    want = formula(c)
+    total, off = float(want["kl"].sum()), float(want["kl_off"].sum())
+    assert abs(float(c.loss[1]) - total) <= off and float(c.loss[1]) >= 0
