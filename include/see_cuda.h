@@ -343,8 +343,9 @@ int see_cuda_preference_loss(see_cuda_backend* h, const see_preference_shape* sh
  * and loss [3] = the sums over the rows that count of weight l, weight kl and weight [r A > clip(r) A].  A row clipped so, by the
  * comparison that is counted, has no gradient but its KL term's; of 16-bit logits l's derivative by logp is within 2^-15 of its value
  * before dlogits are rounded.  old_logp, advantages, weights (NULL: 1), ref_logp (NULL: no KL term, kl_coef 0) and the output logp (0
- * where a row does not count) are [rows] in f32; what they are in rows that do not count does not matter.  clip_low from 0 to 1,
- * clip_high and kl_coef from 0 on, finite.  workspace: at least see_cuda_policy_workspace(rows) bytes, 16-byte aligned. */
+ * where a row does not count) are [rows] in f32; what they are in rows that do not count does not matter.  Where A, a
+ * weight or kl_coef is 0, so is its term, though r or exp(x) be beyond f32.  clip_low from 0 to 1, clip_high and kl_coef from 0 on, finite.
+ * workspace: at least see_cuda_policy_workspace(rows) bytes, 16-byte aligned. */
 typedef struct see_policy_shape {
   int32_t type;
   float logit_scale, clip_low, clip_high, kl_coef;

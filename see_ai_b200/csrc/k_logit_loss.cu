@@ -183,6 +183,11 @@ struct PolicyRow {
 __device__ __forceinline__ PolicyRow PolicyRowOf(const PolicyArgs& p, uint64_t row) {
   return {p.old_logp[row], p.ref_logp ? p.ref_logp[row] : 0.0f, p.advantages[row], p.weights ? p.weights[row] : 1.0f};
 }
+// x y, and 0 where y is 0 beside an x that has grown beyond its type: a ratio of probabilities.  (NaN stays.)
+template <typename F>
+__device__ __forceinline__ F Times(F x, F y) {
+  return y == 0 && x == x ? F(0) : x * y;
+}
 struct PolicyTerms {
   float slope, loss;   // slope: of the loss by logp, with its KL term; loss: without; none of them weighted
   bool clipped;
@@ -190,11 +195,12 @@ struct PolicyTerms {
 __device__ __forceinline__ PolicyTerms PolicyOf(const PolicyArgs& p, const PolicyRow& row, double logp) {
   const float off = static_cast<float>(logp - static_cast<double>(row.old)), above = static_cast<float>(static_cast<double>(row.ref) - logp);
   const float a = row.advantage, r = expf(off), cut = r < 1.0f - p.clip_low ? 1.0f - p.clip_low : r > 1.0f + p.clip_high ? 1.0f + p.clip_high : r;
+  const float by = Times(r, a);
   PolicyTerms t;
-  t.clipped = r * a > cut * a;
-  t.loss = t.clipped ? -(cut * a) : -(r * a);
-  t.slope = t.clipped ? 0.0f : -(r * a);
-  if (p.ref_logp) t.slope -= p.kl_coef * expm1f(above);
+  t.clipped = by > cut * a;
+  t.loss = t.clipped ? -(cut * a) : -by;
+  t.slope = t.clipped ? 0.0f : -by;
+  if (p.ref_logp) t.slope -= Times(expm1f(above), p.kl_coef);
   return t;
 }
 // exp(x) - x - 1, some x^2 / 2: in double, and next to 0 by its series, since the difference would leave none of an f32's digits.
@@ -206,7 +212,7 @@ __device__ __forceinline__ double KlOf(double x) {
 // PolicyFinishKernel counts it on, nor where the slope is what is left of two terms, or little because the policy is next to its
 // reference.  `off` bounds how far that logp is from the double one: ex2.approx and lg2.approx, 2^-22 each (the latter of its result where
 // that is larger than 1), and roundings of 2^-24 and 2^-25 of what it is made of.  (The f32 logp alone: 16384 rows of 250 in bf16 18.5 us,
-// so 19.5; 8192 of 32000 182 both.  The rare path as a call of its own, or in 64 registers: 20.1, 19.8.)
+// so 19.8; 8192 of 32000 182 both.)
 template <typename T>
 __device__ __forceinline__ float SlopeOf(const LogitArgs& a, const PolicyArgs& p, const PolicyRow& row, const RowSums& q) {
   if constexpr (sizeof(T) == 2) {
@@ -223,9 +229,10 @@ __device__ __forceinline__ float SlopeOf(const LogitArgs& a, const PolicyArgs& p
       slope -= by;
       most += p.kl_coef + fabsf(by);
     }
-    if (!(fabsf(beyond) <= 2.0f * off * r || most * off > 0x1p-15f * fabsf(slope))) return row.weight * slope;
+    // (what is beyond f32, and NaN, does not pass either)
+    if (fabsf(beyond) > 2.0f * off * r && most * off < fmaf(0x1p-15f, fabsf(slope), 0x1p-126f)) return row.weight * slope;
   }
-  return row.weight * PolicyOf(p, row, LogpOf<true>(a, q)).slope;
+  return Times(PolicyOf(p, row, LogpOf<true>(a, q)).slope, row.weight);
 }
 
 __device__ __forceinline__ double WarpSum(double v) {
@@ -258,9 +265,9 @@ PolicyFinishKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ 
     if (Counts(a.labels[r], a.classes)) {
       logp = LogpOf<true>(a, {q.x, q.y, q.z, q.w});
       const PolicyTerms t = PolicyOf(p, row, logp);
-      const double kl = p.ref_logp ? KlOf(static_cast<double>(row.ref) - logp) : 0.0;
-      sums[0] += static_cast<double>(row.weight) * fma(static_cast<double>(p.kl_coef), kl, static_cast<double>(t.loss));
-      sums[1] += static_cast<double>(row.weight) * kl;
+      const double kl = p.ref_logp ? KlOf(static_cast<double>(row.ref) - logp) : 0.0, weight = static_cast<double>(row.weight);
+      sums[0] += Times(static_cast<double>(t.loss) + Times(kl, static_cast<double>(p.kl_coef)), weight);
+      sums[1] += Times(kl, weight);
       sums[2] += t.clipped ? static_cast<double>(row.weight) : 0.0;
     }
     p.logp[r] = static_cast<float>(logp);

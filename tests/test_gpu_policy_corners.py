@@ -1,4 +1,4 @@
-"""The policy loss where little decides much: ratios at a corner of the clip, policies next to their reference.
+"""The policy loss where little decides much: ratios at a corner of the clip, policies next to their reference, ratios beyond f32.
 
 Tolerances are logit_reference's, but for two that are narrower or wider there:
 - kl = exp(x) - x - 1 of an x that is off by `off`: |exp(x) - 1| off, and 4 roundings of f32 of kl itself (its own, the weight's product,
@@ -103,3 +103,44 @@ def test_kl_keeps_its_digits(be, rows, dtype, least, most):
     want = formula(c)
     total, off = float(want["kl"].sum()), float(want["kl_off"].sum())
     assert abs(float(c.loss[1]) - total) <= off and float(c.loss[1]) >= 0
+
+
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("rows,classes", [(1300, 250), (33, 250), (200, 5003), (2, 300001)])
+def test_ratios_beyond_f32_times_nothing(be, rows, classes, dtype):
+    """exp(logp - old_logp) or exp(ref_logp - logp) overflows f32 where an advantage, a weight or kl_coef is 0: their terms are 0."""
+    for what in ("advantages", "weights", "kl_coef", "weights of kl"):
+        c = Policy(rows, classes, dtype, seed=13, kl=0.0 if what == "kl_coef" else 0.05)
+        far = torch.arange(rows, device="cuda") % 2 == 0
+        if what in ("advantages", "weights"):
+            c.old = torch.where(far & c.reference.counts, -300.0, c.old)
+            (c.a if what == "advantages" else c.w)[far] = 0.0
+            c.a = torch.where(far, -c.a.abs(), c.a)   # (below 0: no clip takes them)
+        else:
+            c.ref = torch.where(far, 300.0, c.reference.logp.float())
+            if what != "kl_coef":
+                c.w[far] = 0.0
+        c(be)
+        want = formula(c)
+        c.reference.check_dlogits(c.d, want["slope"], want["slope_off"])
+        for i, key in enumerate(("loss", "kl", "clipped")):
+            total = float(want[key].sum())
+            if what == "kl_coef" and key == "kl":   # (beyond f32)
+                assert float(c.loss[1]) == math.inf
+                continue
+            off = float(want[key + "_off"].sum()) if key != "clipped" else 0.0
+            assert abs(float(c.loss[i]) - total) <= off + 2 * R.ULP * abs(total), (what, key)
+
+
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+def test_what_is_not_a_number_is_not_lost_in_a_weight_of_0(be, dtype):
+    for rows, classes in ((1300, 250), (20, 5003)):
+        c = Policy(rows, classes, dtype, seed=14)
+        c.w.zero_()
+        c.a.zero_()
+        row = int(torch.nonzero(c.reference.counts)[3])
+        c.logits[row, 7] = math.nan
+        c(be)
+        assert torch.isnan(c.loss[0]) and torch.isnan(c.d[row]).all()
+        c.d[row] = 0.0
+        assert (c.d == 0).all()
