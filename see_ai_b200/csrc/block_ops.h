@@ -72,6 +72,7 @@ struct LogitArgs {
   uint64_t rows, stride;
   uint32_t classes;
   float scale, k, k_rest;                     // k: scale / ln 2; k_rest: what its rounding leaves, above 0 (of the policy loss: next to nothing)
+  float k_up;                                 // the next power of two from k on
   double inv_k;
   DeviceStatus* status;
 };

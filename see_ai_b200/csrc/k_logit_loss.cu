@@ -6,6 +6,10 @@
 // slope being the loss's derivative by logp.  The product k M is rounded once and the same in every exponent of a row, so that its
 // rounding cancels between e_c and s.  Bound by HBM: logits are read once, dlogits written once.
 //
+// Far from 0, from |k M| = 2^30 on, the rounding of k M alone is beyond what 2^x can make good.  Parts of a row that are that far below 0
+// count as nothing; a row whose maximum is far either way (all classes masked, say) is left to the kernel that comes next, whose warps make
+// its sums from memory (FarRow).  Neighbouring logits are 2^64 apart there: what is not equal to M is next to nothing.
+//
 // A row is walked in units of 16 bytes by address, of which the first and the last may stick out of it, whatever its alignment.  Rows
 // reach registers through a ring in shared memory (LogitRowsKernel); wide rows, and few ones, are shared by the blocks of a cluster.
 // A policy loss's rows that are wider still are walked twice (LogitStreamKernel), a preference loss's that are many and wide go through
@@ -149,14 +153,26 @@ __device__ __forceinline__ double LogOf(float s) {
 }
 
 constexpr double kLow = 5.1e-8;
-// k M as it is used.
+constexpr float kFar = 0x1p30f;
+__device__ __forceinline__ bool IsFar(float mk) { return fabsf(mk) >= kFar; }
+// k M as it is used; -inf: nothing here, or nothing that shows beside a row that is not far.
 template <bool kPolicy>
-__device__ __forceinline__ float Shift(float km) { return kPolicy ? km : ceilf(km); }
+__device__ __forceinline__ float TopOf(const LogitArgs& a, float z) {
+  const float km = __fmul_rn(z, a.k), top = kPolicy ? km : ceilf(km);
+  return top > -kFar ? top : MinusInf();
+}
 
-// Of a row: the label's logit, k M, the sum over the others, the sum over all.
+// Of a row: the label's logit, k M (of a far row: what FarOf makes of M), the sum over the others, the sum over all.
 struct RowSums {
   float z_label, mk, others, s;
 };
+// A logit of a far row: times a power of two, which is exact, and above k, so that what was far is 2^30 at least.  (Beyond f32, where a
+// mask's lowest value may lie: f32's largest number.)
+__device__ __forceinline__ float FarOf(const LogitArgs& a, float z) {
+  const float m = z * a.k_up;
+  return isinf(m) && !isinf(z) ? copysignf(0x1.fffffep127f, m) : m;
+}
+__device__ __forceinline__ float FarPower(const LogitArgs& a, float z, float mk) { return Ex2Approx(FarOf(a, z) - mk); }
 __device__ __forceinline__ float LabelTerm(const LogitArgs& a, float z_label, float mk) {
   return Ex2Approx(fmaf(z_label, a.k_rest, fmaf(z_label, a.k, -mk)));
 }
@@ -164,11 +180,14 @@ __device__ __forceinline__ float LabelTerm(const LogitArgs& a, float z_label, fl
 // decides by a logp agrees with what another one reports.)
 template <bool kPolicy>
 __device__ __forceinline__ double LogpOf(const LogitArgs& a, const RowSums& q) {
-  const float e = LabelTerm(a, q.z_label, q.mk);
+  const bool far = IsFar(q.mk);
+  const float e = far ? FarPower(a, q.z_label, q.mk) : LabelTerm(a, q.z_label, q.mk);
   if (3.0f * q.others < e) {   // -log1p(others / e)
     const double ratio = Quotient(static_cast<double>(q.others), static_cast<double>(e));
     return -LogRatio(Quotient(ratio, 2.0 + ratio));
   }
+  if (far)
+    return fma(static_cast<double>(a.scale), (static_cast<double>(FarOf(a, q.z_label)) - static_cast<double>(q.mk)) / static_cast<double>(a.k_up), -LogOf(q.s));
   const double above = fma(static_cast<double>(a.scale), fma(-static_cast<double>(q.mk), a.inv_k, static_cast<double>(q.z_label)), -LogOf(q.s));
   return kPolicy ? above : above - kLow;
 }
@@ -246,10 +265,55 @@ __device__ __forceinline__ float WarpMax(float v) {
   return r;
 }
 
+// The sums of a far row, by a warp, from memory.  (Of -inf alone: NaN.)
+template <typename T>
+__device__ __noinline__ RowSums FarRow(const LogitArgs& a, uint64_t r, int32_t label) {
+  const Row<T> row(a, r);
+  const uint32_t lane = threadIdx.x & 31;
+  float top = MinusInf(), v[kPerUnit<T>];
+  for (uint32_t u = lane; u < row.units; u += 32) {
+    row.Load(u, v);
+#pragma unroll
+    for (int j = 0; j < kPerUnit<T>; ++j) top = fmaxf(top, v[j]);
+  }
+  const float z_label = ToF32(row.z[label]), mk = FarOf(a, WarpMax(top));
+  float others = 0.0f;
+  for (uint32_t u = lane; u < row.units; u += 32) {
+    row.Load(u, v);
+#pragma unroll
+    for (int j = 0; j < kPerUnit<T>; ++j)
+      if (row.At(u) + j != label) others += FarPower(a, v[j], mk);
+  }
+#pragma unroll
+  for (uint32_t o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xFFFFFFFFu, others, o);
+  return {z_label, mk, others, others + FarPower(a, z_label, mk)};
+}
+// Its dlogits, or of them the units first, first + step, ...
+template <typename T>
+__device__ __noinline__ void FarGradient(const LogitArgs& a, uint64_t r, int32_t label, const RowSums q, float slope, uint32_t first, uint32_t step) {
+  const Row<T> row(a, r);
+  const float by = -slope / q.s;
+  const uint32_t label_unit = (static_cast<uint32_t>(label) + row.skip) / kPerUnit<T>;
+  for (uint32_t u = first; u < row.units; u += step) {
+    float v[kPerUnit<T>];
+    row.Load(u, v);
+#pragma unroll
+    for (int j = 0; j < kPerUnit<T>; ++j) v[j] = slope == 0.0f ? 0.0f : by * FarPower(a, v[j], q.mk);
+    row.Store(u, v);
+    if (u == label_unit) row.d[label] = FromF32<T>(slope == 0.0f ? 0.0f : slope * (q.others / q.s));
+  }
+}
+// Calls far(lane) for each lane of a warp whose row is far; all lanes are here.
+template <typename F>
+__device__ __forceinline__ void EachFar(bool is, F far) {
+  for (uint32_t left = __ballot_sync(0xFFFFFFFFu, is); left != 0; left &= left - 1) far(static_cast<uint32_t>(__ffs(static_cast<int>(left)) - 1));
+}
+
 constexpr uint32_t kFinishThreads = 256;
 
 // From what is kept of the rows: logp and the loss's three sums, a block's rows in its partials; the block that comes last (*arrived,
-// which the rows' kernel has set to 0) adds them up, in the blocks' order.
+// which the rows' kernel has set to 0) adds them up, in the blocks' order.  A far row's dlogits are made here.
+template <typename T>
 __global__ void __launch_bounds__(kFinishThreads)
 PolicyFinishKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PolicyArgs p, const float4* __restrict__ kept,
                    double* __restrict__ partials, uint32_t* __restrict__ arrived) {
@@ -258,19 +322,34 @@ PolicyFinishKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ 
   __shared__ bool last;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sums[3] = {};
-  for (uint64_t r = static_cast<uint64_t>(blockIdx.x) * kFinishThreads + threadIdx.x; r < a.rows; r += static_cast<uint64_t>(gridDim.x) * kFinishThreads) {
+  for (uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * kFinishThreads + warp * 32; r0 < a.rows; r0 += static_cast<uint64_t>(gridDim.x) * kFinishThreads) {
     double logp = 0.0;
-    const float4 q = kept[r];   // (all at once; of a row that does not count, whatever is there)
+    const bool here = r0 + lane < a.rows;
+    const uint64_t r = here ? r0 + lane : r0;
+    const float4 k = kept[r];   // (all at once; of a row that does not count, whatever is there)
     const PolicyRow row = PolicyRowOf(p, r);
-    if (Counts(a.labels[r], a.classes)) {
-      logp = LogpOf<true>(a, {q.x, q.y, q.z, q.w});
+    const int32_t label = a.labels[r];
+    const bool counts = here && Counts(label, a.classes);
+    RowSums q = {k.x, k.y, k.z, k.w};
+    EachFar(counts && IsFar(q.mk), [&](uint32_t which) {
+      const RowSums sums = FarRow<T>(a, r0 + which, __shfl_sync(0xFFFFFFFFu, label, which));
+      if (which == lane) q = sums;
+    });
+    if (counts) {
+      logp = LogpOf<true>(a, q);
       const PolicyTerms t = PolicyOf(p, row, logp);
       const double kl = p.ref_logp ? KlOf(static_cast<double>(row.ref) - logp) : 0.0, weight = static_cast<double>(row.weight);
       sums[0] += Times(static_cast<double>(t.loss) + Times(kl, static_cast<double>(p.kl_coef)), weight);
       sums[1] += Times(kl, weight);
       sums[2] += t.clipped ? static_cast<double>(row.weight) : 0.0;
     }
-    p.logp[r] = static_cast<float>(logp);
+    if (here) p.logp[r] = static_cast<float>(logp);
+    if (a.dlogits == nullptr) continue;
+    EachFar(counts && IsFar(q.mk), [&](uint32_t which) {
+      auto of = [which](float v) { return __shfl_sync(0xFFFFFFFFu, v, which); };
+      const float slope = Times(PolicyOf(p, row, logp).slope, row.weight) * ((p.loss_grad ? *p.loss_grad : 1.0f) * a.scale);
+      FarGradient<T>(a, r0 + which, __shfl_sync(0xFFFFFFFFu, label, which), {of(q.z_label), of(q.mk), of(q.others), of(q.s)}, of(slope), lane, 32);
+    });
   }
   auto block_sum = [&] {   // in warp 0's lanes, the three sums
 #pragma unroll
@@ -523,7 +602,7 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
 #pragma unroll
       for (int i = 0; i < NU; ++i) raw[i] = t + i * threads < count ? mine[t + i * threads] : Nothing<T>();
     }
-    float mk = Shift<kPolicy>(__fmul_rn(Largest<T, NU>(raw), a.k)), sum;   // -inf: nothing here
+    float mk = TopOf<kPolicy>(a, Largest<T, NU>(raw)), sum;
     // A lone slot is filled while the exponentials are made, unless dlogits will be stored meanwhile: loads and stores in turn are
     // faster then (8192 rows of 32000 in bf16: 172 us, early 184; a preference loss of 16 x 512 x 16001 in f32 357, early 344).
     const bool early = plan.slots == 1 && !(kPolicy && a.dlogits);
@@ -597,12 +676,12 @@ LogitRowsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Pol
     T raw_label;
     if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(items[0]);
     else raw_label.bits = static_cast<uint16_t>(items[0]);
-    const float z_label = ToF32(raw_label), mk_label = Shift<kPolicy>(__fmul_rn(z_label, a.k)), all = fmaxf(mk, mk_label);
-    RowSums q = {z_label, all == MinusInf() ? 0.0f : all, sum * factor(mk, all), 0.0f};
+    const float z_label = ToF32(raw_label), mk_label = TopOf<kPolicy>(a, z_label), all = fmaxf(mk, mk_label);
+    RowSums q = {z_label, all, sum * factor(mk, all), 0.0f};
     q.s = q.others + LabelTerm(a, z_label, q.mk);
     if (t == 0 && rank == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
     if constexpr (kPolicy) {
-      if (!a.dlogits) continue;
+      if (!a.dlogits || IsFar(q.mk)) continue;
       const PolicyRow brings = {__uint_as_float(items[1]), __uint_as_float(items[2]), __uint_as_float(items[3]), __uint_as_float(items[4])};
       const float slope = SlopeOf<T>(a, p, brings, q) * grad;
       if (slope == 0.0f) {
@@ -739,7 +818,7 @@ LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Po
       const int32_t e0 = static_cast<int32_t>(u * E) - static_cast<int32_t>(row.skip);
       if ((e0 < 0 || u >= whole_end || u == label_unit) && u < row.units) raw[i] = Only<T>(raw[i], -e0, static_cast<int32_t>(a.classes) - e0, label - e0);
     }
-    float mk = WarpMax(Shift<kPolicy>(__fmul_rn(Largest<T, NU>(raw), a.k)));
+    const float mk = WarpMax(TopOf<kPolicy>(a, Largest<T, NU>(raw)));
     const f32x2 away = Splat2(mk == MinusInf() ? 0.0f : -mk);
     f32x2 sum2 = 0;
 #pragma unroll
@@ -758,12 +837,12 @@ LogitShortKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ Po
     T raw_label;
     if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(label_bits);
     else raw_label.bits = static_cast<uint16_t>(label_bits);
-    const float z_label = ToF32(raw_label), mk_label = Shift<kPolicy>(__fmul_rn(z_label, a.k)), all = fmaxf(mk, mk_label);
-    RowSums q = {z_label, all == MinusInf() ? 0.0f : all, mk == MinusInf() ? 0.0f * sum : sum * Ex2Approx(mk - all), 0.0f};
+    const float z_label = ToF32(raw_label), mk_label = TopOf<kPolicy>(a, z_label), all = fmaxf(mk, mk_label);
+    RowSums q = {z_label, all, mk == MinusInf() ? 0.0f * sum : sum * Ex2Approx(mk - all), 0.0f};
     q.s = q.others + LabelTerm(a, z_label, q.mk);
     if (lane == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
     if constexpr (kPolicy) {
-      if (!a.dlogits) continue;
+      if (!a.dlogits || IsFar(q.mk)) continue;
       const PolicyRow brings = {__uint_as_float(__shfl_sync(0xFFFFFFFFu, item, 1)), __uint_as_float(__shfl_sync(0xFFFFFFFFu, item, 2)),
                                 __uint_as_float(__shfl_sync(0xFFFFFFFFu, item, 3)), __uint_as_float(__shfl_sync(0xFFFFFFFFu, item, 4))};
       const float slope = SlopeOf<T>(a, p, brings, q) * grad;   // (0: zeros come out)
@@ -920,7 +999,7 @@ LogitSumsKernel(const __grid_constant__ LogitArgs a, const Sequences seq, float4
               raw[j] = Only<T>(raw[j], static_cast<int32_t>(row.skip) - e0, static_cast<int32_t>(ends_at) - e0, label + static_cast<int32_t>(row.skip) - e0);
           }
         }
-        const float top = fmaxf(mk, Shift<false>(__fmul_rn(Largest<T, kSumUnits>(raw), a.k)));
+        const float top = fmaxf(mk, TopOf<false>(a, Largest<T, kSumUnits>(raw)));
         __syncwarp();   // the slot is read
         fill();
         const f32x2 away = Splat2(top == MinusInf() ? 0.0f : -top);
@@ -962,8 +1041,8 @@ LogitSumsKernel(const __grid_constant__ LogitArgs a, const Sequences seq, float4
       T raw_label;
       if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(label_bits);
       else raw_label.bits = static_cast<uint16_t>(label_bits);
-      const float z_label = ToF32(raw_label), mk_label = Shift<false>(__fmul_rn(z_label, a.k)), top = fmaxf(mk, mk_label);
-      RowSums q = {z_label, top == MinusInf() ? 0.0f : top, sum * factor(mk, top), 0.0f};
+      const float z_label = ToF32(raw_label), mk_label = TopOf<false>(a, z_label), top = fmaxf(mk, mk_label);
+      RowSums q = {z_label, top, sum * factor(mk, top), 0.0f};
       q.s = q.others + LabelTerm(a, z_label, q.mk);
       kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
     }
@@ -1109,7 +1188,7 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
             raw[i] = Only<T>(raw[i], static_cast<int32_t>(w.skip) - e0, static_cast<int32_t>(ends_at) - e0, label + static_cast<int32_t>(w.skip) - e0);
         }
       }
-      const float top = fmaxf(mk, __fmul_rn(Largest<T, kWalkUnits>(raw), a.k));
+      const float top = fmaxf(mk, TopOf<true>(a, Largest<T, kWalkUnits>(raw)));
       GroupBarrier(kWalkers, group);   // the slot is read
       fill();
       const f32x2 away = Splat2(top == MinusInf() ? 0.0f : -top);
@@ -1151,11 +1230,12 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
     T raw_label;
     if constexpr (sizeof(T) == 4) raw_label = __uint_as_float(items[0]);
     else raw_label.bits = static_cast<uint16_t>(items[0]);
-    const float z_label = ToF32(raw_label), mk_label = __fmul_rn(z_label, a.k), all = fmaxf(mk, mk_label);
-    RowSums q = {z_label, all == MinusInf() ? 0.0f : all, sum * factor(mk, all), 0.0f};
+    const float z_label = ToF32(raw_label), mk_label = TopOf<true>(a, z_label), all = fmaxf(mk, mk_label);
+    RowSums q = {z_label, all, sum * factor(mk, all), 0.0f};
     q.s = q.others + LabelTerm(a, z_label, q.mk);
     if (t == 0) kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
-    if (!twice) continue;
+    if (!twice) continue;   // (a far row is walked again all the same, as its chunks are on their way)
+    const bool far = IsFar(q.mk);
     const PolicyRow brings = {__uint_as_float(items[1]), __uint_as_float(items[2]), __uint_as_float(items[3]), __uint_as_float(items[4])};
     const float slope = SlopeOf<T>(a, p, brings, q) * grad;   // (0: zeros come out)
     const f32x2 by = Splat2(-slope / q.s), away = Splat2(-q.mk);
@@ -1175,6 +1255,7 @@ LogitStreamKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ P
       GroupBarrier(kWalkers, group);   // the slot is read
       fill();
       const uint32_t u0 = chunk * kChunk + t;
+      if (far) continue;
       if (row.alike && (chunk != 0 || w.skip == 0) && (chunk + 1) * kChunk * E <= ends_at) {
         uint4* to = reinterpret_cast<uint4*>(row.d - w.skip) + u0;
 #pragma unroll
@@ -1199,9 +1280,29 @@ __device__ __forceinline__ double Softplus(double x) { return (x > 0.0 ? x : 0.0
 
 constexpr uint32_t kPairThreads = 512;
 
+// The logp of the far ones among a warp's rows first .. first + 31, and those kPairThreads / 2 further on, ... before `end`, whose sums are
+// kept anew.
+template <typename T>
+__device__ __noinline__ double FarRows(const LogitArgs& a, float4* __restrict__ kept, int64_t first, int64_t end) {
+  const uint32_t lane = threadIdx.x & 31;
+  double sum = 0.0;
+  for (int64_t r0 = first; r0 < end; r0 += kPairThreads / 2) {
+    const int64_t r = r0 + lane;
+    const int32_t label = r < end ? a.labels[r] : -1;
+    EachFar(Counts(label, a.classes) && IsFar(kept[r].y), [&](uint32_t which) {
+      const RowSums q = FarRow<T>(a, static_cast<uint64_t>(r0) + which, __shfl_sync(0xFFFFFFFFu, label, which));
+      if (which != lane) return;
+      kept[r] = make_float4(q.z_label, q.mk, q.others, q.s);
+      sum += LogpOf<false>(a, q);
+    });
+  }
+  return sum;
+}
+
 // A pair to a block: the first eight warps sum the chosen rows, the others the rejected ones.  Then each row's kept.x becomes the loss's
 // derivative by its logp, logit_scale and loss_grad included, 0 where it does not count.  losses [pairs]: added up by
 // PreferenceFoldKernel.
+template <typename T>
 __global__ void __launch_bounds__(kPairThreads)
 PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PreferenceArgs p, float4* __restrict__ kept) {
   AwaitPrevious();
@@ -1214,13 +1315,16 @@ PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant
     const int64_t begin = min(max(static_cast<int64_t>(p.starts[s]), static_cast<int64_t>(0)), most);
     const int64_t end = min(static_cast<int64_t>(p.starts[s + 1]), most);
     double sum = 0.0, counted = 0.0;
+    bool far = false;
     for (int64_t r = begin + t; r < end; r += kPairThreads / 2) {
       const float4 q = kept[r];   // (asked for beside the label; of a row that does not count, whatever is there)
       if (Counts(a.labels[r], a.classes)) {
-        sum += LogpOf<false>(a, {q.x, q.y, q.z, q.w});
         counted += 1.0;
+        if (IsFar(q.y)) far = true;
+        else sum += LogpOf<false>(a, {q.x, q.y, q.z, q.w});
       }
     }
+    if (__any_sync(0xFFFFFFFFu, far)) sum += FarRows<T>(a, kept, begin + (t - lane), end);
     sum = WarpSum(sum);
     counted = WarpSum(counted);
     __syncthreads();   // (the last pair's are read)
@@ -1303,6 +1407,10 @@ PreferenceGradientKernel(const __grid_constant__ LogitArgs a, const __grid_const
     const bool counts = Counts(label, a.classes);   // (what is kept of other rows is not set)
     const float slope = counts ? q.x : 0.0f, by = -slope / q.w, mk = q.y;
     const uint32_t label_unit = counts ? (static_cast<uint32_t>(label) + row.skip) / kPerUnit<T> : ~0u;
+    if (counts && IsFar(mk)) {
+      FarGradient<T>(a, static_cast<uint64_t>(r), label, {q.x, q.y, q.z, q.w}, slope, (warp % warps) * 32 + lane, warps * 32);
+      continue;
+    }
     for (uint32_t u0 = (warp % warps) * 32 * kGradUnits + lane; u0 < row.units; u0 += warps * 32 * kGradUnits) {
       uint4 raw[kGradUnits];
       if (slope != 0.0f) {
@@ -1472,7 +1580,7 @@ cudaError_t Policy(const LogitArgs& a, const PolicyArgs& p, float4* kept, uint32
   if (cudaError_t e = RunRows<T, true>(a, p, {}, kept, arrived, sms, s); e != cudaSuccess) return e;
   *launches += 2;
   const uint64_t blocks = (a.rows + kFinishThreads - 1) / kFinishThreads;
-  return Next(PolicyFinishKernel, static_cast<unsigned>(blocks < kPolicyPartials ? blocks : kPolicyPartials), kFinishThreads, 0, s)(
+  return Next(PolicyFinishKernel<T>, static_cast<unsigned>(blocks < kPolicyPartials ? blocks : kPolicyPartials), kFinishThreads, 0, s)(
       a, p, static_cast<const float4*>(kept), partials, arrived);
 }
 
@@ -1482,7 +1590,7 @@ cudaError_t Preference(const LogitArgs& a, const PreferenceArgs& p, float4* kept
     if (cudaError_t e = RunRows<T, false>(a, {}, {p.starts, 2 * p.pairs}, kept, nullptr, sms, s); e != cudaSuccess) return e;
     ++*launches;
   }
-  if (cudaError_t e = Next(PreferencePairsKernel, p.pairs < 4 * sms ? p.pairs : 4 * sms, kPairThreads, 0, s)(a, p, kept); e != cudaSuccess) return e;
+  if (cudaError_t e = Next(PreferencePairsKernel<T>, p.pairs < 4 * sms ? p.pairs : 4 * sms, kPairThreads, 0, s)(a, p, kept); e != cudaSuccess) return e;
   *launches += 2;
   if (!a.dlogits) return Next(PreferenceFoldKernel, 1, 256, 0, s)(p);
   // Warps to a row: as many as its pieces of 128 units keep busy, or, of few rows, as many as there are pieces for.

@@ -36,8 +36,11 @@ k::LogitArgs ArgsOf(const Shape& s, const void* logits, const int32_t* labels, v
   float k = static_cast<float>(exact);
   if (whole && static_cast<double>(k) > exact) k = std::nextafter(k, 0.0f);
   const float rest = whole ? static_cast<float>(exact - static_cast<double>(k)) : 0.0f;
+  int exponent;
+  const bool power = std::frexp(k, &exponent) == 0.5f;
+  const float up = std::ldexp(1.0f, power ? exponent - 1 : exponent);
   return {logits, s.rows ? dlogits : nullptr, labels, s.rows, s.stride, static_cast<uint32_t>(s.classes), s.logit_scale, k,
-          std::max(rest, std::numeric_limits<float>::min()), 1.0 / (whole ? exact : static_cast<double>(k)), status};
+          std::max(rest, std::numeric_limits<float>::denorm_min()), up, 1.0 / (whole ? exact : static_cast<double>(k)), status};
 }
 
 }  // namespace
