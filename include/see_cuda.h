@@ -314,9 +314,9 @@ int see_cuda_join_backward(see_cuda_backend* h, const see_join_shape* shape, con
  * type, stride: elements from a row to the next (0: classes); dlogits: of the same type and stride, NULL: not wanted; it may be logits
  * itself (in place).
  * labels [rows]; a row whose label is not in 0 .. classes - 1 does not count: what its logits are does not matter, and its dlogits are
- * zeros.  logp = log softmax(logit_scale logits)[label]: sums over classes in f32, logp and sums over rows in double.  loss_grad: an f32
- * that dlogits is multiplied by (the scale of the loss), or NULL.  A row that holds a NaN or +inf, or -inf alone, has a NaN loss and NaN
- * dlogits.  Other logits are any finite numbers, a row of the type's lowest value alone among them; those of a magnitude from
+ * zeros.  logp = log softmax(logit_scale logits)[label], logit_scale from 2^-100 to 2^100: sums over classes in f32, logp and sums over
+ * rows in double.  loss_grad: an f32 that dlogits is multiplied by (the scale of the loss), or NULL.  A row that holds a NaN or +inf, or
+ * -inf alone, has a NaN loss and NaN dlogits.  Other logits are any finite numbers, a row of the type's lowest value alone among them; those of a magnitude from
  * 2^126 / logit_scale on are not told from one another.
  * The same call has the same bits; the sums' order goes by the sizes, the alignment and the device's number of SMs. */
 enum { SEE_PREFERENCE_SIGMOID = 0, SEE_PREFERENCE_HINGE = 1, SEE_PREFERENCE_SQUARE = 2 };

@@ -15,7 +15,8 @@ constexpr double kLog2E = 1.4426950408889634;
 template <typename Shape>
 Status CheckLogits(const std::string& what, Shape* s) {
   if (!IsType(s->type)) return std::unexpected(what + ": unknown type");
-  if (!(s->logit_scale > 0.0f) || !std::isfinite(s->logit_scale)) return std::unexpected(what + ": logit_scale is not a finite number above 0");
+  // (logit_scale / ln 2, the power of two above it and what its rounding leaves are f32's)
+  if (!(s->logit_scale >= 0x1p-100f && s->logit_scale <= 0x1p100f)) return std::unexpected(what + ": logit_scale is not from 2^-100 to 2^100");
   if (s->classes == 0 || s->classes > (1u << 20)) return std::unexpected(what + ": 1 to 2^20 classes");
   if (s->rows > 0x7FFFFFFFull) return std::unexpected(what + ": more than 2^31 - 1 rows");
   if (s->stride == 0) s->stride = s->classes;
