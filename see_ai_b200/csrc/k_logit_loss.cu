@@ -227,24 +227,26 @@ __device__ __forceinline__ double KlOf(double x) {
   return fabs(x) < 0x1p-10 ? x * x * fma(x, fma(x, 1.0 / 24.0, 1.0 / 6.0), 0.5) : expm1(x) - x;
 }
 // The loss's weighted derivative by a row's logp, as it goes into dlogits.  Of 16-bit logits, 8 or 11 bits: mostly a logp in f32 is enough,
-// and takes each warp some 40 instructions instead of 100.  It is not next to a corner, where the row is on the side that
+// and takes each warp a third of the instructions.  It is not next to a corner, where the row is on the side that
 // PolicyFinishKernel counts it on, nor where the slope is what is left of two terms, or little because the policy is next to its
-// reference.  `off` bounds how far that logp is from the double one: ex2.approx and lg2.approx, 2^-22 each (the latter of its result where
-// that is larger than 1), and roundings of 2^-24 and 2^-25 of what it is made of.  (The f32 logp alone: 16384 rows of 250 in bf16 18.5 us,
-// so 19.8; 8192 of 32000 182 both.)
+// reference.  `off` bounds how far logp, less what it is compared with, and the exponential of that, relative, are from those of the double
+// one, in 2^-22: lg2.approx 0.7 of 1 or of its result, ex2.approx 1 for the label's term and 1 for the exponential, whose double has 1/2;
+// roundings of 2^-24 or 2^-25, 3.5 of logp, 2.5 of the difference, 0.7 of the logarithm.
+// (Rows of 250 in bf16, 16384 18.7 us, 65536 52.0, as with the f32 logp alone; each in double: f32 logits, 52.6.)
 template <typename T>
 __device__ __forceinline__ float SlopeOf(const LogitArgs& a, const PolicyArgs& p, const PolicyRow& row, const RowSums& q) {
   if constexpr (sizeof(T) == 2) {
-    constexpr float kLn2 = 0.6931471805599453f;
+    constexpr float kLn2 = 0.6931471805599453f, kLog2E = 1.4426950408889634f;
     float log2s;
     asm("lg2.approx.f32 %0, %1;" : "=f"(log2s) : "f"(q.s));
     const float logp = kLn2 * (fmaf(q.z_label, a.k, -q.mk) - log2s);
-    const float off = 0x1p-21f * (1.0f + fabsf(log2s) + fabsf(logp) + fabsf(row.old) + fabsf(row.ref));
-    const float r = expf(logp - row.old);   // beyond: the corner that the advantage's sign chooses
+    const float d = logp - row.old, x = p.ref_logp ? row.ref - logp : 0.0f;
+    const float off = 0x1p-22f * (4.0f + fabsf(log2s) + fabsf(logp) + fabsf(d) + fabsf(x));
+    const float r = Ex2Approx(d * kLog2E);   // beyond: the corner that the advantage's sign chooses
     const float beyond = row.advantage > 0.0f ? r - (1.0f + p.clip_high) : row.advantage < 0.0f ? (1.0f - p.clip_low) - r : -r;
     float slope = beyond > 0.0f ? 0.0f : -(r * row.advantage), most = fabsf(slope);   // most: what the slope is off by, divided by `off`
     if (p.ref_logp) {
-      const float by = p.kl_coef * expm1f(row.ref - logp);
+      const float by = p.kl_coef * (Ex2Approx(x * kLog2E) - 1.0f);
       slope -= by;
       most += p.kl_coef + fabsf(by);
     }
