@@ -290,13 +290,13 @@ __device__ __noinline__ RowSums FarRow(const LogitArgs& a, uint64_t r, int32_t l
   for (uint32_t o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xFFFFFFFFu, others, o);
   return {z_label, mk, others, others + FarPower(a, z_label, mk)};
 }
-// Its dlogits, or of them the units first, first + step, ...
+// Its dlogits, by a warp.
 template <typename T>
-__device__ __noinline__ void FarGradient(const LogitArgs& a, uint64_t r, int32_t label, const RowSums q, float slope, uint32_t first, uint32_t step) {
+__device__ __noinline__ void FarGradient(const LogitArgs& a, uint64_t r, int32_t label, const RowSums q, float slope) {
   const Row<T> row(a, r);
   const float by = -slope / q.s;
   const uint32_t label_unit = (static_cast<uint32_t>(label) + row.skip) / kPerUnit<T>;
-  for (uint32_t u = first; u < row.units; u += step) {
+  for (uint32_t u = threadIdx.x & 31; u < row.units; u += 32) {
     float v[kPerUnit<T>];
     row.Load(u, v);
 #pragma unroll
@@ -350,7 +350,7 @@ PolicyFinishKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ 
     EachFar(counts && IsFar(q.mk), [&](uint32_t which) {
       auto of = [which](float v) { return __shfl_sync(0xFFFFFFFFu, v, which); };
       const float slope = Times(PolicyOf(p, row, logp).slope, row.weight) * ((p.loss_grad ? *p.loss_grad : 1.0f) * a.scale);
-      FarGradient<T>(a, r0 + which, __shfl_sync(0xFFFFFFFFu, label, which), {of(q.z_label), of(q.mk), of(q.others), of(q.s)}, of(slope), lane, 32);
+      FarGradient<T>(a, r0 + which, __shfl_sync(0xFFFFFFFFu, label, which), {of(q.z_label), of(q.mk), of(q.others), of(q.s)}, of(slope));
     });
   }
   auto block_sum = [&] {   // in warp 0's lanes, the three sums
@@ -1301,9 +1301,22 @@ __device__ __noinline__ double FarRows(const LogitArgs& a, float4* __restrict__ 
   return sum;
 }
 
+// Their dlogits; slope: the loss's derivative by the logp of each.
+template <typename T>
+__device__ __noinline__ void FarGradients(const LogitArgs& a, const float4* kept, int64_t first, int64_t end, float slope) {
+  for (int64_t r0 = first; r0 < end; r0 += kPairThreads / 2) {
+    const int64_t r = r0 + (threadIdx.x & 31);
+    const int32_t label = r < end ? a.labels[r] : -1;
+    EachFar(Counts(label, a.classes) && IsFar(kept[r].y), [&](uint32_t which) {
+      const float4 q = kept[r0 + which];   // (the block has met since that was written)
+      FarGradient<T>(a, static_cast<uint64_t>(r0) + which, __shfl_sync(0xFFFFFFFFu, label, which), {q.x, q.y, q.z, q.w}, slope);
+    });
+  }
+}
+
 // A pair to a block: the first eight warps sum the chosen rows, the others the rejected ones.  Then each row's kept.x becomes the loss's
-// derivative by its logp, logit_scale and loss_grad included, 0 where it does not count.  losses [pairs]: added up by
-// PreferenceFoldKernel.
+// derivative by its logp, logit_scale and loss_grad included, 0 where it does not count; far rows get their dlogits.  losses [pairs]:
+// added up by PreferenceFoldKernel.
 template <typename T>
 __global__ void __launch_bounds__(kPairThreads)
 PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant__ PreferenceArgs p, float4* __restrict__ kept) {
@@ -1326,7 +1339,8 @@ PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant
         else sum += LogpOf<false>(a, {q.x, q.y, q.z, q.w});
       }
     }
-    if (__any_sync(0xFFFFFFFFu, far)) sum += FarRows<T>(a, kept, begin + (t - lane), end);
+    far = __any_sync(0xFFFFFFFFu, far);
+    if (far) sum += FarRows<T>(a, kept, begin + (t - lane), end);
     sum = WarpSum(sum);
     counted = WarpSum(counted);
     __syncthreads();   // (the last pair's are read)
@@ -1358,6 +1372,7 @@ PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant
       const double each = slope * beta / static_cast<double>(p.pairs);
       const float of_row = static_cast<float>((side ? -each * per_row[1] : each * per_row[0]) * static_cast<double>(grad));
       for (int64_t r = begin + t; r < end; r += kPairThreads / 2) kept[r].x = Counts(a.labels[r], a.classes) ? of_row : 0.0f;
+      if (far) FarGradients<T>(a, kept, begin + (t - lane), end, of_row);
     }
     if (threadIdx.x != 0) continue;   // (its functions take a microsecond: after the rows)
     const double off = (h - 0.5) / beta;
@@ -1409,21 +1424,18 @@ PreferenceGradientKernel(const __grid_constant__ LogitArgs a, const __grid_const
     const bool counts = Counts(label, a.classes);   // (what is kept of other rows is not set)
     const float slope = counts ? q.x : 0.0f, by = -slope / q.w, mk = q.y;
     const uint32_t label_unit = counts ? (static_cast<uint32_t>(label) + row.skip) / kPerUnit<T> : ~0u;
-    if (counts && IsFar(mk)) {
-      FarGradient<T>(a, static_cast<uint64_t>(r), label, {q.x, q.y, q.z, q.w}, slope, (warp % warps) * 32 + lane, warps * 32);
-      continue;
-    }
-    for (uint32_t u0 = (warp % warps) * 32 * kGradUnits + lane; u0 < row.units; u0 += warps * 32 * kGradUnits) {
+    const uint32_t units = counts && IsFar(mk) ? 0 : row.units;   // (a far row's dlogits are there)
+    for (uint32_t u0 = (warp % warps) * 32 * kGradUnits + lane; u0 < units; u0 += warps * 32 * kGradUnits) {
       uint4 raw[kGradUnits];
       if (slope != 0.0f) {
 #pragma unroll
         for (int i = 0; i < kGradUnits; ++i)
-          if (u0 + i * 32 < row.units) raw[i] = row.RawOnce(u0 + i * 32);
+          if (u0 + i * 32 < units) raw[i] = row.RawOnce(u0 + i * 32);
       }
 #pragma unroll
       for (int i = 0; i < kGradUnits; ++i) {
         const uint32_t u = u0 + i * 32;
-        if (u >= row.units) break;
+        if (u >= units) break;
         float v[kPerUnit<T>];
         if (slope == 0.0f) {
 #pragma unroll
