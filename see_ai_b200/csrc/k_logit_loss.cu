@@ -1365,7 +1365,7 @@ PreferencePairsKernel(const __grid_constant__ LogitArgs a, const __grid_constant
     }
     const double beta = p.beta, h = beta * (ratio[0] - ratio[1]) - static_cast<double>(p.margin), smoothing = p.smoothing;
     double slope;
-    if (p.kind == SEE_PREFERENCE_SIGMOID) slope = smoothing - static_cast<double>(1.0f / (1.0f + expf(static_cast<float>(h))));
+    if (p.kind == SEE_PREFERENCE_SIGMOID) slope = smoothing - 1.0 / (1.0 + exp(h));   // (a difference: f32 would leave no digits of it)
     else if (p.kind == SEE_PREFERENCE_HINGE) slope = h >= 1.0 ? 0.0 : h < 1.0 ? -1.0 : h;   // (NaN stays)
     else slope = 2.0 * (h - 0.5) / (beta * beta);
     if (a.dlogits) {
