@@ -321,7 +321,8 @@ int see_cuda_join_backward(see_cuda_backend* h, const see_join_shape* shape, con
  * The same call has the same bits; the sums' order goes by the sizes, the alignment and the device's number of SMs. */
 enum { SEE_PREFERENCE_SIGMOID = 0, SEE_PREFERENCE_HINGE = 1, SEE_PREFERENCE_SQUARE = 2 };
 /* Sequences 2 i (chosen) and 2 i + 1 (rejected) are a pair; sequence s has the rows starts[s] .. starts[s + 1] - 1 (starts: 2 pairs + 1
- * ascending row numbers).  Rows before the first and behind the last are neither read nor written.  S_s: the sum of logp over the
+ * ascending row numbers).  Rows before the first and behind the last are neither read nor written: dlogits there stay what they were, in
+ * place the logits.  Padding that must become zeros belongs into a sequence, with labels that do not count.  S_s: the sum of logp over the
  * sequence's rows that count, or (average != 0) their average; no such row: 0.  ref_logp [2 pairs]: the reference model's S, NULL: 0.
  *   h_i = beta ((S - ref)[2 i] - (S - ref)[2 i + 1]) - margin,  loss = the average over pairs of
  *   sigmoid: -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h);  hinge: max(0, 1 - h), no gradient at h = 1;

@@ -502,8 +502,8 @@ class CudaBackend:
                         type: int = F32, kind: int = PREFERENCE_SIGMOID, beta: float = 0.1, smoothing: float = 0.0, margin: float = 0.0,
                         logit_scale: float = 1.0, average: bool = False, stride: int = 0):
         """A preference loss of `pairs` of sequences (2 i chosen, 2 i + 1 rejected; sequence s is the rows starts[s] up to
-        starts[s + 1]) over DEVICE pointers, with the gradient of the logits (dlogits 0: not wanted; logits: in place).  The
-        workspace has preference_workspace(rows, pairs) bytes."""
+        starts[s + 1]) over DEVICE pointers, with the gradient of the logits (dlogits 0: not wanted; logits: in place; rows that no
+        sequence has stay as they were).  The workspace has preference_workspace(rows, pairs) bytes."""
         shape = PreferenceShape(type, kind, beta, smoothing, margin, logit_scale, int(average), 0, rows, classes, stride, pairs)
         self._check(self.lib.see_cuda_preference_loss(self.h, shape, logits or None, labels or None, starts or None, ref_logp or None,
                                                       loss_grad or None, loss or None, margins or None, sequence_logp or None,

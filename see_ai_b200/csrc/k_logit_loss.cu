@@ -1574,7 +1574,7 @@ cudaError_t RunRows(const LogitArgs& a, const PolicyArgs& p, const Sequences& se
   } else if (!shared || (a.rows > 2 * sms && (w.threads > kThreads / 2 || a.classes >= 20000))) {
     // Many rows wider than two groups of an SM hold, or of 20000 classes on: with pairs and gradient, 8 x 512 x 32000 in bf16 take 190 us,
     // in groups' registers 195; 16 x 100 x 50001 117 and 128; 16 x 512 x 20001 in f16 244 and 251.  But 16 x 512 x 16000 191 and 182, in
-    // f32 356 and 344.
+    // f32 356 and 344.  (The 20000 are for 16 bits: f32 rows have more than half a block's threads from 16384 classes on.)
     const uint32_t chunks = (all + kSumChunk - 1) / kSumChunk, window = sms * kListed;
     uint32_t warps = kSumWarps;   // to a row: as many as its chunks keep busy
     while (warps > 1 && (chunks + warps - 1) / warps * warps * 15 > chunks * 16) warps /= 2;
