@@ -6,9 +6,9 @@
 // slope being the loss's derivative by logp.  The product k M is rounded once and the same in every exponent of a row, so that its
 // rounding cancels between e_c and s.  Bound by HBM: logits are read once, dlogits written once.
 //
-// Far from 0, from |k M| = 2^30 on, the rounding of k M alone is beyond what 2^x can make good.  Parts of a row that are that far below 0
-// count as nothing; a row whose maximum is far either way (all classes masked, say) is left to the kernel that comes next, whose warps make
-// its sums from memory (FarRow).  Neighbouring logits are 2^64 apart there: what is not equal to M is next to nothing.
+// Far from 0 the rounding of k M becomes more than 2^x can make good.  A row whose maximum is far either way, |k M| from 2^26 on (all
+// classes masked, say), is left to the kernel that comes next, whose warps make its sums from memory with exponents k (z - M) (FarRow).
+// Parts of another row that lie below -2^30 count as nothing beside it.
 //
 // A row is walked in units of 16 bytes by address, of which the first and the last may stick out of it, whatever its alignment.  Rows
 // reach registers through a ring in shared memory (LogitRowsKernel); wide rows, and few ones, are shared by the blocks of a cluster.
@@ -153,26 +153,29 @@ __device__ __forceinline__ double LogOf(float s) {
 }
 
 constexpr double kLow = 5.1e-8;
-constexpr float kFar = 0x1p30f;
+constexpr float kFar = 0x1p26f, kNothing = -0x1p30f;
 __device__ __forceinline__ bool IsFar(float mk) { return fabsf(mk) >= kFar; }
-// k M as it is used; -inf: nothing here, or nothing that shows beside a row that is not far.
+// k M as it is used; -inf: nothing here, or nothing that shows beside a row that is not far.  (Above -2^30 a part's terms are 2^96 at
+// most, and its factor beside a row that is not far is 0.)
 template <bool kPolicy>
 __device__ __forceinline__ float TopOf(const LogitArgs& a, float z) {
   const float km = __fmul_rn(z, a.k), top = kPolicy ? km : ceilf(km);
-  return top > -kFar ? top : MinusInf();
+  return top > kNothing ? top : MinusInf();
 }
 
 // Of a row: the label's logit, k M (of a far row: what FarOf makes of M), the sum over the others, the sum over all.
 struct RowSums {
   float z_label, mk, others, s;
 };
-// A logit of a far row: times a power of two, which is exact, and above k, so that what was far is 2^30 at least.  (Beyond f32, where a
-// mask's lowest value may lie: f32's largest number.)
+// A far row's M is kept times a power of two, which is exact, and above k, so that what was far is 2^26 at least.  (What that takes beyond
+// f32, where a mask's lowest value may lie, is as good as f32's largest number.)
 __device__ __forceinline__ float FarOf(const LogitArgs& a, float z) {
   const float m = z * a.k_up;
   return isinf(m) && !isinf(z) ? copysignf(0x1.fffffep127f, m) : m;
 }
-__device__ __forceinline__ float FarPower(const LogitArgs& a, float z, float mk) { return Ex2Approx(FarOf(a, z) - mk); }
+// z - M of such a row, and 2^(k (z - M)).
+__device__ __forceinline__ float FarOff(const LogitArgs& a, float z, float mk) { return (FarOf(a, z) - mk) / a.k_up; }
+__device__ __forceinline__ float FarPower(const LogitArgs& a, float z, float mk) { return Ex2Approx(FarOff(a, z, mk) * a.k); }
 __device__ __forceinline__ float LabelTerm(const LogitArgs& a, float z_label, float mk) {
   return Ex2Approx(fmaf(z_label, a.k_rest, fmaf(z_label, a.k, -mk)));
 }
@@ -279,15 +282,16 @@ __device__ __noinline__ RowSums FarRow(const LogitArgs& a, uint64_t r, int32_t l
     for (int j = 0; j < kPerUnit<T>; ++j) top = fmaxf(top, v[j]);
   }
   const float z_label = ToF32(row.z[label]), mk = FarOf(a, WarpMax(top));
-  float others = 0.0f;
+  double sum = 0.0;   // (a lane has thousands of terms)
   for (uint32_t u = lane; u < row.units; u += 32) {
     row.Load(u, v);
+    float part = 0.0f;
 #pragma unroll
     for (int j = 0; j < kPerUnit<T>; ++j)
-      if (row.At(u) + j != label) others += FarPower(a, v[j], mk);
+      if (row.At(u) + j != label) part += FarPower(a, v[j], mk);
+    sum += static_cast<double>(part);
   }
-#pragma unroll
-  for (uint32_t o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xFFFFFFFFu, others, o);
+  const float others = static_cast<float>(WarpSum(sum));
   return {z_label, mk, others, others + FarPower(a, z_label, mk)};
 }
 // Its dlogits, by a warp.

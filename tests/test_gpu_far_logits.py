@@ -1,7 +1,6 @@
 """Losses over rows whose largest logit is far from 0: classes masked with large negative numbers or the type's lowest value, all of them or
-all but some, and rows of large positive ones.  What is equal to the largest shares the row; the rest has no chance.
-
-Tolerances are logit_reference's, for off = z - max z is 0 or so far below that nothing is left of it."""
+all but some, and rows of large positive ones.  What is equal to the largest shares the row; the rest has no chance, or, where logits next to
+one another are some units apart, the chance that the formula gives it.  Tolerances are logit_reference's."""
 
 import math
 
@@ -15,8 +14,8 @@ from test_gpu_preference_loss import Preference
 
 pytestmark = pytest.mark.gpu
 
-FAR = {"f32": [-1e9, -3e9, -1e10, -1e20, -1e30, -1e37, 3e9, 1e10, 1e25, 1e37, "lowest"],
-       "bf16": [-1e9, -3e9, -1e10, -1e20, -1e37, 1e10, 1e37, "lowest"],
+FAR = {"f32": [-5e7, -1e8, 2e8, -1e9, -3e9, -1e10, -1e20, -1e30, -1e37, 3e9, 1e10, 1e25, 1e37, "lowest"],
+       "bf16": [-1e8, 3e8, -1e9, -3e9, -1e10, -1e20, -1e37, 1e10, 1e37, "lowest"],
        "f16": [-60000.0, 60000.0, "lowest"]}
 
 
@@ -128,3 +127,47 @@ def test_labels_without_a_chance(be, dtype):
         rest = torch.ones(rows, device="cuda", dtype=torch.bool)
         rest[2:5] = False
         assert ((c.logp.double() - want).abs() <= 4 * R.ULP * want.abs())[rest].all()
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e-3, 0.25])
+@pytest.mark.parametrize("rows,classes", [(1300, 250), (64, 250), (64, 5003), (9, 128003), (9, 300001)])
+def test_neighbours(be, rows, classes, scale):
+    """Rows of one far value and the three f32 numbers below it."""
+    at = [v / scale for v in (1.2e7, -4e7, 5e7, -1e8, 2e8, 7e8, -7.5e8, 1.4e9, -3e9)]
+
+    def fill(logits):
+        for r in range(rows):
+            steps = [torch.tensor(at[r % len(at)], dtype=torch.float32)]
+            for _ in range(3):
+                steps.append(torch.nextafter(steps[-1], torch.tensor(-math.inf)))
+            logits[r] = torch.stack(steps).cuda()[(torch.arange(classes, device="cuda") * 7 + r) % 4]
+
+    c = Policy(rows, classes, "f32", seed=26, kl=0.0, scale=scale)
+    fill(c.logits)
+    c.labels = torch.randint(classes, (rows,), device="cuda", dtype=torch.int32)
+    c.reference = R.Rows(c.logits, c.labels, scale)
+    c.old = (c.reference.logp - 0.1).float()
+    c.a, c.w = torch.randn(rows, device="cuda"), torch.rand(rows, device="cuda")
+    c(be)
+    c.check(c.d)
+    half = rows // 2
+    q = Preference([half, rows - half], classes, "f32", seed=27, reference=False, scale=scale, behind=0)
+    fill(q.logits)
+    q.reference = R.Rows(q.logits, q.labels, scale)
+    q(be)
+    q.check(q.d)
+
+
+@pytest.mark.parametrize("dtype", list(R.DTYPES))
+@pytest.mark.parametrize("rows,classes,stride,begin,d_begin", [(1300, 250, 251, 3, 3), (60, 250, 251, 1, 2), (40, 5003, 5011, 5, 0), (9, 32000, 33001, 7, 7),
+                                                              (9, 128003, 128003, 1, 5)])
+def test_strides_and_alignments(be, rows, classes, stride, begin, d_begin, dtype):
+    c = fill(Policy(rows, classes, dtype, seed=28, kl=0.0, stride=stride, begin=begin, d_begin=d_begin))
+    c.reference = R.Rows(c.logits, c.labels)
+    c.old = (c.reference.logp - 0.1).float()
+    before = c.buf.clone()
+    c(be)
+    c.check(c.d)
+    assert torch.equal(c.buf, before)
+    c.d[:] = 9.0
+    assert (c.d_buf == 9).all()
